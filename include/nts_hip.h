@@ -487,6 +487,80 @@ int nts_message_rows_add(float *rows, const float *records, uint32_t n_records, 
                          uint32_t id_end, nts_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Vertex tables in few bits.  Feature rows in 4 bits, the products of a dense layer on them, and a cache of
+ * keys and values in 8 bits with the attention that reads it.  No counterparts in the reference, whose tables
+ * are fp32 (core/ntsDataloador.hpp:78-88).
+ *
+ * 4-bit rows (OCP microscaling, MXFP4).  A table of rows of F values is two arrays:
+ *   codes   [rows, 16 * B] bytes, B = ceil(F / 32): block b of a row holds its values 32 b .. 32 b + 31, the
+ *           even one of two neighbours in the low half of its byte; values behind F are 0.  A code is a sign
+ *           bit and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  16-byte aligned.
+ *   scales  [rows, 4 * ceil(B / 4)] bytes: byte s scales its block by 2^(s - 127); 255 makes all of the block
+ *           NaN.  4-byte aligned.
+ * Either array may be device memory or mapped host memory for nts_gather_rows_mxfp4 (codes on the host and scales on
+ * the device: one link read per 64 bytes of row); the products take device memory.  A row id that is not below
+ * table_rows (e.g. 0xFFFFFFFF, the padding of a batch) names a row of zeros.  F and N are at most 131,072.
+ * ------------------------------------------------------------------------------------------- */
+
+/* codes, scales = x [n, F] rounded.  Per block: e = max(floor(log2 max|x|) - 2, -127), scale byte e + 127, code = the
+ * one nearest to x * 2^-e, ties to the even code, magnitudes above 6 to 6.  A block that holds an infinity or a NaN gets
+ * scale byte 255.  Every byte of both arrays is written. */
+int nts_mxfp4_quantize(uint8_t *codes, uint8_t *scales, const float *x, uint32_t n, uint32_t F, nts_stream_t stream);
+/* nts_gather_rows_f32 for a 4-bit table: out[i, :] = values of row row_ids[i] (row_ids NULL: row i), exactly. */
+int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids,
+                          uint32_t n, uint32_t F, nts_stream_t stream);
+/* A dense layer on rows gathered by id: out[i, j] (+)= sum_f A[row_ids[i], f] * W[j, f], i < n, j < N, where W is a 4-bit
+ * table of N rows of F values (the layer's weight, a row per output).  Products are exact, sums are kept in 32 bits.
+ * row_ids NULL: row i.  accumulate as in nts_spmm_gather. */
+int nts_mxfp4_product(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids,
+                      uint32_t n, const uint8_t *w_codes, const uint8_t *w_scales, uint32_t N, uint32_t F, int accumulate,
+                      nts_stream_t stream);
+/* Gradients of the product with respect to the values that the two tables stand for (a caller that rounded fp32 weights
+ * passes them on to those unchanged):
+ *   nts_mxfp4_product_grad_rows    gx[i, f] (+)= sum_j gout[i, j] * W[j, f]                [n, F]
+ *   nts_mxfp4_product_grad_weight  gw[j, f] (+)= sum_i gout[i, j] * A[row_ids[i], f]       [N, F]
+ * gout is used in full 32-bit precision.  The second sums in parts whose number depends on n, N and F alone, added in order: the
+ * same bits on every call.  It takes nts_mxfp4_product_grad_weight_work_bytes(n, N, F) bytes of 16-byte-aligned device
+ * memory (0: none), which calls that overlap must not share. */
+int nts_mxfp4_product_grad_rows(float *gx, const float *gout, const uint8_t *w_codes, const uint8_t *w_scales, uint32_t n,
+                                uint32_t N, uint32_t F, int accumulate, nts_stream_t stream);
+size_t nts_mxfp4_product_grad_weight_work_bytes(uint32_t n, uint32_t N, uint32_t F);
+int nts_mxfp4_product_grad_weight(float *gw, const float *gout, const uint8_t *codes, const uint8_t *scales,
+                                  uint32_t table_rows, const uint32_t *row_ids, uint32_t n, uint32_t N, uint32_t F,
+                                  int accumulate, void *work, nts_stream_t stream);
+
+/* Cache of keys and values in 8 bits (device memory):
+ *   cache   [capacity, 2, heads, 16 * ceil(width / 16)] e4m3 values, a vertex's keys before its values, columns
+ *           behind `width` 0; 16-byte aligned
+ *   scales  [ceil(capacity / block_rows), 2, heads] bytes: byte s scales the block_rows rows of a block, for keys or
+ *           values and one head, by 2^(s - 127)
+ * width <= 256, heads <= 1,024, block_rows a power of two up to 1,024.
+ *
+ * nts_kv8_append writes rows first .. first + n - 1 from k and v, both [n, heads * width].  The scale of a block is the
+ * smallest power of two (from 2^-127 up) with max|x| <= 448 * scale over the finite values of its rows, codes are the nearest,
+ * ties to even; infinities and NaN become NaN.  Rows of the first block before `first` stay: the block's scale then never
+ * falls below theirs, and where it grows they are rounded once more at the new scale.  Rows from first + n on keep their bytes
+ * but not their meaning where their block's scale changed: the cache ends at first + n.  Calls on one cache must be
+ * ordered by the caller. */
+int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float *v, uint32_t first, uint32_t n,
+                   uint32_t capacity, uint32_t heads, uint32_t width, uint32_t block_rows, nts_stream_t stream);
+/* Every destination's attention over its neighbours' rows of the cache:
+ *   s[e, h]     = score_scale * < q[d, h, :], K[row(e), h', :] >       e in CSC(d), h' = h / (q_heads / heads)
+ *   out[d, h, :] = sum_e softmax_e(s[e, h]) * V[row(e), h', :],   lse[d, h] = log sum_e exp(s[e, h])
+ * row(e) = ri[e], or mirror[ri[e]] (a sampled layer's `source`, whose row_indices are local).  An edge whose row is not
+ * below cache_rows counts for nothing (a neighbour that is not cached); a destination without any other edge gets
+ * out = 0 and lse = -infinity.  q, out: [Vd, q_heads * width], lse [Vd, q_heads] or NULL; q_heads a multiple of heads.
+ * `edges` = co[Vd] - co[0], at most 2^32 - 2^16.  max_degree: the caller's bound on a destination's edges, 0 = none known;
+ * it only selects the launches.  Up to 256 a wavefront takes a destination; otherwise long rows are cut and their parts
+ * joined in order (the same bits on every call), in nts_kv8_attention_work_bytes(...) bytes of 16-byte-aligned device
+ * memory, which calls that overlap must not share.  Scores and sums are kept in 32 bits. */
+size_t nts_kv8_attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t width, uint32_t max_degree);
+int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
+                      const uint32_t *ri, const uint32_t *mirror, uint32_t Vd, uint32_t edges, uint32_t cache_rows,
+                      uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows, float score_scale,
+                      uint32_t max_degree, void *work, nts_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Sampled-layer index construction on the device (sampCSC, core/coocsc.hpp)
  * ------------------------------------------------------------------------------------------- */
 

@@ -93,6 +93,16 @@ SIGNATURES = {
     "nts_gather_labels_i64": [_vp, _vp, _vp, _u32, _u32, _vp],
     "nts_message_rows_unpack": [_vp, _vp, _u32, _u32, _u32, _u32, _vp],
     "nts_message_rows_add": [_vp, _vp, _u32, _u32, _u32, _u32, _vp],
+    "nts_mxfp4_quantize": [_vp, _vp, _vp, _u32, _u32, _vp],
+    "nts_gather_rows_mxfp4": [_vp, _vp, _vp, _u32, _vp, _u32, _u32, _vp],
+    "nts_mxfp4_product": [_vp, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _int, _vp],
+    "nts_mxfp4_product_grad_rows": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _int, _vp],
+    "nts_mxfp4_product_grad_weight_work_bytes": [_u32, _u32, _u32],
+    "nts_mxfp4_product_grad_weight": [_vp, _vp, _vp, _vp, _u32, _vp, _u32, _u32, _u32, _int, _vp, _vp],
+    "nts_kv8_append": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp],
+    "nts_kv8_attention_work_bytes": [_u32, _u32, _u32, _u32, _u32],
+    "nts_kv8_attention": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32, _u32, _vp,
+                          _vp],
     "nts_sample_hop_work_bytes": [_u32],
     "nts_sample_hop_offsets": [_vp, _vp, _vp, _u32, ctypes.c_int32, _vp, _vp],
     "nts_sample_hop_neighbors": [_vp, _vp, _vp, _vp, _vp, _u32, ctypes.c_int32, ctypes.c_uint64, _vp],
@@ -124,10 +134,12 @@ SIGNATURES = {
 _RESTYPES = {"nts_last_error": ctypes.c_char_p, "nts_fingerprint_finish": _u64, "nts_csr_from_csc_work_bytes": _sz,
              "nts_relabel_sources_work_bytes": _sz, "nts_sample_hop_work_bytes": _sz,
              "nts_chunk_from_edges_work_bytes": _sz, "nts_batch_builder_arena_bytes": _sz,
+             "nts_mxfp4_product_grad_weight_work_bytes": _sz, "nts_kv8_attention_work_bytes": _sz,
              "nts_trace_ranges_emitted": ctypes.c_long, "nts_scratch_alloc_count": ctypes.c_long}
 # Entry points whose int result is a value, not a status.
 _NO_STATUS = {"nts_last_error", "nts_abi_version", "nts_fingerprint_finish", "nts_scratch_alloc_count", "nts_trace_ranges_emitted", "nts_csr_from_csc_work_bytes", "nts_relabel_sources_work_bytes",
-              "nts_sample_hop_work_bytes", "nts_chunk_from_edges_work_bytes", "nts_batch_builder_arena_bytes"}
+              "nts_sample_hop_work_bytes", "nts_chunk_from_edges_work_bytes", "nts_batch_builder_arena_bytes",
+              "nts_mxfp4_product_grad_weight_work_bytes", "nts_kv8_attention_work_bytes"}
 
 
 class SampledLayerDesc(ctypes.Structure):

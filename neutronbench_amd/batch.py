@@ -82,6 +82,13 @@ def load_feature_gpu_cache(cs, layer0, local_feature, table_ptr, cache, source_c
     return hit_pos.numel()
 
 
+def load_feature_mxfp4(cs, layer0, local_feature, table):
+    """X0[i,:] = feature[source[i],:] from a table held in 4 bits (lowbit.MxTable), as floats."""
+    call("nts_gather_rows_mxfp4", ptr(local_feature), ptr(table.codes), ptr(table.scales), table.rows,
+         ptr(layer0.dev_source), layer0.src_size, table.width, cs.stream)
+    cs._end_of_method()
+
+
 def load_label_gpu(cs, top_layer, local_label, global_label):
     classes = 1 if global_label.dim() == 1 else global_label.shape[1]
     if classes > 1:

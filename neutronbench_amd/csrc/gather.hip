@@ -7,7 +7,8 @@
 // zero-copy path, where every wave load becomes PCIe read requests.
 #include <algorithm>
 
-#include "common.hpp"
+#include "launch_size.hpp"
+#include "lowbit.hpp"
 
 namespace nts {
 namespace {
@@ -201,6 +202,36 @@ void launch_rows_any(const RowsArgs &a) {
   return launch_rows_v<float>(a, a.F);
 }
 
+// ---- rows held in 4 bits ------------------------------------------------------------------------------
+// A lane takes eight columns: one word of codes, one scale byte, up to eight floats out.  Lanes of a row are neighbours, so a
+// wavefront reads 256 bytes of codes and writes 2 KB.  An id that the table does not have gives a row of zeros (a padded batch).
+template <typename Index>
+__global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
+                                                             const uint8_t *__restrict__ scales, uint32_t table_rows,
+                                                             const uint32_t *__restrict__ row_ids, uint64_t n_parts, uint32_t F,
+                                                             uint32_t row_parts, uint32_t row_blocks, uint32_t scale_stride) {
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * 256u;
+  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x; t < n_parts; t += step) {
+    const Index i = static_cast<Index>(t) / static_cast<Index>(row_parts);
+    const uint32_t part = static_cast<uint32_t>(static_cast<Index>(t) - i * static_cast<Index>(row_parts));
+    const uint64_t g = row_ids ? row_ids[i] : static_cast<uint64_t>(i);
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (g < table_rows)
+      e2m1_decode8(reinterpret_cast<const uint32_t *>(codes)[g * row_blocks * 4u + part],
+                   e8m0_value(scales[g * scale_stride + part / 4u]), v);
+    const uint32_t col = part * 8u;
+    float *dst = out + static_cast<uint64_t>(i) * F + col;
+    if (col + 8u <= F) {
+      *reinterpret_cast<Quad *>(dst) = Quad{{v[0], v[1], v[2], v[3]}};
+      *reinterpret_cast<Quad *>(dst + 4) = Quad{{v[4], v[5], v[6], v[7]}};
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < 7; ++k)
+        if (col + k < F) dst[k] = v[k];
+    }
+  }
+}
+
 // ---- rows that arrive as message records -----------------------------------------------------------
 // The reference's full-graph GPU operators (ForwardGPUfuseOp, core/ntsDistGPUFusedGraphOp.hpp:49-91) move
 // vertex rows between partitions as records {uint32 vertex id, F floats} in a pinned host buffer, also
@@ -338,6 +369,29 @@ int nts_gather_rows_cached_f32(float *out, const float *table, const float *cach
   RowsArgs a{out, table, cache, row_ids, nullptr, hashmap, n, F, hits, stream};
   launch_rows_any(a);
   NTS_LAUNCH_CHECK("nts_gather_rows_cached_f32");
+  return NTS_OK;
+}
+
+int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids,
+                          uint32_t n, uint32_t F, nts_stream_t stream) {
+  NTS_TRACE_RANGE("nts_gather_rows_mxfp4");
+  if (F == 0 || F > kMostWidth) return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: F is 0 or above 2^17");
+  if (n == 0) return NTS_OK;
+  if (!out || (table_rows && (!codes || !scales))) return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: null pointer");
+  if (!aligned_to(codes, 16) || !aligned_to(scales, 4))
+    return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: codes need 16-byte, scales 4-byte alignment");
+  const uint32_t row_parts = F / 8 + (F % 8 != 0);
+  const uint64_t parts = static_cast<uint64_t>(n) * row_parts;
+  uint64_t blocks = std::min<uint64_t>((parts + 255) / 256, kMostBlocks);
+  if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, host_table_blocks(true));
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  if (parts <= 0xFFFFFFFFull)
+    hipLaunchKernelGGL(gather_mx_rows_kernel<uint32_t>, grid, dim3(256), 0, stream, out, codes, scales, table_rows, row_ids, parts,
+                       F, row_parts, mx_blocks(F), mx_scale_stride(F));
+  else
+    hipLaunchKernelGGL(gather_mx_rows_kernel<uint64_t>, grid, dim3(256), 0, stream, out, codes, scales, table_rows, row_ids, parts,
+                       F, row_parts, mx_blocks(F), mx_scale_stride(F));
+  NTS_LAUNCH_CHECK("nts_gather_rows_mxfp4");
   return NTS_OK;
 }
 

@@ -32,8 +32,10 @@ import time
 import torch
 
 from . import synth
-from .batch import BatchBuilder, FeatureCache, MappedHostTable, load_feature_gpu_cache, load_label_gpu, sample_hop
+from .batch import (BatchBuilder, FeatureCache, MappedHostTable, load_feature_gpu_cache, load_feature_mxfp4, load_label_gpu,
+                    sample_hop)
 from .layout import SampledLayer, as_u32
+from .lowbit import MxProductOp, MxTable
 from .ops import GATAggregateOp, GATAttentionOp, SingleGPUSampleGraphOp
 from .stream import CudaStream
 
@@ -73,7 +75,9 @@ def graph_mode(graph, pipeline, cache=0.0):
 
 
 def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pipeline=1, quiet=False, checksum=False,
-        stage_sync=None, graph=True):
+        stage_sync=None, graph=True, features="f32"):
+    if features not in ("f32", "mxfp4"):
+        raise ValueError("features: f32 or mxfp4")
     cfg = dict(CONFIGS[name])
     graph = graph_mode(graph, pipeline, cfg["cache"])
     dev = torch.device("cuda:0")
@@ -86,8 +90,17 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
     del src, dst
     feat_cpu = synth.normal_features(V, cfg["F"], seed=cfg["seed"] + 40)
     labels = synth.uniform_labels(V, cfg["classes"], seed=cfg["seed"] + 41, device=dev)
-    table = MappedHostTable(feat_cpu)
-    cache = FeatureCache(feat_cpu, out_deg.cpu(), int(V * cfg["cache"]), dev) if cfg["cache"] > 0 else None
+    heads = cfg.get("heads", 0)
+    mx = mx_weight = table = cache = None
+    if features == "mxfp4":
+        # 4-bit rows of the whole graph fit the device memory many times over: no host table, no cache of a part of it.  An
+        # attention configuration starts with a dense layer, whose product reads the rows by id itself.
+        mx = MxTable.quantize(feat_cpu.to(dev))
+        if heads:
+            mx_weight = MxTable.quantize(synth.normal_features(cfg["hidden"], cfg["F"], seed=cfg["seed"] + 43, device=dev))
+    else:
+        table = MappedHostTable(feat_cpu)
+        cache = FeatureCache(feat_cpu, out_deg.cpu(), int(V * cfg["cache"]), dev) if cfg["cache"] > 0 else None
     train_nodes = synth.permutation(V, cfg["seed"] + 42, dev)[:n_train]
     cs = CudaStream()
     # Stages separated by a stream synchronisation, as every reference operator ends with one -- except
@@ -97,7 +110,6 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
     if stage_sync is None:
         stage_sync = not (sampler == "builder" and pipeline > 2)
     tm = Timer(sync=stage_sync)
-    heads = cfg.get("heads", 0)
     n_batches = (n_train + cfg["batch"] - 1) // cfg["batch"]
     if max_batches:
         n_batches = min(n_batches, max_batches)
@@ -131,8 +143,15 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
         return train32[b * cfg["batch"]:(b + 1) * cfg["batch"]]
 
     def gather(stream_obj, layers):
-        x = torch.empty(layers[0].src_size, cfg["F"], device=dev)
-        if cache is not None:
+        if mx_weight is not None:
+            x = MxProductOp(layers[0].dev_source).forward(mx, mx_weight)
+        else:
+            x = torch.empty(layers[0].src_size, cfg["F"], device=dev)
+        if mx is not None:
+            hits = None
+            if mx_weight is None:
+                load_feature_mxfp4(stream_obj, layers[0], x, mx)
+        elif cache is not None:
             hits = load_feature_gpu_cache(stream_obj, layers[0], x, table.dev_ptr, cache)
         else:
             stream_obj.zero_copy_feature_move_gpu(x, table.dev_ptr, layers[0].dev_source, cfg["F"], layers[0].src_size)
@@ -318,10 +337,11 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
     torch.cuda.synchronize()
     epoch_s = time.perf_counter() - t_epoch
     edges_total, hits_total, rows_total = totals["edges"], totals["hits"] + int(hits_on_device.item()), totals["rows"]
-    table.close()
+    if table is not None:
+        table.close()
     out = {
         "config": name, "scale": scale, "vertices": V, "edges": E, "batches": n_batches, "batch_size": cfg["batch"],
-        "warmup_batches": n_warm,
+        "features": features, "warmup_batches": n_warm,
         "fanout_output_side_first": cfg["fanout"], "epoch_s": round(epoch_s, 4),
         "stage_s": {k: round(v, 4) for k, v in tm.t.items()},
         "library_s": round(sum(v for k, v in tm.t.items() if k != "sample" or sampler != "harness"), 4),
@@ -438,6 +458,9 @@ if __name__ == "__main__":
                          "3: transpositions and weights as a second graph on the builder's own stream, beside the "
                          "gather; 0: the launches are enqueued one by one for every batch; default for --pipeline 1: "
                          "3 with a feature cache, 2 without; else 1")
+    ap.add_argument("--features", choices=["f32", "mxfp4"], default="f32",
+                    help="mxfp4: the feature table rounded to 4 bits and held in device memory; attention configurations "
+                         "then read it through the product with the first layer's weight (not with --native)")
     ap.add_argument("--native", action="store_true",
                     help="drive the epoch from C++ (lib/nts_epoch) instead of this module's Python loop")
     ap.add_argument("--write-inputs", metavar="DIR", default=None,
@@ -457,9 +480,11 @@ if __name__ == "__main__":
                         str(int(bool(a.stage_sync)) if a.stage_sync is not None else 1), "--graph",
                         str(graph_mode(True if a.graph is None else a.graph, a.pipeline, cfg["cache"]))]))
     elif a.native:
+        if a.features != "f32":
+            ap.error("--native takes --features f32")
         run_native(a.config, a.scale, a.max_batches, a.warmup_batches, a.pipeline,
                    graph=True if a.graph is None else a.graph, stage_sync=bool(a.stage_sync))
     else:
         run(a.config, a.scale, a.max_batches, a.sampler, a.warmup_batches, a.pipeline,
             stage_sync=None if a.stage_sync is None else bool(a.stage_sync),
-            graph=True if a.graph is None else a.graph)
+            graph=True if a.graph is None else a.graph, features=a.features)
