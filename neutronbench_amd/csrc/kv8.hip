@@ -98,21 +98,22 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // for the edges e of destination d whose source is cached; h' = h / (q_heads / heads).  One pass: the running maximum, sum
 // and weighted sum of values stay in registers and are rescaled when the maximum grows.
 //
-// A lane holds 16 columns of one head: one 16-byte load of a key row and one of a value row.  ND lanes (a power of two) cover a
-// head, `hw` heads lie side by side, and what is left of the wavefront takes further edges of the same destination ("slots"),
-// each with a running softmax of its own, joined at the end.  G query heads that share the head's keys are computed from one
-// load.
+// A lane holds 16 columns of G query heads that share a head of the cache ("unit"): one 16-byte load of a key row and one of a
+// value row serve them.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by side, and further edges of the
+// destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
+// one destination are a walker; a wavefront is one walker or, where rows are short, several.
 struct AttendArgs {
   float *out, *lse;
   const float *q;
   const uint8_t *cache, *scales;
   const uint32_t *co, *ri, *mirror;
   uint32_t Vd, cache_rows, q_heads, heads, D, row_width, block_shift;
-  uint32_t share;                       // query heads per head
-  uint32_t hw_shift;                    // log2 of heads side by side
-  uint32_t head_chunks, share_chunks;   // passes over the edges: blockIdx.y = head chunk * share_chunks + share chunk
+  uint32_t share;          // query heads per head of the cache
+  uint32_t units, per_head;  // units in all and of a head
+  uint32_t passes;           // over the edges, 2^hw_shift units each; neighbouring wavefronts take the passes of one walker
+  uint32_t hw_shift, walker_shift;  // log2 of units side by side, of a walker's lanes
   float score_scale;
-  // edges cut into spans of `span` positions (see below); 0: a wavefront per destination
+  // edges cut into spans of `span` positions (see below)
   uint32_t span, spans;
   uint64_t positions;
   float *partial;
@@ -121,22 +122,59 @@ struct AttendArgs {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int ND, int G>
+// Sum over an aligned group of ND lanes, the same in all of them; the exchanges are part of the additions.
+template <int CTRL>
+__device__ __forceinline__ float add_lane(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int ND>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if (ND > 1) v = add_lane<0xB1>(v);   // neighbours in pairs
+  if (ND > 2) v = add_lane<0x4E>(v);   // pairs in fours
+  if (ND > 4) v = add_lane<0x141>(v);  // fours, mirrored within eight
+  if (ND > 8) v = add_lane<0x140>(v);  // eights, mirrored within sixteen
+  return v;
+}
+
+// What the registers allow, measured: with one query head to a lane four edges at a time and four wavefronts to a SIMD (2.48 M edges, 8
+// query heads of 64: 468 us; three wavefronts 507, two edges 600); with two, two edges and three wavefronts (500 K edges, 16
+// query heads of 128: 233 us; four edges 255, one head to a lane 259).  Four heads to a lane leave one wavefront.
+template <int G>
+constexpr int kAheadOf = G == 1 ? 4 : 2;
+template <int G>
+constexpr int kWavesOf = G == 1 ? 4 : 3;
+
+// NEAR: cache and scales of less than 4 GB each are read through buffer descriptors: 32-bit offsets, and a row that is not there
+// gets an offset beyond the end, which reads zeros without a branch.
+template <int ND, int G, bool NEAR>
 struct Attend {
   const AttendArgs &p;
-  uint32_t dl, kv_head, q_head0, slot, slots;
-  bool live;  // this lane has a head and columns
+  uint32_t dl, kv_head, q_head0, slot, slots, rounds;
+  bool live;  // this lane has a unit and columns
+  uint32_t key_at, row_bytes, values_at;  // the lane's 16 bytes of a row's keys; from there to its values
+  __amdgpu_buffer_rsrc_t cache_words, scale_bytes;
   float q[G][16], acc[G][16], top[G], sum[G];
+  uint32_t col;  // the first of the lane's columns; fewer than 16 of them after join()
 
-  __device__ __forceinline__ Attend(const AttendArgs &args) : p(args) {
-    const uint32_t lane = threadIdx.x & (kWave - 1);
-    dl = lane & (ND - 1);
-    const uint32_t hc = blockIdx.y / p.share_chunks, sc = blockIdx.y - hc * p.share_chunks;
-    kv_head = (hc << p.hw_shift) + ((lane / ND) & ((1u << p.hw_shift) - 1u));
-    slot = lane / (static_cast<uint32_t>(ND) << p.hw_shift);
-    slots = (kWave / ND) >> p.hw_shift;
-    live = kv_head < p.heads && dl * 16u < p.row_width;
-    q_head0 = sc * G;  // within the head's share
+  __device__ __forceinline__ Attend(const AttendArgs &args, uint32_t pass) : p(args) {
+    constexpr uint32_t kShift = ND == 1 ? 0 : ND == 2 ? 1 : ND == 4 ? 2 : ND == 8 ? 3 : 4;
+    const uint32_t l = threadIdx.x & ((1u << p.walker_shift) - 1u);
+    dl = l & (ND - 1);
+    const uint32_t unit = (pass << p.hw_shift) + ((l >> kShift) & ((1u << p.hw_shift) - 1u));
+    rounds = p.walker_shift - p.hw_shift - kShift;
+    slot = l >> (kShift + p.hw_shift);
+    slots = 1u << rounds;
+    live = unit < p.units && dl * 16u < p.row_width;
+    kv_head = unit / p.per_head;
+    q_head0 = (unit - kv_head * p.per_head) * G;  // within the head's share
+    row_bytes = 2u * p.heads * p.row_width;
+    values_at = p.heads * p.row_width;
+    key_at = kv_head * p.row_width + dl * 16u;
+    if (NEAR) {
+      const uint32_t blocks = p.cache_rows ? ((p.cache_rows - 1u) >> p.block_shift) + 1u : 0u;
+      cache_words = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.cache), 0, p.cache_rows * row_bytes, 0x00027000);
+      scale_bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.scales), 0, blocks * 2u * p.heads, 0x00027000);
+    }
   }
 
   __device__ __forceinline__ void begin(uint32_t row) {
@@ -144,106 +182,202 @@ struct Attend {
     for (int g = 0; g < G; ++g) {
       top[g] = -INFINITY;
       sum[g] = 0.0f;
-      const bool there = live && q_head0 + g < p.share;
-      const float *src = p.q + (static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head0 + g) * p.D + dl * 16u;
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        acc[g][i] = 0.0f;
-        q[g][i] = there && dl * 16u + i < p.D ? src[i] : 0.0f;
+      for (int i = 0; i < 16; ++i) acc[g][i] = q[g][i] = 0.0f;
+      if (live && q_head0 + g < p.share) {
+        const float *src = p.q + (static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head0 + g) * p.D + dl * 16u;
+        if (dl * 16u + 16u <= p.D) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const Quad four = *reinterpret_cast<const Quad *>(src + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q[g][i + k] = four.v[k];
+          }
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 15; ++i)
+            if (dl * 16u + i < p.D) q[g][i] = src[i];
+        }
       }
     }
   }
 
-  // Edges [j0, j1) of the destination whose edges begin at `first`.
-  __device__ __forceinline__ void edges(uint32_t first, uint32_t j0, uint32_t j1) {
+  // The cache row of edge j, or a row that no cache has for an edge behind the last.
+  __device__ __forceinline__ uint32_t cache_row(const uint32_t *ids, uint32_t j, uint32_t j1) const {
+    uint32_t r = ids[min(j, j1 - 1u)];
+    if (p.mirror) r = p.mirror[r];
+    return j < j1 ? r : 0xFFFFFFFFu;
+  }
+
+  // Edges of a slot whose rows are requested together.
+  static constexpr int kAhead = kAheadOf<G>;
+  template <int U>
+  __device__ __forceinline__ void step(const uint32_t *row) {
+    u32x4 kc[U], vc[U];
+    uint32_t kb[U], vb[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      there[u] = row[u] < p.cache_rows;
+      if (NEAR) {
+        const bool read = there[u] && live;
+        const uint32_t at = read ? row[u] * row_bytes + key_at : 0xFFFFFF00u;
+        const uint32_t scale_at = read ? (row[u] >> p.block_shift) * 2u * p.heads + kv_head : 0xFFFFFF00u;
+        kc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, 0, 0);
+        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, values_at, 0);
+        kb[u] = __builtin_amdgcn_raw_buffer_load_b8(scale_bytes, scale_at, 0, 0);
+        vb[u] = __builtin_amdgcn_raw_buffer_load_b8(scale_bytes, scale_at, p.heads, 0);
+      } else {
+        kc[u] = vc[u] = u32x4{0, 0, 0, 0};
+        kb[u] = vb[u] = 0;
+        if (there[u] && live) {
+          const uint8_t *at = p.cache + static_cast<uint64_t>(row[u]) * row_bytes + key_at;
+          kc[u] = *reinterpret_cast<const u32x4 *>(at);
+          vc[u] = *reinterpret_cast<const u32x4 *>(at + values_at);
+          const uint8_t *s = p.scales + static_cast<uint64_t>(row[u] >> p.block_shift) * 2u * p.heads + kv_head;
+          kb[u] = s[0];
+          vb[u] = s[p.heads];
+        }
+      }
+    }
     const float unit = p.score_scale * kLog2e;
-    for (uint32_t j = j0; j < j1; j += slots) {
-      const bool mine = j + slot < j1;
-      uint32_t g_row = 0xFFFFFFFFu;
-      if (mine) {
-        g_row = p.ri[static_cast<uint64_t>(first) + j + slot];
-        if (p.mirror) g_row = p.mirror[g_row];
-      }
-      const bool there = g_row < p.cache_rows;
-      float k[16], v[16];
-      float ks = 0.0f, vs = 0.0f;
-      uint4 kc = make_uint4(0, 0, 0, 0), vc = kc;
-      if (there && live) {
-        const uint8_t *row = p.cache + (static_cast<uint64_t>(g_row) * 2u * p.heads + kv_head) * p.row_width + dl * 16u;
-        kc = *reinterpret_cast<const uint4 *>(row);
-        vc = *reinterpret_cast<const uint4 *>(row + static_cast<uint64_t>(p.heads) * p.row_width);
-        const uint8_t *s = p.scales + static_cast<uint64_t>(g_row >> p.block_shift) * 2u * p.heads + kv_head;
-        ks = e8m0_value(s[0]);
-        vs = e8m0_value(s[p.heads]);
-      }
-      e4m3_decode4(kc.x, k), e4m3_decode4(kc.y, k + 4), e4m3_decode4(kc.z, k + 8), e4m3_decode4(kc.w, k + 12);
-      e4m3_decode4(vc.x, v), e4m3_decode4(vc.y, v + 4), e4m3_decode4(vc.z, v + 8), e4m3_decode4(vc.w, v + 12);
+    float s[G][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float k[16];
+      e4m3_decode4(kc[u][0], k), e4m3_decode4(kc[u][1], k + 4), e4m3_decode4(kc[u][2], k + 8), e4m3_decode4(kc[u][3], k + 12);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float s = 0.0f;
+        float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s = fmaf(q[g][i], k[i], s);
-        s = group_sum<ND>(s) * ks * unit;
-        if (there) add(g, s, vs, v);
+        for (int i = 0; i < 16; ++i) dot = fmaf(q[g][i], k[i], dot);
+        dot = __builtin_amdgcn_ldexpf(lanes_sum<ND>(dot) * unit, static_cast<int>(kb[u]) - 127);
+        s[g][u] = there[u] ? dot : -INFINITY;
+      }
+    }
+    float base[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float now = top[g];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now = fmaxf(now, s[g][u]);
+      base[g] = now == -INFINITY ? 0.0f : now;
+      const float keep = __builtin_amdgcn_exp2f(top[g] - base[g]);
+      top[g] = now;
+      sum[g] *= keep;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[g][i] *= keep;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[16];
+      e4m3_decode4(vc[u][0], v), e4m3_decode4(vc[u][1], v + 4), e4m3_decode4(vc[u][2], v + 8), e4m3_decode4(vc[u][3], v + 12);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float w = __builtin_amdgcn_exp2f(s[g][u] - base[g]);
+        sum[g] += w;
+        const float wv = __builtin_amdgcn_ldexpf(w, static_cast<int>(vb[u]) - 127);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[g][i] = fmaf(wv, v[i], acc[g][i]);
       }
     }
   }
 
-  __device__ __forceinline__ void add(int g, float s, float vs, const float *v) {
-    const float now = fmaxf(top[g], s);
-    const float base = now == -INFINITY ? 0.0f : now;
-    const float keep = __builtin_amdgcn_exp2f(top[g] - base), w = __builtin_amdgcn_exp2f(s - base);
-    top[g] = now;
-    sum[g] = fmaf(sum[g], keep, w);
-    const float wv = w * vs;
+  // Edges [j0, j1) of the destination whose edges begin at `first`; the next step's rows are looked up ahead.
+  __device__ __forceinline__ void edges(uint32_t first, uint32_t j0, uint32_t j1) {
+    if (j0 >= j1) return;
+    const uint32_t *ids = p.ri + first;
+    uint32_t row[kAhead];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[g][i] = fmaf(wv, v[i], acc[g][i] * keep);
+    for (int u = 0; u < kAhead; ++u) row[u] = cache_row(ids, j0 + u * slots + slot, j1);
+    uint32_t j = j0;
+    for (; j1 - j > kAhead * slots; j += kAhead * slots) {
+      uint32_t next[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next[u] = cache_row(ids, j + (kAhead + u) * slots + slot, j1);
+      step<kAhead>(row);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) row[u] = next[u];
+    }
+    if (j1 - j > kAhead / 2 * slots)
+      step<kAhead>(row);
+    else if (kAhead == 2 || j1 - j <= slots)
+      step<1>(row);
+    else
+      step<2>(row);
   }
 
-  // Joins the slots: every slot ends up with the whole.
+  // Joins the slots.  Each round halves a lane's columns: it hands one half to the lane of the other slot and takes in that one's
+  // part of its own half, so 16 columns and 2^r slots take 8 + 4 + .. exchanges instead of 16 a round.
   __device__ __forceinline__ void join() {
-    for (uint32_t m = static_cast<uint32_t>(ND) << p.hw_shift; m < static_cast<uint32_t>(kWave); m <<= 1) {
+    col = dl * 16u;
+    const uint32_t lanes = 1u << (p.walker_shift - rounds);
+#pragma unroll
+    for (uint32_t r = 0; r < 6; ++r) {
+      if (r >= rounds) break;
+      const uint32_t m = lanes << r;
+      const int half = r < 4 ? 8 >> r : 0;
+      const bool upper = (slot >> r) & 1u;
+      if (half && upper) col += half;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float other = __shfl_xor(top[g], m, kWave), more = __shfl_xor(sum[g], m, kWave);
         const float now = fmaxf(top[g], other), base = now == -INFINITY ? 0.0f : now;
         const float a = __builtin_amdgcn_exp2f(top[g] - base), b = __builtin_amdgcn_exp2f(other - base);
         top[g] = now;
-        sum[g] = sum[g] * a + more * b;
+        // both sides of the exchange add in the same order: the lower slot's part first
+        sum[g] = upper ? more * b + sum[g] * a : sum[g] * a + more * b;
+        if (half) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[g][i] = acc[g][i] * a + __shfl_xor(acc[g][i], m, kWave) * b;
+          for (int i = 0; i < (half ? half : 1); ++i) {
+            const float mine = upper ? acc[g][i + half] : acc[g][i], give = upper ? acc[g][i] : acc[g][i + half];
+            acc[g][i] = mine * a + __shfl_xor(give, m, kWave) * b;
+          }
+        } else {
+          acc[g][0] = acc[g][0] * a + __shfl_xor(acc[g][0], m, kWave) * b;
+        }
       }
     }
   }
 
-  __device__ __forceinline__ void write(uint32_t row) {
-    if (slot != 0 || !live) return;
+  // A lane's columns after join(), times `factor`, to a row of D columns.
+  __device__ __forceinline__ void store(float *dst, int g, float factor) const {
+    const uint32_t count = rounds < 4 ? 16u >> rounds : 1u;
+    if (slot >> 4) return;  // further slots hold the same columns
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i += 4) {
+      if (i >= count) break;
+      if (count >= 4 && col + i + 4u <= p.D) {
+        *reinterpret_cast<Quad *>(dst + col + i) = Quad{{acc[g][i] * factor, acc[g][i + 1] * factor, acc[g][i + 2] * factor, acc[g][i + 3] * factor}};
+      } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+          if (i + k < count && col + i + k < p.D) dst[col + i + k] = acc[g][i + k] * factor;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void write(uint32_t row) const {
+    if (!live) return;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (q_head0 + g >= p.share) continue;
       const uint64_t at = static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head0 + g;
-      float *dst = p.out + at * p.D + dl * 16u;
-      const float inv = sum[g] == 0.0f ? 0.0f : 1.0f / sum[g];
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i)
-        if (dl * 16u + i < p.D) dst[i] = acc[g][i] * inv;
-      if (p.lse && dl == 0) p.lse[at] = sum[g] == 0.0f ? -INFINITY : (top[g] + __builtin_amdgcn_logf(sum[g])) * kLn2;
+      store(p.out + at * p.D, g, sum[g] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[g]));
+      if (p.lse && dl == 0 && slot == 0) p.lse[at] = sum[g] == 0.0f ? -INFINITY : (top[g] + __builtin_amdgcn_logf(sum[g])) * kLn2;
     }
   }
 
   // A part of a destination's edges: top, sum and weighted sums of every query head, for join_spans_kernel.
-  __device__ __forceinline__ void write_partial(uint32_t record) {
-    if (slot != 0 || !live) return;
-    const uint64_t size = static_cast<uint64_t>(p.q_heads) * (p.D + 2u);
+  __device__ __forceinline__ void write_partial(uint64_t record) const {
+    if (!live) return;
+    float *dst = p.partial + record * p.q_heads * (p.D + 2u);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (q_head0 + g >= p.share) continue;
-      float *dst = p.partial + record * size;
       const uint32_t h = kv_head * p.share + q_head0 + g;
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i)
-        if (dl * 16u + i < p.D) dst[static_cast<uint64_t>(h) * p.D + dl * 16u + i] = acc[g][i];
-      if (dl == 0) {
+      store(dst + static_cast<uint64_t>(h) * p.D, g, 1.0f);
+      if (dl == 0 && slot == 0) {
         dst[static_cast<uint64_t>(p.q_heads) * p.D + h] = top[g];
         dst[static_cast<uint64_t>(p.q_heads) * (p.D + 1u) + h] = sum[g];
       }
@@ -251,12 +385,21 @@ struct Attend {
   }
 };
 
-// A wavefront per destination.
-template <int ND, int G>
-__global__ __launch_bounds__(256) void kv8_attend_rows_kernel(AttendArgs p) {
-  Attend<ND, G> a(p);
-  const uint64_t waves = static_cast<uint64_t>(gridDim.x) * (256 / kWave);
-  for (uint64_t row = wave_of_grid(); row < p.Vd; row += waves) {
+__device__ __forceinline__ uint64_t walker_of_grid(const AttendArgs &p, uint32_t *pass) {
+  const uint64_t w = (static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x) >> p.walker_shift;
+  *pass = p.passes == 1 ? 0u : static_cast<uint32_t>(w % p.passes);
+  return p.passes == 1 ? w : w / p.passes;
+}
+
+// A walker per destination.
+template <int ND, int G, bool NEAR>
+__global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_rows_kernel(AttendArgs p) {
+  uint32_t pass;
+  uint64_t row = walker_of_grid(p, &pass);
+  Attend<ND, G, NEAR> a(p, pass);
+  const uint64_t walkers = (static_cast<uint64_t>(gridDim.x) * 256u >> p.walker_shift) / p.passes;  // whole rounds of passes
+  if (row >= walkers) return;
+  for (; row < p.Vd; row += walkers) {
     const uint32_t first = p.co[row], degree = p.co[row + 1] - first;
     a.begin(static_cast<uint32_t>(row));
     a.edges(first, 0, degree);
@@ -266,127 +409,201 @@ __global__ __launch_bounds__(256) void kv8_attend_rows_kernel(AttendArgs p) {
 }
 
 // Long rows are shared out and short ones bundled without a look at the degrees on the host: destinations and edges are
-// lined up -- destination r takes position r + co[r] - co[0], its edges the positions behind it -- and every wavefront walks
-// one span of `span` positions.  Destinations that lie within the span are written at once; a part of one that reaches over
-// the span's end or its beginning goes to the span's two records (0: began in an earlier span, 1: goes on in the next), and
-// join_spans_kernel adds the parts in order.  No atomics: the same bits on every call.
+// lined up -- destination r takes position r + co[r] - co[0], its edges the positions behind it -- and every walker takes the
+// destinations that begin within its span of `span` positions.  A destination of more than `span` edges is cut at the
+// spans' ends: every span that it reaches into sums its part into a record (1: the destination begins in this span, 0: in an
+// earlier one) and join_spans_kernel adds the parts in order.  No atomics: the same bits on every call.
 __device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r + (co[r] - co0); }
 
-// The last destination at or before position x: 64 candidates a step.
-__device__ __forceinline__ uint32_t destination_at(const uint32_t *co, uint32_t co0, uint32_t Vd, uint64_t x) {
-  const uint32_t lane = threadIdx.x & (kWave - 1);
+// The last destination at or before position x: a candidate for every lane of the walker a step.
+__device__ __forceinline__ uint32_t destination_at(const uint32_t *co, uint32_t co0, uint32_t Vd, uint64_t x, uint32_t walker_shift) {
+  const uint32_t lanes = 1u << walker_shift, lane = threadIdx.x & (lanes - 1u);
+  const uint64_t group = lanes == 64u ? ~0ull : ((1ull << lanes) - 1ull) << ((threadIdx.x & 63u) & ~(lanes - 1u));
   uint32_t lo = 0, hi = Vd;  // position_of(lo) <= x, the answer is in [lo, hi)
   while (hi - lo > 1) {
-    const uint32_t step = (hi - lo + kWave - 1) / kWave;
-    const uint64_t r = static_cast<uint64_t>(lo) + static_cast<uint64_t>(lane) * step;
+    const uint32_t step = lanes == 1u ? (hi - lo) / 2u : (hi - lo - 1u) / lanes + 1u;
+    const uint64_t r = static_cast<uint64_t>(lo) + static_cast<uint64_t>(lanes == 1u ? 1u : lane) * step;
     const bool before = r < hi && position_of(co, co0, r) <= x;
-    const uint32_t count = __popcll(__ballot(before));  // the first lane always counts
-    const uint32_t next = lo + (count - 1) * step;
+    if (lanes == 1u) {
+      if (before) lo += step; else hi = lo + step;
+      continue;
+    }
+    const uint32_t count = __popcll(__ballot(before) & group);  // lane 0 always counts
+    const uint32_t next = lo + (count - 1u) * step;
     hi = hi - next > step ? next + step : hi;
     lo = next;
   }
   return lo;
 }
 
-template <int ND, int G>
-__global__ __launch_bounds__(256) void kv8_attend_spans_kernel(AttendArgs p) {
-  const uint32_t span = static_cast<uint32_t>(wave_of_grid());
+template <int ND, int G, bool NEAR>
+__global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_spans_kernel(AttendArgs p) {
+  uint32_t pass;
+  const uint64_t span = walker_of_grid(p, &pass);
   if (span >= p.spans) return;
-  Attend<ND, G> a(p);
-  const uint64_t begin = static_cast<uint64_t>(span) * p.span, end = min(begin + p.span, p.positions);
+  Attend<ND, G, NEAR> a(p, pass);
+  const uint64_t begin = span * p.span, end = min(begin + p.span, p.positions);
   const uint32_t co0 = p.co[0];
-  uint32_t row = wave_first(destination_at(p.co, co0, p.Vd, begin));
   uint32_t tail = kNoSlot;
-  for (; row < p.Vd; ++row) {
+  for (uint32_t row = destination_at(p.co, co0, p.Vd, begin, p.walker_shift); row < p.Vd; ++row) {
     const uint32_t first = p.co[row], degree = p.co[row + 1] - first;
     const uint64_t at = static_cast<uint64_t>(row) + (first - co0);  // the destination's own position, its edges behind it
     if (at >= end) break;
+    const bool cut = degree > p.span;
+    if (at < begin && !cut) continue;  // the earlier span has done it
     const uint32_t j0 = at + 1 < begin ? static_cast<uint32_t>(min<uint64_t>(begin - at - 1, degree)) : 0u;
-    const uint32_t j1 = static_cast<uint32_t>(min<uint64_t>(degree, end - at - 1));
+    const uint32_t j1 = cut ? static_cast<uint32_t>(min<uint64_t>(degree, end - at - 1)) : degree;
+    if (j0 >= j1 && at < begin) continue;
     a.begin(row);
     a.edges(first, j0, j1);
     a.join();
-    const bool goes_on = j1 < degree;
-    if (at < begin) {
-      if (degree && j0 < degree) a.write_partial(span * 2u);
-    } else if (goes_on) {
-      a.write_partial(span * 2u + 1u);
-      tail = row;
-    } else {
+    if (!cut) {
       a.write(row);
+      continue;
     }
-    if (goes_on) break;
+    a.write_partial(span * 2u + (at < begin ? 0u : 1u));
+    if (at >= begin) tail = row;
   }
-  if (blockIdx.y == 0 && (threadIdx.x & (kWave - 1)) == 0) p.tail_row[span] = tail;
+  if (pass == 0 && (threadIdx.x & ((1u << p.walker_shift) - 1u)) == 0) p.tail_row[span] = tail;
 }
 
-// The destinations that reach over a span's end: a block each, columns in parallel, parts in order.
-__global__ __launch_bounds__(256) void join_spans_kernel(AttendArgs p) {
-  const uint32_t span = blockIdx.x, row = p.tail_row[span];
-  if (row == kNoSlot) return;
-  const uint64_t last_at = static_cast<uint64_t>(row) + (p.co[row + 1] - p.co[0]);  // position of its last edge
-  const uint32_t last = static_cast<uint32_t>(min<uint64_t>(last_at / p.span, p.spans - 1u));
+// The destinations that were cut: 64 columns a block, its wavefronts take every kJoinWaves-th part, and the first adds up
+// what they have, in order.
+constexpr uint32_t kJoinWaves = 8, kJoinSpans = 8;
+__global__ __launch_bounds__(kJoinWaves *kWave) void join_spans_kernel(AttendArgs p) {
+  __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave];
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block();
+  const uint32_t columns = p.q_heads * p.D, c = blockIdx.y * kWave + lane, h = min(c, columns - 1u) / p.D;
   const uint64_t size = static_cast<uint64_t>(p.q_heads) * (p.D + 2u);
-  const uint32_t columns = p.q_heads * p.D;
-  for (uint32_t c = threadIdx.x; c < columns; c += 256) {
-    const uint32_t h = c / p.D;
+  for (uint32_t k = 0; k < kJoinSpans; ++k) {
+    const uint64_t span = static_cast<uint64_t>(blockIdx.x) * kJoinSpans + k;
+    if (span >= p.spans) break;
+    const uint32_t row = p.tail_row[span];
+    if (row == kNoSlot) continue;
+    const uint64_t last_at = static_cast<uint64_t>(row) + (p.co[row + 1] - p.co[0]);  // position of its last edge
+    const uint64_t last = min<uint64_t>(last_at / p.span, p.spans - 1u);
     float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (uint32_t s = span; s <= last; ++s) {
-      const float *from = p.partial + (static_cast<uint64_t>(s) * 2u + (s == span ? 1u : 0u)) * size;
-      const float t = from[columns + h], l = from[columns + p.q_heads + h], v = from[c];
-      const float now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
-      const float a = __builtin_amdgcn_exp2f(top - base), b = __builtin_amdgcn_exp2f(t - base);
+    const float *const from = p.partial + min(c, columns - 1u);
+    for (uint64_t s = span + wave; s <= last; s += 4 * kJoinWaves) {
+      float t[4], l[4], v[4];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint64_t at = s + u * kJoinWaves;
+        t[u] = -INFINITY, l[u] = v[u] = 0.0f;
+        if (at <= last) {
+          const uint64_t record = (at * 2u + (at == span ? 1u : 0u)) * size;
+          t[u] = p.partial[record + columns + h];
+          l[u] = p.partial[record + columns + p.q_heads + h];
+          v[u] = from[record];
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) now = fmaxf(now, t[u]);
+      const float base = now == -INFINITY ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
       top = now;
-      sum = sum * a + l * b;
-      acc = acc * a + v * b;
+      sum *= a;
+      acc *= a;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float b = __builtin_amdgcn_exp2f(t[u] - base);
+        sum = fmaf(l[u], b, sum);
+        acc = fmaf(v[u], b, acc);
+      }
     }
-    const uint64_t at = static_cast<uint64_t>(row) * p.q_heads + h;
-    p.out[static_cast<uint64_t>(row) * columns + c] = sum == 0.0f ? 0.0f : acc / sum;
-    if (p.lse && c == h * p.D) p.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    tops[wave][lane] = top, sums[wave][lane] = sum, accs[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && c < columns) {
+      for (uint32_t w = 1; w < kJoinWaves; ++w) {
+        const float t = tops[w][lane], now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
+        const float a = __builtin_amdgcn_exp2f(top - base), b = __builtin_amdgcn_exp2f(t - base);
+        top = now;
+        sum = sum * a + sums[w][lane] * b;
+        acc = acc * a + accs[w][lane] * b;
+      }
+      p.out[static_cast<uint64_t>(row) * columns + c] = sum == 0.0f ? 0.0f : acc / sum;
+      if (p.lse && c == h * p.D)
+        p.lse[static_cast<uint64_t>(row) * p.q_heads + h] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+    __syncthreads();
   }
 }
 
 constexpr uint32_t kMostHeadWidth = 256, kMostHeads = 1024, kMostBlockRows = 1024;
-// Above this bound (or without one) a row may be long enough to keep one wavefront busy after the others are done.
+// Above this bound (or without one) a row may be long enough to keep one walker busy after the others are done.
 constexpr uint32_t kMostRowEdges = 256;
-
-// Bytes of a span's two records.
-uint64_t records_bytes(uint32_t q_heads, uint32_t D) { return 2ull * q_heads * (D + 2u) * sizeof(float); }
-// Positions of a span, for `positions` of them: 8,192 spans fill the chip (fewer where their records would take more than
-// 256 MB), none of fewer than 64 positions.
-uint32_t span_length(uint64_t positions, uint32_t q_heads, uint32_t D) {
-  const uint64_t spans = std::max<uint64_t>(256, std::min<uint64_t>(8192, (256ull << 20) / records_bytes(q_heads, D)));
-  const uint64_t wanted = (positions + spans - 1) / spans;
-  return static_cast<uint32_t>(std::max<uint64_t>(wanted, 64));
-}
 bool by_spans(uint32_t max_degree) { return max_degree == 0 || max_degree > kMostRowEdges; }
-
-template <int ND, int G>
-int launch_attend(const AttendArgs &p, hipStream_t stream) {
-  const uint32_t passes = p.head_chunks * p.share_chunks;
-  if (!p.span) {
-    const uint64_t blocks = std::min<uint64_t>((static_cast<uint64_t>(p.Vd) + 3) / 4, kMostBlocks / passes);
-    hipLaunchKernelGGL((kv8_attend_rows_kernel<ND, G>), dim3(static_cast<uint32_t>(blocks), passes), dim3(256), 0, stream, p);
-    NTS_LAUNCH_CHECK("nts_kv8_attention");
-    return NTS_OK;
-  }
-  hipLaunchKernelGGL((kv8_attend_spans_kernel<ND, G>), dim3((p.spans + 3) / 4, passes), dim3(256), 0, stream, p);
-  NTS_LAUNCH_CHECK("nts_kv8_attention");
-  if (p.spans > 1) {
-    hipLaunchKernelGGL(join_spans_kernel, dim3(p.spans), dim3(256), 0, stream, p);
-    NTS_LAUNCH_CHECK("join_spans_kernel");
-  }
-  return NTS_OK;
-}
-template <int ND>
-int launch_attend_g(const AttendArgs &p, uint32_t g, hipStream_t stream) {
-  return g == 1 ? launch_attend<ND, 1>(p, stream) : g == 2 ? launch_attend<ND, 2>(p, stream) : launch_attend<ND, 4>(p, stream);
-}
 
 uint32_t next_power(uint32_t v) {
   uint32_t p = 1;
   while (p < v) p <<= 1;
   return p;
+}
+uint32_t shift_of(uint32_t power) { return static_cast<uint32_t>(__builtin_ctz(power)); }
+
+// How the lanes are laid out.  `slot_edges`: edges of a row for each of its slots.
+struct Lanes {
+  uint32_t nd, g, units, per_head, hw_shift, walker_shift;
+};
+Lanes lanes_for(uint32_t q_heads, uint32_t heads, uint32_t D, uint64_t slot_edges) {
+  Lanes l;
+  const uint32_t share = q_heads / heads;
+  l.nd = next_power(kv8_row_width(D) / 16);
+  // Query heads of a head side by side as long as all fit a wavefront (their loads of the same row meet in the L1, and few
+  // registers leave many wavefronts); two to a lane where the edges would have to be walked more than once.
+  l.g = 1;
+    if (share > 1 && l.nd * heads * share > static_cast<uint32_t>(kWave)) l.g = 2;
+  l.per_head = ceil_div(share, l.g);
+  l.units = heads * l.per_head;
+  const uint32_t hw = std::min(kWave / l.nd, next_power(l.units));
+  l.hw_shift = shift_of(hw);
+  const uint32_t slots = std::min<uint32_t>(kWave / (l.nd * hw), next_power(static_cast<uint32_t>(std::min<uint64_t>(slot_edges, 64))));
+  l.walker_shift = shift_of(l.nd * hw * slots);
+  return l;
+}
+
+// Bytes of a span's two records.
+uint64_t records_bytes(uint32_t q_heads, uint32_t D) { return 2ull * q_heads * (D + 2u) * sizeof(float); }
+// Positions of a span: `walkers` spans fill the chip (fewer where their records would take more than 256 MB), none of fewer
+// than 64 positions.
+uint32_t span_length(uint64_t positions, uint32_t q_heads, uint32_t D) {
+  const uint64_t most = std::max<uint64_t>(256, std::min<uint64_t>(16384, (256ull << 20) / records_bytes(q_heads, D)));
+  const uint64_t spans = std::min(most, std::max<uint64_t>(1024, positions / 256));
+  const uint64_t wanted = (positions + spans - 1) / spans;
+  return static_cast<uint32_t>(std::max<uint64_t>(wanted, 64));
+}
+
+template <int ND, int G, bool NEAR>
+int launch_attend(const AttendArgs &p, hipStream_t stream) {
+  const uint32_t walkers = 256u >> p.walker_shift;  // a block's
+  if (!p.span) {
+    const uint64_t blocks = std::min<uint64_t>((static_cast<uint64_t>(p.Vd) * p.passes + walkers - 1) / walkers, kMostBlocks);
+    hipLaunchKernelGGL((kv8_attend_rows_kernel<ND, G, NEAR>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, p);
+    NTS_LAUNCH_CHECK("nts_kv8_attention");
+    return NTS_OK;
+  }
+  hipLaunchKernelGGL((kv8_attend_spans_kernel<ND, G, NEAR>), dim3(ceil_div(static_cast<uint64_t>(p.spans) * p.passes, walkers)), dim3(256), 0, stream, p);
+  NTS_LAUNCH_CHECK("nts_kv8_attention");
+  if (p.spans > 1) {  // with one span no destination has more edges than it has positions
+    hipLaunchKernelGGL(join_spans_kernel, dim3(ceil_div(p.spans, kJoinSpans), ceil_div(static_cast<uint64_t>(p.q_heads) * p.D, kWave)),
+                       dim3(kJoinWaves * kWave), 0, stream, p);
+    NTS_LAUNCH_CHECK("join_spans_kernel");
+  }
+  return NTS_OK;
+}
+template <int ND, bool NEAR>
+int launch_attend_g(const AttendArgs &p, uint32_t g, hipStream_t stream) {
+  return g == 1 ? launch_attend<ND, 1, NEAR>(p, stream) : launch_attend<ND, 2, NEAR>(p, stream);
+}
+template <bool NEAR>
+int launch_attend_nd(const AttendArgs &p, const Lanes &l, hipStream_t stream) {
+  switch (l.nd) {
+    case 1: return launch_attend_g<1, NEAR>(p, l.g, stream);
+    case 2: return launch_attend_g<2, NEAR>(p, l.g, stream);
+    case 4: return launch_attend_g<4, NEAR>(p, l.g, stream);
+    case 8: return launch_attend_g<8, NEAR>(p, l.g, stream);
+    default: return launch_attend_g<16, NEAR>(p, l.g, stream);
+  }
 }
 
 size_t attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t D, uint32_t max_degree) {
@@ -457,12 +674,12 @@ int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cac
   p.block_shift = static_cast<uint32_t>(__builtin_ctz(block_rows));
   p.share = q_heads / heads;
   p.score_scale = score_scale;
-  const uint32_t nd = next_power(p.row_width / 16);
-  const uint32_t hw = std::min(kWave / nd, next_power(heads));
-  p.hw_shift = static_cast<uint32_t>(__builtin_ctz(hw));
-  const uint32_t g = p.share >= 3 ? 4 : p.share;
-  p.head_chunks = ceil_div(heads, hw);
-  p.share_chunks = ceil_div(p.share, g);
+  // Slots: where a bound is known most rows reach it, and a slot that works through 16 edges costs least (60,000 rows of 10
+  // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four); averages hide longer rows (2.48 M edges in 169 K rows:
+  // 229 us with four slots for 15 edges on average, 264 with two, 572 with one).
+  const Lanes l = lanes_for(q_heads, heads, width, by_spans(max_degree) ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
+  p.units = l.units, p.per_head = l.per_head, p.hw_shift = l.hw_shift, p.walker_shift = l.walker_shift;
+  p.passes = ceil_div(l.units, 1u << l.hw_shift);
   if (by_spans(max_degree)) {
     if (!work || !aligned_to(work, 16)) return fail_in(call, "needs nts_kv8_attention_work_bytes of 16-byte-aligned work");
     p.positions = static_cast<uint64_t>(Vd) + edges;
@@ -471,13 +688,8 @@ int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cac
     p.partial = static_cast<float *>(work);
     p.tail_row = reinterpret_cast<uint32_t *>(p.partial + static_cast<uint64_t>(p.spans) * 2u * q_heads * (width + 2u));
   }
-  switch (nd) {
-    case 1: return launch_attend_g<1>(p, g, stream);
-    case 2: return launch_attend_g<2>(p, g, stream);
-    case 4: return launch_attend_g<4>(p, g, stream);
-    case 8: return launch_attend_g<8>(p, g, stream);
-    default: return launch_attend_g<16>(p, g, stream);
-  }
+  const uint64_t bytes = 2ull * heads * std::max(static_cast<uint64_t>(cache_rows) * p.row_width, static_cast<uint64_t>(cache_rows) / block_rows + 1);
+  return bytes < 0xFFFF0000ull ? launch_attend_nd<true>(p, l, stream) : launch_attend_nd<false>(p, l, stream);
 }
 
 }  // extern "C"
