@@ -73,81 +73,346 @@ struct ProductArgs {
   MxRows w;
   uint32_t N, row_blocks, scale_stride;
   int accumulate;
+  bool streamed;  // rows of whole 16-byte stores: the output, which nothing here reads again, goes past the caches
 };
 
 __device__ __forceinline__ i32x8 operand(i32x4 c) { return i32x8{c.x, c.y, c.z, c.w, 0, 0, 0, 0}; }
 
-// A lane's part of 128 values of a row: block `block` of it; zeros (and a scale of 1) where there is no such block or row.
-__device__ __forceinline__ void load_part(const MxRows &t, uint64_t row, bool there, uint32_t block, const ProductArgs &p,
-                                          i32x4 *codes, uint32_t *scale) {
-  *codes = i32x4{0, 0, 0, 0};
-  *scale = 127u;
-  if (there && block < p.row_blocks) {
-    *codes = *reinterpret_cast<const i32x4 *>(t.codes + (row * p.row_blocks + block) * 16u);
-    *scale = t.scales[row * p.scale_stride + block];
+// Four neighbouring columns of an output row.
+__device__ __forceinline__ void write_columns(const ProductArgs &p, uint64_t i, uint64_t c, f32x4 v) {
+  float *dst = p.out + i * p.N + c;
+  if (c + 4u <= p.N) {
+    if (p.accumulate) {
+      const Quad old = *reinterpret_cast<const Quad *>(dst);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += old.v[k];
+    }
+    if (p.streamed)
+      __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(dst));
+    else
+      *reinterpret_cast<Quad *>(dst) = Quad{{v.x, v.y, v.z, v.w}};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (c + k < p.N) dst[k] = p.accumulate ? dst[k] + v[k] : v[k];
   }
 }
 
-template <int MT, int NT>
-__global__ __launch_bounds__(256) void mx_product_kernel(ProductArgs p) {
-  const uint32_t lane = threadIdx.x & (kWave - 1), r = lane & 15u, part = lane >> 4;
-  const uint64_t tiles_n = (p.N + 16u * NT - 1) / (16u * NT), tiles_m = (static_cast<uint64_t>(p.n) + 16u * MT - 1) / (16u * MT);
-  const uint64_t waves = static_cast<uint64_t>(gridDim.x) * (256 / kWave);
-  for (uint64_t tile = wave_of_grid(); tile < tiles_m * tiles_n; tile += waves) {
-    const uint64_t tm = tile / tiles_n, tn = tile - tm * tiles_n;
-    uint64_t row[MT], col[NT];
-    bool row_there[MT], col_there[NT];
+// 16 rows by 16 columns; the scales are bytes `wb` of `sw` and `ab` of `sa`, constants once inlined.
+__device__ __forceinline__ f32x4 multiply_16(i32x4 w, i32x4 a, f32x4 c, int wb, uint32_t sw, int ab, uint32_t sa) {
+#define NTS_MX_MFMA(WB, AB) \
+  __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(a), c, 4, 4, WB, static_cast<int>(sw), AB, static_cast<int>(sa))
+#define NTS_MX_MFMA_A(WB) (ab == 0 ? NTS_MX_MFMA(WB, 0) : ab == 1 ? NTS_MX_MFMA(WB, 1) : ab == 2 ? NTS_MX_MFMA(WB, 2) : NTS_MX_MFMA(WB, 3))
+  return wb == 0 ? NTS_MX_MFMA_A(0) : wb == 1 ? NTS_MX_MFMA_A(1) : wb == 2 ? NTS_MX_MFMA_A(2) : NTS_MX_MFMA_A(3);
+#undef NTS_MX_MFMA_A
+#undef NTS_MX_MFMA
+}
+
+// Few rows (a prediction for one vertex or some): the weight is what has to be read, once, and its latency is what counts.  A
+// block takes 16 columns and 16 * MT rows; its wavefronts take every kFewWaves-th 128 values of the rows, two at a time, and the
+// first adds up what they have, in order.
+constexpr uint32_t kFewWaves = 8;
+template <int MT>
+__global__ __launch_bounds__(kFewWaves *kWave) void mx_product_few_kernel(ProductArgs p) {
+  __shared__ f32x4 sums[kFewWaves - 1][MT][kWave];
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
+  const uint64_t col = blockIdx.x * 16ull + r;
+  uint64_t row[MT];
+  bool there[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const uint64_t i = (tm * MT + m) * 16u + r;
-      row_there[m] = i < p.n;
-      row[m] = row_there[m] ? (p.row_ids ? p.row_ids[i] : i) : 0u;
-      row_there[m] = row_there[m] && row[m] < p.table_rows;
+  for (int m = 0; m < MT; ++m) {
+    const uint64_t i = (blockIdx.y * MT + m) * 16ull + r;
+    row[m] = 0;
+    there[m] = i < p.n;
+    if (there[m]) row[m] = p.row_ids ? p.row_ids[i] : i;
+    there[m] = there[m] && row[m] < p.table_rows;
+  }
+  f32x4 acc[MT] = {};
+  // a lane's part of 128 values of a row; zeros (and a scale that is none's) where there is no such block or row
+  auto load = [&](const MxRows &t, uint64_t row, bool there, uint32_t block, i32x4 *codes, uint32_t *scale) {
+    *codes = i32x4{0, 0, 0, 0};
+    *scale = 127u;
+    if (there && block < p.row_blocks) {
+      *codes = *reinterpret_cast<const i32x4 *>(t.codes + (row * p.row_blocks + block) * 16u);
+      *scale = t.scales[row * p.scale_stride + block];
+    }
+  };
+  for (uint32_t base = wave * 4u; base < p.row_blocks; base += kFewWaves * 8u) {
+    i32x4 w[2], a[2][MT];
+    uint32_t sw[2], sa[2][MT];
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t block = base + u * kFewWaves * 4u + part;
+      load(p.w, col, col < p.N, block, &w[u], &sw[u]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) load(p.a, row[m], there[m], block, &a[u][m], &sa[u][m]);
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      col[j] = (tn * NT + j) * 16u + r;
-      col_there[j] = col[j] < p.N;
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = multiply_16(w[u], a[u][m], acc[m], 0, sw[u], 0, sa[u][m]);
+  }
+  if (wave) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sums[wave - 1][m][lane] = acc[m];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWaves - 1; ++k) acc[m] += sums[k][m][lane];
+    const uint64_t i = (blockIdx.y * MT + m) * 16ull + r;
+    if (i < p.n) write_columns(p, i, blockIdx.x * 16ull + part * 4u, acc[m]);
+  }
+}
+
+// Many rows: a block of WM x WN wavefronts takes BM rows by BN columns through LDS, a stage of 32 * PARTS values at a time: 64
+// or 128 bytes a row.  The loads write a stage to LDS themselves (no registers between) while the one before it is
+// multiplied.  Part c of row r lies at c ^ (r * PARTS / 16) % PARTS, so that the 16 lanes that read one part of 16 rows meet all
+// banks once.
+// Measured (65,536 rows of 4,096 values by 4,096 columns): 785 us, 2.8 PFLOP/s, where a library's bf16 product of that size
+// takes 1,599.  Without loads and stores 417 us, with the stores 687: the stores of a block's tile, 256 KB, are not hidden behind
+// another's products.  Past the caches they cost less than through them (1,043 -> 900 us).  Registers in place of loads into LDS 1,170;
+// stages of 64 bytes, of which the L2 fetches whole lines, 973 (128 x 128); operands asked for a step ahead 893 -> 785.
+typedef __attribute__((address_space(3))) void *LdsPointer;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00027000);
+}
+// 16 bytes a lane from `from` + offset + at to 1,024 consecutive bytes of LDS.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t *to, uint32_t offset, uint32_t at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPointer)to, 16, offset, at, 0, 0);
+}
+__device__ __forceinline__ void load_to_lds(const uint8_t *from, uint8_t *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (LdsPointer)to, 16, 0, 0);
+}
+constexpr uint32_t kNowhere = 0xFFFFFF00u;  // an offset behind the end of any buffer: reads zeros
+__device__ __attribute__((aligned(16))) uint8_t zero_part[16];  // zeros for the loads that go by address
+
+// Waits for the wavefront's loads and LDS accesses, then for the block.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// NEAR: both tables' codes are less than 4 GB and are read through buffer descriptors, by 32-bit offsets.
+template <int BM, int BN, int WM, int WN, int PARTS, bool NEAR>
+__global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(ProductArgs p, uint32_t tiles_n) {
+  constexpr int kThreads = WM * WN * kWave, kWaves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int kRows = BM + BN, kBytes = PARTS * 16, kLoadRows = kWave / PARTS, kLoads = kRows / kLoadRows / kWaves;
+  constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads, kSpread = 16 / PARTS;
+  static_assert(PARTS == 4 || PARTS == 8, "a row's part of a stage");
+  static_assert(kLoads * kLoadRows * kWaves == kRows && BM % (kLoadRows * kWaves) == 0, "a load's rows are all of A or all of W");
+  static_assert(kLoadRows * kWaves / kSpread % PARTS == 0, "rows of a wavefront's loads are alike in their parts");
+  static_assert(BM % (WM * 64) == 0 && BN % (WN * 64) == 0, "whole words of scales");
+  __shared__ __attribute__((aligned(16))) uint8_t tile0[kRows * kBytes], tile1[kRows * kBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t tile_scales[2][kRows * PARTS];
+  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
+  const uint64_t tm = blockIdx.x / tiles_n;
+  const uint32_t tn = static_cast<uint32_t>(blockIdx.x - tm * tiles_n);
+  // the row of A's or W's table that row `row` of a stage holds; false: none
+  auto table_row = [&](uint32_t row, uint64_t *g) {
+    if (row < BM) {
+      const uint64_t at = tm * BM + row;
+      if (at >= p.n) return false;
+      *g = p.row_ids ? p.row_ids[at] : at;
+      return *g < p.table_rows;
     }
-    f32x4 acc[MT][NT] = {};
-    for (uint32_t base = 0; base < p.row_blocks; base += 4) {
-      i32x4 a[MT], w[NT];
-      uint32_t sa[MT], sw[NT];
+    *g = static_cast<uint64_t>(tn) * BN + row - BM;
+    return *g < p.N;
+  };
+  // A wavefront's load writes 1,024 consecutive bytes of LDS, 16 a lane: kLoadRows rows of a stage.  Which part of its row a lane
+  // fetches is what places the parts as the reads want them.
+  const auto a_codes = buffer_of(p.a.codes, p.table_rows * p.row_blocks * 16u), w_codes = buffer_of(p.w.codes, p.N * p.row_blocks * 16u);
+  uint32_t src[kLoads];
+  const uint8_t *far[kLoads];
+  const uint32_t chunk = (lane ^ ((wave * kLoadRows + lane / PARTS) / kSpread)) % PARTS;  // the same in all of the lane's rows
 #pragma unroll
-      for (int m = 0; m < MT; ++m) load_part(p.a, row[m], row_there[m], base + part, p, &a[m], &sa[m]);
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t row = (i * kWaves + wave) * kLoadRows + lane / PARTS;
+    uint64_t g = 0;
+    const bool there = table_row(row, &g);
+    src[i] = there ? (static_cast<uint32_t>(g) * p.row_blocks + chunk) * 16u : kNowhere;
+    far[i] = there ? (row < BM ? p.a.codes : p.w.codes) + (g * p.row_blocks + chunk) * 16u : nullptr;
+  }
+  auto request = [&](uint8_t *tile, uint32_t base) {  // blocks base .. base + PARTS - 1
+    const bool inside = base + chunk < p.row_blocks;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) load_part(p.w, col[j], col_there[j], base + part, p, &w[j], &sw[j]);
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          acc[m][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[j]), operand(a[m]), acc[m][j], 4, 4, 0,
-                                                                       static_cast<int>(sw[j]), 0, static_cast<int>(sa[m]));
+    for (int i = 0; i < kLoads; ++i) {
+      uint8_t *to = tile + (i * kWaves + wave) * 1024u;
+      if (NEAR)
+        load_to_lds((i + 1) * kLoadRows * kWaves <= BM ? a_codes : w_codes, to, inside ? src[i] : kNowhere, base * 16u);
+      else
+        load_to_lds(inside && far[i] ? far[i] + base * 16ull : zero_part, to);
     }
+  };
+  // Scales: 16 of a row at a time into registers, PARTS of them to LDS with each stage, as words that hold those of one block of
+  // four rows that are 16 apart: four products take theirs from one word.
+  const uint8_t *scale_src[kScaleRows];
+  bool has_scales[kScaleRows];
+  u32x4 words[kScaleRows];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const uint64_t i = (tm * MT + m) * 16u + r;
-      if (i >= p.n) continue;
+  for (int i = 0; i < kScaleRows; ++i) {
+    const uint32_t row = t + i * kThreads;
+    uint64_t g = 0;
+    has_scales[i] = row < kRows && table_row(row, &g);
+    scale_src[i] = has_scales[i] ? (row < BM ? p.a.scales : p.w.scales) + g * p.scale_stride : p.w.scales;
+  }
+  auto request_scales = [&](uint32_t base) {  // behind a row's end: any bytes of it
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint64_t c = (tn * NT + j) * 16u + part * 4u;
-        float *dst = p.out + i * p.N + c;
-        if (c + 4u <= p.N) {
-          Quad q{{acc[m][j].x, acc[m][j].y, acc[m][j].z, acc[m][j].w}};
-          if (p.accumulate) {
-            const Quad old = *reinterpret_cast<const Quad *>(dst);
+    for (int i = 0; i < kScaleRows; ++i) {
+      if (base + 16u <= p.scale_stride) {
+        struct __attribute__((packed, aligned(4))) Words {
+          u32x4 v;
+        };
+        words[i] = reinterpret_cast<const Words *>(scale_src[i] + base)->v;
+      } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q.v[k] += old.v[k];
-          }
-          *reinterpret_cast<Quad *>(dst) = q;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 3; ++k)
-            if (c + k < p.N) dst[k] = p.accumulate ? dst[k] + acc[m][j][k] : acc[m][j][k];
-        }
+        for (uint32_t k = 0; k < 4; ++k)
+          words[i][k] = *reinterpret_cast<const uint32_t *>(scale_src[i] + min(base + k * 4u, p.scale_stride - 4u));
       }
     }
+  };
+  auto keep_scales = [&](uint32_t half, uint32_t s, uint32_t base) {
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) {
+      const uint32_t row = t + i * kThreads;
+      if (row >= kRows) continue;
+      uint8_t *to = &tile_scales[half][(row / 64u * 16u + row % 16u) * 4u + row / 16u % 4u];
+#pragma unroll
+      for (uint32_t k = 0; k < PARTS; k += 4) {
+        // scales of a row that is not there and behind the last block are 0, whatever the table has
+        uint32_t word = has_scales[i] ? words[i][(s % 16u + k) / 4u] : 0u;
+        if (base + k + 4u > p.row_blocks) word &= base + k < p.row_blocks ? (1u << (8u * (p.row_blocks - base - k))) - 1u : 0u;
+        to[k * kRows] = static_cast<uint8_t>(word);
+        to[(k + 1u) * kRows] = static_cast<uint8_t>(word >> 8);
+        to[(k + 2u) * kRows] = static_cast<uint8_t>(word >> 16);
+        to[(k + 3u) * kRows] = static_cast<uint8_t>(word >> 24);
+      }
+    }
+  };
+  const uint32_t m0 = wave / WN * (BM / WM), n0 = BM + wave % WN * (BN / WN);
+  f32x4 acc[MT][NT] = {};
+  // Each step of NT products asks for the next one's operands first; the fences keep the compiler from asking for all at once,
+  // which the registers do not hold, and from putting the products off behind the barrier.
+  auto multiply = [&](const uint8_t *tile, uint32_t half) {
+    const uint32_t at = r * kBytes + ((part ^ (r / kSpread)) % PARTS) * 16u;
+    const uint8_t *words_at = &tile_scales[half][part * kRows + r * 4u];
+    constexpr int kDeep = PARTS / 4;
+    i32x4 w[2][NT], a[2];
+    uint32_t sw[2][NT / 4], sa[2][MT / 4];
+    auto columns = [&](int k) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w[k & 1][j] = *reinterpret_cast<const i32x4 *>(&tile[(n0 + j * 16u) * kBytes + (at ^ (k * 64u))]);
+#pragma unroll
+      for (int j = 0; j < NT; j += 4)
+        sw[k & 1][j / 4] = *reinterpret_cast<const uint32_t *>(words_at + k * 4 * kRows + (n0 / 16u + j) * 16u);
+#pragma unroll
+      for (int m = 0; m < MT; m += 4)
+        sa[k & 1][m / 4] = *reinterpret_cast<const uint32_t *>(words_at + k * 4 * kRows + (m0 / 16u + m) * 16u);
+    };
+    auto rows = [&](int k, int m) { a[m & 1] = *reinterpret_cast<const i32x4 *>(&tile[(m0 + m * 16u) * kBytes + (at ^ (k * 64u))]); };
+    columns(0);
+    rows(0, 0);
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m + 1 < MT) rows(k, m + 1);
+        if (m + 2 == MT && k + 1 < kDeep) columns(k + 1);
+        if (m + 1 == MT && k + 1 < kDeep) rows(k + 1, 0);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[m][j] = multiply_16(w[k & 1][j], a[m & 1], acc[m][j], j % 4, sw[k & 1][j / 4], m % 4, sa[k & 1][m / 4]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[m][j]));
+  };
+  request_scales(0);
+  request(tile0, 0);
+  keep_scales(0, 0, 0);
+  // two stages a turn, so that the halves are constants; one behind the last block is zeros that no memory is read for
+  for (uint32_t base = 0; base < p.row_blocks; base += 2 * PARTS) {
+#pragma unroll
+    for (uint32_t s = 0; s < 2 * PARTS; s += PARTS) {
+      const uint32_t half = s / PARTS, next = base + s + PARTS;
+      stage_barrier();
+      if (next % 16u == 0) request_scales(next);
+      request(half ? tile0 : tile1, next);
+      multiply(half ? tile1 : tile0, half);
+      keep_scales(half ^ 1u, next % 16u, next);
+    }
   }
+  stage_barrier();  // no load may reach the LDS any more
+  // A lane has four columns of 16 rows: stores of 64 bytes a row.  Through LDS, 16 rows at a time, they become 256 bytes a row (part c
+  // of row r at c ^ r).
+  f32x4 *const mine = reinterpret_cast<f32x4 *>(tile0) + wave * 256u;
+  static_assert(NT == 4 && kWaves * 4096 <= kRows * kBytes, "64 columns, and room for 16 rows of every wavefront");
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) mine[r * 16u + ((j * 4u + part) ^ r)] = acc[m][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t row = k * 4u + lane / 16u;
+      const uint64_t i = tm * BM + m0 + m * 16u + row;
+      const f32x4 v = mine[row * 16u + ((lane & 15u) ^ row)];
+      if (i < p.n) write_columns(p, i, static_cast<uint64_t>(tn) * BN + (n0 - BM) + (lane & 15u) * 4u, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int PARTS, bool NEAR>
+void launch_tiled(const ProductArgs &p, hipStream_t stream) {
+  // rows in turns of at most 2^22 tiles, far below what a launch may have
+  const uint32_t tiles_n = ceil_div(p.N, BN), turn = std::max(1u, (1u << 22) / tiles_n) * BM;
+  for (uint64_t first = 0; first < p.n; first += turn) {
+    ProductArgs q = p;
+    q.out = p.out + first * p.N;
+    q.n = static_cast<uint32_t>(std::min<uint64_t>(turn, p.n - first));
+    if (p.row_ids) {
+      q.row_ids = p.row_ids + first;
+    } else {
+      q.a.codes = p.a.codes + first * p.row_blocks * 16u;
+      q.a.scales = p.a.scales + first * p.scale_stride;
+      q.table_rows = p.table_rows > first ? static_cast<uint32_t>(p.table_rows - first) : 0u;
+    }
+    hipLaunchKernelGGL((mx_product_tiled_kernel<BM, BN, WM, WN, PARTS, NEAR>), dim3(ceil_div(q.n, BM) * tiles_n), dim3(WM * WN * kWave), 0,
+                       stream, q, tiles_n);
+  }
+}
+
+void launch_product(const ProductArgs &p, hipStream_t stream) {
+#ifdef KIND
+  if (KIND == 1) return launch_tiled<128, 128, 2, 2, 4, true>(p, stream);
+  if (KIND == 2) return launch_tiled<128, 128, 2, 2, 8, true>(p, stream);
+  if (KIND == 3) return launch_tiled<256, 256, 2, 4, 8, true>(p, stream);
+  if (KIND == 4) return launch_tiled<256, 64, 4, 1, 4, true>(p, stream);
+  if (KIND == 5) return launch_tiled<256, 128, 2, 2, 4, true>(p, stream);
+  if (KIND == 6) return launch_tiled<128, 256, 1, 4, 4, true>(p, stream);
+#endif
+  if (p.n <= 64) {
+    const uint32_t mt = p.n <= 16 ? 1 : p.n <= 32 ? 2 : 4;
+    const dim3 grid(ceil_div(p.N, 16), ceil_div(p.n, 16 * mt)), block(kFewWaves * kWave);
+    if (mt == 1) hipLaunchKernelGGL(mx_product_few_kernel<1>, grid, block, 0, stream, p);
+    else if (mt == 2) hipLaunchKernelGGL(mx_product_few_kernel<2>, grid, block, 0, stream, p);
+    else hipLaunchKernelGGL(mx_product_few_kernel<4>, grid, block, 0, stream, p);
+    return;
+  }
+  const uint64_t row_bytes = p.row_blocks * 16ull;
+  if (std::max(p.table_rows, p.N) * row_bytes >= 0xFFFF0000ull) return launch_tiled<128, 128, 2, 2, 4, false>(p, stream);
+  // The larger tile where there are enough of them to fill the chip a few times and rows are long: 65,536 rows of 4,096 by 4,096
+  // columns 782 us against 973; 65,536 of 1,024 by 1,024: 111 against 113; 232,965 of 602 by 256: 108 against 99.
+  if (p.row_blocks >= 32 && static_cast<uint64_t>(ceil_div(p.n, 256)) * ceil_div(p.N, 256) >= 1024)
+    return launch_tiled<256, 256, 2, 4, 8, true>(p, stream);
+  launch_tiled<128, 128, 2, 2, 4, true>(p, stream);
 }
 
 // ---- gradients --------------------------------------------------------------------------------------
@@ -303,10 +568,9 @@ int nts_mxfp4_product(float *out, const uint8_t *codes, const uint8_t *scales, u
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product: null pointer");
   if (!table_aligned(codes, scales) || !table_aligned(w_codes, w_scales))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product: codes need 16-byte, scales 4-byte alignment");
-  const ProductArgs p{out, {codes, scales}, table_rows, row_ids, n, {w_codes, w_scales}, N, mx_blocks(F), mx_scale_stride(F), accumulate};
-  const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, 32)) * ceil_div(N, 64);
-  hipLaunchKernelGGL((mx_product_kernel<2, 4>), dim3(static_cast<uint32_t>(std::min<uint64_t>((tiles + 3) / 4, kMostBlocks))),
-                     dim3(256), 0, stream, p);
+  const ProductArgs p{out, {codes, scales}, table_rows, row_ids, n, {w_codes, w_scales}, N, mx_blocks(F), mx_scale_stride(F), accumulate,
+                      N % 4 == 0 && aligned_to(out, 16)};
+  launch_product(p, stream);
   NTS_LAUNCH_CHECK("nts_mxfp4_product");
   return NTS_OK;
 }
