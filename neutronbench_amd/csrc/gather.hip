@@ -203,33 +203,51 @@ void launch_rows_any(const RowsArgs &a) {
 }
 
 // ---- rows held in 4 bits ------------------------------------------------------------------------------
-// A lane takes eight columns: one word of codes, one scale byte, up to eight floats out.  Lanes of a row are neighbours, so a
-// wavefront reads 256 bytes of codes and writes 2 KB.  An id that the table does not have gives a row of zeros (a padded batch).
-template <typename Index>
+// A group of G lanes takes a row, four columns a lane and step: two bytes of codes, one scale byte, 16 bytes out, so that the
+// group's stores are pieces of 16 G bytes.  An id that the table does not have gives a row of zeros (a padded batch).
+// Bound by its stores.  streamed: past the caches, for an output that the L2s do not hold anyway (400,000 rows of 640 values 291 ->
+// 177 us, 5.8 TB/s written; of 602, whose rows end inside lines, 303 -> 284; 2.45 M of 100: 290 -> 262).  Eight columns a lane, two
+// stores 32 bytes apart, 305 -> 351 with 602; two or four steps or rows at a time, 325 .. 390: a wavefront that writes to several
+// places at once is the slower one.
+template <int G>
 __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales, uint32_t table_rows,
-                                                             const uint32_t *__restrict__ row_ids, uint64_t n_parts, uint32_t F,
-                                                             uint32_t row_parts, uint32_t row_blocks, uint32_t scale_stride) {
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * 256u;
-  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x; t < n_parts; t += step) {
-    const Index i = static_cast<Index>(t) / static_cast<Index>(row_parts);
-    const uint32_t part = static_cast<uint32_t>(static_cast<Index>(t) - i * static_cast<Index>(row_parts));
-    const uint64_t g = row_ids ? row_ids[i] : static_cast<uint64_t>(i);
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (g < table_rows)
-      e2m1_decode8(reinterpret_cast<const uint32_t *>(codes)[g * row_blocks * 4u + part],
-                   e8m0_value(scales[g * scale_stride + part / 4u]), v);
-    const uint32_t col = part * 8u;
-    float *dst = out + static_cast<uint64_t>(i) * F + col;
-    if (col + 8u <= F) {
-      *reinterpret_cast<Quad *>(dst) = Quad{{v[0], v[1], v[2], v[3]}};
-      *reinterpret_cast<Quad *>(dst + 4) = Quad{{v[4], v[5], v[6], v[7]}};
-    } else {
-#pragma unroll
-      for (uint32_t k = 0; k < 7; ++k)
-        if (col + k < F) dst[k] = v[k];
+                                                             const uint32_t *__restrict__ row_ids, uint32_t n, uint32_t F,
+                                                             uint32_t row_blocks, uint32_t scale_stride, bool streamed) {
+  constexpr uint32_t kGroups = 256 / G;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * kGroups;
+  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kGroups + threadIdx.x / G; i < n; i += step) {
+    const uint64_t g = row_ids ? row_ids[i] : i;
+    const bool there = g < table_rows;
+    const uint8_t *row_codes = codes + (there ? g : 0u) * row_blocks * 16u, *row_scales = scales + (there ? g : 0u) * scale_stride;
+    for (uint32_t col = (threadIdx.x & (G - 1)) * 4u; col < F; col += G * 4u) {
+      uint32_t half = 0, scale = 0;
+      if (there) {
+        half = *reinterpret_cast<const uint16_t *>(row_codes + col / 2u);
+        scale = row_scales[col / kMxBlock];
+      }
+      float v[4];
+      e2m1_decode4(half, e8m0_value(scale), v);
+      float *dst = out + i * F + col;
+      if (col + 4u <= F) {
+        store_quad(dst, FloatQuad{v[0], v[1], v[2], v[3]}, streamed);
+      } else {
+        dst[0] = v[0];
+        if (col + 1u < F) dst[1] = v[1];
+        if (col + 2u < F) dst[2] = v[2];
+      }
     }
   }
+}
+
+template <int G>
+void launch_mx_rows(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids, uint32_t n,
+                    uint32_t F, hipStream_t stream) {
+  constexpr uint64_t per_block = 256 / G;
+    uint64_t blocks = std::min<uint64_t>((n + per_block - 1) / per_block, kMostBlocks);
+  if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, host_table_blocks(true));
+  hipLaunchKernelGGL(gather_mx_rows_kernel<G>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, out, codes, scales,
+                     table_rows, row_ids, n, F, mx_blocks(F), mx_scale_stride(F), static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes);
 }
 
 // ---- rows that arrive as message records -----------------------------------------------------------
@@ -380,17 +398,13 @@ int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scale
   if (!out || (table_rows && (!codes || !scales))) return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: null pointer");
   if (!aligned_to(codes, 16) || !aligned_to(scales, 4))
     return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: codes need 16-byte, scales 4-byte alignment");
-  const uint32_t row_parts = F / 8 + (F % 8 != 0);
-  const uint64_t parts = static_cast<uint64_t>(n) * row_parts;
-  uint64_t blocks = std::min<uint64_t>((parts + 255) / 256, kMostBlocks);
-  if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, host_table_blocks(true));
-  const dim3 grid(static_cast<uint32_t>(blocks));
-  if (parts <= 0xFFFFFFFFull)
-    hipLaunchKernelGGL(gather_mx_rows_kernel<uint32_t>, grid, dim3(256), 0, stream, out, codes, scales, table_rows, row_ids, parts,
-                       F, row_parts, mx_blocks(F), mx_scale_stride(F));
-  else
-    hipLaunchKernelGGL(gather_mx_rows_kernel<uint64_t>, grid, dim3(256), 0, stream, out, codes, scales, table_rows, row_ids, parts,
-                       F, row_parts, mx_blocks(F), mx_scale_stride(F));
+  switch (group_for(ceil_div(F, 4))) {
+    case 4: launch_mx_rows<4>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
+    case 8: launch_mx_rows<8>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
+    case 16: launch_mx_rows<16>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
+    case 32: launch_mx_rows<32>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
+    default: launch_mx_rows<64>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
+  }
   NTS_LAUNCH_CHECK("nts_gather_rows_mxfp4");
   return NTS_OK;
 }

@@ -37,9 +37,9 @@ __device__ __forceinline__ void append_values(const AppendArgs &p, const float *
   }
   const float *at = src + static_cast<uint64_t>(row - p.first) * p.heads * p.D + col;
   if (col + 4u <= p.D) {
-    const Quad q = *reinterpret_cast<const Quad *>(at);
+    const FloatQuad q = *reinterpret_cast<const FloatQuad *>(at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+    for (int i = 0; i < 4; ++i) v[i] = q[i];
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < 3; ++i)
@@ -189,9 +189,9 @@ struct Attend {
         if (dl * 16u + 16u <= p.D) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const Quad four = *reinterpret_cast<const Quad *>(src + i);
+            const FloatQuad four = *reinterpret_cast<const FloatQuad *>(src + i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q[g][i + k] = four.v[k];
+            for (int k = 0; k < 4; ++k) q[g][i + k] = four[k];
           }
         } else {
 #pragma unroll
@@ -348,7 +348,7 @@ struct Attend {
     for (uint32_t i = 0; i < 16; i += 4) {
       if (i >= count) break;
       if (count >= 4 && col + i + 4u <= p.D) {
-        *reinterpret_cast<Quad *>(dst + col + i) = Quad{{acc[g][i] * factor, acc[g][i + 1] * factor, acc[g][i + 2] * factor, acc[g][i + 3] * factor}};
+        *reinterpret_cast<FloatQuad *>(dst + col + i) = FloatQuad{acc[g][i] * factor, acc[g][i + 1] * factor, acc[g][i + 2] * factor, acc[g][i + 3] * factor};
       } else {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)

@@ -16,6 +16,9 @@ constexpr uint32_t kMostWidth = 1u << 17;  // columns (and outputs) of a row: th
 // Columns of a row that the cache of 8-bit keys and values keeps: whole 16-byte loads.
 inline __host__ __device__ uint32_t kv8_row_width(uint32_t D) { return (D + 15) / 16 * 16; }
 
+// An output from this size on is more than the L2s hold (8 of 4 MB) and is written past them.
+constexpr uint64_t kStreamedBytes = 32ull << 20;
+
 #if defined(__HIPCC__)
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -25,9 +28,17 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // Four floats at an address that is a multiple of four bytes only: global memory takes a 16-byte access there.
-struct __attribute__((packed, aligned(4))) Quad {
-  float v[4];
-};
+typedef float FloatQuad __attribute__((ext_vector_type(4), aligned(4)));
+// Stores them, past the caches if `streamed`.  The empty statements keep the compiler from making one plain store of the two.
+__device__ __forceinline__ void store_quad(float *to, FloatQuad v, bool streamed) {
+  if (streamed) {
+    asm volatile("");
+    __builtin_nontemporal_store(v, reinterpret_cast<FloatQuad *>(to));
+    asm volatile("");
+  } else {
+    *reinterpret_cast<FloatQuad *>(to) = v;
+  }
+}
 
 __device__ __forceinline__ float e8m0_value(uint32_t b) {
   return b == 0u ? __uint_as_float(0x00400000u) : b == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(b << 23);
@@ -35,6 +46,11 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
 // 2^-(b - 127) for the bytes that the quantisers write (0 .. 252): a normal float.
 __device__ __forceinline__ float e8m0_inverse(uint32_t b) { return __uint_as_float((254u - b) << 23); }
 
+// The four e2m1 values of the lower half of a word, lowest four bits first, times `scale`.
+__device__ __forceinline__ void e2m1_decode4(uint32_t word, float scale, float *v) {
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 1);
+  v[0] = a.x * scale, v[1] = a.y * scale, v[2] = b.x * scale, v[3] = b.y * scale;
+}
 // The eight e2m1 values of a word, lowest four bits first, times `scale`.
 __device__ __forceinline__ void e2m1_decode8(uint32_t word, float scale, float *v) {
   const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 1),

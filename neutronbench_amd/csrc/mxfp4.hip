@@ -12,44 +12,61 @@ namespace {
 // Per block of 32 values of a row: e = floor(log2 max|x|) - 2, so that the largest value lies in [4, 8) of the code's range
 // 0 .. 6 (7 and more become 6), then every x 2^-e to the nearest code.  Eight lanes take a block, four floats each; the
 // maximum is one of integers, since the bits of |x| order as the values do and infinities and NaN lie above them.
+// Blocks of a lane group that are requested together (2.45 M rows of 100: 282 us with four, 4.1 TB/s; 325 with one, 291 with two).
+constexpr uint32_t kQuantizeAhead = 4;
 template <typename Index>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                                                           const float *__restrict__ x, uint64_t n_blocks, uint32_t F,
                                                           uint32_t row_blocks, uint32_t scale_stride) {
   const uint32_t sub = threadIdx.x & 7u;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * 32u;
-  for (uint64_t b = static_cast<uint64_t>(blockIdx.x) * 32u + threadIdx.x / 8u; b < n_blocks; b += step) {
-    const Index row = static_cast<Index>(b) / static_cast<Index>(row_blocks);
-    const uint32_t kb = static_cast<uint32_t>(static_cast<Index>(b) - row * static_cast<Index>(row_blocks));
-    const uint32_t col = kb * kMxBlock + sub * 4u;
-    const float *src = x + static_cast<uint64_t>(row) * F + col;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (col + 4u <= F) {
-      const Quad q = *reinterpret_cast<const Quad *>(src);
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * (32u * kQuantizeAhead);
+  for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * (32u * kQuantizeAhead) + threadIdx.x / 8u; first < n_blocks; first += step) {
+    float v[kQuantizeAhead][4];
+    uint64_t row[kQuantizeAhead];
+    uint32_t kb[kQuantizeAhead];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = q.v[i];
-    } else {
+    for (uint32_t u = 0; u < kQuantizeAhead; ++u) {
+      const uint64_t b = first + u * 32u;
+      const Index r = static_cast<Index>(b) / static_cast<Index>(row_blocks);
+      kb[u] = static_cast<uint32_t>(static_cast<Index>(b) - r * static_cast<Index>(row_blocks));
+      row[u] = r;
+      const uint32_t col = kb[u] * kMxBlock + sub * 4u;
+      const float *src = x + row[u] * F + col;
 #pragma unroll
-      for (uint32_t i = 0; i < 3; ++i)
-        if (col + i < F) v[i] = src[i];
+      for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
+      if (b >= n_blocks) continue;
+      if (col + 4u <= F) {
+        const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] = q[i];
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i)
+          if (col + i < F) v[u][i] = src[i];
+      }
     }
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (uint32_t u = 0; u < kQuantizeAhead; ++u) {
+      const uint64_t b = first + u * 32u;
+      uint32_t top = 0;
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, kWave)));
-    const uint32_t exponent = top >> 23;
-    const bool fine = exponent < 255u;
-    const uint32_t byte = !fine ? 255u : (exponent > 2u ? exponent - 2u : 0u);
-    const float inverse = e8m0_inverse(fine ? byte : 0u);
-    uint32_t word = 0;
+      for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) word |= e2m1_encode(v[i], inverse) << (4 * i);
-    reinterpret_cast<uint16_t *>(codes)[b * 8u + sub] = static_cast<uint16_t>(fine ? word : 0u);
-    // the block's scale, and the bytes that fill the last block's row up to whole words
-    const uint32_t at = kb + sub;
-    if (sub == 0 || (kb + 1 == row_blocks && at < scale_stride))
-      scales[static_cast<uint64_t>(row) * scale_stride + at] = static_cast<uint8_t>(sub == 0 ? byte : 0u);
+      for (int m = 1; m < 8; m <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, kWave)));
+      if (b >= n_blocks) continue;
+      const uint32_t exponent = top >> 23;
+      const bool fine = exponent < 255u;
+      const uint32_t byte = !fine ? 255u : (exponent > 2u ? exponent - 2u : 0u);
+      const float inverse = e8m0_inverse(fine ? byte : 0u);
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word |= e2m1_encode(v[u][i], inverse) << (4 * i);
+      reinterpret_cast<uint16_t *>(codes)[b * 8u + sub] = static_cast<uint16_t>(fine ? word : 0u);
+      // the block's scale, and the bytes that fill the last block's row up to whole words
+      const uint32_t at = kb[u] + sub;
+      if (sub == 0 || (kb[u] + 1 == row_blocks && at < scale_stride))
+        scales[row[u] * scale_stride + at] = static_cast<uint8_t>(sub == 0 ? byte : 0u);
+    }
   }
 }
 
@@ -73,7 +90,7 @@ struct ProductArgs {
   MxRows w;
   uint32_t N, row_blocks, scale_stride;
   int accumulate;
-  bool streamed;  // rows of whole 16-byte stores: the output, which nothing here reads again, goes past the caches
+  bool streamed;  // the output goes past the caches
 };
 
 __device__ __forceinline__ i32x8 operand(i32x4 c) { return i32x8{c.x, c.y, c.z, c.w, 0, 0, 0, 0}; }
@@ -83,14 +100,11 @@ __device__ __forceinline__ void write_columns(const ProductArgs &p, uint64_t i, 
   float *dst = p.out + i * p.N + c;
   if (c + 4u <= p.N) {
     if (p.accumulate) {
-      const Quad old = *reinterpret_cast<const Quad *>(dst);
+      const FloatQuad old = *reinterpret_cast<const FloatQuad *>(dst);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += old.v[k];
+      for (int k = 0; k < 4; ++k) v[k] += old[k];
     }
-    if (p.streamed)
-      __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(dst));
-    else
-      *reinterpret_cast<Quad *>(dst) = Quad{{v.x, v.y, v.z, v.w}};
+    store_quad(dst, FloatQuad{v.x, v.y, v.z, v.w}, p.streamed);
   } else {
 #pragma unroll
     for (int k = 0; k < 3; ++k)
@@ -390,14 +404,6 @@ void launch_tiled(const ProductArgs &p, hipStream_t stream) {
 }
 
 void launch_product(const ProductArgs &p, hipStream_t stream) {
-#ifdef KIND
-  if (KIND == 1) return launch_tiled<128, 128, 2, 2, 4, true>(p, stream);
-  if (KIND == 2) return launch_tiled<128, 128, 2, 2, 8, true>(p, stream);
-  if (KIND == 3) return launch_tiled<256, 256, 2, 4, 8, true>(p, stream);
-  if (KIND == 4) return launch_tiled<256, 64, 4, 1, 4, true>(p, stream);
-  if (KIND == 5) return launch_tiled<256, 128, 2, 2, 4, true>(p, stream);
-  if (KIND == 6) return launch_tiled<128, 256, 1, 4, 4, true>(p, stream);
-#endif
   if (p.n <= 64) {
     const uint32_t mt = p.n <= 16 ? 1 : p.n <= 32 ? 2 : 4;
     const dim3 grid(ceil_div(p.N, 16), ceil_div(p.n, 16 * mt)), block(kFewWaves * kWave);
@@ -420,11 +426,12 @@ void launch_product(const ProductArgs &p, hipStream_t stream) {
 //   weight:  gw[j, f] (+)= sum_i g[i, j] A[row_ids[i], f]        P = g^T, Q = A by id,    R = n terms
 // Q's 4-bit values times their scales are exact in bf16 (one bit of fraction, eight of exponent).  g is split into three bf16
 // terms of eight bits of fraction each by cutting off bits, which is exact and cannot overflow, so three bf16 products summed
-// in 32 bits keep the accuracy of a 32-bit product.  A block of four wavefronts takes 64 rows of the result by 64
-// columns, 32 terms at a time through LDS, where both operands lie with the terms of a row or column side by side.
+// in 32 bits keep the accuracy of a 32-bit product.  A block of four wavefronts takes 128 rows of the result by 128
+// columns, 32 terms at a time through LDS, where both operands lie with the terms of a row or column side by side; the next
+// terms are on their way into registers meanwhile.
 // The weight's gradient has few results and many terms: blockIdx.z takes its part of the terms, the parts' sums are added in
 // order by a second launch, so results do not depend on scheduling.
-constexpr uint32_t kGradRows = 64, kGradCols = 64, kGradTerms = 32, kGradPitch = kGradTerms + 8;
+constexpr uint32_t kGradTile = 128, kGradTerms = 32, kGradPitch = kGradTerms + 8;
 
 struct GradArgs {
   float *out;        // [M, F], or the parts' sums [parts, M, F]
@@ -435,93 +442,173 @@ struct GradArgs {
   uint32_t M, R, F, g_stride, row_blocks, scale_stride;
   uint32_t part_terms;  // terms a part sums (a multiple of kGradTerms)
   int accumulate;
+  bool streamed;  // the output goes past the caches
 };
 
-// x = hi + mid + lo as bf16 bits, exactly for finite x; an infinity or NaN goes to hi alone.
-__device__ __forceinline__ void split3(float x, uint16_t *hi, uint16_t *mid, uint16_t *lo) {
+// x = hi + mid + lo, each the upper half of its word, exactly for finite x; an infinity or NaN goes to hi alone.
+__device__ __forceinline__ void split3(float x, uint32_t *hi, uint32_t *mid, uint32_t *lo) {
   const uint32_t b = __float_as_uint(x);
   const bool fine = (b & 0x7F800000u) != 0x7F800000u;
-  const float h = __uint_as_float(b & 0xFFFF0000u);
-  const float rest = fine ? x - h : 0.0f;
+  const float rest = fine ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f;
   const float m = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
-  *hi = static_cast<uint16_t>((b >> 16) | ((b & 0x7FFFFFFFu) > 0x7F800000u ? 0x40u : 0u));
-  *mid = static_cast<uint16_t>(__float_as_uint(m) >> 16);
-  *lo = static_cast<uint16_t>(__float_as_uint(rest - m) >> 16);
+  *hi = b | ((b & 0x7FFFFFFFu) > 0x7F800000u ? 0x400000u : 0u);  // a NaN whose upper bits are an infinity's
+  *mid = __float_as_uint(m);
+  *lo = __float_as_uint(rest - m);
 }
+// The upper halves of two words.
+__device__ __forceinline__ uint32_t upper_halves(uint32_t first, uint32_t second) { return __builtin_amdgcn_perm(second, first, 0x07060302u); }
 
 template <bool WEIGHT>
-__global__ __launch_bounds__(256) void mx_grad_kernel(GradArgs p) {
-  __shared__ __attribute__((aligned(16))) uint16_t sp[3][kGradRows][kGradPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t sq[kGradCols][kGradPitch];
-  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave, r = lane & 15u, part = lane >> 4;
-  const uint64_t m0 = static_cast<uint64_t>(blockIdx.x) * kGradRows;
-  const uint32_t f0 = blockIdx.y * kGradCols;
+__global__ __launch_bounds__(256, 2) void mx_grad_kernel(GradArgs p) {
+  __shared__ __attribute__((aligned(16))) uint16_t sp[3][kGradTile][kGradPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t sq[kGradTile][kGradPitch];
+  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
+  const uint64_t m0 = static_cast<uint64_t>(blockIdx.x) * kGradTile;
+  const uint32_t f0 = blockIdx.y * kGradTile;
   const uint64_t begin = static_cast<uint64_t>(blockIdx.z) * p.part_terms;
   const uint64_t end = min(static_cast<uint64_t>(p.R), begin + p.part_terms);
-  f32x4 acc[4] = {};
-  for (uint64_t k0 = begin; k0 < end; k0 += kGradTerms) {
-    __syncthreads();
+  // P: a thread takes 16 terms of one row: neighbouring threads have neighbouring rows where those are g's columns, otherwise two
+  // threads share a row.  Q: half of the threads take eight columns of four terms.
+  const uint32_t pm = WEIGHT ? t & 127u : t >> 1, pk = (WEIGHT ? t >> 7 : t & 1u) * 16u;
+  const uint32_t qf = (t & 15u) * 8u, qk = (t >> 4) * 4u;
+  const bool q_mine = t < 128u && f0 + qf < p.F;
+  float g[16];
+  uint32_t word[4], scale[4];
+  auto request = [&](uint64_t k0) {
+    const uint64_t m = m0 + pm;
+    if (WEIGHT) {
+      const float *src = p.g + (k0 + pk) * p.g_stride + m;
 #pragma unroll
-    for (uint32_t i = 0; i < kGradRows * kGradTerms / 256; ++i) {
-      const uint32_t at = i * 256 + t;
-      const uint32_t m = WEIGHT ? at % kGradRows : at / kGradTerms, k = WEIGHT ? at / kGradRows : at % kGradTerms;
-      float v = 0.0f;
-      if (m0 + m < p.M && k0 + k < end)
-        v = WEIGHT ? p.g[(k0 + k) * p.g_stride + m0 + m] : p.g[(m0 + m) * p.g_stride + k0 + k];
-      split3(v, &sp[0][m][k], &sp[1][m][k], &sp[2][m][k]);
-    }
-    {
-      const uint32_t k = t / 8u, f = (t & 7u) * 8u;
-      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      if (k0 + k < end && f0 + f < p.F) {
-        const uint64_t row = WEIGHT && p.row_ids ? p.row_ids[k0 + k] : k0 + k;
-        if (row < p.q_rows)
-          e2m1_decode8(*reinterpret_cast<const uint32_t *>(p.q.codes + row * p.row_blocks * 16u + (f0 + f) / 2u),
-                       e8m0_value(p.q.scales[row * p.scale_stride + (f0 + f) / kMxBlock]), v);
+      for (uint32_t i = 0; i < 16; ++i) g[i] = m < p.M && k0 + pk + i < end ? src[static_cast<uint64_t>(i) * p.g_stride] : 0.0f;
+    } else {
+      const float *src = p.g + m * p.g_stride + k0 + pk;
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 4) {
+        if (m < p.M && k0 + pk + i + 4u <= end) {
+          const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src + i);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) g[i + k] = q[k];
+        } else {
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) g[i + k] = m < p.M && k0 + pk + i + k < end ? src[i + k] : 0.0f;
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq[f + i][k] = static_cast<uint16_t>(__float_as_uint(v[i]) >> 16);
     }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      word[i] = scale[i] = 0;
+      const uint64_t k = k0 + qk + i;
+      if (q_mine && k < end) {
+        const uint64_t row = WEIGHT && p.row_ids ? p.row_ids[k] : k;
+        if (row < p.q_rows) {
+          word[i] = *reinterpret_cast<const uint32_t *>(p.q.codes + row * p.row_blocks * 16u + (f0 + qf) / 2u);
+          scale[i] = p.q.scales[row * p.scale_stride + (f0 + qf) / kMxBlock];
+        }
+      }
+    }
+  };
+  auto keep = [&]() {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i += 8) {
+      uint32_t s[3][8];
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) split3(g[i + k], &s[0][k], &s[1][k], &s[2][k]);
+#pragma unroll
+      for (int c = 0; c < 3; ++c)
+        *reinterpret_cast<u32x4 *>(&sp[c][pm][pk + i]) = u32x4{upper_halves(s[c][0], s[c][1]), upper_halves(s[c][2], s[c][3]),
+                                                               upper_halves(s[c][4], s[c][5]), upper_halves(s[c][6], s[c][7])};
+    }
+    if (t < 128u) {
+      float v[4][8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e2m1_decode8(word[i], e8m0_value(scale[i]), v[i]);
+#pragma unroll
+      for (int f = 0; f < 8; ++f)
+        *reinterpret_cast<uint2 *>(&sq[qf + f][qk]) =
+            make_uint2(upper_halves(__float_as_uint(v[0][f]), __float_as_uint(v[1][f])), upper_halves(__float_as_uint(v[2][f]), __float_as_uint(v[3][f])));
+    }
+  };
+  const uint32_t wm = wave / 2u * 64u, wf = wave % 2u * 64u;
+  f32x4 acc[4][4] = {};
+  request(begin);
+  for (uint64_t k0 = begin; k0 < end; k0 += kGradTerms) {
+    keep();
     __syncthreads();
+    if (k0 + kGradTerms < end) request(k0 + kGradTerms);
     bf16x8 q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8 *>(&sq[j * 16 + r][part * 8]);
+    for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8 *>(&sq[wf + j * 16 + r][part * 8]);
 #pragma unroll
-    for (int s = 0; s < 3; ++s) {
-      const bf16x8 g = *reinterpret_cast<const bf16x8 *>(&sp[s][wave * 16 + r][part * 8]);
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[j], g, acc[j], 0, 0, 0);
-    }
+      for (int s = 0; s < 3; ++s) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8 *>(&sp[s][wm + m * 16 + r][part * 8]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[j], a, acc[m][j], 0, 0, 0);
+      }
+    __syncthreads();
   }
-  const uint64_t m = m0 + wave * 16 + r;
-  if (m >= p.M) return;
-  float *out = p.out + (static_cast<uint64_t>(blockIdx.z) * p.M + m) * p.F;
+  // rows of 64 columns through LDS, as the product's
+  f32x4 *const mine = reinterpret_cast<f32x4 *>(&sp[0][0][0]) + wave * 256u;
+  static_assert(sizeof(sp) >= 4 * 256 * sizeof(f32x4), "room for 16 rows of every wavefront");
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int m = 0; m < 4; ++m) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t f = f0 + j * 16 + part * 4 + i;
-      if (f < p.F) out[f] = p.accumulate ? out[f] + acc[j][i] : acc[j][i];
+    for (int j = 0; j < 4; ++j) mine[r * 16u + ((j * 4u + part) ^ r)] = acc[m][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t row = k * 4u + lane / 16u, f = f0 + wf + (lane & 15u) * 4u;
+      const uint64_t i = m0 + wm + m * 16u + row;
+      f32x4 v = mine[row * 16u + ((lane & 15u) ^ row)];
+      if (i >= p.M) continue;
+      float *dst = p.out + (static_cast<uint64_t>(blockIdx.z) * p.M + i) * p.F + f;
+      if (f + 4u <= p.F) {
+        if (p.accumulate) {
+          const FloatQuad old = *reinterpret_cast<const FloatQuad *>(dst);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] += old[c];
+        }
+          store_quad(dst, FloatQuad{v.x, v.y, v.z, v.w}, p.streamed);
+      } else {
+#pragma unroll
+        for (uint32_t c = 0; c < 3; ++c)
+          if (f + c < p.F) dst[c] = p.accumulate ? dst[c] + v[c] : v[c];
+      }
     }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
-// out (+)= the sum of `parts` arrays of `count` floats, in order.
+// out (+)= the sum of `parts` arrays of `count` floats, in order: four wavefronts take every fourth part of 64 values, eight
+// loads at a time, and the first adds up what they have.
 __global__ __launch_bounds__(256) void sum_parts_kernel(float *__restrict__ out, const float *__restrict__ from, uint64_t count,
                                                         uint32_t parts, int accumulate) {
-  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<uint64_t>(gridDim.x) * 256) {
-    float sum = 0.0f;
-    for (uint32_t k = 0; k < parts; ++k) sum += from[k * count + i];
-    out[i] = accumulate ? out[i] + sum : sum;
+  __shared__ float sums[3][kWave];
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block();
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kWave + lane;
+  float sum = 0.0f;
+  if (i < count) {
+#pragma unroll 8
+    for (uint32_t k = wave; k < parts; k += 4) sum += from[k * count + i];
   }
+  if (wave) sums[wave - 1][lane] = sum;
+  __syncthreads();
+  if (wave || i >= count) return;
+  sum += sums[0][lane];
+  sum += sums[1][lane];
+  sum += sums[2][lane];
+  out[i] = accumulate ? out[i] + sum : sum;
 }
 
 struct Parts {
   uint32_t count, terms;
 };
-// Parts of the weight's gradient: enough blocks for the chip, none of fewer than 256 terms.
+// Parts of the weight's gradient: 512 blocks, two for a compute unit, and none of fewer than 256 terms (169,343 rows of 640 by 640:
+// 1.0 ms with 512, 2.0 with 256, 1.0 with 1,024).
 Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
-  const uint64_t tiles = static_cast<uint64_t>(ceil_div(N, kGradRows)) * ceil_div(F, kGradCols);
-  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(1024 / tiles, n / 256));
+  const uint64_t tiles = static_cast<uint64_t>(ceil_div(N, kGradTile)) * ceil_div(F, kGradTile);
+  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(512 / tiles, n / 256));
   const uint64_t terms = (n + want - 1) / want;
   Parts p;
   p.terms = static_cast<uint32_t>(std::min<uint64_t>((terms + kGradTerms - 1) / kGradTerms * kGradTerms, 0xFFFFFFE0u));
@@ -546,7 +633,7 @@ int nts_mxfp4_quantize(uint8_t *codes, uint8_t *scales, const float *x, uint32_t
   if (!table_aligned(codes, scales)) return fail(NTS_ERR_INVALID, "nts_mxfp4_quantize: codes need 16-byte, scales 4-byte alignment");
   const uint32_t row_blocks = mx_blocks(F);
   const uint64_t blocks = static_cast<uint64_t>(n) * row_blocks;
-  const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>((blocks + 31) / 32, kMostBlocks)));
+  const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>((blocks + 32 * kQuantizeAhead - 1) / (32 * kQuantizeAhead), kMostBlocks)));
   if (blocks <= 0xFFFFFFFFull)
     hipLaunchKernelGGL(mx_quantize_kernel<uint32_t>, grid, dim3(256), 0, stream, codes, scales, x, blocks, F, row_blocks,
                        mx_scale_stride(F));
@@ -569,7 +656,7 @@ int nts_mxfp4_product(float *out, const uint8_t *codes, const uint8_t *scales, u
   if (!table_aligned(codes, scales) || !table_aligned(w_codes, w_scales))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product: codes need 16-byte, scales 4-byte alignment");
   const ProductArgs p{out, {codes, scales}, table_rows, row_ids, n, {w_codes, w_scales}, N, mx_blocks(F), mx_scale_stride(F), accumulate,
-                      N % 4 == 0 && aligned_to(out, 16)};
+                      static_cast<uint64_t>(n) * N * sizeof(float) >= kStreamedBytes};
   launch_product(p, stream);
   NTS_LAUNCH_CHECK("nts_mxfp4_product");
   return NTS_OK;
@@ -585,14 +672,15 @@ int nts_mxfp4_product_grad_rows(float *gx, const float *gout, const uint8_t *w_c
   if (!table_aligned(w_codes, w_scales))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product_grad_rows: codes need 16-byte, scales 4-byte alignment");
   const uint32_t terms = ceil_div(N, kGradTerms) * kGradTerms;
-  const GradArgs p{gx, gout, {w_codes, w_scales}, N, nullptr, n, N, F, N, mx_blocks(F), mx_scale_stride(F), terms, accumulate};
+  const GradArgs p{gx, gout, {w_codes, w_scales}, N, nullptr, n, N, F, N, mx_blocks(F), mx_scale_stride(F), terms, accumulate,
+                   static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes};
   // launches of at most 2^24 - 1 blocks: rows of the result in turns
-  const uint32_t cols = ceil_div(F, kGradCols), turn = std::max(1u, kMostBlocks / cols) * kGradRows;
+  const uint32_t cols = ceil_div(F, kGradTile), turn = kMostBlocks / cols * kGradTile;
   for (uint64_t first = 0; first < n; first += turn) {
     GradArgs q = p;
     q.out = gx + first * F, q.g = gout + first * N;
     q.M = static_cast<uint32_t>(std::min<uint64_t>(turn, n - first));
-    hipLaunchKernelGGL((mx_grad_kernel<false>), dim3(ceil_div(q.M, kGradRows), cols, 1), dim3(256), 0, stream, q);
+    hipLaunchKernelGGL((mx_grad_kernel<false>), dim3(ceil_div(q.M, kGradTile), cols, 1), dim3(256), 0, stream, q);
     NTS_LAUNCH_CHECK("nts_mxfp4_product_grad_rows");
   }
   return NTS_OK;
@@ -617,15 +705,14 @@ int nts_mxfp4_product_grad_weight(float *gw, const float *gout, const uint8_t *c
   const Parts parts = weight_parts(n, N, F);
   if (parts.count > 1 && (!work || !aligned_to(work, 16)))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product_grad_weight: needs nts_mxfp4_product_grad_weight_work_bytes of 16-byte-aligned work");
-  GradArgs p{gw, gout, {codes, scales}, table_rows, row_ids, N, n, F, N, mx_blocks(F), mx_scale_stride(F), parts.terms, accumulate};
+  GradArgs p{gw, gout, {codes, scales}, table_rows, row_ids, N, n, F, N, mx_blocks(F), mx_scale_stride(F), parts.terms, accumulate, false};
   if (parts.count > 1) p.out = static_cast<float *>(work), p.accumulate = 0;
-  hipLaunchKernelGGL((mx_grad_kernel<true>), dim3(ceil_div(N, kGradRows), ceil_div(F, kGradCols), parts.count), dim3(256), 0,
+  hipLaunchKernelGGL((mx_grad_kernel<true>), dim3(ceil_div(N, kGradTile), ceil_div(F, kGradTile), parts.count), dim3(256), 0,
                      stream, p);
   NTS_LAUNCH_CHECK("nts_mxfp4_product_grad_weight");
   if (parts.count > 1) {
     const uint64_t count = static_cast<uint64_t>(N) * F;
-    hipLaunchKernelGGL(sum_parts_kernel, dim3(static_cast<uint32_t>(std::min<uint64_t>((count + 255) / 256, 65536))), dim3(256),
-                       0, stream, gw, static_cast<const float *>(work), count, parts.count, accumulate);
+    hipLaunchKernelGGL(sum_parts_kernel, dim3(ceil_div(count, kWave)), dim3(256), 0, stream, gw, static_cast<const float *>(work), count, parts.count, accumulate);
     NTS_LAUNCH_CHECK("sum_parts_kernel");
   }
   return NTS_OK;
