@@ -551,9 +551,9 @@ int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float 
  * below cache_rows counts for nothing (a neighbour that is not cached); a destination without any other edge gets
  * out = 0 and lse = -infinity.  q, out: [Vd, q_heads * width], lse [Vd, q_heads] or NULL; q_heads a multiple of heads.
  * `edges` = co[Vd] - co[0], at most 2^32 - 2^16.  max_degree: the caller's bound on a destination's edges, 0 = none known;
- * it only selects the launches.  Up to 256 a wavefront takes a destination; otherwise long rows are cut and their parts
- * joined in order (the same bits on every call), in nts_kv8_attention_work_bytes(...) bytes of 16-byte-aligned device
- * memory, which calls that overlap must not share.  Scores and sums are kept in 32 bits. */
+ * it only selects the launches (one, or where rows may be long and are many, two: long rows are cut and their parts joined
+ * in order).  The same bits on every call.  `work`: nts_kv8_attention_work_bytes(...) bytes (0: none) of 16-byte-aligned
+ * device memory, which calls that overlap must not share.  Scores and sums are kept in 32 bits. */
 size_t nts_kv8_attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t width, uint32_t max_degree);
 int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
                       const uint32_t *ri, const uint32_t *mirror, uint32_t Vd, uint32_t edges, uint32_t cache_rows,

@@ -113,6 +113,7 @@ struct AttendArgs {
   uint32_t passes;           // over the edges, 2^hw_shift units each; neighbouring wavefronts take the passes of one walker
   uint32_t hw_shift, walker_shift;  // log2 of units side by side, of a walker's lanes
   float score_scale;
+  bool blocks;  // a block per destination
   // edges cut into spans of `span` positions (see below)
   uint32_t span, spans;
   uint64_t positions;
@@ -144,12 +145,13 @@ constexpr int kAheadOf = G == 1 ? 4 : 2;
 template <int G>
 constexpr int kWavesOf = G == 1 ? 4 : 3;
 
-// NEAR: cache and scales of less than 4 GB each are read through buffer descriptors: 32-bit offsets, and a row that is not there
-// gets an offset beyond the end, which reads zeros without a branch.
+// NEAR: cache and scales of less than 4 GB each and of at most 2^24 rows are read through buffer descriptors: 32-bit offsets from
+// 24-bit products, and a row that is not there gets an offset beyond the end, which reads zeros without a branch.
 template <int ND, int G, bool NEAR>
 struct Attend {
   const AttendArgs &p;
-  uint32_t dl, kv_head, q_head0, slot, slots, rounds;
+  uint32_t dl, kv_head, q_head0, slot, rounds;
+  uint32_t lane_edge, edge_step;  // the lane's first edge of a destination, and how far its next one lies behind it
   bool live;  // this lane has a unit and columns
   uint32_t key_at, row_bytes, values_at;  // the lane's 16 bytes of a row's keys; from there to its values
   __amdgpu_buffer_rsrc_t cache_words, scale_bytes;
@@ -163,7 +165,8 @@ struct Attend {
     const uint32_t unit = (pass << p.hw_shift) + ((l >> kShift) & ((1u << p.hw_shift) - 1u));
     rounds = p.walker_shift - p.hw_shift - kShift;
     slot = l >> (kShift + p.hw_shift);
-    slots = 1u << rounds;
+    lane_edge = slot;
+    edge_step = 1u << rounds;
     live = unit < p.units && dl * 16u < p.row_width;
     kv_head = unit / p.per_head;
     q_head0 = (unit - kv_head * p.per_head) * G;  // within the head's share
@@ -221,8 +224,8 @@ struct Attend {
       there[u] = row[u] < p.cache_rows;
       if (NEAR) {
         const bool read = there[u] && live;
-        const uint32_t at = read ? row[u] * row_bytes + key_at : 0xFFFFFF00u;
-        const uint32_t scale_at = read ? (row[u] >> p.block_shift) * 2u * p.heads + kv_head : 0xFFFFFF00u;
+        const uint32_t at = read ? __umul24(row[u], row_bytes) + key_at : 0xFFFFFF00u;
+        const uint32_t scale_at = read ? __umul24(row[u] >> p.block_shift, 2u * p.heads) + kv_head : 0xFFFFFF00u;
         kc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, 0, 0);
         vc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, values_at, 0);
         kb[u] = __builtin_amdgcn_raw_buffer_load_b8(scale_bytes, scale_at, 0, 0);
@@ -289,19 +292,19 @@ struct Attend {
     const uint32_t *ids = p.ri + first;
     uint32_t row[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) row[u] = cache_row(ids, j0 + u * slots + slot, j1);
+    for (int u = 0; u < kAhead; ++u) row[u] = cache_row(ids, j0 + u * edge_step + lane_edge, j1);
     uint32_t j = j0;
-    for (; j1 - j > kAhead * slots; j += kAhead * slots) {
+    for (; j1 - j > kAhead * edge_step; j += kAhead * edge_step) {
       uint32_t next[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) next[u] = cache_row(ids, j + (kAhead + u) * slots + slot, j1);
+      for (int u = 0; u < kAhead; ++u) next[u] = cache_row(ids, j + (kAhead + u) * edge_step + lane_edge, j1);
       step<kAhead>(row);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) row[u] = next[u];
     }
-    if (j1 - j > kAhead / 2 * slots)
+    if (j1 - j > kAhead / 2 * edge_step)
       step<kAhead>(row);
-    else if (kAhead == 2 || j1 - j <= slots)
+    else if (kAhead == 2 || j1 - j <= edge_step)
       step<1>(row);
     else
       step<2>(row);
@@ -340,19 +343,19 @@ struct Attend {
     }
   }
 
-  // A lane's columns after join(), times `factor`, to a row of D columns.
-  __device__ __forceinline__ void store(float *dst, int g, float factor) const {
+  // A lane's columns after join(), times `factor`, to a row of `columns`.
+  __device__ __forceinline__ void store(float *dst, int g, float factor, uint32_t columns) const {
     const uint32_t count = rounds < 4 ? 16u >> rounds : 1u;
     if (slot >> 4) return;  // further slots hold the same columns
 #pragma unroll
     for (uint32_t i = 0; i < 16; i += 4) {
       if (i >= count) break;
-      if (count >= 4 && col + i + 4u <= p.D) {
+      if (count >= 4 && col + i + 4u <= columns) {
         *reinterpret_cast<FloatQuad *>(dst + col + i) = FloatQuad{acc[g][i] * factor, acc[g][i + 1] * factor, acc[g][i + 2] * factor, acc[g][i + 3] * factor};
       } else {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
-          if (i + k < count && col + i + k < p.D) dst[col + i + k] = acc[g][i + k] * factor;
+          if (i + k < count && col + i + k < columns) dst[col + i + k] = acc[g][i + k] * factor;
       }
     }
   }
@@ -363,7 +366,7 @@ struct Attend {
     for (int g = 0; g < G; ++g) {
       if (q_head0 + g >= p.share) continue;
       const uint64_t at = static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head0 + g;
-      store(p.out + at * p.D, g, sum[g] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[g]));
+      store(p.out + at * p.D, g, sum[g] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[g]), p.D);
       if (p.lse && dl == 0 && slot == 0) p.lse[at] = sum[g] == 0.0f ? -INFINITY : (top[g] + __builtin_amdgcn_logf(sum[g])) * kLn2;
     }
   }
@@ -376,7 +379,7 @@ struct Attend {
     for (int g = 0; g < G; ++g) {
       if (q_head0 + g >= p.share) continue;
       const uint32_t h = kv_head * p.share + q_head0 + g;
-      store(dst + static_cast<uint64_t>(h) * p.D, g, 1.0f);
+      store(dst + static_cast<uint64_t>(h) * p.D, g, 1.0f, p.D);
       if (dl == 0 && slot == 0) {
         dst[static_cast<uint64_t>(p.q_heads) * p.D + h] = top[g];
         dst[static_cast<uint64_t>(p.q_heads) * (p.D + 1u) + h] = sum[g];
@@ -408,12 +411,66 @@ __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_rows_kernel(Atten
   }
 }
 
+// A block per destination, for few destinations of up to some thousand edges: its wavefronts share the edges and join through
+// LDS, in one launch (one vertex with 300 neighbours: @BLK@).
+constexpr uint32_t kBlockWaves = 16;
+template <int ND, int G, bool NEAR>
+__global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(AttendArgs p) {
+  __shared__ float tops[kBlockWaves * kWave * G / ND], sums[kBlockWaves * kWave * G / ND], accs[kBlockWaves * kWave * 16 * G];
+  const uint32_t row = blockIdx.x / p.passes, pass = blockIdx.x - row * p.passes, wave = wave_of_block();
+  const uint32_t hw = 1u << p.hw_shift, first = p.co[row], degree = p.co[row + 1] - first;
+  {
+    Attend<ND, G, NEAR> a(p, pass);
+    a.lane_edge += wave * a.edge_step;
+    a.edge_step *= kBlockWaves;
+    a.begin(row);
+    a.edges(first, 0, degree);
+    a.join();
+    if (a.live) {
+      const uint32_t unit = (threadIdx.x & (kWave - 1)) / ND % hw;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint32_t at = (wave * hw + unit) * G + g;
+        a.store(accs + at * (ND * 16u), g, 1.0f, ND * 16u);
+        if (a.dl == 0 && a.slot == 0) {
+          tops[at] = a.top[g];
+          sums[at] = a.sum[g];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < hw * G * ND * 16u; i += kBlockWaves * kWave) {
+    const uint32_t at = i / (ND * 16u), c = i % (ND * 16u), unit = pass * hw + at / G;
+    const uint32_t kv_head = unit / p.per_head, q_head = (unit - kv_head * p.per_head) * G + at % G;
+    if (unit >= p.units || c >= p.D || q_head >= p.share) continue;
+    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < kBlockWaves; ++w) top = fmaxf(top, tops[w * hw * G + at]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (uint32_t w = 0; w < kBlockWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(tops[w * hw * G + at] - base);
+      sum = fmaf(sums[w * hw * G + at], f, sum);
+      acc = fmaf(accs[(w * hw * G + at) * (ND * 16u) + c], f, acc);
+    }
+    const uint64_t h = static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head;
+    p.out[h * p.D + c] = sum == 0.0f ? 0.0f : acc / sum;
+    if (p.lse && c == 0) p.lse[h] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  }
+}
+
 // Long rows are shared out and short ones bundled without a look at the degrees on the host: destinations and edges are
-// lined up -- destination r takes position r + co[r] - co[0], its edges the positions behind it -- and every walker takes the
-// destinations that begin within its span of `span` positions.  A destination of more than `span` edges is cut at the
+// lined up -- destination r takes kRowCost positions from r * kRowCost + co[r] - co[0] on, which is what beginning and writing a
+// row costs in edges, and its edges the positions behind them -- and every walker takes the destinations that begin within its
+// span of `span` positions.  A destination of more than `span` edges is cut at the
 // spans' ends: every span that it reaches into sums its part into a record (1: the destination begins in this span, 0: in an
 // earlier one) and join_spans_kernel adds the parts in order.  No atomics: the same bits on every call.
-__device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r + (co[r] - co0); }
+#ifndef RC
+#define RC 8
+#endif
+constexpr uint32_t kRowCost = RC;
+__device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r * kRowCost + (co[r] - co0); }
 
 // The last destination at or before position x: a candidate for every lane of the walker a step.
 __device__ __forceinline__ uint32_t destination_at(const uint32_t *co, uint32_t co0, uint32_t Vd, uint64_t x, uint32_t walker_shift) {
@@ -447,12 +504,12 @@ __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_spans_kernel(Atte
   uint32_t tail = kNoSlot;
   for (uint32_t row = destination_at(p.co, co0, p.Vd, begin, p.walker_shift); row < p.Vd; ++row) {
     const uint32_t first = p.co[row], degree = p.co[row + 1] - first;
-    const uint64_t at = static_cast<uint64_t>(row) + (first - co0);  // the destination's own position, its edges behind it
+    const uint64_t at = static_cast<uint64_t>(row) * kRowCost + (first - co0), edges_at = at + kRowCost;
     if (at >= end) break;
     const bool cut = degree > p.span;
     if (at < begin && !cut) continue;  // the earlier span has done it
-    const uint32_t j0 = at + 1 < begin ? static_cast<uint32_t>(min<uint64_t>(begin - at - 1, degree)) : 0u;
-    const uint32_t j1 = cut ? static_cast<uint32_t>(min<uint64_t>(degree, end - at - 1)) : degree;
+    const uint32_t j0 = edges_at < begin ? static_cast<uint32_t>(min<uint64_t>(begin - edges_at, degree)) : 0u;
+    const uint32_t j1 = !cut ? degree : edges_at < end ? static_cast<uint32_t>(min<uint64_t>(degree, end - edges_at)) : 0u;
     if (j0 >= j1 && at < begin) continue;
     a.begin(row);
     a.edges(first, j0, j1);
@@ -469,25 +526,27 @@ __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_spans_kernel(Atte
 
 // The destinations that were cut: 64 columns a block, its wavefronts take every kJoinWaves-th part, and the first adds up
 // what they have, in order.
-constexpr uint32_t kJoinWaves = 8, kJoinSpans = 8;
+constexpr uint32_t kJoinWaves = 16, kJoinSpans = 8, kJoinAhead = 8;
 __global__ __launch_bounds__(kJoinWaves *kWave) void join_spans_kernel(AttendArgs p) {
   __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave];
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block();
   const uint32_t columns = p.q_heads * p.D, c = blockIdx.y * kWave + lane, h = min(c, columns - 1u) / p.D;
   const uint64_t size = static_cast<uint64_t>(p.q_heads) * (p.D + 2u);
+  const uint64_t span0 = static_cast<uint64_t>(blockIdx.x) * kJoinSpans;
+  const uint32_t rows = lane < kJoinSpans && span0 + lane < p.spans ? p.tail_row[span0 + lane] : kNoSlot;
+  if (__ballot(rows != kNoSlot) == 0) return;  // the same in every wavefront
   for (uint32_t k = 0; k < kJoinSpans; ++k) {
-    const uint64_t span = static_cast<uint64_t>(blockIdx.x) * kJoinSpans + k;
-    if (span >= p.spans) break;
-    const uint32_t row = p.tail_row[span];
+    const uint64_t span = span0 + k;
+    const uint32_t row = wave_read(rows, k);
     if (row == kNoSlot) continue;
-    const uint64_t last_at = static_cast<uint64_t>(row) + (p.co[row + 1] - p.co[0]);  // position of its last edge
+    const uint64_t last_at = static_cast<uint64_t>(row) * kRowCost + (kRowCost - 1u) + (p.co[row + 1] - p.co[0]);  // its last edge's
     const uint64_t last = min<uint64_t>(last_at / p.span, p.spans - 1u);
     float top = -INFINITY, sum = 0.0f, acc = 0.0f;
     const float *const from = p.partial + min(c, columns - 1u);
-    for (uint64_t s = span + wave; s <= last; s += 4 * kJoinWaves) {
-      float t[4], l[4], v[4];
+    for (uint64_t s = span + wave; s <= last; s += kJoinAhead * kJoinWaves) {
+      float t[kJoinAhead], l[kJoinAhead], v[kJoinAhead];
 #pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
+      for (uint32_t u = 0; u < kJoinAhead; ++u) {
         const uint64_t at = s + u * kJoinWaves;
         t[u] = -INFINITY, l[u] = v[u] = 0.0f;
         if (at <= last) {
@@ -499,13 +558,13 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_spans_kernel(AttendArg
       }
       float now = top;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) now = fmaxf(now, t[u]);
+      for (uint32_t u = 0; u < kJoinAhead; ++u) now = fmaxf(now, t[u]);
       const float base = now == -INFINITY ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
       top = now;
       sum *= a;
       acc *= a;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (uint32_t u = 0; u < kJoinAhead; ++u) {
         const float b = __builtin_amdgcn_exp2f(t[u] - base);
         sum = fmaf(l[u], b, sum);
         acc = fmaf(v[u], b, acc);
@@ -532,7 +591,14 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_spans_kernel(AttendArg
 constexpr uint32_t kMostHeadWidth = 256, kMostHeads = 1024, kMostBlockRows = 1024;
 // Above this bound (or without one) a row may be long enough to keep one walker busy after the others are done.
 constexpr uint32_t kMostRowEdges = 256;
-bool by_spans(uint32_t max_degree) { return max_degree == 0 || max_degree > kMostRowEdges; }
+// Up to so many destinations and edges a block takes a destination, whatever the degrees.
+constexpr uint32_t kBlockRows = 64, kBlockEdges = 4096;
+bool by_blocks(uint32_t Vd, uint32_t edges, uint32_t max_degree) {
+  return Vd <= kBlockRows && edges <= kBlockEdges && (max_degree == 0 || max_degree > 16);
+}
+bool by_spans(uint32_t Vd, uint32_t edges, uint32_t max_degree) {
+  return !by_blocks(Vd, edges, max_degree) && (max_degree == 0 || max_degree > kMostRowEdges);
+}
 
 uint32_t next_power(uint32_t v) {
   uint32_t p = 1;
@@ -575,6 +641,11 @@ uint32_t span_length(uint64_t positions, uint32_t q_heads, uint32_t D) {
 
 template <int ND, int G, bool NEAR>
 int launch_attend(const AttendArgs &p, hipStream_t stream) {
+  if (p.blocks) {
+    hipLaunchKernelGGL((kv8_attend_block_kernel<ND, G, NEAR>), dim3(p.Vd * p.passes), dim3(kBlockWaves * kWave), 0, stream, p);
+    NTS_LAUNCH_CHECK("nts_kv8_attention");
+    return NTS_OK;
+  }
   const uint32_t walkers = 256u >> p.walker_shift;  // a block's
   if (!p.span) {
     const uint64_t blocks = std::min<uint64_t>((static_cast<uint64_t>(p.Vd) * p.passes + walkers - 1) / walkers, kMostBlocks);
@@ -607,8 +678,8 @@ int launch_attend_nd(const AttendArgs &p, const Lanes &l, hipStream_t stream) {
 }
 
 size_t attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t D, uint32_t max_degree) {
-  if (!by_spans(max_degree)) return 0;
-  const uint64_t positions = static_cast<uint64_t>(Vd) + edges;
+  if (!by_spans(Vd, edges, max_degree)) return 0;
+  const uint64_t positions = static_cast<uint64_t>(Vd) * kRowCost + edges;
   const uint32_t span = span_length(positions, q_heads, D);
   const uint64_t spans = (positions + span - 1) / span;
   return static_cast<size_t>(spans * (records_bytes(q_heads, D) + sizeof(uint32_t)));
@@ -677,19 +748,21 @@ int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cac
   // Slots: where a bound is known most rows reach it, and a slot that works through 16 edges costs least (60,000 rows of 10
   // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four); averages hide longer rows (2.48 M edges in 169 K rows:
   // 229 us with four slots for 15 edges on average, 264 with two, 572 with one).
-  const Lanes l = lanes_for(q_heads, heads, width, by_spans(max_degree) ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
+  const bool blocks = by_blocks(Vd, edges, max_degree), spans = by_spans(Vd, edges, max_degree);
+  const Lanes l = lanes_for(q_heads, heads, width, blocks ? kWave : spans ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
   p.units = l.units, p.per_head = l.per_head, p.hw_shift = l.hw_shift, p.walker_shift = l.walker_shift;
   p.passes = ceil_div(l.units, 1u << l.hw_shift);
-  if (by_spans(max_degree)) {
+  p.blocks = blocks;
+  if (spans) {
     if (!work || !aligned_to(work, 16)) return fail_in(call, "needs nts_kv8_attention_work_bytes of 16-byte-aligned work");
-    p.positions = static_cast<uint64_t>(Vd) + edges;
+    p.positions = static_cast<uint64_t>(Vd) * kRowCost + edges;
     p.span = span_length(p.positions, q_heads, width);
     p.spans = static_cast<uint32_t>((p.positions + p.span - 1) / p.span);
     p.partial = static_cast<float *>(work);
     p.tail_row = reinterpret_cast<uint32_t *>(p.partial + static_cast<uint64_t>(p.spans) * 2u * q_heads * (width + 2u));
   }
   const uint64_t bytes = 2ull * heads * std::max(static_cast<uint64_t>(cache_rows) * p.row_width, static_cast<uint64_t>(cache_rows) / block_rows + 1);
-  return bytes < 0xFFFF0000ull ? launch_attend_nd<true>(p, l, stream) : launch_attend_nd<false>(p, l, stream);
+  return bytes < 0xFFFF0000ull && cache_rows <= (1u << 24) ? launch_attend_nd<true>(p, l, stream) : launch_attend_nd<false>(p, l, stream);
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@ out and rounded).
 
 Work is enqueued on torch's current stream of the operands' device.
 """
+import contextlib
 import math
 
 import torch
@@ -28,8 +29,20 @@ def kv8_row_width(width):
     return -(-width // 16) * 16
 
 
+# The raw handle of torch's current stream; a Stream object for it takes 2 us more to make, a fifth of a small call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device made current for a call, if it is not."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _floats(t, columns, what):
@@ -72,7 +85,7 @@ class MxTable:
         code_shape, scale_shape = mx_shapes(n, width)
         codes = allocate(torch.empty, code_shape, dtype=torch.uint8, device=x.device)
         scales = allocate(torch.empty, scale_shape, dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             call("nts_mxfp4_quantize", ptr(codes), ptr(scales), ptr(x), n, width, _stream(x.device))
         return cls(codes, scales, width)
 
@@ -88,7 +101,7 @@ class MxTable:
             if out.shape[0] != n:
                 raise ValueError(f"out: {n} rows")
         _same_device(self.device, row_ids, out)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             call("nts_gather_rows_mxfp4", ptr(out), ptr(self.codes), ptr(self.scales), self.rows, ptr(row_ids), n, self.width,
                  _stream(self.device))
         return out
@@ -115,7 +128,7 @@ class MxProductOp:
         _same_device(dev, weight.codes, self.row_ids)
         n = self._rows(table)
         y = allocate(torch.empty, n, weight.rows, dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
+        with _on(dev):
             call("nts_mxfp4_product", ptr(y), ptr(table.codes), ptr(table.scales), table.rows, ptr(self.row_ids), n,
                  ptr(weight.codes), ptr(weight.scales), weight.rows, table.width, 0, _stream(dev))
         self.table, self.weight = table, weight
@@ -130,7 +143,7 @@ class MxProductOp:
         _same_device(dev, g_out)
         stream = _stream(dev)
         gx = None
-        with torch.cuda.device(dev):
+        with _on(dev):
             if self.rows_grad:
                 gx = allocate(torch.empty, n, F, dtype=torch.float32, device=dev)
                 call("nts_mxfp4_product_grad_rows", ptr(gx), ptr(g_out), ptr(weight.codes), ptr(weight.scales), n, N, F, 0, stream)
@@ -182,7 +195,7 @@ class Kv8Cache:
         if v.shape[0] != n or first < 0 or first > self.rows or first + n > self.capacity:
             raise ValueError(f"k and v: as many rows, from at most row {self.rows} on, up to row {self.capacity}")
         _same_device(self.device, k, v)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             call("nts_kv8_append", ptr(self.cache), ptr(self.scales), ptr(k), ptr(v), first, n, self.capacity, self.heads,
                  self.width, self.block_rows, _stream(self.device))
         self.rows = first + n
@@ -210,7 +223,7 @@ class NeighborAttentionOp:
         scale = 1.0 / math.sqrt(D) if self.scale is None else self.scale
         out = allocate(torch.empty, sg.v_size, H * D, dtype=torch.float32, device=dev)
         lse = allocate(torch.empty, sg.v_size, H, dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
+        with _on(dev):
             size = call("nts_kv8_attention_work_bytes", sg.v_size, sg.e_size, H, D, bound)
             work = allocate(torch.empty, size, dtype=torch.uint8, device=dev) if size else None
             call("nts_kv8_attention", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(sg.dev_c_o()),

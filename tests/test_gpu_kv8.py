@@ -77,7 +77,14 @@ def graph_of(degrees, V, seed, missing=0.0, offset=0):
     return co, ri
 
 
-def check(device, degrees, V, q_heads, heads, D, block, seed=1, missing=0.0, bound=0, offset=0, mirrored=False, rows=None,
+def check(device, degrees, *args, **kwargs):
+    """As they are, and with enough destinations without neighbours behind them that none gets a block of its own."""
+    check_one(device, degrees, *args, **kwargs)
+    if len(degrees) <= 64:
+        check_one(device, list(degrees) + [0] * 65, *args, **kwargs)
+
+
+def check_one(device, degrees, V, q_heads, heads, D, block, seed=1, missing=0.0, bound=0, offset=0, mirrored=False, rows=None,
           scale=None, spread=1.0):
     degrees = np.asarray(degrees, dtype=np.int64)
     Vd = len(degrees)
@@ -163,17 +170,17 @@ def test_a_nan_key_reaches_its_destinations_alone(device):
     k, v = keys(V, heads * D, 1), keys(V, heads * D, 2)
     k[9, 3] = np.nan
     ref.kv8_append(cache, scales, k, v, 0, D, block)
-    for bound in (0, 8):
-        co = np.array([0, 3, 6, 8], dtype=np.uint32)
+    for Vd, bound in ((3, 0), (3, 8), (80, 0)):
+        co = np.array([0, 3, 6] + [8] * (Vd - 2), dtype=np.uint32)
         ri = np.array([1, 9, 2, 3, 4, 5, 8, 10], dtype=np.uint32)
         layer = SampledLayer()
-        layer.v_size, layer.e_size, layer.max_in_degree = 3, 8, bound
+        layer.v_size, layer.e_size, layer.max_in_degree = Vd, 8, bound
         layer.dev_column_offset, layer.dev_row_indices = dev(co, device), dev(ri, device)
         op = lowbit.NeighborAttentionOp(layer, heads)
-        out = op.forward(torch.randn(3, heads * D, device=device), lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, block))
-        nan = torch.isnan(out.view(3, heads, D)).cpu()
+        out = op.forward(torch.randn(Vd, heads * D, device=device), lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, block))
+        nan = torch.isnan(out.view(Vd, heads, D)).cpu()
         assert nan[0, 0].all() and not nan[0, 1].any() and not nan[1:].any()
-        assert torch.isnan(op.lse[0, 0]) and torch.isfinite(op.lse[1:]).all()
+        assert torch.isnan(op.lse[0, 0]) and torch.isfinite(op.lse[1:3]).all()
 
 
 def test_without_the_logarithms_and_beyond_the_rows(device):
@@ -215,14 +222,13 @@ def test_a_cache_beyond_32_bits(device):
     first = (V - 30) % block  # the same place within a block
     ref.kv8_append(small, scales, k, v, first, D, block)
     assert (kv.cache[-30:].cpu().numpy() == small[first:first + 30]).all()
-    co = np.array([0, 30, 33], dtype=np.uint32)
     local = np.concatenate([np.arange(30), [0, 29, 7]])
-    layer = SampledLayer()
-    layer.v_size, layer.e_size = 2, 33
-    layer.dev_column_offset, layer.dev_row_indices = dev(co, device), dev((local + V - 30).astype(np.uint32), device)
-    q = np.random.default_rng(3).standard_normal((2, heads * D)).astype(np.float32)
-    for bound in (0, 30):
-        layer.max_in_degree = bound
+    for Vd, bound in ((2, 0), (2, 30), (70, 0), (70, 30)):
+        co = np.array([0, 30] + [33] * (Vd - 1), dtype=np.uint32)
+        layer = SampledLayer()
+        layer.v_size, layer.e_size, layer.max_in_degree = Vd, 33, bound
+        layer.dev_column_offset, layer.dev_row_indices = dev(co, device), dev((local + V - 30).astype(np.uint32), device)
+        q = np.random.default_rng(3).standard_normal((Vd, heads * D)).astype(np.float32)
         got = lowbit.NeighborAttentionOp(layer, heads, 0.125).forward(dev(q, device), kv).cpu().numpy()
         want, _, tol, _ = ref.attention(q, ref.kv8_values(small, scales, D, block), co.astype(np.int64), local + first, 46, heads, 0.125)
         assert (np.abs(got - want) <= tol).all()

@@ -99,14 +99,16 @@ def test_attention():
     for text, changed in (("heads", dict(heads=0)), ("heads", dict(heads=1025)), ("width", dict(width=0)),
                           ("width", dict(width=257)), ("block_rows", dict(block_rows=48)), ("alignment", dict(cache=P + 4)),
                           ("q_heads", dict(q_heads=0)), ("q_heads", dict(q_heads=6)), ("q_heads", dict(q_heads=1028)),
-                          ("edges", dict(edges=0xFFFF0001)), ("work", dict(work=0)), ("work", dict(work=P + 8)),
-                          ("work", dict(work=0, max_degree=257))):
+                          ("edges", dict(edges=0xFFFF0001)), ("work", dict(work=0, edges=100000)),
+                          ("work", dict(work=P + 8, Vd=1000)), ("work", dict(work=0, edges=100000, max_degree=257))):
         refused(text, name, *attention(**changed))
     for hole in ("out", "q", "cache", "scales", "co", "ri"):
         refused("null pointer", name, *attention(**{hole: 0}))
     assert abi.status(name, *attention(Vd=0, out=0, q=0, co=0)) == abi.NTS_OK
     sizes = abi.call(name + "_work_bytes", 1000, 100000, 8, 32, 0)
     assert sizes > 0 and abi.call(name + "_work_bytes", 1000, 100000, 8, 32, 257) == sizes
+    assert abi.call(name + "_work_bytes", 64, 4096, 8, 32, 0) == 0  # a block of wavefronts for each destination
+    assert abi.call(name + "_work_bytes", 64, 4097, 8, 32, 0) > 0 and abi.call(name + "_work_bytes", 65, 4096, 8, 32, 0) > 0
     for bad in ((8, 32, 25), (0, 32, 0), (8, 0, 0), (8, 257, 0)):
         assert abi.call(name + "_work_bytes", 1000, 100000, *bad) == 0
 
