@@ -206,10 +206,11 @@ void launch_rows_any(const RowsArgs &a) {
 // A group of G lanes takes a row, four columns a lane and step: two bytes of codes, one scale byte, 16 bytes out, so that the
 // group's stores are pieces of 16 G bytes.  An id that the table does not have gives a row of zeros (a padded batch).
 // Bound by its stores.  streamed: past the caches, for an output that the L2s do not hold anyway (400,000 rows of 640 values 291 ->
-// 177 us, 5.8 TB/s written; of 602, whose rows end inside lines, 303 -> 284; 2.45 M of 100: 290 -> 262).  Eight columns a lane, two
-// stores 32 bytes apart, 305 -> 351 with 602; two or four steps or rows at a time, 325 .. 390: a wavefront that writes to several
-// places at once is the slower one.
-template <int G>
+// 164 us, 6.2 TB/s written; 2.45 M of 100: 290 -> 262).  400,000 rows of 602, which begin and end inside lines: 303 through the caches, 284
+// past them, 243 with quads that are whole 16-byte pieces of memory, 196 with the shared lines through the caches.  Eight
+// columns a lane, two stores 32 bytes apart, or two or four steps or rows at a time: 305 .. 390; a wavefront that writes to
+// several places at once is the slower one.
+template <int G, bool SHIFTED>
 __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales, uint32_t table_rows,
                                                              const uint32_t *__restrict__ row_ids, uint32_t n, uint32_t F,
@@ -220,17 +221,37 @@ __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__
     const uint64_t g = row_ids ? row_ids[i] : i;
     const bool there = g < table_rows;
     const uint8_t *row_codes = codes + (there ? g : 0u) * row_blocks * 16u, *row_scales = scales + (there ? g : 0u) * scale_stride;
-    for (uint32_t col = (threadIdx.x & (G - 1)) * 4u; col < F; col += G * 4u) {
-      uint32_t half = 0, scale = 0;
+    // SHIFTED: some rows, of an even number of columns, begin two floats behind a multiple of 16 bytes: two columns first, so that
+    // the quads are whole 16-byte pieces of memory.
+    float *const row = out + i * F;
+    const uint32_t skip = SHIFTED && (reinterpret_cast<uintptr_t>(row) & 15u) == 8u ? 2u : 0u;
+    // From 1 KB on the lines that a row shares with its neighbours go through the caches, where the two parts meet.
+    const bool wide = F >= 256u;
+    const uintptr_t lines = wide ? (reinterpret_cast<uintptr_t>(row) + 127u) & ~static_cast<uintptr_t>(127) : 0u;
+    const uintptr_t lines_end = wide ? reinterpret_cast<uintptr_t>(row + F) & ~static_cast<uintptr_t>(127) : ~static_cast<uintptr_t>(0);
+    const uint32_t lane = threadIdx.x & (G - 1);
+    if (skip && lane == 0) {
+      float v[4];
+      e2m1_decode4(there ? row_codes[0] : 0u, e8m0_value(there ? row_scales[0] : 0u), v);
+      row[0] = v[0];
+      row[1] = v[1];
+    }
+    for (uint32_t col = skip + lane * 4u; col < F; col += G * 4u) {
+      uint32_t half = 0, scale = 0, scale2 = 0;
       if (there) {
-        half = *reinterpret_cast<const uint16_t *>(row_codes + col / 2u);
-        scale = row_scales[col / kMxBlock];
+        typedef uint16_t __attribute__((aligned(1))) Two;
+        half = !SHIFTED || col + 2u < F ? *reinterpret_cast<const Two *>(row_codes + col / 2u) : row_codes[col / 2u];
+        scale = scale2 = row_scales[col / kMxBlock];
+        if (SHIFTED && col % kMxBlock == kMxBlock - 2u && col + 2u < F) scale2 = row_scales[col / kMxBlock + 1u];
       }
       float v[4];
-      e2m1_decode4(half, e8m0_value(scale), v);
-      float *dst = out + i * F + col;
+      e2m1_decode4(half, 1.0f, v);
+      const float s = e8m0_value(scale), s2 = e8m0_value(scale2);
+      v[0] *= s, v[1] *= s, v[2] *= s2, v[3] *= s2;
+      float *dst = row + col;
       if (col + 4u <= F) {
-        store_quad(dst, FloatQuad{v[0], v[1], v[2], v[3]}, streamed);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
+        store_quad(dst, FloatQuad{v[0], v[1], v[2], v[3]}, streamed && at >= lines && at < lines_end);
       } else {
         dst[0] = v[0];
         if (col + 1u < F) dst[1] = v[1];
@@ -244,10 +265,14 @@ template <int G>
 void launch_mx_rows(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids, uint32_t n,
                     uint32_t F, hipStream_t stream) {
   constexpr uint64_t per_block = 256 / G;
-    uint64_t blocks = std::min<uint64_t>((n + per_block - 1) / per_block, kMostBlocks);
-  if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, host_table_blocks(true));
-  hipLaunchKernelGGL(gather_mx_rows_kernel<G>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, out, codes, scales,
-                     table_rows, row_ids, n, F, mx_blocks(F), mx_scale_stride(F), static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes);
+  uint64_t blocks = std::min<uint64_t>((n + per_block - 1) / per_block, kMostBlocks);
+  // codes in host memory: rows are an eighth as long as in floats, so more of them have to be on their way (300,000 rows of 602:
+  // 3.96 ms with 128 blocks, 2.82 with 256, 2.77 with 1,024; in floats 13.4)
+  if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, 2u * host_table_blocks(true));
+  const bool shifted = F % 2 == 0 && (F % 4 != 0 || !aligned_to(out, 16));
+  const auto kernel = shifted ? gather_mx_rows_kernel<G, true> : gather_mx_rows_kernel<G, false>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, out, codes, scales, table_rows,
+                     row_ids, n, F, mx_blocks(F), mx_scale_stride(F), static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes);
 }
 
 // ---- rows that arrive as message records -----------------------------------------------------------

@@ -108,9 +108,9 @@ struct AttendArgs {
   const uint8_t *cache, *scales;
   const uint32_t *co, *ri, *mirror;
   uint32_t Vd, cache_rows, q_heads, heads, D, row_width, block_shift;
-  uint32_t share;          // query heads per head of the cache
-  uint32_t units, per_head;  // units in all and of a head
-  uint32_t passes;           // over the edges, 2^hw_shift units each; neighbouring wavefronts take the passes of one walker
+  uint32_t share;             // query heads per head of the cache
+  uint32_t units, per_head;   // units in all and of a head
+  uint32_t passes;            // over the edges, 2^hw_shift units each; neighbouring wavefronts take the passes of one walker
   uint32_t hw_shift, walker_shift;  // log2 of units side by side, of a walker's lanes
   float score_scale;
   bool blocks;  // a block per destination
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_rows_kernel(Atten
 }
 
 // A block per destination, for few destinations of up to some thousand edges: its wavefronts share the edges and join through
-// LDS, in one launch (one vertex with 300 neighbours: @BLK@).
+// LDS, in one launch (one vertex with 300 neighbours: 6 us on the device, where spans and their join take 13).
 constexpr uint32_t kBlockWaves = 16;
 template <int ND, int G, bool NEAR>
 __global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(AttendArgs p) {
@@ -463,13 +463,10 @@ __global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(At
 // Long rows are shared out and short ones bundled without a look at the degrees on the host: destinations and edges are
 // lined up -- destination r takes kRowCost positions from r * kRowCost + co[r] - co[0] on, which is what beginning and writing a
 // row costs in edges, and its edges the positions behind them -- and every walker takes the destinations that begin within its
-// span of `span` positions.  A destination of more than `span` edges is cut at the
-// spans' ends: every span that it reaches into sums its part into a record (1: the destination begins in this span, 0: in an
-// earlier one) and join_spans_kernel adds the parts in order.  No atomics: the same bits on every call.
-#ifndef RC
-#define RC 8
-#endif
-constexpr uint32_t kRowCost = RC;
+// span of `span` positions.  A destination of more than `span` edges is cut at the spans' ends: every span that it reaches into
+// sums its part into a record (1: the destination begins in this span, 0: in an earlier one) and join_spans_kernel adds the
+// parts in order.  No atomics: the same bits on every call.
+constexpr uint32_t kRowCost = 8;  // 2.48 M edges in 169 K rows, 4 heads of 32: 194 us; 4: 209, 16: 192, 1: 230
 __device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r * kRowCost + (co[r] - co0); }
 
 // The last destination at or before position x: a candidate for every lane of the walker a step.
@@ -617,8 +614,7 @@ Lanes lanes_for(uint32_t q_heads, uint32_t heads, uint32_t D, uint64_t slot_edge
   l.nd = next_power(kv8_row_width(D) / 16);
   // Query heads of a head side by side as long as all fit a wavefront (their loads of the same row meet in the L1, and few
   // registers leave many wavefronts); two to a lane where the edges would have to be walked more than once.
-  l.g = 1;
-    if (share > 1 && l.nd * heads * share > static_cast<uint32_t>(kWave)) l.g = 2;
+  l.g = share > 1 && l.nd * heads * share > static_cast<uint32_t>(kWave) ? 2 : 1;
   l.per_head = ceil_div(share, l.g);
   l.units = heads * l.per_head;
   const uint32_t hw = std::min(kWave / l.nd, next_power(l.units));
@@ -630,8 +626,9 @@ Lanes lanes_for(uint32_t q_heads, uint32_t heads, uint32_t D, uint64_t slot_edge
 
 // Bytes of a span's two records.
 uint64_t records_bytes(uint32_t q_heads, uint32_t D) { return 2ull * q_heads * (D + 2u) * sizeof(float); }
-// Positions of a span: `walkers` spans fill the chip (fewer where their records would take more than 256 MB), none of fewer
-// than 64 positions.
+// Positions of a span: 256, so that a part's record is little beside its edges, but spans for all wavefronts that the chip holds
+// where there are few positions (none of fewer than 64), and no more spans than fill it four times over or have records of
+// 256 MB.
 uint32_t span_length(uint64_t positions, uint32_t q_heads, uint32_t D) {
   const uint64_t most = std::max<uint64_t>(256, std::min<uint64_t>(16384, (256ull << 20) / records_bytes(q_heads, D)));
   const uint64_t spans = std::min(most, std::max<uint64_t>(1024, positions / 256));

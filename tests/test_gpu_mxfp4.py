@@ -100,6 +100,25 @@ def test_gather_by_id(device, F):
     assert (out[777:] == 7.0).all()
 
 
+@pytest.mark.parametrize("F", [1, 6, 32, 47, 64, 100, 130, 256, 602, 1433])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_gather_to_any_float(device, F, shift):
+    """An output that begins at any multiple of four bytes, the whole table with its last row, large enough to be written past
+    the caches and small."""
+    for V, n in ((50, 50), (70, 9_000_000 // F)):
+        x = rows_of(V, F, seed=F + shift)
+        codes, scales, t = table_of(x, device)
+        ids = np.random.default_rng(shift).integers(0, V + 1, n).astype(np.uint32)
+        ids[-1] = V - 1
+        out = torch.full((n * F + 8,), 7.0, device=device)
+        call("nts_gather_rows_mxfp4", ptr(out[shift:]), ptr(t.codes), ptr(t.scales), V, ptr(dev(ids, device)), n, F, stream())
+        values = np.concatenate([ref.mx_values(codes, scales, F).astype(np.float32), np.zeros((1, F), dtype=np.float32)])
+        want = torch.from_numpy(values).to(device)[torch.from_numpy(ids.astype(np.int64)).to(device)].reshape(-1)
+        got = out[shift:shift + n * F]
+        assert ((got == want) | (torch.isnan(got) & torch.isnan(want))).all()
+        assert (out[:shift] == 7.0).all() and (out[shift + n * F:] == 7.0).all()
+
+
 def test_gather_from_mapped_host_memory(device):
     F, V = 100, 5000
     x = rows_of(V, F, seed=5)
@@ -149,6 +168,27 @@ def test_product(device, n, N, F, accumulate):
         want, scale = want + start, scale + np.abs(start)
     close(out[:n], want, scale, F + 1)
     assert (out[n:] == 3.0).all()
+
+
+@pytest.mark.parametrize("n,N,F,accumulate", [(66001, 1030, 1001, 0), (65600, 1024, 1056, 1), (40000, 1793, 2048, 0)])
+def test_product_in_the_larger_tiles(device, n, N, F, accumulate):
+    """Against 64-bit products on the device, whose operands torch reads from the same rows."""
+    V = 300
+    ca, sa, a = table_of(rows_of(V, F, n, special=False), device)
+    cw, sw, w = table_of(rows_of(N, F, N, special=False), device)
+    ids = np.random.default_rng(n).integers(0, V, n).astype(np.uint32)
+    ids[7::1000] = 0xFFFFFFFF
+    dids = dev(ids, device)
+    x = torch.from_numpy(np.concatenate([ref.mx_values(ca, sa, F), np.zeros((1, F))])).to(device)
+    x, wv = x[torch.from_numpy(np.minimum(ids, V).astype(np.int64)).to(device)], torch.from_numpy(ref.mx_values(cw, sw, F)).to(device)
+    start = torch.randn(n, N, device=device)
+    out = start.clone()
+    call("nts_mxfp4_product", ptr(out), ptr(a.codes), ptr(a.scales), V, ptr(dids), n, ptr(w.codes), ptr(w.scales), N, F,
+         accumulate, stream())
+    want, scale = torch.mm(x, wv.t().contiguous()), torch.mm(x.abs(), wv.abs().t().contiguous())
+    if accumulate:
+        want, scale = want + start, scale + start.abs()
+    assert bool(((out.double() - want).abs() <= (F + 1) * 2.0 ** -23 * scale + 2.0 ** -120).all())
 
 
 def test_product_without_ids_is_the_whole_table(device):
@@ -319,6 +359,8 @@ def test_a_table_beyond_32_bits(device):
     wv = ref.mx_values(cw, sw, F)
     op = lowbit.MxProductOp(ids, rows_grad=False)
     close(op.forward(t, w), want @ wv.T, np.abs(want) @ np.abs(wv).T, F)
+    many = lowbit.MxProductOp(ids.repeat(22))
+    close(many.forward(t, w), np.tile(want @ wv.T, (22, 1)), np.tile(np.abs(want) @ np.abs(wv).T, (22, 1)), F)
     g = np.random.default_rng(1).standard_normal((6, 20)).astype(np.float32)
     op.backward(dev(g, device))
     close(op.get_additional_grad(), g.T.astype(np.float64) @ want, np.abs(g.T.astype(np.float64)) @ np.abs(want), 3 * 6 + 1100)
