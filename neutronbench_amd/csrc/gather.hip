@@ -206,11 +206,9 @@ void launch_rows_any(const RowsArgs &a) {
 // A group of G lanes takes a row, four columns a lane and step: two bytes of codes, one scale byte, 16 bytes out, so that the
 // group's stores are pieces of 16 G bytes.  An id that the table does not have gives a row of zeros (a padded batch).
 // Bound by its stores.  streamed: past the caches, for an output that the L2s do not hold anyway (400,000 rows of 640 values 291 ->
-// 164 us, 6.2 TB/s written; 2.45 M of 100: 290 -> 262).  400,000 rows of 602, which begin and end inside lines: 303 through the caches, 284
-// past them, 243 with quads that are whole 16-byte pieces of memory, 196 with the shared lines through the caches.  Eight
-// columns a lane, two stores 32 bytes apart, or two or four steps or rows at a time: 305 .. 390; a wavefront that writes to
-// several places at once is the slower one.
-template <int G, bool SHIFTED>
+// 165 us, 6.2 TB/s written; 2.45 M of 100: 290 -> 262).  Eight columns a lane, two stores 32 bytes apart, or two or four steps or rows
+// at a time take longer: a wavefront that writes to several places at once is the slower one.
+template <int G>
 __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales, uint32_t table_rows,
                                                              const uint32_t *__restrict__ row_ids, uint32_t n, uint32_t F,
@@ -221,41 +219,91 @@ __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__
     const uint64_t g = row_ids ? row_ids[i] : i;
     const bool there = g < table_rows;
     const uint8_t *row_codes = codes + (there ? g : 0u) * row_blocks * 16u, *row_scales = scales + (there ? g : 0u) * scale_stride;
-    // SHIFTED: some rows, of an even number of columns, begin two floats behind a multiple of 16 bytes: two columns first, so that
-    // the quads are whole 16-byte pieces of memory.
-    float *const row = out + i * F;
-    const uint32_t skip = SHIFTED && (reinterpret_cast<uintptr_t>(row) & 15u) == 8u ? 2u : 0u;
-    // From 1 KB on the lines that a row shares with its neighbours go through the caches, where the two parts meet.
-    const bool wide = F >= 256u;
-    const uintptr_t lines = wide ? (reinterpret_cast<uintptr_t>(row) + 127u) & ~static_cast<uintptr_t>(127) : 0u;
-    const uintptr_t lines_end = wide ? reinterpret_cast<uintptr_t>(row + F) & ~static_cast<uintptr_t>(127) : ~static_cast<uintptr_t>(0);
-    const uint32_t lane = threadIdx.x & (G - 1);
-    if (skip && lane == 0) {
-      float v[4];
-      e2m1_decode4(there ? row_codes[0] : 0u, e8m0_value(there ? row_scales[0] : 0u), v);
-      row[0] = v[0];
-      row[1] = v[1];
-    }
-    for (uint32_t col = skip + lane * 4u; col < F; col += G * 4u) {
-      uint32_t half = 0, scale = 0, scale2 = 0;
+    for (uint32_t col = (threadIdx.x & (G - 1)) * 4u; col < F; col += G * 4u) {
+      uint32_t half = 0, scale = 0;
       if (there) {
-        typedef uint16_t __attribute__((aligned(1))) Two;
-        half = !SHIFTED || col + 2u < F ? *reinterpret_cast<const Two *>(row_codes + col / 2u) : row_codes[col / 2u];
-        scale = scale2 = row_scales[col / kMxBlock];
-        if (SHIFTED && col % kMxBlock == kMxBlock - 2u && col + 2u < F) scale2 = row_scales[col / kMxBlock + 1u];
+        half = *reinterpret_cast<const uint16_t *>(row_codes + col / 2u);
+        scale = row_scales[col / kMxBlock];
       }
       float v[4];
-      e2m1_decode4(half, 1.0f, v);
-      const float s = e8m0_value(scale), s2 = e8m0_value(scale2);
-      v[0] *= s, v[1] *= s, v[2] *= s2, v[3] *= s2;
-      float *dst = row + col;
+      e2m1_decode4(half, e8m0_value(scale), v);
+      float *dst = out + i * F + col;
       if (col + 4u <= F) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(dst);
-        store_quad(dst, FloatQuad{v[0], v[1], v[2], v[3]}, streamed && at >= lines && at < lines_end);
+        store_quad(dst, FloatQuad{v[0], v[1], v[2], v[3]}, streamed);
       } else {
         dst[0] = v[0];
         if (col + 1u < F) dst[1] = v[1];
         if (col + 2u < F) dst[2] = v[2];
+      }
+    }
+  }
+}
+
+// The same for large outputs whose rows do not fill whole lines: a wavefront takes kFlatSteps KB of the output in a piece, wherever
+// rows begin in it, so that every line has one writer.  F is even, so a lane's four columns are two pairs that each lie in one row
+// and one block of it.  NARROW: rows of less than 256 columns, of which a wavefront's 256 may reach into many; that costs a
+// division a pair and pays only where rows are no multiple of 16 bytes.
+// 400,000 rows of 602: 284 us a row at a time, 168 in pieces; of 600: 234, 167; 1 M rows of 256: 196, 172; of 50: 73, 53; but of
+// 100: 98, 93 and of 128: 103, 113.
+constexpr uint32_t kFlatSteps = 4;
+template <bool NARROW>
+__global__ __launch_bounds__(256) void gather_mx_flat_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
+                                                             const uint8_t *__restrict__ scales, uint32_t table_rows,
+                                                             const uint32_t *__restrict__ row_ids, uint32_t n, uint32_t F,
+                                                             uint32_t row_blocks, uint32_t scale_stride) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  const uint64_t total = static_cast<uint64_t>(n) * F, waves = static_cast<uint64_t>(gridDim.x) * (256 / kWave);
+  for (uint64_t piece = wave_of_grid(); piece * (kFlatSteps * 256u) < total; piece += waves) {
+    const uint64_t begin = piece * (kFlatSteps * 256u);
+    uint64_t row = begin / F;
+    uint32_t col = static_cast<uint32_t>(begin - row * F);  // both the same in all lanes
+    uint32_t code[kFlatSteps][2], scale[kFlatSteps][2];
+#pragma unroll
+    for (uint32_t k = 0; k < kFlatSteps; ++k) {
+      uint64_t g0 = ~0ull, g1 = ~0ull;
+      if (!NARROW) {
+        if (row < n) g0 = row_ids ? row_ids[row] : row;
+        if (row + 1 < n) g1 = row_ids ? row_ids[row + 1] : row + 1;
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        uint32_t at = col + lane * 4u + h * 2u;
+        uint64_t g;
+        if (NARROW) {
+          const uint32_t ahead = at / F;
+          const uint64_t r = row + ahead;
+          at -= ahead * F;
+          g = r >= n ? ~0ull : row_ids ? row_ids[r] : r;
+        } else {
+          g = at >= F ? g1 : g0;
+          if (at >= F) at -= F;
+        }
+        code[k][h] = scale[k][h] = 0;
+        if (g < table_rows) {
+          code[k][h] = codes[g * row_blocks * 16u + at / 2u];
+          scale[k][h] = scales[g * scale_stride + at / kMxBlock];
+        }
+      }
+      col += 256u;
+      if (NARROW) {
+        row += col / F;
+        col %= F;
+      } else if (col >= F) {
+        ++row;
+        col -= F;
+      }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kFlatSteps; ++k) {
+      const uint64_t at = begin + k * 256u + lane * 4u;
+      float v[4];
+      e2m1_decode4(code[k][0] | code[k][1] << 8, 1.0f, v);
+      const float s = e8m0_value(scale[k][0]), s2 = e8m0_value(scale[k][1]);
+      if (at + 4u <= total) {
+        store_quad(out + at, FloatQuad{v[0] * s, v[1] * s, v[2] * s2, v[3] * s2}, true);
+      } else if (at < total) {  // total is even
+        out[at] = v[0] * s;
+        out[at + 1] = v[1] * s;
       }
     }
   }
@@ -269,9 +317,7 @@ void launch_mx_rows(float *out, const uint8_t *codes, const uint8_t *scales, uin
   // codes in host memory: rows are an eighth as long as in floats, so more of them have to be on their way (300,000 rows of 602:
   // 3.96 ms with 128 blocks, 2.82 with 256, 2.77 with 1,024; in floats 13.4)
   if (table_in_host_memory(codes)) blocks = std::min<uint64_t>(blocks, 2u * host_table_blocks(true));
-  const bool shifted = F % 2 == 0 && (F % 4 != 0 || !aligned_to(out, 16));
-  const auto kernel = shifted ? gather_mx_rows_kernel<G, true> : gather_mx_rows_kernel<G, false>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, out, codes, scales, table_rows,
+  hipLaunchKernelGGL(gather_mx_rows_kernel<G>, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream, out, codes, scales, table_rows,
                      row_ids, n, F, mx_blocks(F), mx_scale_stride(F), static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes);
 }
 
@@ -423,6 +469,15 @@ int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scale
   if (!out || (table_rows && (!codes || !scales))) return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: null pointer");
   if (!aligned_to(codes, 16) || !aligned_to(scales, 4))
     return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: codes need 16-byte, scales 4-byte alignment");
+  if (static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes && F % 2 == 0 && F >= 16 && (F % 4 != 0 || F == 256 || (F > 256 && F % 32 != 0)) &&
+      aligned_to(out, 128) && !table_in_host_memory(codes)) {
+    const uint64_t pieces = (static_cast<uint64_t>(n) * F + kFlatSteps * 256 - 1) / (kFlatSteps * 256);
+    const auto kernel = F < 256 ? gather_mx_flat_kernel<true> : gather_mx_flat_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(std::min<uint64_t>((pieces + 3) / 4, kMostBlocks))), dim3(256), 0, stream,
+                       out, codes, scales, table_rows, row_ids, n, F, mx_blocks(F), mx_scale_stride(F));
+    NTS_LAUNCH_CHECK("nts_gather_rows_mxfp4");
+    return NTS_OK;
+  }
   switch (group_for(ceil_div(F, 4))) {
     case 4: launch_mx_rows<4>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
     case 8: launch_mx_rows<8>(out, codes, scales, table_rows, row_ids, n, F, stream); break;
