@@ -504,13 +504,14 @@ int nts_message_rows_add(float *rows, const float *records, uint32_t n_records, 
 
 /* codes, scales = x [n, F] rounded.  Per block: e = max(floor(log2 max|x|) - 2, -127), scale byte e + 127, code = the
  * one nearest to x * 2^-e, ties to the even code, magnitudes above 6 to 6.  A block that holds an infinity or a NaN gets
- * scale byte 255.  Every byte of both arrays is written. */
+ * scale byte 255.  Every byte of both arrays is written.  n * B is less than 2^32. */
 int nts_mxfp4_quantize(uint8_t *codes, uint8_t *scales, const float *x, uint32_t n, uint32_t F, nts_stream_t stream);
 /* nts_gather_rows_f32 for a 4-bit table: out[i, :] = values of row row_ids[i] (row_ids NULL: row i), exactly. */
 int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids,
                           uint32_t n, uint32_t F, nts_stream_t stream);
 /* A dense layer on rows gathered by id: out[i, j] (+)= sum_f A[row_ids[i], f] * W[j, f], i < n, j < N, where W is a 4-bit
- * table of N rows of F values (the layer's weight, a row per output).  Products are exact, sums are kept in 32 bits.
+ * table of N rows of F values (the layer's weight, a row per output).  Products are exact, sums are kept in 32 bits (what
+ * lies beyond the range of floats is infinite, what lies below 2^-126 may be lost).
  * row_ids NULL: row i.  accumulate as in nts_spmm_gather. */
 int nts_mxfp4_product(float *out, const uint8_t *codes, const uint8_t *scales, uint32_t table_rows, const uint32_t *row_ids,
                       uint32_t n, const uint8_t *w_codes, const uint8_t *w_scales, uint32_t N, uint32_t F, int accumulate,

@@ -205,7 +205,7 @@ void launch_rows_any(const RowsArgs &a) {
 // ---- rows held in 4 bits ------------------------------------------------------------------------------
 // A group of G lanes takes a row, four columns a lane and step: two bytes of codes, one scale byte, 16 bytes out, so that the
 // group's stores are pieces of 16 G bytes.  An id that the table does not have gives a row of zeros (a padded batch).
-// Bound by its stores.  streamed: past the caches, for an output that the L2s do not hold anyway (400,000 rows of 640 values 291 ->
+// Bound by its stores.  streamed: past the caches, for an output that these do not hold anyway (400,000 rows of 640 values 291 ->
 // 165 us, 6.2 TB/s written; 2.45 M of 100: 290 -> 262).  Eight columns a lane, two stores 32 bytes apart, or two or four steps or rows
 // at a time take longer: a wavefront that writes to several places at once is the slower one.
 template <int G>
@@ -243,8 +243,8 @@ __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__
 // rows begin in it, so that every line has one writer.  F is even, so a lane's four columns are two pairs that each lie in one row
 // and one block of it.  NARROW: rows of less than 256 columns, of which a wavefront's 256 may reach into many; that costs a
 // division a pair and pays only where rows are no multiple of 16 bytes.
-// 400,000 rows of 602: 284 us a row at a time, 168 in pieces; of 600: 234, 167; 1 M rows of 256: 196, 172; of 50: 73, 53; but of
-// 100: 98, 93 and of 128: 103, 113.
+// 400,000 rows of 602: 284 us a row at a time, 168 in pieces; of 600: 234, 167; 1 M rows of 256: 196, 172; of 50: 73, 53 (streamed
+// both); but of 100: 98, 93 and of 128: 103, 113.
 constexpr uint32_t kFlatSteps = 4;
 template <bool NARROW>
 __global__ __launch_bounds__(256) void gather_mx_flat_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,

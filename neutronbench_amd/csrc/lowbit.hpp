@@ -16,7 +16,9 @@ constexpr uint32_t kMostWidth = 1u << 17;  // columns (and outputs) of a row: th
 // Columns of a row that the cache of 8-bit keys and values keeps: whole 16-byte loads.
 inline __host__ __device__ uint32_t kv8_row_width(uint32_t D) { return (D + 15) / 16 * 16; }
 
-// An output from this size on is more than the L2s hold (8 of 4 MB) and is written past them.
+// An output from this size on is more than the L2s hold (8 of 4 MB) and is written past the caches.  Its reader does not seem to miss
+// it there: twelve batches of a Products-shaped epoch, whose 94 MB of gathered features the aggregation reads next, take 11.4 ms
+// with this bound and 11.5 with one of 256 MB, which nothing in them reaches.
 constexpr uint64_t kStreamedBytes = 32ull << 20;
 
 #if defined(__HIPCC__)

@@ -136,6 +136,8 @@ class MxProductOp:
 
     def backward(self, g_out):
         table, weight = self.table, self.weight
+        if table is None:
+            raise ValueError("backward before forward")
         n, N, F, dev = self._rows(table), weight.rows, table.width, table.device
         _floats(g_out, N, "g_out")
         if g_out.shape[0] != n:
@@ -175,8 +177,8 @@ class Kv8Cache:
         return self
 
     def _hold(self, cache, scales, width, block_rows, rows):
-        if cache.dim() != 4 or block_rows < 1:
-            raise ValueError("cache: [capacity, 2, heads, row width], block_rows at least 1")
+        if cache.dim() != 4 or cache.shape[2] < 1 or not 1 <= width <= 256 or block_rows < 1 or block_rows & (block_rows - 1):
+            raise ValueError("cache: [capacity, 2, heads, row width], width 1 .. 256, block_rows a power of two")
         capacity, _, heads, _ = cache.shape
         _bytes(cache, (capacity, 2, heads, kv8_row_width(width)), "cache")
         _bytes(scales, (-(-capacity // block_rows), 2, heads), "scales")
@@ -218,7 +220,12 @@ class NeighborAttentionOp:
             raise ValueError(f"q: a row for each of {sg.v_size} destinations; q_heads: a multiple of {cache.heads}")
         if mirror is not None:
             _indices(mirror, "mirror")
-        _same_device(dev, q, mirror, sg.dev_c_o(), sg.dev_r_i())
+        co, ri = sg.dev_c_o(), sg.dev_r_i()
+        _indices(co, "column_offset")
+        _indices(ri, "row_indices")
+        if co.numel() != sg.v_size + 1 or ri.numel() < sg.e_size:
+            raise ValueError(f"layer: offsets of {sg.v_size} destinations and {sg.e_size} edges")
+        _same_device(dev, q, mirror, co, ri)
         bound = getattr(sg, "max_in_degree", 0)
         scale = 1.0 / math.sqrt(D) if self.scale is None else self.scale
         out = allocate(torch.empty, sg.v_size, H * D, dtype=torch.float32, device=dev)
@@ -226,8 +233,8 @@ class NeighborAttentionOp:
         with _on(dev):
             size = call("nts_kv8_attention_work_bytes", sg.v_size, sg.e_size, H, D, bound)
             work = allocate(torch.empty, size, dtype=torch.uint8, device=dev) if size else None
-            call("nts_kv8_attention", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(sg.dev_c_o()),
-                 ptr(sg.dev_r_i()), ptr(mirror), sg.v_size, sg.e_size, cache.rows, H, cache.heads, D, cache.block_rows, scale,
+            call("nts_kv8_attention", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(co),
+                 ptr(ri), ptr(mirror), sg.v_size, sg.e_size, cache.rows, H, cache.heads, D, cache.block_rows, scale,
                  bound, ptr(work), _stream(dev))
         self.lse = lse
         return out

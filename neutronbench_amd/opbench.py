@@ -19,7 +19,8 @@ import torch
 from . import synth
 from .abi import call, ptr
 from .batch import MappedHostTable
-from .layout import SpmmPlan, as_u32
+from .layout import SampledLayer, SpmmPlan, as_u32
+from .lowbit import Kv8Cache, MxProductOp, MxTable, NeighborAttentionOp
 
 HBM_PEAK = 8.0e12
 
@@ -144,6 +145,25 @@ def main():
                                                        ptr(ids), ptr(hashmap), n, Ff, ptr(hits), s), miss * 4 * Ff,
            f"{n} rows, {n - miss} from the HBM cache, {miss} over PCIe; bytes = PCIe payload")
     host.close()
+
+    held = Ff // 32 + (Ff % 32 != 0)
+    mx = MxTable.quantize(table_dev)
+    report("nts_mxfp4_quantize", lambda: MxTable.quantize(table_dev), V * (4 * Ff + 17 * held), f"{V} rows of {Ff} floats")
+    report("nts_gather_rows_mxfp4", lambda: mx.gather(ids, o), n * (17 * held + 4 + 4 * Ff), f"{n} random rows of {Ff} values")
+    weight = MxTable.quantize(torch.randn(F, Ff, device=dev))
+    op = MxProductOp(ids)
+    g = torch.randn(n, F, device=dev)
+    held = n * (17 * held + 4)
+    report("nts_mxfp4_product", lambda: op.forward(mx, weight), held + 4 * n * F, f"{n} random rows of {Ff} values by {F} outputs")
+    report("nts_mxfp4_product_grad_rows, _grad_weight", lambda: op.backward(g), held + 4 * n * (2 * F + Ff), "the same")
+    del g, op
+    kv = Kv8Cache(V, H, Fh, device=dev)
+    k, v = torch.randn(V, F, device=dev), torch.randn(V, F, device=dev)
+    report("nts_kv8_append", lambda: kv.append(k, v, 0), V * 2 * F * 5, f"{V} vertices, {H} heads of {Fh}")
+    layer = SampledLayer()
+    layer.v_size, layer.e_size, layer.dev_column_offset, layer.dev_row_indices = V, E, co32, ri32
+    attention = NeighborAttentionOp(layer, H)
+    report("nts_kv8_attention", lambda: attention.forward(k, kv), E * (2 * F + 4) + V * (8 * F + 4 * H), whole + f", F'={F}")
 
 
 if __name__ == "__main__":

@@ -24,6 +24,7 @@ def test_quantize():
         refused("null pointer", "nts_mxfp4_quantize", *args, 4, 8, 0)
     refused("alignment", "nts_mxfp4_quantize", P + 8, P, P, 4, 8, 0)
     refused("alignment", "nts_mxfp4_quantize", P, P + 2, P, 4, 8, 0)
+    refused("2^32 blocks", "nts_mxfp4_quantize", P, P, P, 0x80000000, 33, 0)
     assert abi.status("nts_mxfp4_quantize", 0, 0, 0, 0, 8, 0) == abi.NTS_OK
 
 
@@ -138,7 +139,7 @@ def test_python_objects_check_their_operands():
         lowbit.MxProductOp().forward(table(6, 100), table(6, 96))
     cache, scales = torch.zeros(40, 2, 3, 32, dtype=torch.uint8), torch.zeros(3, 2, 3, dtype=torch.uint8)
     kv = lowbit.Kv8Cache.over(cache, scales, 20, 16, rows=10)
-    for bad in ((cache, scales, 33, 16), (cache, scales, 20, 8), (cache[:, :1], scales, 20, 16), (cache[:, 0], scales, 20, 16),
+    for bad in ((cache[:, :, :0], scales[:, :, :0], 20, 16), (cache, scales, 0, 16), (cache[:10], scales, 20, 5), (cache, scales, 33, 16), (cache, scales, 20, 8), (cache[:, :1], scales, 20, 16), (cache[:, 0], scales, 20, 16),
                 (cache, scales, 20, 0)):
         with pytest.raises(ValueError):
             lowbit.Kv8Cache.over(*bad)
@@ -150,6 +151,15 @@ def test_python_objects_check_their_operands():
             kv.append(*bad)
     layer = SampledLayer()
     layer.v_size, layer.dev_column_offset, layer.dev_row_indices = 4, torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        lowbit.MxProductOp().backward(torch.zeros(4, 8))
+    with pytest.raises(ValueError):  # five offsets for five destinations
+        layer.v_size = 5
+        lowbit.NeighborAttentionOp(layer, 6).forward(torch.zeros(5, 120), kv)
+    layer.v_size, layer.e_size = 4, 1
+    with pytest.raises(ValueError):  # fewer edges than the layer says
+        lowbit.NeighborAttentionOp(layer, 6).forward(torch.zeros(4, 120), kv)
+    layer.e_size = 0
     for q_heads, q in ((6, torch.zeros(5, 120)), (6, torch.zeros(4, 100)), (4, torch.zeros(4, 80))):
         with pytest.raises(ValueError):
             lowbit.NeighborAttentionOp(layer, q_heads).forward(q, kv)
