@@ -14,7 +14,7 @@ namespace {
 // A wavefront takes one block of rows, one of keys and values and one head: the largest finite magnitude first, then the codes.
 // The scale is the smallest power of two with max <= 448 * scale, so every value lies within e4m3's range.  Rows of the block
 // that were there before `first` keep their place: the scale is at least theirs, and they are rounded once more where it grew
-// (exactly, unless the value falls among e4m3's subnormals).  Both passes read through the caches the second time.
+// (exactly, unless the value falls among e4m3's subnormals).
 struct AppendArgs {
   uint8_t *cache;
   uint8_t *scales;
@@ -47,6 +47,10 @@ __device__ __forceinline__ void append_values(const AppendArgs &p, const float *
   }
 }
 
+// Bound by memory: 2.45 M rows of 4 heads of 32, blocks of 16, 623 us, 5.0 TB/s of floats read and bytes written (read twice, the
+// second time from the caches: 712 .. 770).
+// HELD: blocks of at most 64 * HELD quads, which the lanes hold between the passes; 0: of any size, read twice.
+template <int HELD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
   const uint64_t waves = static_cast<uint64_t>(gridDim.x) * (256 / kWave);
@@ -63,14 +67,30 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     const float held_scale = e8m0_value(old);
     const uint32_t total = rows * p.quads;
     uint32_t top = 0;
-    for (uint32_t j = lane; j < total; j += kWave) {
-      const uint32_t r = j / p.quads;
-      float v[4];
-      append_values(p, src, held, held_scale, static_cast<uint32_t>(row0) + r, j - r * p.quads, v);
+    auto largest = [&](const float *v) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
         if (b < 0x7F800000u) top = max(top, b);
+      }
+    };
+    float kept[HELD ? HELD : 1][4];
+    if (HELD) {
+#pragma unroll
+      for (uint32_t k = 0; k < HELD; ++k) {
+        const uint32_t j = k * kWave + lane, r = j / p.quads;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kept[k][i] = 0.0f;
+        if (j < total) append_values(p, src, held, held_scale, static_cast<uint32_t>(row0) + r, j - r * p.quads, kept[k]);
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < HELD; ++k) largest(kept[k]);
+    } else {
+      for (uint32_t j = lane; j < total; j += kWave) {
+        const uint32_t r = j / p.quads;
+        float v[4];
+        append_values(p, src, held, held_scale, static_cast<uint32_t>(row0) + r, j - r * p.quads, v);
+        largest(v);
       }
     }
 #pragma unroll
@@ -79,15 +99,22 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     const uint32_t up = (top >> 23) + ((top & 0x7FFFFFu) > 0x600000u ? 1u : 0u);
     const uint32_t byte = max(old, up > 8u ? up - 8u : 0u);
     const float inverse = e8m0_inverse(min(byte, 253u));
-    for (uint32_t j = lane; j < total; j += kWave) {
+    auto put = [&](uint32_t j, float *v) {
       const uint32_t r = j / p.quads;
       const uint32_t row = static_cast<uint32_t>(row0) + r, quad = j - r * p.quads;
-      if (row < p.first && byte == old) continue;
-      float v[4];
-      append_values(p, src, held, held_scale, row, quad, v);
+      if (row < p.first && byte == old) return;
+      if (!HELD) append_values(p, src, held, held_scale, row, quad, v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] *= inverse;
       *reinterpret_cast<uint32_t *>(held + static_cast<uint64_t>(row) * 2u * p.heads * p.quads * 4u + quad * 4u) = e4m3_encode4(v);
+    };
+    if (HELD) {
+#pragma unroll
+      for (uint32_t k = 0; k < HELD; ++k)
+        if (k * kWave + lane < total) put(k * kWave + lane, kept[k]);
+    } else {
+      float v[4];
+      for (uint32_t j = lane; j < total; j += kWave) put(j, v);
     }
     if (lane == 0) *scale = static_cast<uint8_t>(byte);
   }
@@ -102,6 +129,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // value row serve them.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by side, and further edges of the
 // destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
 // one destination are a walker; a wavefront is one walker or, where rows are short, several.
+// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 428 us, of which 400 in the walkers, that is 1.3 GB of rows, queries
+// and results at 3.3 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 24 a lane to convert and
+// multiply 16 columns of a key and a value, as many again to look up, scale, rescale, join and write.
 struct AttendArgs {
   float *out, *lse;
   const float *q;
@@ -138,7 +168,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // What the registers allow, measured: with one query head to a lane four edges at a time and four wavefronts to a SIMD (2.48 M edges, 8
-// query heads of 64: 468 us; three wavefronts 507, two edges 600); with two, two edges and three wavefronts (500 K edges, 16
+// query heads of 64: 468 us at the time; three wavefronts 507, two edges 600); with two, two edges and three wavefronts (500 K edges, 16
 // query heads of 128: 233 us; four edges 255, one head to a lane 259).  Four heads to a lane leave one wavefront.
 template <int G>
 constexpr int kAheadOf = G == 1 ? 4 : 2;
@@ -523,7 +553,7 @@ __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_spans_kernel(Atte
 
 // The destinations that were cut: 64 columns a block, its wavefronts take every kJoinWaves-th part, and the first adds up
 // what they have, in order.
-constexpr uint32_t kJoinWaves = 16, kJoinSpans = 8, kJoinAhead = 8;
+constexpr uint32_t kJoinWaves = 8, kJoinSpans = 32, kJoinAhead = 16;
 __global__ __launch_bounds__(kJoinWaves *kWave) void join_spans_kernel(AttendArgs p) {
   __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave];
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block();
@@ -715,7 +745,9 @@ int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float 
   const AppendArgs p{cache, scales, k, v, first, n, heads, width, kv8_row_width(width) / 4, block_rows, first_block,
                      blocks * 2u * heads};
   const uint64_t grid = std::min<uint64_t>((p.units + 3) / 4, kMostBlocks);
-  hipLaunchKernelGGL(kv8_append_kernel, dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream, p);
+  const uint32_t quads = block_rows * p.quads;
+  const auto kernel = quads <= 2 * kWave ? kv8_append_kernel<2> : quads <= 8 * kWave ? kv8_append_kernel<8> : kv8_append_kernel<0>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream, p);
   NTS_LAUNCH_CHECK("nts_kv8_append");
   return NTS_OK;
 }

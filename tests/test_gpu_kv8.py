@@ -31,7 +31,7 @@ def empty(capacity, heads, D, block, fill=0):
             np.full((-(-capacity // block), 2, heads), fill, dtype=np.uint8))
 
 
-@pytest.mark.parametrize("heads,D,block", [(1, 1, 1), (1, 16, 4), (4, 32, 16), (3, 20, 16), (2, 47, 8), (8, 128, 64), (5, 256, 32),
+@pytest.mark.parametrize("heads,D,block", [(1, 1, 1), (1, 16, 4), (4, 32, 16), (3, 20, 16), (2, 47, 8), (2, 64, 16), (3, 47, 32), (8, 128, 64), (5, 256, 32),
                                            (2, 100, 1024)])
 def test_append_in_pieces(device, heads, D, block):
     """Pieces that begin and end inside blocks, on blocks, and one row at a time; later rows larger, so that scales grow."""
