@@ -7,6 +7,7 @@ package is the thin Python host layer used by the tests and the benchmark:
 * ``stream``  ``CudaStream``, a mirror of the reference's ``Cuda_Stream`` class over the ABI;
 * ``ops``     mirrors of the reference's graph operators (forward()/backward() objects);
 * ``layout``  device-resident full-graph chunks and sampled layers;
+* ``lowbit``  vertex tables in few bits: 4-bit rows and products on them, a cache of 8-bit keys and values;
 * ``synth``   seeded synthetic graphs / features of the benchmark shapes.
 
 There is no CPU fallback: every operator calls the HIP library.

@@ -130,8 +130,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
 // one destination are a walker; a wavefront is one walker or, where rows are short, several.
 // 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 428 us, of which 400 in the walkers, that is 1.3 GB of rows, queries
-// and results at 3.3 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 24 a lane to convert and
-// multiply 16 columns of a key and a value, as many again to look up, scale, rescale, join and write.
+// and results at 3.3 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
+// convert and multiply 16 columns of a key and a value, about as many again to look up, scale, rescale, join and write.
 struct AttendArgs {
   float *out, *lse;
   const float *q;

@@ -475,34 +475,44 @@ __global__ __launch_bounds__(256, 2) void mx_grad_kernel(GradArgs p) {
   uint32_t word[4], scale[4];
   auto request = [&](uint64_t k0) {
     const uint64_t m = m0 + pm;
-    if (WEIGHT) {
-      const float *src = p.g + (k0 + pk) * p.g_stride + m;
+    if (k0 + kGradTerms <= end) {  // the same in all threads: no look at every term (weight's gradient of 640 by 640: 1,100 -> 540 us)
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) g[i] = m < p.M && k0 + pk + i < end ? src[static_cast<uint64_t>(i) * p.g_stride] : 0.0f;
-    } else {
-      const float *src = p.g + m * p.g_stride + k0 + pk;
+      for (uint32_t i = 0; i < 16; ++i) g[i] = 0.0f;
+      if (m < p.M) {
+        if (WEIGHT) {
+          const float *src = p.g + (k0 + pk) * p.g_stride + m;
 #pragma unroll
-      for (uint32_t i = 0; i < 16; i += 4) {
-        if (m < p.M && k0 + pk + i + 4u <= end) {
-          const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src + i);
-#pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) g[i + k] = q[k];
+          for (uint32_t i = 0; i < 16; ++i) g[i] = src[static_cast<uint64_t>(i) * p.g_stride];
         } else {
+          const float *src = p.g + m * p.g_stride + k0 + pk;
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) g[i + k] = m < p.M && k0 + pk + i + k < end ? src[i + k] : 0.0f;
+          for (uint32_t i = 0; i < 16; i += 4) {
+            const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src + i);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) g[i + k] = q[k];
+          }
         }
       }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const uint64_t k = k0 + pk + i;
+        g[i] = m < p.M && k < end ? p.g[WEIGHT ? k * p.g_stride + m : m * p.g_stride + k] : 0.0f;
+      }
+    }
+    uint32_t id[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint64_t k = k0 + qk + i;
+      id[i] = kNoSlot;
+      if (q_mine && k < end) id[i] = WEIGHT && p.row_ids ? p.row_ids[k] : static_cast<uint32_t>(k);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       word[i] = scale[i] = 0;
-      const uint64_t k = k0 + qk + i;
-      if (q_mine && k < end) {
-        const uint64_t row = WEIGHT && p.row_ids ? p.row_ids[k] : k;
-        if (row < p.q_rows) {
-          word[i] = *reinterpret_cast<const uint32_t *>(p.q.codes + row * p.row_blocks * 16u + (f0 + qf) / 2u);
-          scale[i] = p.q.scales[row * p.scale_stride + (f0 + qf) / kMxBlock];
-        }
+      if (id[i] < p.q_rows) {
+        word[i] = *reinterpret_cast<const uint32_t *>(p.q.codes + static_cast<uint64_t>(id[i]) * p.row_blocks * 16u + (f0 + qf) / 2u);
+        scale[i] = p.q.scales[static_cast<uint64_t>(id[i]) * p.scale_stride + (f0 + qf) / kMxBlock];
       }
     }
   };

@@ -16,7 +16,9 @@ Everything goes through the C ABI: neighbour sampling of each hop, relabelling, 
 weights, gathers, aggregation.  --sampler builder (default) builds all layers of a batch in one
 stream-ordered sequence with one read-back (nts_batch_builder_*; "sample" then holds sampling and
 structure together); --sampler library goes hop by hop through the per-step entry points;
---sampler harness uses the torch sampler of the test harness instead.  Stages are separated by
+--sampler harness uses the torch sampler of the test harness instead.  --features mxfp4 rounds the feature
+table to 4 bits and holds it in device memory: the gather reads it there, and in the gat configuration the
+first dense layer is part of the pass, as a product that gathers the rows itself.  Stages are separated by
 stream synchronisation, as every reference operator synchronises its stream.  --pipeline 2 samples
 the next batch on a second stream while the current one is gathered and aggregated; --pipeline P >= 3
 keeps P batches in flight: P - 2 are sampled ahead, each on a stream of its own, and the next
