@@ -47,8 +47,8 @@ __device__ __forceinline__ void append_values(const AppendArgs &p, const float *
   }
 }
 
-// Bound by memory: 2.45 M rows of 4 heads of 32, blocks of 16, 623 us, 5.0 TB/s of floats read and bytes written (read twice, the
-// second time from the caches: 712 .. 770).
+// Bound by memory: 2.45 M rows of 4 heads of 32, blocks of 16, 534 us, 5.9 TB/s of floats read and bytes written (read twice, the
+// second time from the caches: 712; alone in a loop 540 .. 650).
 // HELD: blocks of at most 64 * HELD quads, which the lanes hold between the passes; 0: of any size, read twice.
 template <int HELD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // value row serve them.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by side, and further edges of the
 // destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
 // one destination are a walker; a wavefront is one walker or, where rows are short, several.
-// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 428 us, of which 400 in the walkers, that is 1.3 GB of rows, queries
-// and results at 3.3 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
+// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 413 us, of which 385 in the walkers, that is 1.3 GB of rows, queries
+// and results at 3.4 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
 // convert and multiply 16 columns of a key and a value, about as many again to look up, scale, rescale, join and write.
 struct AttendArgs {
   float *out, *lse;

@@ -184,10 +184,10 @@ __global__ __launch_bounds__(kFewWaves *kWave) void mx_product_few_kernel(Produc
 // or 128 bytes a row.  The loads write a stage to LDS themselves (no registers between) while the one before it is
 // multiplied.  Part c of row r lies at c ^ (r * PARTS / 16) % PARTS, so that the 16 lanes that read one part of 16 rows meet all
 // banks once.
-// Measured (65,536 rows of 4,096 values by 4,096 columns): 785 us, 2.8 PFLOP/s, where a library's bf16 product of that size
-// takes 1,599.  Without loads and stores 417 us, with the stores 687: the stores of a block's tile, 256 KB, are not hidden behind
-// another's products.  Past the caches they cost less than through them (1,043 -> 900 us).  Registers in place of loads into LDS 1,170;
-// stages of 64 bytes, of which the L2 fetches whole lines, 973 (128 x 128); operands asked for a step ahead 893 -> 785.
+// Measured (65,536 rows of 4,096 values by 4,096 columns): 693 us, 3.2 PFLOP/s, where a library's bf16 product of that size
+// takes 1,599.  Without loads and stores 411 us, with the stores 493, with the loads 686: bound by the loads of codes into LDS and the
+// waits for them.  Steps: registers in place of loads into LDS 1,170; stores past the caches 1,043 -> 900; operands asked for a step
+// ahead 893 -> 785; results turned in LDS and stored as whole lines 785 -> 693.  128 x 128 with stages of 64 bytes takes 933.
 typedef __attribute__((address_space(3))) void *LdsPointer;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00027000);
@@ -414,7 +414,7 @@ void launch_product(const ProductArgs &p, hipStream_t stream) {
   const uint64_t row_bytes = p.row_blocks * 16ull;
   if (std::max(p.table_rows, p.N) * row_bytes >= 0xFFFF0000ull) return launch_tiled<128, 128, 2, 2, 4, false>(p, stream);
   // The larger tile where there are enough of them to fill the chip a few times and rows are long: 65,536 rows of 4,096 by 4,096
-  // columns 782 us against 973; 65,536 of 1,024 by 1,024: 111 against 113; 232,965 of 602 by 256: 108 against 99.
+  // columns 718 us against 933; 65,536 of 1,024 by 1,024: 85 against 90; 232,965 of 602 by 256: 86 against 79.
   if (p.row_blocks >= 32 && static_cast<uint64_t>(ceil_div(p.n, 256)) * ceil_div(p.N, 256) >= 1024)
     return launch_tiled<256, 256, 2, 4, 8, true>(p, stream);
   launch_tiled<128, 128, 2, 2, 4, true>(p, stream);
@@ -614,7 +614,7 @@ struct Parts {
   uint32_t count, terms;
 };
 // Parts of the weight's gradient: 512 blocks, two for a compute unit, and none of fewer than 256 terms (169,343 rows of 640 by 640:
-// 1.0 ms with 512, 2.0 with 256, 1.0 with 1,024).
+// 0.54 ms with 512; when that took 1.0, 256 took 2.0 and 1,024 took 1.0).
 Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
   const uint64_t tiles = static_cast<uint64_t>(ceil_div(N, kGradTile)) * ceil_div(F, kGradTile);
   const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(512 / tiles, n / 256));
