@@ -184,7 +184,7 @@ struct Attend {
   uint32_t lane_edge, edge_step;  // the lane's first edge of a destination, and how far its next one lies behind it
   bool live;  // this lane has a unit and columns
   uint32_t key_at, row_bytes, values_at;  // the lane's 16 bytes of a row's keys; from there to its values
-  __amdgpu_buffer_rsrc_t cache_words, scale_bytes;
+  __amdgpu_buffer_rsrc_t keys, values, key_scales, value_scales;
   float q[G][16], acc[G][16], top[G], sum[G];
   uint32_t col;  // the first of the lane's columns; fewer than 16 of them after join()
 
@@ -205,8 +205,13 @@ struct Attend {
     key_at = kv_head * p.row_width + dl * 16u;
     if (NEAR) {
       const uint32_t blocks = p.cache_rows ? ((p.cache_rows - 1u) >> p.block_shift) + 1u : 0u;
-      cache_words = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.cache), 0, p.cache_rows * row_bytes, 0x00027000);
-      scale_bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.scales), 0, blocks * 2u * p.heads, 0x00027000);
+      // one for keys and one for values, so that an offset is one register and one behind the end stays there
+      uint8_t *const cache = const_cast<uint8_t *>(p.cache), *const scales = const_cast<uint8_t *>(p.scales);
+      const uint32_t bytes = p.cache_rows * row_bytes, scales_bytes = blocks * 2u * p.heads;
+      keys = __builtin_amdgcn_make_buffer_rsrc(cache, 0, bytes, 0x00027000);
+      values = __builtin_amdgcn_make_buffer_rsrc(cache + values_at, 0, bytes ? bytes - values_at : 0u, 0x00027000);
+      key_scales = __builtin_amdgcn_make_buffer_rsrc(scales, 0, scales_bytes, 0x00027000);
+      value_scales = __builtin_amdgcn_make_buffer_rsrc(scales + p.heads, 0, scales_bytes ? scales_bytes - p.heads : 0u, 0x00027000);
     }
   }
 
@@ -256,10 +261,10 @@ struct Attend {
         const bool read = there[u] && live;
         const uint32_t at = read ? __umul24(row[u], row_bytes) + key_at : 0xFFFFFF00u;
         const uint32_t scale_at = read ? __umul24(row[u] >> p.block_shift, 2u * p.heads) + kv_head : 0xFFFFFF00u;
-        kc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, 0, 0);
-        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(cache_words, at, values_at, 0);
-        kb[u] = __builtin_amdgcn_raw_buffer_load_b8(scale_bytes, scale_at, 0, 0);
-        vb[u] = __builtin_amdgcn_raw_buffer_load_b8(scale_bytes, scale_at, p.heads, 0);
+        kc[u] = __builtin_amdgcn_raw_buffer_load_b128(keys, at, 0, 0);
+        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(values, at, 0, 0);
+        kb[u] = __builtin_amdgcn_raw_buffer_load_b8(key_scales, scale_at, 0, 0);
+        vb[u] = __builtin_amdgcn_raw_buffer_load_b8(value_scales, scale_at, 0, 0);
       } else {
         kc[u] = vc[u] = u32x4{0, 0, 0, 0};
         kb[u] = vb[u] = 0;
