@@ -199,7 +199,10 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t
 __device__ __forceinline__ void load_to_lds(const uint8_t *from, uint8_t *to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (LdsPointer)to, 16, 0, 0);
 }
-constexpr uint32_t kNowhere = 0xFFFFFF00u;  // an offset behind the end of any buffer: reads zeros
+// An offset behind the end of any buffer, which reads zeros: also with a stage's 16 bytes times kMostWidth / 32 blocks added, of
+// which the last begins within any table that has a row.
+constexpr uint32_t kNowhere = 0xFFFF0000u;
+static_assert(kNowhere + (kMostWidth / kMxBlock - 1) * 16u > kNowhere, "the sum fits 32 bits");
 __device__ __attribute__((aligned(16))) uint8_t zero_part[16];  // zeros for the loads that go by address
 
 // Waits for the wavefront's loads and LDS accesses, then for the block.
@@ -252,11 +255,14 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(Prod
   }
   auto request = [&](uint8_t *tile, uint32_t base) {  // blocks base .. base + PARTS - 1
     const bool inside = base + chunk < p.row_blocks;
+    // never behind the end of a table: the hardware may compare an offset with the table's length less this
+    const uint32_t at = min(base, p.row_blocks - 1u) * 16u, a_at = p.table_rows ? at : 0u;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       uint8_t *to = tile + (i * kWaves + wave) * 1024u;
+      const bool of_a = (i + 1) * kLoadRows * kWaves <= BM;
       if (NEAR)
-        load_to_lds((i + 1) * kLoadRows * kWaves <= BM ? a_codes : w_codes, to, inside ? src[i] : kNowhere, base * 16u);
+        load_to_lds(of_a ? a_codes : w_codes, to, inside ? src[i] : kNowhere, of_a ? a_at : at);
       else
         load_to_lds(inside && far[i] ? far[i] + base * 16ull : zero_part, to);
     }

@@ -191,6 +191,27 @@ def test_product_in_the_larger_tiles(device, n, N, F, accumulate):
     assert bool(((out.double() - want).abs() <= (F + 1) * 2.0 ** -23 * scale + 2.0 ** -120).all())
 
 
+@pytest.mark.parametrize("n,V,N,F", [(70, 1, 1, 1), (200, 1, 1, 32), (200, 1, 2, 100), (200, 0, 3, 300), (130, 2, 1, 1433), (90, 1, 1, 8300),
+                                     (262200, 2, 1, 1000), (262200, 1, 2, 1433)])
+def test_product_of_tables_of_few_rows(device, n, V, N, F):
+    """Many rows by id from tables that are shorter than a stage of the product's; ids that the table does not have give zeros."""
+    xw = rows_of(N, F, n + N, special=False)
+    cw, sw, w = table_of(xw, device)
+    ids = np.random.default_rng(n).integers(0, max(V, 1), n).astype(np.uint32)
+    ids[3::7] = 0xFFFFFFFF
+    ids[5::7] = V
+    if V:
+        ca, sa, a = table_of(rows_of(V, F, n + F, special=False), device)
+        x = ref.mx_values(ca, sa, F)
+    else:
+        a = lowbit.MxTable(*(torch.empty(s, dtype=torch.uint8, device=device) for s in lowbit.mx_shapes(0, F)), F)
+        x = np.zeros((0, F))
+    x, wv = np.concatenate([x, np.zeros((1, F))])[np.minimum(ids, V)], ref.mx_values(cw, sw, F)
+    got = lowbit.MxProductOp(dev(ids, device)).forward(a, w)
+    close(got, x @ wv.T, np.abs(x) @ np.abs(wv).T, F)
+    assert not got.cpu().numpy()[ids >= V].any()
+
+
 def test_product_without_ids_is_the_whole_table(device):
     ca, sa, a = table_of(rows_of(130, 96, 1, special=False), device)
     cw, sw, w = table_of(rows_of(50, 96, 2, special=False), device)
