@@ -75,6 +75,25 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t *__restrict__ 
 // l / 16, which are 16 consecutive bytes of the row, and that block's scale.  So the operands go from memory to registers as
 // they lie.  W is the first operand: a lane then ends up with four neighbouring columns of one output row.
 
+// Blocks are handed to the eight chiplets, each with an L2 of its own, in turn.  Where there are kXcdTiles tiles of rows or more, a
+// chiplet takes `group` of them at a time, every column of tiles for all of the group before the next: blocks that run together share
+// rows and columns.  With fewer, tiles in turn fill the chip more evenly.  Product of 232,965 rows of 602 by 256: 79.5 -> 65.5 us, the
+// rows' gradient of 169,343 by 640 by 640: 607 -> 489.
+constexpr uint32_t kXcdTiles = 64;
+__device__ __forceinline__ void tile_of(uint32_t tiles_n, bool by_xcd, uint32_t group, uint32_t *tm, uint32_t *tn) {
+  if (by_xcd) {
+    const uint32_t x = blockIdx.x / 8u, of = group * tiles_n, within = x % of;
+    *tm = (x / of * group + within % group) * 8u + blockIdx.x % 8u;
+    *tn = within / group;
+  } else {
+    *tm = blockIdx.x / tiles_n;
+    *tn = blockIdx.x % tiles_n;
+  }
+}
+uint32_t tile_blocks(uint32_t tiles_m, uint32_t tiles_n, uint32_t group) {
+  return (tiles_m >= kXcdTiles ? ceil_div(tiles_m, 8 * group) * 8u * group : tiles_m) * tiles_n;
+}
+
 struct MxRows {
   const uint8_t *codes;
   const uint8_t *scales;
@@ -213,9 +232,10 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
+constexpr uint32_t kRowGroup = 8;  // 65,536 x 4,096 by 4,096: 718 us; groups of 4: 737, of 2: 752, tiles in turn 737
 // NEAR: both tables' codes are less than 4 GB and are read through buffer descriptors, by 32-bit offsets.
 template <int BM, int BN, int WM, int WN, int PARTS, bool NEAR>
-__global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(ProductArgs p, uint32_t tiles_n) {
+__global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(ProductArgs p, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr int kThreads = WM * WN * kWave, kWaves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
   constexpr int kRows = BM + BN, kBytes = PARTS * 16, kLoadRows = kWave / PARTS, kLoads = kRows / kLoadRows / kWaves;
   constexpr int kScaleRows = (kRows + kThreads - 1) / kThreads, kSpread = 16 / PARTS;
@@ -226,8 +246,10 @@ __global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(Prod
   __shared__ __attribute__((aligned(16))) uint8_t tile0[kRows * kBytes], tile1[kRows * kBytes];
   __shared__ __attribute__((aligned(16))) uint8_t tile_scales[2][kRows * PARTS];
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
-  const uint64_t tm = blockIdx.x / tiles_n;
-  const uint32_t tn = static_cast<uint32_t>(blockIdx.x - tm * tiles_n);
+  uint32_t tile_m, tn;
+  tile_of(tiles_n, tiles_m >= kXcdTiles, kRowGroup, &tile_m, &tn);
+  if (tile_m >= tiles_m) return;
+  const uint64_t tm = tile_m;
   // the row of A's or W's table that row `row` of a stage holds; false: none
   auto table_row = [&](uint32_t row, uint64_t *g) {
     if (row < BM) {
@@ -403,8 +425,9 @@ void launch_tiled(const ProductArgs &p, hipStream_t stream) {
       q.a.scales = p.a.scales + first * p.scale_stride;
       q.table_rows = p.table_rows > first ? static_cast<uint32_t>(p.table_rows - first) : 0u;
     }
-    hipLaunchKernelGGL((mx_product_tiled_kernel<BM, BN, WM, WN, PARTS, NEAR>), dim3(ceil_div(q.n, BM) * tiles_n), dim3(WM * WN * kWave), 0,
-                       stream, q, tiles_n);
+    const uint32_t tiles_m = ceil_div(q.n, BM);
+    hipLaunchKernelGGL((mx_product_tiled_kernel<BM, BN, WM, WN, PARTS, NEAR>), dim3(tile_blocks(tiles_m, tiles_n, kRowGroup)), dim3(WM * WN * kWave), 0,
+                       stream, q, tiles_m, tiles_n);
   }
 }
 
@@ -433,10 +456,18 @@ void launch_product(const ProductArgs &p, hipStream_t stream) {
 // terms of eight bits of fraction each by cutting off bits, which is exact and cannot overflow, so three bf16 products summed
 // in 32 bits keep the accuracy of a 32-bit product.  A block of four wavefronts takes 128 rows of the result by 128
 // columns, 32 terms at a time through LDS, where both operands lie with the terms of a row or column side by side; the next
-// terms are on their way into registers meanwhile.
+// terms are on their way into registers meanwhile.  What that costs is the waits for them, vector instructions (30 % of the
+// time) and LDS; the matrix units are busy for a third.
 // The weight's gradient has few results and many terms: blockIdx.z takes its part of the terms, the parts' sums are added in
 // order by a second launch, so results do not depend on scheduling.
-constexpr uint32_t kGradTile = 128, kGradTerms = 32, kGradPitch = kGradTerms + 8;
+constexpr uint32_t kGradTile = 128, kGradTerms = 32;
+// Where 8 of a row's 32 terms lie: as in the product, so that the 16 lanes that read one part of 16 rows meet all banks once.
+constexpr uint32_t kGradQ = kGradTile * kGradTerms + kGradTile;
+// Q's rows are written 8 apart by neighbouring lanes: 16 bytes more behind every eighth spread those over the banks as well.
+__device__ __forceinline__ uint32_t grad_q_at(uint32_t row, uint32_t part) {
+  return row * kGradTerms + ((row >> 3) + ((part + (row >> 2) - (row >> 3)) & 3u)) * 8u;
+}
+__device__ __forceinline__ uint32_t grad_at(uint32_t row, uint32_t part) { return row * kGradTerms + ((part ^ (row >> 2)) & 3u) * 8u; }
 
 struct GradArgs {
   float *out;        // [M, F], or the parts' sums [parts, M, F]
@@ -445,127 +476,210 @@ struct GradArgs {
   uint32_t q_rows;   // rows of Q's table: an id beyond them names a row of zeros
   const uint32_t *row_ids;
   uint32_t M, R, F, g_stride, row_blocks, scale_stride;
-  uint32_t part_terms;  // terms a part sums (a multiple of kGradTerms)
+  uint32_t part_terms;        // terms a part sums (a multiple of kGradTerms)
+  uint32_t tiles_m, tiles_f;  // of the rows' gradient
   int accumulate;
   bool streamed;  // the output goes past the caches
 };
 
 // x = hi + mid + lo, each the upper half of its word, exactly for finite x; an infinity or NaN goes to hi alone.
-__device__ __forceinline__ void split3(float x, uint32_t *hi, uint32_t *mid, uint32_t *lo) {
+__device__ __forceinline__ void split3(float x, bool finite, uint32_t *hi, uint32_t *mid, uint32_t *lo) {
   const uint32_t b = __float_as_uint(x);
-  const bool fine = (b & 0x7F800000u) != 0x7F800000u;
+  const bool fine = finite || (b & 0x7F800000u) != 0x7F800000u;
   const float rest = fine ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f;
   const float m = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
-  *hi = b | ((b & 0x7FFFFFFFu) > 0x7F800000u ? 0x400000u : 0u);  // a NaN whose upper bits are an infinity's
+  *hi = b | (!finite && (b & 0x7FFFFFFFu) > 0x7F800000u ? 0x400000u : 0u);  // a NaN whose upper bits are an infinity's
   *mid = __float_as_uint(m);
   *lo = __float_as_uint(rest - m);
 }
 // The upper halves of two words.
 __device__ __forceinline__ uint32_t upper_halves(uint32_t first, uint32_t second) { return __builtin_amdgcn_perm(second, first, 0x07060302u); }
 
-template <bool WEIGHT>
-__global__ __launch_bounds__(256, 2) void mx_grad_kernel(GradArgs p) {
-  __shared__ __attribute__((aligned(16))) uint16_t sp[3][kGradTile][kGradPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t sq[kGradTile][kGradPitch];
+// Whole stages load without branches, so that a wait is for the oldest loads alone: rows and columns of the tile that the result does
+// not have read some other of it, ids that the table does not have read its first row and count as zeros.  What is left of the
+// terms is loaded one by one.
+// Weight: two stages of loads are on their way while a third is multiplied (640 by 640 over 169,343 rows: 832 -> 624 us, 128 by 128: 41 ->
+// 33); it has blocks for two on a compute unit anyway.  Rows: one stage, and the registers for three blocks, are better (169,343 by
+// 128 by 128: 38 us against 46).
+template <bool WEIGHT, bool IDS>
+__global__ __launch_bounds__(256, WEIGHT ? 2 : 3) void mx_grad_kernel(GradArgs p) {
+  __shared__ __attribute__((aligned(16))) uint16_t sp0[3][kGradTile * kGradTerms], sp1[3][kGradTile * kGradTerms], sq0[kGradQ], sq1[kGradQ];
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
-  const uint64_t m0 = static_cast<uint64_t>(blockIdx.x) * kGradTile;
-  const uint32_t f0 = blockIdx.y * kGradTile;
+  uint32_t tm = blockIdx.x, tf = blockIdx.y;
+  if (!WEIGHT) {
+    tile_of(p.tiles_f, p.tiles_m >= kXcdTiles, 1, &tm, &tf);
+    if (tm >= p.tiles_m) return;
+  }
+  const uint64_t m0 = static_cast<uint64_t>(tm) * kGradTile;
+  const uint32_t f0 = tf * kGradTile;
   const uint64_t begin = static_cast<uint64_t>(blockIdx.z) * p.part_terms;
   const uint64_t end = min(static_cast<uint64_t>(p.R), begin + p.part_terms);
   // P: a thread takes 16 terms of one row: neighbouring threads have neighbouring rows where those are g's columns, otherwise two
-  // threads share a row.  Q: half of the threads take eight columns of four terms.
-  const uint32_t pm = WEIGHT ? t & 127u : t >> 1, pk = (WEIGHT ? t >> 7 : t & 1u) * 16u;
-  const uint32_t qf = (t & 15u) * 8u, qk = (t >> 4) * 4u;
-  const bool q_mine = t < 128u && f0 + qf < p.F;
-  float g[16];
-  uint32_t word[4], scale[4];
-  auto request = [&](uint64_t k0) {
-    const uint64_t m = m0 + pm;
-    if (k0 + kGradTerms <= end) {  // the same in all threads: no look at every term (weight's gradient of 640 by 640: 1,100 -> 540 us)
+  // threads share a row.  Q: four columns of four terms.
+  const uint32_t pm = WEIGHT ? (wave & 1u) * kWave + lane : t >> 1, pk = WEIGHT ? (wave >> 1) * 16u : (t & 1u) * 16u;
+  const uint32_t qf = (t & 31u) * 4u, qk = (t >> 5) * 4u;
+  const uint32_t m = static_cast<uint32_t>(min(m0 + pm, p.M - 1ull)), col = f0 + qf < p.F ? f0 + qf : 0u;
+  float g[2][16];
+  uint32_t code[2][4], scale[2][4], absent[2], id[4];
+  auto look_up = [&](uint32_t stage, uint32_t *ids) __attribute__((always_inline)) {
+    const uint64_t k0 = begin + static_cast<uint64_t>(stage) * kGradTerms;
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) g[i] = 0.0f;
-      if (m < p.M) {
-        if (WEIGHT) {
-          const float *src = p.g + (k0 + pk) * p.g_stride + m;
+    for (uint32_t i = 0; i < 4; ++i) ids[i] = IDS ? (p.row_ids + k0)[qk + i] : static_cast<uint32_t>(k0) + qk + i;
+  };
+  auto request = [&](uint32_t stage, const uint32_t *ids, int u) __attribute__((always_inline)) {
+    const uint64_t k0 = begin + static_cast<uint64_t>(stage) * kGradTerms;
+    if (WEIGHT) {
 #pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) g[i] = src[static_cast<uint64_t>(i) * p.g_stride];
-        } else {
-          const float *src = p.g + m * p.g_stride + k0 + pk;
-#pragma unroll
-          for (uint32_t i = 0; i < 16; i += 4) {
-            const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src + i);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) g[i + k] = q[k];
-          }
-        }
-      }
+      for (uint32_t i = 0; i < 16; ++i) g[u][i] = (p.g + (k0 + pk + i) * p.g_stride)[m];
     } else {
+      const float *src = p.g + static_cast<uint64_t>(m) * p.g_stride + k0 + pk;
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        const uint64_t k = k0 + pk + i;
-        g[i] = m < p.M && k < end ? p.g[WEIGHT ? k * p.g_stride + m : m * p.g_stride + k] : 0.0f;
+      for (uint32_t i = 0; i < 16; i += 4) {
+        const FloatQuad q = *reinterpret_cast<const FloatQuad *>(src + i);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) g[u][i + k] = q[k];
       }
     }
-    uint32_t id[4];
+    absent[u] = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t row = ids[i] < p.q_rows ? ids[i] : 0u;
+      if (ids[i] >= p.q_rows) absent[u] |= 1u << i;
+      code[u][i] = *reinterpret_cast<const uint16_t *>(p.q.codes + static_cast<uint64_t>(row) * (p.row_blocks * 16u) + col / 2u);
+      scale[u][i] = p.q.scales[static_cast<uint64_t>(row) * p.scale_stride + col / kMxBlock];
+    }
+  };
+  auto request_some = [&](uint64_t k0) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const uint64_t k = k0 + pk + i;
+      g[0][i] = k < end ? p.g[WEIGHT ? k * p.g_stride + m : static_cast<uint64_t>(m) * p.g_stride + k] : 0.0f;
+    }
+    absent[0] = 0;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       const uint64_t k = k0 + qk + i;
-      id[i] = kNoSlot;
-      if (q_mine && k < end) id[i] = WEIGHT && p.row_ids ? p.row_ids[k] : static_cast<uint32_t>(k);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      word[i] = scale[i] = 0;
-      if (id[i] < p.q_rows) {
-        word[i] = *reinterpret_cast<const uint32_t *>(p.q.codes + static_cast<uint64_t>(id[i]) * p.row_blocks * 16u + (f0 + qf) / 2u);
-        scale[i] = p.q.scales[static_cast<uint64_t>(id[i]) * p.scale_stride + (f0 + qf) / kMxBlock];
+      uint32_t row = kNoSlot;
+      if (k < end) row = IDS ? p.row_ids[k] : static_cast<uint32_t>(k);
+      code[0][i] = scale[0][i] = 0;
+      if (row < p.q_rows) {
+        code[0][i] = *reinterpret_cast<const uint16_t *>(p.q.codes + static_cast<uint64_t>(row) * (p.row_blocks * 16u) + col / 2u);
+        scale[0][i] = p.q.scales[static_cast<uint64_t>(row) * p.scale_stride + col / kMxBlock];
       }
     }
   };
-  auto keep = [&]() {
+  auto keep_g = [&](int u, uint16_t (*sp)[kGradTile * kGradTerms], bool finite) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t i = 0; i < 16; i += 8) {
       uint32_t s[3][8];
 #pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) split3(g[i + k], &s[0][k], &s[1][k], &s[2][k]);
+      for (uint32_t k = 0; k < 8; ++k) split3(g[u][i + k], finite, &s[0][k], &s[1][k], &s[2][k]);
 #pragma unroll
       for (int c = 0; c < 3; ++c)
-        *reinterpret_cast<u32x4 *>(&sp[c][pm][pk + i]) = u32x4{upper_halves(s[c][0], s[c][1]), upper_halves(s[c][2], s[c][3]),
+        *reinterpret_cast<u32x4 *>(&sp[c][grad_at(pm, (pk + i) / 8u)]) = u32x4{upper_halves(s[c][0], s[c][1]), upper_halves(s[c][2], s[c][3]),
                                                                upper_halves(s[c][4], s[c][5]), upper_halves(s[c][6], s[c][7])};
     }
-    if (t < 128u) {
-      float v[4][8];
+  };
+  auto keep = [&](int u) __attribute__((always_inline)) {
+    uint16_t(*const sp)[kGradTile * kGradTerms] = u ? sp1 : sp0;
+    uint16_t *const sq = u ? sq1 : sq0;
+    float probe = 0.0f;  // NaN where one of them is an infinity or NaN
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e2m1_decode8(word[i], e8m0_value(scale[i]), v[i]);
+    for (uint32_t i = 0; i < 16; ++i) probe = fmaf(g[u][i], 0.0f, probe);
+    if (probe == 0.0f)
+      keep_g(u, sp, true);
+    else
+      keep_g(u, sp, false);
+    float v[4][4];
 #pragma unroll
-      for (int f = 0; f < 8; ++f)
-        *reinterpret_cast<uint2 *>(&sq[qf + f][qk]) =
-            make_uint2(upper_halves(__float_as_uint(v[0][f]), __float_as_uint(v[1][f])), upper_halves(__float_as_uint(v[2][f]), __float_as_uint(v[3][f])));
+    for (int i = 0; i < 4; ++i) {
+      const bool there = !(absent[u] >> i & 1u);
+      e2m1_decode4(there ? code[u][i] : 0u, there ? e8m0_value(scale[u][i]) : 0.0f, v[i]);
     }
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+      *reinterpret_cast<uint2 *>(&sq[grad_q_at(qf + f, qk / 8u) + qk % 8u]) =
+          make_uint2(upper_halves(__float_as_uint(v[0][f]), __float_as_uint(v[1][f])), upper_halves(__float_as_uint(v[2][f]), __float_as_uint(v[3][f])));
   };
   const uint32_t wm = wave / 2u * 64u, wf = wave % 2u * 64u;
   f32x4 acc[4][4] = {};
-  request(begin);
-  for (uint64_t k0 = begin; k0 < end; k0 += kGradTerms) {
-    keep();
-    __syncthreads();
-    if (k0 + kGradTerms < end) request(k0 + kGradTerms);
+  auto multiply = [&](int u) __attribute__((always_inline)) {
+    uint16_t(*const sp)[kGradTile * kGradTerms] = u ? sp1 : sp0;
+    const uint16_t *const sq = u ? sq1 : sq0;
     bf16x8 q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8 *>(&sq[wf + j * 16 + r][part * 8]);
+    for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8 *>(&sq[grad_q_at(wf + j * 16 + r, part)]);
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int s = 0; s < 3; ++s) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8 *>(&sp[s][wm + m * 16 + r][part * 8]);
+        const bf16x8 a = *reinterpret_cast<const bf16x8 *>(&sp[s][grad_at(wm + i * 16 + r, part)]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[j], a, acc[m][j], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[j], a, acc[i][j], 0, 0, 0);
       }
-    __syncthreads();
+  };
+  // Stages take the halves of LDS in turn, so one barrier a stage is enough: who writes a half has passed the barrier behind its last reads.
+  const uint32_t full = p.q_rows && end > begin ? static_cast<uint32_t>((end - begin) / kGradTerms) : 0u;
+  if (!WEIGHT && full) {
+    uint32_t ids[4];
+    look_up(0, ids);
+    request(0, ids, 0);
+    for (uint32_t s = 0; s < full; ++s) {
+      keep(0);
+      __syncthreads();
+      if (s + 1u < full) {
+        look_up(s + 1u, ids);
+        request(s + 1u, ids, 0);
+      }
+      multiply(0);
+      __syncthreads();
+    }
+  } else if (full) {
+    const uint32_t last = full - 1u;
+    uint32_t id0[4], id1[4];
+    look_up(0, id0);
+    look_up(min(1u, last), id1);
+    look_up(min(2u, last), id);
+    request(0, id0, 0);
+    request(min(1u, last), id1, 1);
+    uint32_t s = 0;
+    auto stage = [&](int u, bool ahead) __attribute__((always_inline)) {
+      keep(u);
+      __syncthreads();
+      if (ahead) {
+        uint32_t next[4];
+        look_up(min(s + 3u, last), next);
+        request(s + 2u, id, u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) id[i] = next[i];
+      }
+      multiply(u);
+      ++s;
+    };
+    while (s + 3u < full) {
+      stage(0, true);
+      stage(1, true);
+    }
+    if (s + 2u < full) {  // three left, two or one
+      stage(0, true);
+      stage(1, false);
+      stage(0, false);
+    } else {
+      stage(0, false);
+      if (s < full) stage(1, false);
+    }
   }
+  for (uint64_t k0 = begin + static_cast<uint64_t>(full) * kGradTerms; k0 < end; k0 += kGradTerms) {
+    request_some(k0);
+    __syncthreads();
+    keep(0);
+    __syncthreads();
+    multiply(0);
+  }
+  __syncthreads();
   // rows of 64 columns through LDS, as the product's
-  f32x4 *const mine = reinterpret_cast<f32x4 *>(&sp[0][0][0]) + wave * 256u;
-  static_assert(sizeof(sp) >= 4 * 256 * sizeof(f32x4), "room for 16 rows of every wavefront");
+  f32x4 *const mine = reinterpret_cast<f32x4 *>(&sp0[0][0]) + wave * 256u;
+  static_assert(sizeof(sp0) >= 4 * 256 * sizeof(f32x4), "room for 16 rows of every wavefront");
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -584,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void mx_grad_kernel(GradArgs p) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) v[c] += old[c];
         }
-          store_quad(dst, FloatQuad{v.x, v.y, v.z, v.w}, p.streamed);
+        store_quad(dst, FloatQuad{v.x, v.y, v.z, v.w}, p.streamed);
       } else {
 #pragma unroll
         for (uint32_t c = 0; c < 3; ++c)
@@ -620,7 +734,7 @@ struct Parts {
   uint32_t count, terms;
 };
 // Parts of the weight's gradient: 512 blocks, two for a compute unit, and none of fewer than 256 terms (169,343 rows of 640 by 640:
-// 0.54 ms with 512; when that took 1.0, 256 took 2.0 and 1,024 took 1.0).
+// 0.62 ms with 512; when that took 1.0, 256 took 2.0 and 1,024 took 1.0).
 Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
   const uint64_t tiles = static_cast<uint64_t>(ceil_div(N, kGradTile)) * ceil_div(F, kGradTile);
   const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(512 / tiles, n / 256));
@@ -683,16 +797,17 @@ int nts_mxfp4_product_grad_rows(float *gx, const float *gout, const uint8_t *w_c
   if (!gx || !gout || !w_codes || !w_scales) return fail(NTS_ERR_INVALID, "nts_mxfp4_product_grad_rows: null pointer");
   if (!table_aligned(w_codes, w_scales))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product_grad_rows: codes need 16-byte, scales 4-byte alignment");
-  const uint32_t terms = ceil_div(N, kGradTerms) * kGradTerms;
-  const GradArgs p{gx, gout, {w_codes, w_scales}, N, nullptr, n, N, F, N, mx_blocks(F), mx_scale_stride(F), terms, accumulate,
+  const uint32_t terms = ceil_div(N, kGradTerms) * kGradTerms, cols = ceil_div(F, kGradTile);
+  const GradArgs p{gx, gout, {w_codes, w_scales}, N, nullptr, n, N, F, N, mx_blocks(F), mx_scale_stride(F), terms, 0u, cols, accumulate,
                    static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes};
   // launches of at most 2^24 - 1 blocks: rows of the result in turns
-  const uint32_t cols = ceil_div(F, kGradTile), turn = kMostBlocks / cols * kGradTile;
+  const uint32_t turn = (kMostBlocks / cols - kXcdTiles) * kGradTile;
   for (uint64_t first = 0; first < n; first += turn) {
     GradArgs q = p;
     q.out = gx + first * F, q.g = gout + first * N;
     q.M = static_cast<uint32_t>(std::min<uint64_t>(turn, n - first));
-    hipLaunchKernelGGL((mx_grad_kernel<false>), dim3(ceil_div(q.M, kGradTile), cols, 1), dim3(256), 0, stream, q);
+    q.tiles_m = ceil_div(q.M, kGradTile);
+    hipLaunchKernelGGL((mx_grad_kernel<false, false>), dim3(tile_blocks(q.tiles_m, cols, 1)), dim3(256), 0, stream, q);
     NTS_LAUNCH_CHECK("nts_mxfp4_product_grad_rows");
   }
   return NTS_OK;
@@ -717,10 +832,10 @@ int nts_mxfp4_product_grad_weight(float *gw, const float *gout, const uint8_t *c
   const Parts parts = weight_parts(n, N, F);
   if (parts.count > 1 && (!work || !aligned_to(work, 16)))
     return fail(NTS_ERR_INVALID, "nts_mxfp4_product_grad_weight: needs nts_mxfp4_product_grad_weight_work_bytes of 16-byte-aligned work");
-  GradArgs p{gw, gout, {codes, scales}, table_rows, row_ids, N, n, F, N, mx_blocks(F), mx_scale_stride(F), parts.terms, accumulate, false};
+  GradArgs p{gw, gout, {codes, scales}, table_rows, row_ids, N, n, F, N, mx_blocks(F), mx_scale_stride(F), parts.terms, 0u, 0u, accumulate, false};
   if (parts.count > 1) p.out = static_cast<float *>(work), p.accumulate = 0;
-  hipLaunchKernelGGL((mx_grad_kernel<true>), dim3(ceil_div(N, kGradTile), ceil_div(F, kGradTile), parts.count), dim3(256), 0,
-                     stream, p);
+  hipLaunchKernelGGL((row_ids ? mx_grad_kernel<true, true> : mx_grad_kernel<true, false>),
+                     dim3(ceil_div(N, kGradTile), ceil_div(F, kGradTile), parts.count), dim3(256), 0, stream, p);
   NTS_LAUNCH_CHECK("nts_mxfp4_product_grad_weight");
   if (parts.count > 1) {
     const uint64_t count = static_cast<uint64_t>(N) * F;

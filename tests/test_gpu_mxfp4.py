@@ -270,6 +270,24 @@ def test_gradients(device, n, N, F, accumulate):
         close(got, want, scale, 3 * terms + 1100)
 
 
+@pytest.mark.parametrize("n", [32, 63, 96, 128, 160, 193, 600])
+@pytest.mark.parametrize("V", [0, 1, 40, 700])
+def test_gradient_of_the_weight_by_stages(device, n, V):
+    """From one whole stage of rows on, without ids, and from tables that end before the last row."""
+    N, F = 37, 70
+    rng = np.random.default_rng(n + V)
+    g = rng.standard_normal((n, N)).astype(np.float32)
+    x = np.zeros((n, F))
+    if V:
+        ca, sa, a = table_of(rows_of(V, F, V, special=False), device)
+        x[:V] = ref.mx_values(ca, sa, F)[:n]
+    gw, dg = torch.full((N, F), 5.0, device=device), dev(g, device)
+    work = torch.empty(call("nts_mxfp4_product_grad_weight_work_bytes", n, N, F), dtype=torch.uint8, device=device)
+    call("nts_mxfp4_product_grad_weight", ptr(gw), ptr(dg), ptr(a.codes) if V else 0, ptr(a.scales) if V else 0, V, 0, n, N, F, 0,
+         ptr(work) if work.numel() else 0, stream())
+    close(gw, g.astype(np.float64).T @ x, np.abs(g).astype(np.float64).T @ np.abs(x), 3 * n + 1100)
+
+
 def test_gradients_are_the_products_differences(device):
     """The product is linear in each table's values: <g, y(A, W) - y(A, W')> = <gw, W - W'>, and alike for the rows."""
     n, N, F = 300, 40, 100
