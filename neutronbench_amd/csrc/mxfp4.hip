@@ -206,7 +206,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void mx_product_few_kernel(Produc
 // Measured (65,536 rows of 4,096 values by 4,096 columns): 693 us, 3.2 PFLOP/s, where a library's bf16 product of that size
 // takes 1,599.  Without loads and stores 411 us, with the stores 493, with the loads 686: bound by the loads of codes into LDS and the
 // waits for them.  Steps: registers in place of loads into LDS 1,170; stores past the caches 1,043 -> 900; operands asked for a step
-// ahead 893 -> 785; results turned in LDS and stored as whole lines 785 -> 693.  128 x 128 with stages of 64 bytes takes 933.
+// ahead 893 -> 785; results turned in LDS and stored as whole lines 785 -> 693.  128 x 128 with stages of 64 bytes takes 912.
 typedef __attribute__((address_space(3))) void *LdsPointer;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00027000);
@@ -442,9 +442,10 @@ void launch_product(const ProductArgs &p, hipStream_t stream) {
   }
   const uint64_t row_bytes = p.row_blocks * 16ull;
   if (std::max(p.table_rows, p.N) * row_bytes >= 0xFFFF0000ull) return launch_tiled<128, 128, 2, 2, 4, false>(p, stream);
-  // The larger tile where there are enough of them to fill the chip a few times and rows are long: 65,536 rows of 4,096 by 4,096
-  // columns 718 us against 933; 65,536 of 1,024 by 1,024: 85 against 90; 232,965 of 602 by 256: 86 against 79.
-  if (p.row_blocks >= 32 && static_cast<uint64_t>(ceil_div(p.n, 256)) * ceil_div(p.N, 256) >= 1024)
+  // The larger tile where there are enough of them to fill the chip twice and rows are long: 65,536 rows of 4,096 by 4,096 columns
+  // 715 us against 912; 8,192 of 2,048 by 4,096: 61.5 against 64; but 65,536 of 1,024 by 1,024: 81 against 75; 232,965 of 602 by
+  // 256: 86 against 66.
+  if (p.row_blocks >= 64 && static_cast<uint64_t>(ceil_div(p.n, 256)) * ceil_div(p.N, 256) >= 512)
     return launch_tiled<256, 256, 2, 4, 8, true>(p, stream);
   launch_tiled<128, 128, 2, 2, 4, true>(p, stream);
 }

@@ -170,7 +170,7 @@ def test_product(device, n, N, F, accumulate):
     assert (out[n:] == 3.0).all()
 
 
-@pytest.mark.parametrize("n,N,F,accumulate", [(66001, 1030, 1001, 0), (65600, 1024, 1056, 1), (40000, 1793, 2048, 0)])
+@pytest.mark.parametrize("n,N,F,accumulate", [(66001, 1030, 1001, 0), (65600, 1024, 1056, 1), (40000, 1793, 2048, 0), (20100, 1797, 2100, 1)])
 def test_product_in_the_larger_tiles(device, n, N, F, accumulate):
     """Against 64-bit products on the device, whose operands torch reads from the same rows."""
     V = 300
@@ -192,7 +192,7 @@ def test_product_in_the_larger_tiles(device, n, N, F, accumulate):
 
 
 @pytest.mark.parametrize("n,V,N,F", [(70, 1, 1, 1), (200, 1, 1, 32), (200, 1, 2, 100), (200, 0, 3, 300), (130, 2, 1, 1433), (90, 1, 1, 8300),
-                                     (262200, 2, 1, 1000), (262200, 1, 2, 1433)])
+                                     (262200, 2, 1, 1000), (131100, 1, 2, 2100)])
 def test_product_of_tables_of_few_rows(device, n, V, N, F):
     """Many rows by id from tables that are shorter than a stage of the product's; ids that the table does not have give zeros."""
     xw = rows_of(N, F, n + N, special=False)
