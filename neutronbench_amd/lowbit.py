@@ -75,19 +75,24 @@ class MxTable:
         _bytes(codes, code_shape, "codes")
         _bytes(scales, scale_shape, "scales")
         _same_device(codes.device, scales)
-        self.codes, self.scales, self.rows, self.width, self.device = codes, scales, codes.shape[0], width, codes.device
+        self._hold(codes, scales, codes.shape[0], width, codes.device)
+
+    def _hold(self, codes, scales, rows, width, device):
+        self.codes, self.scales, self.rows, self.width, self.device = codes, scales, rows, width, device
 
     @classmethod
     def quantize(cls, x):
         """The rows of x [n, width] rounded to the nearest values their blocks can hold."""
         _floats(x, None, "x")
-        n, width = x.shape
+        (n, width), dev = x.shape, x.device
         code_shape, scale_shape = mx_shapes(n, width)
-        codes = allocate(torch.empty, code_shape, dtype=torch.uint8, device=x.device)
-        scales = allocate(torch.empty, scale_shape, dtype=torch.uint8, device=x.device)
-        with _on(x.device):
-            call("nts_mxfp4_quantize", ptr(codes), ptr(scales), ptr(x), n, width, _stream(x.device))
-        return cls(codes, scales, width)
+        codes = allocate(torch.empty, code_shape, dtype=torch.uint8, device=dev)
+        scales = allocate(torch.empty, scale_shape, dtype=torch.uint8, device=dev)
+        with _on(dev):
+            call("nts_mxfp4_quantize", ptr(codes), ptr(scales), ptr(x), n, width, _stream(dev))
+        self = cls.__new__(cls)  # its own arrays need no checks
+        self._hold(codes, scales, n, width, dev)
+        return self
 
     def gather(self, row_ids=None, out=None):
         """The rows as floats: all of them, or those that row_ids names (an id beyond the table: zeros)."""
