@@ -167,17 +167,15 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// What the registers allow, measured: with one query head to a lane four edges at a time and four wavefronts to a SIMD (2.48 M edges, 8
-// query heads of 64: 468 us at the time; three wavefronts 507, two edges 600); with two, two edges and three wavefronts (500 K edges, 16
-// query heads of 128: 233 us; four edges 255, one head to a lane 259).  Four heads to a lane leave one wavefront.
+// What the registers allow, measured: with one query head to a lane four wavefronts to a SIMD (2.48 M edges, 8 query heads of 64: 468 us at
+// the time; three 507, two edges at a time 600); with two, two wavefronts (500 K edges, 16 query heads of 128: 205 us; three and two
+// edges at a time 227, one head to a lane 259; but 2.48 M ragged edges 1,355 against 1,330).  Four heads to a lane leave one.
 template <int G>
-constexpr int kAheadOf = G == 1 ? 4 : 2;
-template <int G>
-constexpr int kWavesOf = G == 1 ? 4 : 3;
+constexpr int kWavesOf = G == 1 ? 4 : 2;
 
 // NEAR: cache and scales of less than 4 GB each and of at most 2^24 rows are read through buffer descriptors: 32-bit offsets from
 // 24-bit products, and a row that is not there gets an offset beyond the end, which reads zeros without a branch.
-template <int ND, int G, bool NEAR>
+template <int ND, int G, bool NEAR, int AHEAD = 4>
 struct Attend {
   const AttendArgs &p;
   uint32_t dl, kv_head, q_head0, slot, rounds;
@@ -247,8 +245,8 @@ struct Attend {
     return j < j1 ? r : 0xFFFFFFFFu;
   }
 
-  // Edges of a slot whose rows are requested together.
-  static constexpr int kAhead = kAheadOf<G>;
+  // Edges of a slot whose rows are requested together: AHEAD, 2 or 4.
+  static constexpr int kAhead = AHEAD;
   template <int U>
   __device__ __forceinline__ void step(const uint32_t *row) {
     u32x4 kc[U], vc[U];
@@ -455,7 +453,7 @@ __global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(At
   const uint32_t row = blockIdx.x / p.passes, pass = blockIdx.x - row * p.passes, wave = wave_of_block();
   const uint32_t hw = 1u << p.hw_shift, first = p.co[row], degree = p.co[row + 1] - first;
   {
-    Attend<ND, G, NEAR> a(p, pass);
+    Attend<ND, G, NEAR, G == 1 ? 4 : 2> a(p, pass);  // what 128 registers hold
     a.lane_edge += wave * a.edge_step;
     a.edge_step *= kBlockWaves;
     a.begin(row);
