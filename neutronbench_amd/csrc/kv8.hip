@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // value row serve them.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by side, and further edges of the
 // destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
 // one destination are a walker; a wavefront is one walker or, where rows are short, several.
-// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 413 us, of which 385 in the walkers, that is 1.3 GB of rows, queries
-// and results at 3.4 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
+// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 392 us, of which 362 in the walkers, that is 1.3 GB of rows, queries
+// and results at 3.7 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
 // convert and multiply 16 columns of a key and a value, about as many again to look up, scale, rescale, join and write.
 struct AttendArgs {
   float *out, *lse;

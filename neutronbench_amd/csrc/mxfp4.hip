@@ -203,10 +203,11 @@ __global__ __launch_bounds__(kFewWaves *kWave) void mx_product_few_kernel(Produc
 // or 128 bytes a row.  The loads write a stage to LDS themselves (no registers between) while the one before it is
 // multiplied.  Part c of row r lies at c ^ (r * PARTS / 16) % PARTS, so that the 16 lanes that read one part of 16 rows meet all
 // banks once.
-// Measured (65,536 rows of 4,096 values by 4,096 columns): 693 us, 3.2 PFLOP/s, where a library's bf16 product of that size
+// Measured (65,536 rows of 4,096 values by 4,096 columns): 684 us, 3.2 PFLOP/s, where a library's bf16 product of that size
 // takes 1,599.  Without loads and stores 411 us, with the stores 493, with the loads 686: bound by the loads of codes into LDS and the
 // waits for them.  Steps: registers in place of loads into LDS 1,170; stores past the caches 1,043 -> 900; operands asked for a step
-// ahead 893 -> 785; results turned in LDS and stored as whole lines 785 -> 693.  128 x 128 with stages of 64 bytes takes 912.
+// ahead 893 -> 785; results turned in LDS and stored as whole lines
+// 785 -> 693.  128 x 128 with stages of 64 bytes takes 912.
 typedef __attribute__((address_space(3))) void *LdsPointer;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00027000);
