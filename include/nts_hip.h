@@ -549,8 +549,8 @@ int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float 
  *   s[e, h]     = score_scale * < q[d, h, :], K[row(e), h', :] >       e in CSC(d), h' = h / (q_heads / heads)
  *   out[d, h, :] = sum_e softmax_e(s[e, h]) * V[row(e), h', :],   lse[d, h] = log sum_e exp(s[e, h])
  * row(e) = ri[e], or mirror[ri[e]] (a sampled layer's `source`, whose row_indices are local).  An edge whose row is not
- * below cache_rows counts for nothing (a neighbour that is not cached); a destination without any other edge gets
- * out = 0 and lse = -infinity.  q, out: [Vd, q_heads * width], lse [Vd, q_heads] or NULL; q_heads a multiple of heads.
+ * below cache_rows counts for nothing (a neighbour that is not cached); a destination without any other edge, or
+ * all of whose scores are -infinity, gets out = 0 and lse = -infinity.  q, out: [Vd, q_heads * width], lse [Vd, q_heads] or NULL; q_heads a multiple of heads.
  * `edges` = co[Vd] - co[0], at most 2^32 - 2^16.  max_degree: the caller's bound on a destination's edges, 0 = none known;
  * it only selects the launches (one, or where rows may be long and are many, two: long rows are cut and their parts joined
  * in order).  The same bits on every call.  `work`: nts_kv8_attention_work_bytes(...) bytes (0: none) of 16-byte-aligned

@@ -1,5 +1,7 @@
 """The cache of 8-bit keys and values and the attention over it against plain implementations in 64 bits: the cache's bytes
 are exact, the attention's tolerance is derived in lowbit_ref.attention."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -181,6 +183,27 @@ def test_a_nan_key_reaches_its_destinations_alone(device):
         nan = torch.isnan(out.view(Vd, heads, D)).cpu()
         assert nan[0, 0].all() and not nan[0, 1].any() and not nan[1:].any()
         assert torch.isnan(op.lse[0, 0]) and torch.isfinite(op.lse[1:3]).all()
+
+
+@pytest.mark.parametrize("Vd,bound", [(3, 0), (3, 8), (80, 0)])
+def test_scores_of_minus_infinity(device, Vd, bound):
+    """A destination all of whose scores are -infinity is one without neighbours; +infinity is NaN, in its head alone."""
+    heads, D, V = 2, 16, 32
+    cache, scales = empty(V, heads, D, 4)
+    ref.kv8_append(cache, scales, np.ones((V, heads * D), dtype=np.float32), keys(V, heads * D, 2), 0, D, 4)
+    layer = SampledLayer()
+    layer.v_size, layer.e_size, layer.max_in_degree = Vd, 8, bound
+    layer.dev_column_offset = dev(np.array([0, 3, 6] + [8] * (Vd - 2), dtype=np.uint32), device)
+    layer.dev_row_indices = dev(np.array([1, 9, 2, 3, 4, 5, 8, 10], dtype=np.uint32), device)
+    q = torch.ones(Vd, heads * D, device=device)
+    q[0, 3], q[1, D + 2] = -math.inf, math.inf
+    op = lowbit.NeighborAttentionOp(layer, heads)
+    out = op.forward(q, lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, 4)).view(Vd, heads, D).cpu()
+    lse = op.lse.cpu()
+    assert (out[0, 0] == 0).all() and lse[0, 0] == -math.inf
+    assert torch.isnan(out[1, 1]).all()
+    assert torch.isfinite(out[0, 1]).all() and torch.isfinite(out[1, 0]).all() and torch.isfinite(out[2]).all()
+    assert torch.isfinite(lse[0, 1]) and torch.isfinite(lse[1, 0]) and torch.isfinite(lse[2]).all()
 
 
 def test_without_the_logarithms_and_beyond_the_rows(device):
