@@ -7,6 +7,7 @@ import torch
 
 from .abi import SampledLayerDesc, allocate, call, ptr
 from .layout import SampledLayer, as_u32
+from .lowbit import _floats, _indices, _same_device
 from .stream import CudaStream
 
 
@@ -83,7 +84,15 @@ def load_feature_gpu_cache(cs, layer0, local_feature, table_ptr, cache, source_c
 
 
 def load_feature_mxfp4(cs, layer0, local_feature, table):
-    """X0[i,:] = feature[source[i],:] from a table held in 4 bits (lowbit.MxTable), as floats."""
+    """X0[i,:] = feature[source[i],:] from a table held in 4 bits (lowbit.MxTable), as floats.  local_feature has table.width
+    columns and src_size rows or more; those behind src_size stay as they were."""
+    _floats(local_feature, table.width, "local_feature")
+    if local_feature.shape[0] < layer0.src_size:
+        raise ValueError(f"local_feature: {layer0.src_size} rows")
+    _indices(layer0.dev_source, "dev_source")
+    if layer0.dev_source.numel() < layer0.src_size:
+        raise ValueError(f"layer: {layer0.src_size} sources")
+    _same_device(table.device, local_feature, layer0.dev_source)
     call("nts_gather_rows_mxfp4", ptr(local_feature), ptr(table.codes), ptr(table.scales), table.rows,
          ptr(layer0.dev_source), layer0.src_size, table.width, cs.stream)
     cs._end_of_method()

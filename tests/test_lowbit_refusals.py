@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import lowbit_ref as ref
-from neutronbench_amd import abi, lowbit
+from neutronbench_amd import abi, batch, lowbit
 from neutronbench_amd.layout import SampledLayer
 
 P = 4096  # stands for a device pointer with any alignment that is asked for: refused calls never follow it
@@ -163,6 +163,21 @@ def test_python_objects_check_their_operands():
     for q_heads, q in ((6, torch.zeros(5, 120)), (6, torch.zeros(4, 100)), (4, torch.zeros(4, 80))):
         with pytest.raises(ValueError):
             lowbit.NeighborAttentionOp(layer, q_heads).forward(q, kv)
+
+
+def test_a_batchs_rows_need_an_output_of_their_size():
+    """load_feature_mxfp4 against outputs that are too narrow, too wide, too short, of another type or strided, and layers whose
+    id array is shorter than they say."""
+    layer = SampledLayer()
+    layer.src_size, layer.dev_source = 4, torch.zeros(4, dtype=torch.int32)
+    good = torch.zeros(4, 100)
+    for bad in (good[:, :96], torch.zeros(4, 104), good[:3], good.double(), torch.zeros(100, 4).t(), torch.zeros(400)):
+        with pytest.raises(ValueError):
+            batch.load_feature_mxfp4(None, layer, bad, table(6, 100))
+    for ids in (torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int64), torch.zeros(8, dtype=torch.int32)[::2]):
+        layer.dev_source = ids
+        with pytest.raises(ValueError):
+            batch.load_feature_mxfp4(None, layer, good, table(6, 100))
 
 
 def test_reference_rounding():
