@@ -548,8 +548,9 @@ int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float 
 /* Every destination's attention over its neighbours' rows of the cache:
  *   s[e, h]     = score_scale * < q[d, h, :], K[row(e), h', :] >       e in CSC(d), h' = h / (q_heads / heads)
  *   out[d, h, :] = sum_e softmax_e(s[e, h]) * V[row(e), h', :],   lse[d, h] = log sum_e exp(s[e, h])
- * row(e) = ri[e], or mirror[ri[e]] (a sampled layer's `source`, whose row_indices are local).  An edge whose row is not
- * below cache_rows counts for nothing (a neighbour that is not cached); a destination without any other edge, or
+ * row(e) = ri[e], or mirror[ri[e]] (a sampled layer's `source`, whose row_indices are local; mirror then has an entry at
+ * least, and ri[e] is below their number or 0xFFFFFFFF, an edge without a row).  An edge without a row, or whose row is not
+ * below cache_rows, counts for nothing (a neighbour that is not cached); a destination without any other edge, or
  * all of whose scores are -infinity, gets out = 0 and lse = -infinity.  q, out: [Vd, q_heads * width], lse [Vd, q_heads] or NULL; q_heads a multiple of heads.
  * `edges` = co[Vd] - co[0], at most 2^32 - 2^16.  max_degree: the caller's bound on a destination's edges, 0 = none known;
  * it only selects the launches (one, or where rows may be long and are many, two: long rows are cut and their parts joined
@@ -560,6 +561,11 @@ int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cac
                       const uint32_t *ri, const uint32_t *mirror, uint32_t Vd, uint32_t edges, uint32_t cache_rows,
                       uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows, float score_scale,
                       uint32_t max_degree, void *work, nts_stream_t stream);
+/* The same by a mirror whose length is known: an edge whose ri[e] is not below mirror_rows has no row, whatever the id. */
+int nts_kv8_attention_local(float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
+                            const uint32_t *ri, const uint32_t *mirror, uint32_t mirror_rows, uint32_t Vd, uint32_t edges,
+                            uint32_t cache_rows, uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows,
+                            float score_scale, uint32_t max_degree, void *work, nts_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Sampled-layer index construction on the device (sampCSC, core/coocsc.hpp)

@@ -103,6 +103,8 @@ SIGNATURES = {
     "nts_kv8_attention_work_bytes": [_u32, _u32, _u32, _u32, _u32],
     "nts_kv8_attention": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32, _u32, _vp,
                           _vp],
+    "nts_kv8_attention_local": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32, _u32,
+                                _vp, _vp],
     "nts_sample_hop_work_bytes": [_u32],
     "nts_sample_hop_offsets": [_vp, _vp, _vp, _u32, ctypes.c_int32, _vp, _vp],
     "nts_sample_hop_neighbors": [_vp, _vp, _vp, _vp, _vp, _u32, ctypes.c_int32, ctypes.c_uint64, _vp],

@@ -137,6 +137,7 @@ struct AttendArgs {
   const float *q;
   const uint8_t *cache, *scales;
   const uint32_t *co, *ri, *mirror;
+  uint32_t mirror_rows;  // entries of mirror: an id beyond them names no row
   uint32_t Vd, cache_rows, q_heads, heads, D, row_width, block_shift;
   uint32_t share;             // query heads per head of the cache
   uint32_t units, per_head;   // units in all and of a head
@@ -241,8 +242,14 @@ struct Attend {
   // The cache row of edge j, or a row that no cache has for an edge behind the last.
   __device__ __forceinline__ uint32_t cache_row(const uint32_t *ids, uint32_t j, uint32_t j1) const {
     uint32_t r = ids[min(j, j1 - 1u)];
-    if (p.mirror) r = p.mirror[r];
-    return j < j1 ? r : 0xFFFFFFFFu;
+    bool there = j < j1;
+    if (p.mirror) {
+      // Without a branch: an id beyond the mirror reads its first entry (20,000 rows of 25 edges, 16 query heads on 4 of 128: 212 us;
+      // with one 240, without a look at the length 208).
+      there = there && r < p.mirror_rows;
+      r = p.mirror[there ? r : 0u];
+    }
+    return there ? r : 0xFFFFFFFFu;
   }
 
   // Edges of a slot whose rows are requested together: AHEAD, 2 or 4.
@@ -729,6 +736,42 @@ int fail_in(const char *call, const char *why) {
   return fail(NTS_ERR_INVALID, text);
 }
 
+int attend(const char *call, float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
+           const uint32_t *ri, const uint32_t *mirror, uint32_t mirror_rows, uint32_t Vd, uint32_t edges, uint32_t cache_rows,
+           uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows, float score_scale, uint32_t max_degree, void *work,
+           hipStream_t stream) {
+  if (const char *why = bad_cache(cache, heads, width, block_rows)) return fail_in(call, why);
+  if (q_heads == 0 || q_heads % heads || q_heads > kMostHeads) return fail_in(call, "q_heads is no multiple of heads up to 1,024");
+  if (edges > 0xFFFF0000u) return fail_in(call, "more than 2^32 - 2^16 edges");
+  if (Vd == 0) return NTS_OK;
+  if (!out || !q || !co || (edges && !ri) || (edges && cache_rows && (!cache || !scales))) return fail_in(call, "null pointer");
+  AttendArgs p{};
+  p.out = out, p.lse = lse, p.q = q, p.cache = cache, p.scales = scales, p.co = co, p.ri = ri, p.mirror = mirror;
+  p.mirror_rows = mirror_rows;
+  p.Vd = Vd, p.cache_rows = cache_rows, p.q_heads = q_heads, p.heads = heads, p.D = width, p.row_width = kv8_row_width(width);
+  p.block_shift = static_cast<uint32_t>(__builtin_ctz(block_rows));
+  p.share = q_heads / heads;
+  p.score_scale = score_scale;
+  // Slots: where a bound is known most rows reach it, and a slot that works through 16 edges costs least (60,000 rows of 10
+  // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four); averages hide longer rows (2.48 M edges in 169 K rows:
+  // 229 us with four slots for 15 edges on average, 264 with two, 572 with one).
+  const bool blocks = by_blocks(Vd, edges, max_degree), spans = by_spans(Vd, edges, max_degree);
+  const Lanes l = lanes_for(q_heads, heads, width, blocks ? kWave : spans ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
+  p.units = l.units, p.per_head = l.per_head, p.hw_shift = l.hw_shift, p.walker_shift = l.walker_shift;
+  p.passes = ceil_div(l.units, 1u << l.hw_shift);
+  p.blocks = blocks;
+  if (spans) {
+    if (!work || !aligned_to(work, 16)) return fail_in(call, "needs nts_kv8_attention_work_bytes of 16-byte-aligned work");
+    p.positions = static_cast<uint64_t>(Vd) * kRowCost + edges;
+    p.span = span_length(p.positions, q_heads, width);
+    p.spans = static_cast<uint32_t>((p.positions + p.span - 1) / p.span);
+    p.partial = static_cast<float *>(work);
+    p.tail_row = reinterpret_cast<uint32_t *>(p.partial + static_cast<uint64_t>(p.spans) * 2u * q_heads * (width + 2u));
+  }
+  const uint64_t bytes = 2ull * heads * std::max(static_cast<uint64_t>(cache_rows) * p.row_width, static_cast<uint64_t>(cache_rows) / block_rows + 1);
+  return bytes < 0xFFFF0000ull && cache_rows <= (1u << 24) ? launch_attend_nd<true>(p, l, stream) : launch_attend_nd<false>(p, l, stream);
+}
+
 }  // namespace
 }  // namespace nts
 
@@ -764,37 +807,20 @@ int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cac
                       const uint32_t *ri, const uint32_t *mirror, uint32_t Vd, uint32_t edges, uint32_t cache_rows,
                       uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows, float score_scale,
                       uint32_t max_degree, void *work, nts_stream_t stream) {
-  const char *const call = "nts_kv8_attention";
   NTS_TRACE_RANGE("nts_kv8_attention");
-  if (const char *why = bad_cache(cache, heads, width, block_rows)) return fail_in(call, why);
-  if (q_heads == 0 || q_heads % heads || q_heads > kMostHeads) return fail_in(call, "q_heads is no multiple of heads up to 1,024");
-  if (edges > 0xFFFF0000u) return fail_in(call, "more than 2^32 - 2^16 edges");
-  if (Vd == 0) return NTS_OK;
-  if (!out || !q || !co || (edges && !ri) || (edges && cache_rows && (!cache || !scales))) return fail_in(call, "null pointer");
-  AttendArgs p{};
-  p.out = out, p.lse = lse, p.q = q, p.cache = cache, p.scales = scales, p.co = co, p.ri = ri, p.mirror = mirror;
-  p.Vd = Vd, p.cache_rows = cache_rows, p.q_heads = q_heads, p.heads = heads, p.D = width, p.row_width = kv8_row_width(width);
-  p.block_shift = static_cast<uint32_t>(__builtin_ctz(block_rows));
-  p.share = q_heads / heads;
-  p.score_scale = score_scale;
-  // Slots: where a bound is known most rows reach it, and a slot that works through 16 edges costs least (60,000 rows of 10
-  // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four); averages hide longer rows (2.48 M edges in 169 K rows:
-  // 229 us with four slots for 15 edges on average, 264 with two, 572 with one).
-  const bool blocks = by_blocks(Vd, edges, max_degree), spans = by_spans(Vd, edges, max_degree);
-  const Lanes l = lanes_for(q_heads, heads, width, blocks ? kWave : spans ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
-  p.units = l.units, p.per_head = l.per_head, p.hw_shift = l.hw_shift, p.walker_shift = l.walker_shift;
-  p.passes = ceil_div(l.units, 1u << l.hw_shift);
-  p.blocks = blocks;
-  if (spans) {
-    if (!work || !aligned_to(work, 16)) return fail_in(call, "needs nts_kv8_attention_work_bytes of 16-byte-aligned work");
-    p.positions = static_cast<uint64_t>(Vd) * kRowCost + edges;
-    p.span = span_length(p.positions, q_heads, width);
-    p.spans = static_cast<uint32_t>((p.positions + p.span - 1) / p.span);
-    p.partial = static_cast<float *>(work);
-    p.tail_row = reinterpret_cast<uint32_t *>(p.partial + static_cast<uint64_t>(p.spans) * 2u * q_heads * (width + 2u));
-  }
-  const uint64_t bytes = 2ull * heads * std::max(static_cast<uint64_t>(cache_rows) * p.row_width, static_cast<uint64_t>(cache_rows) / block_rows + 1);
-  return bytes < 0xFFFF0000ull && cache_rows <= (1u << 24) ? launch_attend_nd<true>(p, l, stream) : launch_attend_nd<false>(p, l, stream);
+  return attend("nts_kv8_attention", out, lse, q, cache, scales, co, ri, mirror, 0xFFFFFFFFu, Vd, edges, cache_rows, q_heads, heads,
+                width, block_rows, score_scale, max_degree, work, stream);
+}
+
+int nts_kv8_attention_local(float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
+                            const uint32_t *ri, const uint32_t *mirror, uint32_t mirror_rows, uint32_t Vd, uint32_t edges,
+                            uint32_t cache_rows, uint32_t q_heads, uint32_t heads, uint32_t width, uint32_t block_rows,
+                            float score_scale, uint32_t max_degree, void *work, nts_stream_t stream) {
+  NTS_TRACE_RANGE("nts_kv8_attention_local");
+  if (mirror_rows && !mirror) return fail_in("nts_kv8_attention_local", "null pointer");
+  // a mirror without entries names no row of the cache, like a cache without rows
+  return attend("nts_kv8_attention_local", out, lse, q, cache, scales, co, ri, mirror_rows ? mirror : nullptr, mirror_rows, Vd, edges,
+                mirror_rows ? cache_rows : 0u, q_heads, heads, width, block_rows, score_scale, max_degree, work, stream);
 }
 
 }  // extern "C"

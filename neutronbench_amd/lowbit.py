@@ -218,7 +218,7 @@ class NeighborAttentionOp:
 
     def forward(self, q, cache, mirror=None):
         """mirror: the cache row of every local source (a sampled layer's dev_source where the cache holds all vertices);
-        None: row_indices name cache rows.  Rows that the cache does not hold are left out."""
+        None: row_indices name cache rows.  Sources beyond mirror and rows that the cache does not hold are left out."""
         sg, H, D, dev = self.sg, self.q_heads, cache.width, cache.device
         _floats(q, H * D, "q")
         if q.shape[0] != sg.v_size or H % cache.heads:
@@ -238,8 +238,12 @@ class NeighborAttentionOp:
         with _on(dev):
             size = call("nts_kv8_attention_work_bytes", sg.v_size, sg.e_size, H, D, bound)
             work = allocate(torch.empty, size, dtype=torch.uint8, device=dev) if size else None
-            call("nts_kv8_attention", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(co),
-                 ptr(ri), ptr(mirror), sg.v_size, sg.e_size, cache.rows, H, cache.heads, D, cache.block_rows, scale,
-                 bound, ptr(work), _stream(dev))
+            if mirror is None:
+                call("nts_kv8_attention", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(co), ptr(ri), 0,
+                     sg.v_size, sg.e_size, cache.rows, H, cache.heads, D, cache.block_rows, scale, bound, ptr(work), _stream(dev))
+            else:
+                call("nts_kv8_attention_local", ptr(out), ptr(lse), ptr(q), ptr(cache.cache), ptr(cache.scales), ptr(co), ptr(ri),
+                     ptr(mirror), mirror.numel(), sg.v_size, sg.e_size, cache.rows, H, cache.heads, D, cache.block_rows, scale,
+                     bound, ptr(work), _stream(dev))
         self.lse = lse
         return out

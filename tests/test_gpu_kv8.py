@@ -159,6 +159,44 @@ def test_offsets_that_do_not_begin_at_zero_and_local_sources(device):
     check(device, [5, 0, 7, 25, 2], 200, 8, 2, 64, 16, mirrored=True, missing=0.2, bound=25)
 
 
+@pytest.mark.parametrize("degrees,bound", [([3, 0, 40, 1], 0), ([3, 0, 4, 9, 16], 16), ([3, 0, 5, 700, 1] * 20, 0)])
+@pytest.mark.parametrize("known", [True, False])
+def test_local_sources_beyond_the_mirror(device, degrees, bound, known):
+    """A block a destination, a walker a row, and spans: sources that the mirror does not have count for nothing.  Where its length is
+    not passed that is 0xFFFFFFFF alone."""
+    Vd, V, heads, D, n_local = len(degrees), 90, 2, 32, 37
+    rng = np.random.default_rng(8)
+    cache, scales = empty(V, heads, D, 16)
+    ref.kv8_append(cache, scales, keys(V, heads * D, 1), keys(V, heads * D, 2), 0, D, 16)
+    co, ri = graph_of(np.array(degrees), n_local, 4)
+    ri[::3] = 0xFFFFFFFF
+    if known:
+        ri[1::7], ri[2::11] = n_local, 0x80000000
+    mirror = rng.permutation(V)[:n_local].astype(np.uint32)
+    row = np.where(ri < n_local, mirror[np.minimum(ri, n_local - 1)], np.uint32(0xFFFFFFFF))
+    q = rng.standard_normal((Vd, heads * D)).astype(np.float32)
+    want, lse, tol, ltol = ref.attention(q, ref.kv8_values(cache, scales, D, 16), co.astype(np.int64), row, V, heads, 0.125)
+    layer = SampledLayer()
+    layer.v_size, layer.e_size, layer.max_in_degree = Vd, ri.size, bound
+    layer.dev_column_offset, layer.dev_row_indices = dev(co, device), dev(ri, device)
+    kv, dq, dm = lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, 16), dev(q, device), dev(mirror, device)
+    if known:
+        op = lowbit.NeighborAttentionOp(layer, heads, 0.125)
+        out, glse = op.forward(dq, kv, dm), op.lse
+        none = op.forward(dq, kv, dm[:0])
+        assert not none.any() and (op.lse == -math.inf).all()
+    else:
+        out, glse = torch.empty(Vd, heads * D, device=device), torch.empty(Vd, heads, device=device)
+        size = call("nts_kv8_attention_work_bytes", Vd, ri.size, heads, D, bound)
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        call("nts_kv8_attention", ptr(out), ptr(glse), ptr(dq), ptr(kv.cache), ptr(kv.scales), ptr(layer.dev_column_offset),
+             ptr(layer.dev_row_indices), ptr(dm), Vd, ri.size, V, heads, heads, D, 16, 0.125, bound, ptr(work), stream())
+    out, glse = out.cpu().numpy(), glse.cpu().numpy()
+    some = np.isfinite(lse)
+    assert (np.abs(out - want) <= tol).all() and (np.isfinite(glse) == some).all()
+    assert (np.abs(glse[some] - lse[some]) <= ltol[some]).all()
+
+
 def test_peaked_and_flat_scores(device):
     """Scores of several hundred (one neighbour takes all) and all equal (a scale of 0)."""
     check(device, [30, 700, 1, 5], 300, 4, 2, 32, 16, spread=40.0)

@@ -114,6 +114,23 @@ def test_attention():
         assert abi.call(name + "_work_bytes", 1000, 100000, *bad) == 0
 
 
+def test_attention_by_local_sources():
+    """The same refusals where the mirror's length is known, and a mirror that is not there."""
+    name = "nts_kv8_attention_local"
+
+    def local(mirror=P, mirror_rows=40, **changed):
+        args = attention(**changed)
+        return args[:7] + [mirror, mirror_rows] + args[8:]
+
+    for text, changed in (("heads", dict(heads=0)), ("width", dict(width=257)), ("block_rows", dict(block_rows=48)),
+                          ("alignment", dict(cache=P + 4)), ("q_heads", dict(q_heads=6)), ("edges", dict(edges=0xFFFF0001)),
+                          ("work", dict(work=0, edges=100000)), ("null pointer", dict(mirror=0))):
+        refused(text, name, *local(**changed))
+    for hole in ("out", "q", "cache", "scales", "co", "ri"):
+        refused("null pointer", name, *local(**{hole: 0}))
+    assert abi.status(name, *local(Vd=0, mirror=0, mirror_rows=0)) == abi.NTS_OK
+
+
 def table(rows, width):
     codes, scales = lowbit.mx_shapes(rows, width)
     return lowbit.MxTable(torch.zeros(codes, dtype=torch.uint8), torch.zeros(scales, dtype=torch.uint8), width)
