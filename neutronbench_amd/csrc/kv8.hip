@@ -98,7 +98,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     // 448 = 1.75 * 2^8
     const uint32_t up = (top >> 23) + ((top & 0x7FFFFFu) > 0x600000u ? 1u : 0u);
     const uint32_t byte = max(old, up > 8u ? up - 8u : 0u);
-    const float inverse = e8m0_inverse(min(byte, 253u));
+    // 2^-127 and 2^-128, which only rows from elsewhere can ask for, lie below the normal floats
+    const float inverse = byte < 254u ? e8m0_inverse(byte) : __uint_as_float(0x00400000u >> (byte - 254u));
     auto put = [&](uint32_t j, float *v) {
       const uint32_t r = j / p.quads;
       const uint32_t row = static_cast<uint32_t>(row0) + r, quad = j - r * p.quads;

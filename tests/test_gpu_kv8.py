@@ -71,6 +71,24 @@ def test_append_again_from_the_middle(device):
         kv.append(dev(k, device), dev(v, device), 64)
 
 
+@pytest.mark.parametrize("byte", [0, 130, 247, 253, 254, 255])
+@pytest.mark.parametrize("D,block", [(16, 8), (64, 64), (250, 128)])
+def test_append_behind_rows_of_any_scale(device, byte, D, block):
+    """A cache from elsewhere whose begun block has any scale byte: the new rows are rounded at that scale or a larger one."""
+    heads, first, n = 2, 5, block
+    cache, scales = empty(2 * block, heads, D, block)
+    rng = np.random.default_rng(byte + D)
+    cache[:first, :, :, :D] = rng.integers(0, 0x7F, (first, 2, heads, D)) if byte < 240 else rng.integers(0, 2, (first, 2, heads, D))
+    scales[0] = byte
+    k = (rng.standard_normal((n, heads * D)) * np.exp2(rng.integers(-130, 126, (n, heads * D)))).astype(np.float32)
+    v = np.full((n, heads * D), np.float32(3.4028235e38)) if byte > 130 else k[::-1].copy()
+    kv = lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, block, rows=first)
+    ref.kv8_append(cache, scales, k, v, first, D, block)
+    kv.append(dev(k, device), dev(v, device))
+    assert (kv.scales.cpu().numpy() == scales).all()
+    assert (kv.cache.cpu().numpy() == cache).all()
+
+
 def graph_of(degrees, V, seed, missing=0.0, offset=0):
     rng = np.random.default_rng(seed)
     co = np.concatenate([[0], np.cumsum(degrees)]).astype(np.uint32) + np.uint32(offset)
