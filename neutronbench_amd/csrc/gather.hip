@@ -239,12 +239,16 @@ __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__
   }
 }
 
-// The same for large outputs whose rows do not fill whole lines: a wavefront takes kFlatSteps KB of the output in a piece, wherever
+// The same for large outputs of rows of fewer than 512 columns or of broken lines: a wavefront takes kFlatSteps KB of the output in a piece, wherever
 // rows begin in it, so that every line has one writer.  F is even, so a lane's four columns are two pairs that each lie in one row
 // and one block of it.  NARROW: rows of less than 256 columns, of which a wavefront's 256 may reach into many; that costs a
-// division a pair and pays only where rows are no multiple of 16 bytes.
-// 400,000 rows of 602: 284 us a row at a time, 168 in pieces; of 600: 234, 167; 1 M rows of 256: 196, 172; of 50: 73, 53 (streamed
-// both); but of 100: 98, 93 and of 128: 103, 113.
+// division a pair and is taken only where rows are no multiple of 16 bytes.
+// 963 MB of output by random ids, us a row at a time and in pieces.  From a table of 232,965 rows, which the last-level cache holds:
+// rows of 602 284, 168; of 258 232, 172; of 256 165, 148; of 320 183, 161; of 384 163, 154; of 448 157, 157; of 512 151, 150; of 768
+// 157, 151; of 1,024 156, 150.  From 2.45 M rows, which it does not: of 602 276, 271; of 258 356, 270; of 256 216, 191; of 320 297,
+// 262; of 384 271, 259; of 448 264, 263; but of 512 243, 254; of 768 239, 259; of 1,024 231, 262.  So rows of whole lines go in pieces up to
+// 512 columns.  Narrow ones, near and far: of 50 73, 53 (1 M rows) and 303, 287; of 130 far 328, 219; of 100
+// 98, 93 (1 M rows) and 241, 217; but of 128 183, 221 and 194, 203.
 constexpr uint32_t kFlatSteps = 4;
 template <bool NARROW>
 __global__ __launch_bounds__(256) void gather_mx_flat_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
@@ -469,7 +473,7 @@ int nts_gather_rows_mxfp4(float *out, const uint8_t *codes, const uint8_t *scale
   if (!out || (table_rows && (!codes || !scales))) return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: null pointer");
   if (!aligned_to(codes, 16) || !aligned_to(scales, 4))
     return fail(NTS_ERR_INVALID, "nts_gather_rows_mxfp4: codes need 16-byte, scales 4-byte alignment");
-  if (static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes && F % 2 == 0 && F >= 16 && (F % 4 != 0 || F == 256 || (F > 256 && F % 32 != 0)) &&
+  if (static_cast<uint64_t>(n) * F * sizeof(float) >= kStreamedBytes && F % 2 == 0 && F >= 16 && (F % 4 != 0 || (F >= 256 && (F < 512 || F % 32 != 0))) &&
       aligned_to(out, 128) && !table_in_host_memory(codes)) {
     const uint64_t pieces = (static_cast<uint64_t>(n) * F + kFlatSteps * 256 - 1) / (kFlatSteps * 256);
     const auto kernel = F < 256 ? gather_mx_flat_kernel<true> : gather_mx_flat_kernel<false>;

@@ -119,6 +119,21 @@ def test_gather_to_any_float(device, F, shift):
         assert (out[:shift] == 7.0).all() and (out[shift + n * F:] == 7.0).all()
 
 
+@pytest.mark.parametrize("F", [288, 384, 512, 1024, 1280])
+@pytest.mark.parametrize("by_id", [True, False])
+def test_gather_of_rows_of_whole_lines(device, F, by_id):
+    """Large outputs of rows that fill whole lines, which pieces of the output may begin and end within."""
+    V, n = 50, 9_000_000 // F
+    codes, scales, t = table_of(rows_of(V, F, seed=F), device)
+    values = np.concatenate([ref.mx_values(codes, scales, F).astype(np.float32), np.zeros((1, F), dtype=np.float32)])
+    ids = np.random.default_rng(F).integers(0, V + 1, n) if by_id else np.minimum(np.arange(n), V)
+    out = torch.full((n + 1, F), 7.0, device=device)
+    dids = dev(ids.astype(np.uint32), device) if by_id else None
+    call("nts_gather_rows_mxfp4", ptr(out), ptr(t.codes), ptr(t.scales), V, ptr(dids), n, F, stream())
+    want = torch.from_numpy(values).to(device)[torch.from_numpy(ids).to(device)]
+    assert ((out[:n] == want) | (torch.isnan(out[:n]) & torch.isnan(want))).all() and (out[n] == 7.0).all()
+
+
 def test_gather_from_mapped_host_memory(device):
     F, V = 100, 5000
     x = rows_of(V, F, seed=5)
