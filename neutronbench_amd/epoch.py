@@ -99,7 +99,8 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
         # attention configuration starts with a dense layer, whose product reads the rows by id itself.
         mx = MxTable.quantize(feat_cpu.to(dev))
         if heads:
-            mx_weight = MxTable.quantize(synth.normal_features(cfg["hidden"], cfg["F"], seed=cfg["seed"] + 43, device=dev))
+            weight = synth.normal_features(cfg["hidden"], cfg["F"], seed=cfg["seed"] + 43, device=dev)
+            mx_weight = MxTable.quantize(weight * cfg["F"] ** -0.5)  # rows of about the features' size
     else:
         table = MappedHostTable(feat_cpu)
         cache = FeatureCache(feat_cpu, out_deg.cpu(), int(V * cfg["cache"]), dev) if cfg["cache"] > 0 else None
@@ -166,7 +167,7 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
         """Forward through the layers (input side first), then backward in reverse order."""
         ops = []
         for l, layer in enumerate(layers):
-            width = cfg["F"] if l == 0 else cfg["hidden"]
+            width = cfg["F"] if l == 0 and mx_weight is None else cfg["hidden"]  # with mx_weight the dense layer has been
             if x.shape[1] != width or x.shape[0] != layer.src_size:
                 x = synth.normal_features(layer.src_size, width, seed=l, device=dev)  # stands in for the dense layer
             t0 = time.perf_counter()

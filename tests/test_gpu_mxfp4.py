@@ -12,7 +12,7 @@ import torch
 
 import lowbit_ref as ref
 from gpu_util import dev, stream
-from neutronbench_amd import epoch, lowbit
+from neutronbench_amd import epoch, lowbit, synth
 from neutronbench_amd.abi import call, ptr
 from neutronbench_amd.batch import BatchBuilder, load_feature_mxfp4
 from neutronbench_amd.stream import CudaStream
@@ -466,6 +466,32 @@ def test_an_epoch_on_rows_in_4_bits(device, config, scale):
     assert plain["features"] == "f32"
     with pytest.raises(ValueError):
         epoch.run(config, features="int3")
+
+
+@pytest.mark.parametrize("pipeline", [1, 2, 4])
+def test_the_attention_epoch_reads_the_products_rows(device, monkeypatch, pipeline):
+    """The first layer's input in the attention configuration: the batch's rows times the first layer's weight."""
+    seen = []
+
+    class Recorded(epoch.GATAggregateOp):
+        def forward(self, x, alpha):
+            seen.append((self.sg.dev_source.tensor().clone(), x.clone()))
+            return super().forward(x, alpha)
+
+    monkeypatch.setattr(epoch, "GATAggregateOp", Recorded)
+    scale, cfg = 0.05, epoch.CONFIGS["gat"]
+    V, F, hops = int(cfg["V"] * scale), cfg["F"], len(cfg["fanout"])
+    out = epoch.run("gat", scale=scale, max_batches=3, warmup_batches=0, pipeline=pipeline, quiet=True, features="mxfp4")
+    assert len(seen) == out["batches"] * hops == 3 * hops
+    x = ref.mx_values(*ref.mx_quantize(synth.normal_features(V, F, seed=cfg["seed"] + 40).numpy()), F)
+    weight = synth.normal_features(cfg["hidden"], F, seed=cfg["seed"] + 43, device=device).cpu().numpy() * np.float32(F ** -0.5)
+    w = ref.mx_values(*ref.mx_quantize(weight), F)
+    rows = 0
+    for ids, got in seen[::hops]:  # input side first
+        at = ids.cpu().numpy().view(np.uint32).astype(np.int64)
+        close(got, x[at] @ w.T, np.abs(x[at]) @ np.abs(w).T, F)
+        rows += at.size
+    assert rows == out["gathered_rows"]
 
 
 def test_a_sampled_layers_rows(device):
