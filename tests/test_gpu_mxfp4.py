@@ -285,6 +285,56 @@ def test_gradients(device, n, N, F, accumulate):
         close(got, want, scale, 3 * terms + 1100)
 
 
+@pytest.mark.parametrize("n,N,F", GRADS)
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_gradients_within_their_own_roundings(device, n, N, F, accumulate):
+    """A value of g is three exact terms whose magnitudes add up to its own, so a result is a chain of at most 3 terms roundings
+    within a part, one for each part and one for what was there: each off by 2^-23 of the magnitudes at most."""
+    ca, sa, a = table_of(rows_of(150, F, n + F, special=False), device)
+    cw, sw, w = table_of(rows_of(N, F, n + N, special=False), device)
+    rng = np.random.default_rng(n + 2)
+    ids = rng.integers(0, 150, n).astype(np.uint32)
+    g = rng.standard_normal((n, N)).astype(np.float32)
+    gx0, gw0 = rng.standard_normal((n, F)).astype(np.float32), rng.standard_normal((N, F)).astype(np.float32)
+    gx, gw, dg, dids = (dev(v, device) for v in (gx0, gw0, g, ids))
+    call("nts_mxfp4_product_grad_rows", ptr(gx), ptr(dg), ptr(w.codes), ptr(w.scales), n, N, F, accumulate, stream())
+    size = call("nts_mxfp4_product_grad_weight_work_bytes", n, N, F)
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    call("nts_mxfp4_product_grad_weight", ptr(gw), ptr(dg), ptr(a.codes), ptr(a.scales), 150, ptr(dids), n, N, F, accumulate,
+         ptr(work), stream())
+    x, wv, g64 = ref.mx_rows(ca, sa, F, ids), ref.mx_values(cw, sw, F), g.astype(np.float64)
+    for got, start, p, q, steps in ((gx, gx0, g64, wv, 3 * N + 1), (gw, gw0, g64.T, x, 3 * n + max(1, size // (4 * N * F)) + 1)):
+        want, scale = p @ q, np.abs(p) @ np.abs(q)
+        if accumulate:
+            want, scale = want + start, scale + np.abs(start)
+        close(got, want, scale, steps)
+
+
+@pytest.mark.parametrize("n,N,F", [(1, 1, 1), (40, 33, 70), (70, 128, 128), (97, 200, 40), (600, 40, 130), (20000, 17, 100)])
+@pytest.mark.parametrize("by_id", [True, False])
+def test_gradients_keep_every_bit_of_g(device, n, N, F, by_id):
+    """One term other than zero to a result, a power of two times a value of g whose 24 bits are in use: the gradient is that
+    product, exactly."""
+    rng = np.random.default_rng(n + N)
+    power = lambda *shape: (rng.choice([-1.0, 1.0], shape) * np.exp2(rng.integers(0, 3, shape))).astype(np.float32)
+    columns, term, row = np.arange(F), np.arange(F) * 5 % N, np.arange(F) * 7919 % n
+    xw, xa = np.zeros((N, F), dtype=np.float32), np.zeros((n, F), dtype=np.float32)
+    xw[term, columns], xa[row, columns] = power(F), power(F)
+    g = rng.standard_normal((n, N)).astype(np.float32)
+    g = (g.view(np.uint32) | 1).view(np.float32)
+    ids = rng.permutation(n) if by_id else np.arange(n)
+    stored = np.empty_like(xa)
+    stored[ids] = xa
+    ca, sa, a = table_of(stored, device)
+    cw, sw, w = table_of(xw, device)
+    assert (ref.mx_values(ca, sa, F) == stored).all() and (ref.mx_values(cw, sw, F) == xw).all()
+    op = lowbit.MxProductOp(dev(ids.astype(np.uint32), device) if by_id else None)
+    op.forward(a, w)
+    gx = op.backward(dev(g, device)).cpu().numpy()
+    assert (gx == g[:, term] * xw[term, columns]).all()
+    assert (op.get_additional_grad().cpu().numpy() == g[row].T * xa[row, columns]).all()
+
+
 @pytest.mark.parametrize("n", [32, 63, 96, 128, 160, 193, 600])
 @pytest.mark.parametrize("V", [0, 1, 40, 700])
 def test_gradient_of_the_weight_by_stages(device, n, V):
