@@ -463,13 +463,16 @@ if __name__ == "__main__":
                          "3 with a feature cache, 2 without; else 1")
     ap.add_argument("--features", choices=["f32", "mxfp4"], default="f32",
                     help="mxfp4: the feature table rounded to 4 bits and held in device memory; attention configurations "
-                         "then read it through the product with the first layer's weight (not with --native)")
+                         "then read it through the product with the first layer's weight (not with --native or "
+                         "--write-inputs)")
     ap.add_argument("--native", action="store_true",
                     help="drive the epoch from C++ (lib/nts_epoch) instead of this module's Python loop")
     ap.add_argument("--write-inputs", metavar="DIR", default=None,
                     help="only write the configuration's arrays for lib/nts_epoch to DIR and print the command line "
                          "that runs the epoch on them (to run the program under a profiler)")
     a = ap.parse_args()
+    if a.features != "f32" and (a.native or a.write_inputs):
+        ap.error("--native and --write-inputs take --features f32")
     if a.write_inputs:
         import os
 
@@ -483,8 +486,6 @@ if __name__ == "__main__":
                         str(int(bool(a.stage_sync)) if a.stage_sync is not None else 1), "--graph",
                         str(graph_mode(True if a.graph is None else a.graph, a.pipeline, cfg["cache"]))]))
     elif a.native:
-        if a.features != "f32":
-            ap.error("--native takes --features f32")
         run_native(a.config, a.scale, a.max_batches, a.warmup_batches, a.pipeline,
                    graph=True if a.graph is None else a.graph, stage_sync=bool(a.stage_sync))
     else:

@@ -1,4 +1,10 @@
 """Host logic of the epoch runners that needs no GPU."""
+import os
+import subprocess
+import sys
+
+import pytest
+
 from neutronbench_amd import epoch
 
 
@@ -24,3 +30,12 @@ def test_every_configuration_names_what_the_native_driver_needs():
             assert key in cfg, (name, key)
         assert cfg["hidden"] % max(cfg.get("heads", 0), 1) == 0
         assert all(f != 0 for f in cfg["fanout"]) and 1 <= len(cfg["fanout"]) <= 8
+
+
+@pytest.mark.parametrize("option", [["--native"], ["--write-inputs", "inputs"]])
+def test_the_native_driver_takes_float_features_only(option, tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(epoch.__file__)))
+    env = {**os.environ, "PYTHONPATH": root}
+    got = subprocess.run([sys.executable, "-m", "neutronbench_amd.epoch", "--config", "arxiv", "--features", "mxfp4", *option],
+                         cwd=tmp_path, env=env, capture_output=True, text=True)
+    assert got.returncode == 2 and "--features f32" in got.stderr and not os.listdir(tmp_path)
