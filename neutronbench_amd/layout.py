@@ -95,6 +95,7 @@ class FullGraphChunk:
             self.plan_forward = SpmmPlan(column_offset, V, self.E, chunk_edges, row_indices, V, n_slabs)
             self.plan_backward = SpmmPlan(row_offset, V, self.E, chunk_edges, column_indices, V, n_slabs)
         self.plan_build_s = time.perf_counter() - t0  # both schedules (host side, read-backs and uploads included)
+        self.v_size, self.e_size = V, self.E  # as a layer whose sources are the vertices themselves (dev_c_o, dev_r_i)
 
     @classmethod
     def from_edges(cls, src, dst, V, chunk_edges=0, n_slabs=1):
@@ -140,6 +141,12 @@ class FullGraphChunk:
         with torch.cuda.device(device):
             call("nts_scratch_trim")  # the graph is loaded: the memory that making its schedules took is the program's again
         return chunk
+
+    def dev_c_o(self):
+        return self.column_offset_gpu
+
+    def dev_r_i(self):
+        return self.row_indices_gpu
 
 
 class SampledLayer:

@@ -210,7 +210,8 @@ class Kv8Cache:
 
 class NeighborAttentionOp:
     """out[d, h, :] = sum over d's edges of softmax(scale * <q[d, h], K[row, h']>) V[row, h'], read from a Kv8Cache; the log of
-    each softmax's denominator is in `lse` afterwards.  The cached rows are constants: there is no backward."""
+    each softmax's denominator is in `lse` afterwards.  layer: a SampledLayer, or a FullGraphChunk, whose row_indices are vertices.
+    The cached rows are constants: there is no backward."""
 
     def __init__(self, layer, q_heads, scale=None):
         self.sg, self.q_heads, self.scale = layer, q_heads, scale

@@ -8,9 +8,10 @@ import torch
 
 import lowbit_ref as ref
 from gpu_util import dev, stream
-from neutronbench_amd import lowbit
+from neutronbench_amd import lowbit, synth
 from neutronbench_amd.abi import call, ptr
-from neutronbench_amd.layout import SampledLayer
+from neutronbench_amd.batch import BatchBuilder
+from neutronbench_amd.layout import FullGraphChunk, SampledLayer
 
 pytestmark = pytest.mark.gpu
 
@@ -213,6 +214,32 @@ def test_local_sources_beyond_the_mirror(device, degrees, bound, known):
     some = np.isfinite(lse)
     assert (np.abs(out - want) <= tol).all() and (np.isfinite(glse) == some).all()
     assert (np.abs(glse[some] - lse[some]) <= ltol[some]).all()
+
+
+def test_the_whole_graph_and_a_builders_layers(device):
+    """Attention over a FullGraphChunk, whose sources are vertices, and over the layers that a BatchBuilder makes of the same graph,
+    whose `source` is the mirror; neighbours that are not cached among both."""
+    V, heads, D, rows = 700, 2, 32, 650
+    src, dst = (t.to(device) for t in synth.rmat_edges(V, 9000, seed=3, device=device, sort=True))
+    cache, scales = empty(V, heads, D, 16)
+    ref.kv8_append(cache, scales, keys(V, heads * D, 1), keys(V, heads * D, 2), 0, D, 16)
+    kv = lowbit.Kv8Cache.over(dev(cache, device), dev(scales, device), D, 16, rows=rows)
+    values, rng = ref.kv8_values(cache, scales, D, 16), np.random.default_rng(4)
+    chunk = FullGraphChunk.from_edges(src, dst, V)
+    builder = BatchBuilder(chunk.column_offset_gpu, chunk.row_indices_gpu, [5, 40], 64)
+    batch = builder.sample(dev(rng.choice(V, 64, replace=False).astype(np.uint32), device), 1)
+    for layer in (chunk, *batch):
+        mirror = layer.dev_source if layer is not chunk else None
+        q = rng.standard_normal((layer.v_size, heads * D)).astype(np.float32)
+        op = lowbit.NeighborAttentionOp(layer, heads, 0.125)
+        out = op.forward(dev(q, device), kv, mirror).cpu().numpy()
+        co, ri = (a.cpu().numpy().view(np.uint32) for a in (layer.dev_c_o(), layer.dev_r_i()))
+        row = ri if mirror is None else mirror.cpu().numpy().view(np.uint32)[ri]
+        want, lse, tol, ltol = ref.attention(q, values, co.astype(np.int64), row, rows, heads, 0.125)
+        assert (np.abs(out - want) <= tol).all()
+        got, some = op.lse.cpu().numpy(), np.isfinite(lse)
+        assert (np.isfinite(got) == some).all() and (np.abs(got[some] - lse[some]) <= ltol[some]).all()
+    builder.close()
 
 
 def test_peaked_and_flat_scores(device):
