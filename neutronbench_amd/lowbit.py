@@ -170,6 +170,7 @@ class Kv8Cache:
     head, for keys and values each.  `rows` is how many the cache holds."""
 
     def __init__(self, capacity, heads, width, block_rows=16, device="cuda"):
+        self._check(heads, width, block_rows)
         cache = allocate(torch.zeros, (capacity, 2, heads, kv8_row_width(width)), dtype=torch.uint8, device=device)
         scales = allocate(torch.zeros, (-(-capacity // block_rows), 2, heads), dtype=torch.uint8, device=device)
         self._hold(cache, scales, width, block_rows, 0)
@@ -181,10 +182,16 @@ class Kv8Cache:
         self._hold(cache, scales, width, block_rows, cache.shape[0] if rows is None else rows)
         return self
 
+    @staticmethod
+    def _check(heads, width, block_rows):
+        if not 1 <= heads <= 1024 or not 1 <= width <= 256 or not 1 <= block_rows <= 1024 or block_rows & (block_rows - 1):
+            raise ValueError("cache: 1 .. 1,024 heads, width 1 .. 256, block_rows a power of two up to 1,024")
+
     def _hold(self, cache, scales, width, block_rows, rows):
-        if cache.dim() != 4 or cache.shape[2] < 1 or not 1 <= width <= 256 or block_rows < 1 or block_rows & (block_rows - 1):
-            raise ValueError("cache: [capacity, 2, heads, row width], width 1 .. 256, block_rows a power of two")
+        if cache.dim() != 4:
+            raise ValueError("cache: [capacity, 2, heads, row width]")
         capacity, _, heads, _ = cache.shape
+        self._check(heads, width, block_rows)
         _bytes(cache, (capacity, 2, heads, kv8_row_width(width)), "cache")
         _bytes(scales, (-(-capacity // block_rows), 2, heads), "scales")
         _same_device(cache.device, scales)

@@ -182,6 +182,15 @@ def test_python_objects_check_their_operands():
             lowbit.NeighborAttentionOp(layer, q_heads).forward(q, kv)
 
 
+def test_a_caches_shape_is_checked_before_it_is_made():
+    for heads, width, block in ((0, 8, 16), (1025, 8, 16), (4, 0, 16), (4, 257, 16), (4, 8, 0), (4, 8, 12), (4, 8, 2048), (4, 8, -4)):
+        with pytest.raises(ValueError):
+            lowbit.Kv8Cache(1 << 50, heads, width, block, device="cpu")
+    with pytest.raises(ValueError):  # blocks of more rows than any call takes
+        lowbit.Kv8Cache.over(torch.zeros(10, 2, 1, 16, dtype=torch.uint8), torch.zeros(1, 2, 1, dtype=torch.uint8), 16, 2048)
+    assert lowbit.Kv8Cache(40, 3, 20, 16, device="cpu").rows == 0
+
+
 def test_a_batchs_rows_need_an_output_of_their_size():
     """load_feature_mxfp4 against outputs that are too narrow, too wide, too short, of another type or strided, and layers whose
     id array is shorter than they say."""
