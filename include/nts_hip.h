@@ -555,7 +555,9 @@ int nts_kv8_append(uint8_t *cache, uint8_t *scales, const float *k, const float 
  * `edges` = co[Vd] - co[0], at most 2^32 - 2^16.  max_degree: the caller's bound on a destination's edges, 0 = none known;
  * it only selects the launches (one, or where rows may be long and are many, two: long rows are cut and their parts joined
  * in order).  The same bits on every call.  `work`: nts_kv8_attention_work_bytes(...) bytes (0: none) of 16-byte-aligned
- * device memory, which calls that overlap must not share.  Scores and sums are kept in 32 bits. */
+ * device memory, which calls that overlap must not share.  Scores and sums are kept in 32 bits: the sum over columns of q times
+ * the codes before their scale, the weighted sum of values before the division; what leaves the range of floats there is infinite (and
+ * NaN where the scores' maximum is), what lies below 2^-126 may be lost. */
 size_t nts_kv8_attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t width, uint32_t max_degree);
 int nts_kv8_attention(float *out, float *lse, const float *q, const uint8_t *cache, const uint8_t *scales, const uint32_t *co,
                       const uint32_t *ri, const uint32_t *mirror, uint32_t Vd, uint32_t edges, uint32_t cache_rows,

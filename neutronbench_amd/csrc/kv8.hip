@@ -47,8 +47,9 @@ __device__ __forceinline__ void append_values(const AppendArgs &p, const float *
   }
 }
 
-// Bound by memory: 2.45 M rows of 4 heads of 32, blocks of 16, 534 us, 5.9 TB/s of floats read and bytes written (read twice, the
-// second time from the caches: 712; alone in a loop 540 .. 650).
+// Bound by memory and by vector instructions, which are under way all of the time: 2.45 M rows of 4 heads of 32, blocks of 16, 563 us
+// after other work, 5.6 TB/s of floats read and bytes written; 603 one after the other.  Read twice, the second time from the
+// caches: 712.
 // HELD: blocks of at most 64 * HELD quads, which the lanes hold between the passes; 0: of any size, read twice.
 template <int HELD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
@@ -130,9 +131,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
 // value row serve them.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by side, and further edges of the
 // destination go to further such sets of lanes ("slots"), each with a running softmax of its own, joined at the end.  All slots of
 // one destination are a walker; a wavefront is one walker or, where rows are short, several.
-// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 392 us, of which 362 in the walkers, that is 1.3 GB of rows, queries
-// and results at 3.7 TB/s.  Bound by vector instructions (70 % of the time; without reading rows 333 us): 48 a lane and edge to
-// convert and multiply 16 columns of a key and a value, about as many again to look up, scale, rescale, join and write.
+// 2.48 M edges of 169,343 destinations, 8 query heads on 2 of 64: 394 us after other work, of which some 29 in the join; that is 1.3 GB of
+// rows, queries and results at 3.6 TB/s in the walkers.  Bound by vector instructions (64 % of the time; without reading rows 333 us when
+// the whole took 392): 48 a lane and edge to convert and multiply 16 columns of a key and a value, about as many again to look up,
+// scale, rescale, join and write.
 struct AttendArgs {
   float *out, *lse;
   const float *q;
@@ -407,6 +409,8 @@ struct Attend {
     for (int g = 0; g < G; ++g) {
       if (q_head0 + g >= p.share) continue;
       const uint64_t at = static_cast<uint64_t>(row) * p.q_heads + kv_head * p.share + q_head0 + g;
+      // the reciprocal is within one step of 32 bits, and its product another half; divided correctly 418 us instead of 415 (the
+      // edges above, one call after the other)
       store(p.out + at * p.D, g, sum[g] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[g]), p.D);
       if (p.lse && dl == 0 && slot == 0) p.lse[at] = sum[g] == 0.0f ? -INFINITY : (top[g] + __builtin_amdgcn_logf(sum[g])) * kLn2;
     }
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(At
 // span of `span` positions.  A destination of more than `span` edges is cut at the spans' ends: every span that it reaches into
 // sums its part into a record (1: the destination begins in this span, 0: in an earlier one) and join_spans_kernel adds the
 // parts in order.  No atomics: the same bits on every call.
-constexpr uint32_t kRowCost = 8;  // 2.48 M edges in 169 K rows, 4 heads of 32: 194 us; 4: 209, 16: 192, 1: 230
+constexpr uint32_t kRowCost = 8;  // 2.48 M edges in 169 K rows, 4 heads of 32: 194 us when chosen (201 now); 4: 209, 16: 192, 1: 230
 __device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r * kRowCost + (co[r] - co0); }
 
 // The last destination at or before position x: a candidate for every lane of the walker a step.
@@ -669,7 +673,7 @@ Lanes lanes_for(uint32_t q_heads, uint32_t heads, uint32_t D, uint64_t slot_edge
 uint64_t records_bytes(uint32_t q_heads, uint32_t D) { return 2ull * q_heads * (D + 2u) * sizeof(float); }
 // Positions of a span: 256, so that a part's record is little beside its edges, but spans for all wavefronts that the chip holds
 // where there are few positions (none of fewer than 64), and no more spans than fill it four times over or have records of
-// 256 MB.
+// 256 MB, but up to 256 spans whatever theirs take (of 1,024 heads of 256: 516 MB).
 uint32_t span_length(uint64_t positions, uint32_t q_heads, uint32_t D) {
   const uint64_t most = std::max<uint64_t>(256, std::min<uint64_t>(16384, (256ull << 20) / records_bytes(q_heads, D)));
   const uint64_t spans = std::min(most, std::max<uint64_t>(1024, positions / 256));
@@ -754,8 +758,8 @@ int attend(const char *call, float *out, float *lse, const float *q, const uint8
   p.share = q_heads / heads;
   p.score_scale = score_scale;
   // Slots: where a bound is known most rows reach it, and a slot that works through 16 edges costs least (60,000 rows of 10
-  // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four); averages hide longer rows (2.48 M edges in 169 K rows:
-  // 229 us with four slots for 15 edges on average, 264 with two, 572 with one).
+  // edges, 4 heads of 32: 37 us with one slot, 42 with two, 51 with four when chosen, 40 now); averages hide longer rows (2.48 M edges
+  // in 169 K rows: 229 us with four slots for 15 edges on average, 264 with two, 572 with one when chosen, 201 now).
   const bool blocks = by_blocks(Vd, edges, max_degree), spans = by_spans(Vd, edges, max_degree);
   const Lanes l = lanes_for(q_heads, heads, width, blocks ? kWave : spans ? (static_cast<uint64_t>(edges) / Vd + 4) / 4 : (max_degree + 15) / 16);
   p.units = l.units, p.per_head = l.per_head, p.hw_shift = l.hw_shift, p.walker_shift = l.walker_shift;

@@ -12,7 +12,8 @@ namespace {
 // Per block of 32 values of a row: e = floor(log2 max|x|) - 2, so that the largest value lies in [4, 8) of the code's range
 // 0 .. 6 (7 and more become 6), then every x 2^-e to the nearest code.  Eight lanes take a block, four floats each; the
 // maximum is one of integers, since the bits of |x| order as the values do and infinities and NaN lie above them.
-// Blocks of a lane group that are requested together (2.45 M rows of 100: 282 us with four, 4.1 TB/s; 325 with one, 291 with two).
+// Blocks of a lane group that are requested together (2.45 M rows of 100: 282 us with four, 325 with one, 291 with two; 295 under a
+// kernel trace, 3.9 TB/s).
 constexpr uint32_t kQuantizeAhead = 4;
 __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                                                           const float *__restrict__ x, uint32_t n_blocks, uint32_t F,
@@ -203,11 +204,11 @@ __global__ __launch_bounds__(kFewWaves *kWave) void mx_product_few_kernel(Produc
 // or 128 bytes a row.  The loads write a stage to LDS themselves (no registers between) while the one before it is
 // multiplied.  Part c of row r lies at c ^ (r * PARTS / 16) % PARTS, so that the 16 lanes that read one part of 16 rows meet all
 // banks once.
-// Measured (65,536 rows of 4,096 values by 4,096 columns): 684 us, 3.2 PFLOP/s, where a library's bf16 product of that size
-// takes 1,599.  Without loads and stores 411 us, with the stores 493, with the loads 686: bound by the loads of codes into LDS and the
+// Measured (65,536 rows of 4,096 values by 4,096 columns): 700 us, 3.1 PFLOP/s (684 .. 715 from card to card), where a library's bf16
+// product of that size takes 1,580 and its rate times four would take 394.  The matrix units are busy for 34 % of the time.  When the
+// whole took 684: 411 without loads and stores, 493 with the stores, 686 with the loads: bound by the loads of codes into LDS and the
 // waits for them.  Steps: registers in place of loads into LDS 1,170; stores past the caches 1,043 -> 900; operands asked for a step
-// ahead 893 -> 785; results turned in LDS and stored as whole lines
-// 785 -> 693.  128 x 128 with stages of 64 bytes takes 912.
+// ahead 893 -> 785; results turned in LDS and stored as whole lines 785 -> 693.  128 x 128 with stages of 64 bytes takes 912.
 typedef __attribute__((address_space(3))) void *LdsPointer;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00027000);
@@ -233,7 +234,7 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
-constexpr uint32_t kRowGroup = 8;  // 65,536 x 4,096 by 4,096: 718 us; groups of 4: 737, of 2: 752, tiles in turn 737
+constexpr uint32_t kRowGroup = 8;  // 65,536 x 4,096 by 4,096, one after the other: 718 us; groups of 4 737, of 2 752, tiles in turn 737
 // NEAR: both tables' codes are less than 4 GB and are read through buffer descriptors, by 32-bit offsets.
 template <int BM, int BN, int WM, int WN, int PARTS, bool NEAR>
 __global__ __launch_bounds__(WM *WN *kWave, 2) void mx_product_tiled_kernel(ProductArgs p, uint32_t tiles_m, uint32_t tiles_n) {
@@ -458,8 +459,9 @@ void launch_product(const ProductArgs &p, hipStream_t stream) {
 // terms of eight bits of fraction each by cutting off bits, which is exact and cannot overflow, so three bf16 products summed
 // in 32 bits keep the accuracy of a 32-bit product.  A block of four wavefronts takes 128 rows of the result by 128
 // columns, 32 terms at a time through LDS, where both operands lie with the terms of a row or column side by side; the next
-// terms are on their way into registers meanwhile.  What that costs is the waits for them, vector instructions (30 % of the
-// time) and LDS; the matrix units are busy for a third.
+// terms are on their way into registers meanwhile.  What that costs is the waits for them, vector instructions and LDS: over
+// 169,343 rows of 128 by 128 vector instructions are under way for 29 % of the time and the matrix units busy for 15 (rows) and 17
+// (weight); of 640 by 640 for 54 and 38 (rows), 44 and 31 (weight).
 // The weight's gradient has few results and many terms: blockIdx.z takes its part of the terms, the parts' sums are added in
 // order by a second launch, so results do not depend on scheduling.
 constexpr uint32_t kGradTile = 128, kGradTerms = 32;
@@ -500,8 +502,8 @@ __device__ __forceinline__ uint32_t upper_halves(uint32_t first, uint32_t second
 // Whole stages load without branches, so that a wait is for the oldest loads alone: rows and columns of the tile that the result does
 // not have read some other of it, ids that the table does not have read its first row and count as zeros.  What is left of the
 // terms is loaded one by one.
-// Weight: two stages of loads are on their way while a third is multiplied (640 by 640 over 169,343 rows: 832 -> 624 us, 128 by 128: 41 ->
-// 33); it has blocks for two on a compute unit anyway.  Rows: one stage, and the registers for three blocks, are better (169,343 by
+// Weight: two stages of loads are on their way while a third is multiplied (640 by 640 over 169,343 rows: 832 -> 624 us, with the parts'
+// sum, 128 by 128: 41 -> 33); it has blocks for two on a compute unit anyway.  Rows: one stage, and the registers for three blocks, are better (169,343 by
 // 128 by 128: 38 us against 46).
 template <bool WEIGHT, bool IDS>
 __global__ __launch_bounds__(256, WEIGHT ? 2 : 3) void mx_grad_kernel(GradArgs p) {

@@ -56,3 +56,17 @@ def test_registers(kernels, kernel, most):
     found = [k for name, k in kernels.items() if kernel in name]
     assert len(found) == 1
     assert found[0][".vgpr_count"] <= most and found[0][".vgpr_spill_count"] == 0
+
+
+@pytest.mark.parametrize("kernel,number,most", [
+    ("gather_mx_", 7, 64), ("mx_quantize_kernel", 1, 64), ("kv8_append_kernelILi2E", 1, 64), ("kv8_append_kernelILi0E", 1, 64),
+    ("mx_product_tiled_kernelILi128E", 2, 128), ("mx_product_tiled_kernelILi256E", 1, 256),
+    ("mx_grad_kernelILb0E", 1, 168),  # the gradient of the rows: three blocks on a compute unit
+    ("mx_grad_kernelILb1E", 2, 256),
+] + [(f"kv8_attend_rows_kernelILi{n}ELi{g}E", 2, 128 if g == 1 else 256) for n in (1, 2, 4, 8, 16) for g in (1, 2)])
+def test_registers_of_tables_in_few_bits(kernels, kernel, number, most):
+    """As many wavefronts on a SIMD as the launches count on, and no vector register in scratch memory."""
+    found = [k for name, k in kernels.items() if kernel in name]
+    assert len(found) == number
+    for k in found:
+        assert k[".vgpr_count"] <= most and k[".vgpr_spill_count"] == 0 and k[".private_segment_fixed_size"] == 0
