@@ -239,8 +239,8 @@ __global__ __launch_bounds__(256) void gather_mx_rows_kernel(float *__restrict__
   }
 }
 
-// The same for large outputs of rows of fewer than 512 columns or of broken lines: a wavefront takes kFlatSteps KB of the output in a piece, wherever
-// rows begin in it, so that every line has one writer.  F is even, so a lane's four columns are two pairs that each lie in one row
+// The same for large outputs of rows of fewer than 512 columns or of broken lines: a wavefront takes kFlatSteps KB of the output in a
+// piece, wherever rows begin in it, so that every line has one writer.  F is even, so a lane's four columns are two pairs that each lie in one row
 // and one block of it.  NARROW: rows of less than 256 columns, of which a wavefront's 256 may reach into many; that costs a
 // division a pair and is taken only where rows are no multiple of 16 bytes.
 // 963 MB of output by random ids, us a row at a time and in pieces.  From a table of 232,965 rows, which the last-level cache holds:

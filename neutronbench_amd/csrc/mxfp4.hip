@@ -502,9 +502,9 @@ __device__ __forceinline__ uint32_t upper_halves(uint32_t first, uint32_t second
 // Whole stages load without branches, so that a wait is for the oldest loads alone: rows and columns of the tile that the result does
 // not have read some other of it, ids that the table does not have read its first row and count as zeros.  What is left of the
 // terms is loaded one by one.
-// Weight: two stages of loads are on their way while a third is multiplied (640 by 640 over 169,343 rows: 832 -> 624 us, with the parts'
-// sum, 128 by 128: 41 -> 33); it has blocks for two on a compute unit anyway.  Rows: one stage, and the registers for three blocks, are better (169,343 by
-// 128 by 128: 38 us against 46).
+// Weight: two stages of loads are on their way while a third is multiplied (640 by 640 over 169,343 rows: 832 -> 624 us, with the
+// parts' sum, 128 by 128: 41 -> 33); it has blocks for two on a compute unit anyway.  Rows: one stage, and the registers for three
+// blocks, are better (169,343 by 128 by 128: 38 us against 46).
 template <bool WEIGHT, bool IDS>
 __global__ __launch_bounds__(256, WEIGHT ? 2 : 3) void mx_grad_kernel(GradArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t sp0[3][kGradTile * kGradTerms], sp1[3][kGradTile * kGradTerms], sq0[kGradQ], sq1[kGradQ];
