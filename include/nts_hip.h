@@ -570,6 +570,76 @@ int nts_kv8_attention_local(float *out, float *lse, const float *q, const uint8_
                             float score_scale, uint32_t max_degree, void *work, nts_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Layers of vertices in training (what the reference's toolkits leave to libtorch between the graph operators: mm(W), relu,
+ * dropout of vertexForward, toolkits/GCN_GPU_NEIGHBOR.hpp:715-728) and attention with dot products as scores, which it lacks
+ * ------------------------------------------------------------------------------------------- */
+
+/* Types of the dense operands.  All sums, softmax statistics and activations are computed in 32 bits; an output is rounded once.
+ * Arrays need the alignment of one value. */
+enum nts_type { NTS_F32 = 0, NTS_BF16 = 1, NTS_F16 = 2 };
+
+/* Dropout from a counter: nothing is stored, and the backward pass draws the same numbers again.  Ten rounds of Philox-4x32 with
+ * the 64-bit seed as key make eight 16-bit numbers (the low half of a word before the high one) of every counter:
+ *   value (row r, column c)        number c % 8 of counter (c / 8, r, step, 0)
+ *   edge (src, dst), query head h  number h % 8 of counter (src, dst, step, 1 + h / 8); parallel edges share theirs
+ * A value is dropped where its number is below t = p * 65536, rounded to the nearest whole number; what is kept is multiplied by
+ * 65536 / (65536 - t); what is dropped is 0, whatever it was.  Operators of one training step need different seeds.
+ * step_device: a device word that the step is read from instead of `step` when the kernels run (a captured graph, whose
+ * replays draw other numbers once the word has changed); NULL otherwise.  step_kept: a device word that receives the step that was
+ * used (may be NULL): passed as the backward pass's step_device it lets the program advance its step in between. */
+typedef struct nts_dropout {
+  float p; /* within 0 .. 1 */
+  uint32_t step;
+  uint64_t seed;
+  const uint32_t *step_device;
+  uint32_t *step_kept;
+} nts_dropout_t;
+
+/* out [n, F] = dropout of in [n, F], F up to 2^17; out may be in.  The gradient of `in` is the same call on the gradient of out. */
+int nts_dropout(void *out, const void *in, int type, uint32_t n, uint32_t F, const nts_dropout_t *dropout, nts_stream_t stream);
+
+/* Attention of every destination over its edges' sources, with gradients (nts_kv8_attention reads keys and values in 8 bits and
+ * has none).  q, out and their gradients [Vd, q_heads, width], k, v and theirs [Vs, heads, width]; q_heads a multiple of heads up to
+ * 1,024, head h of q reads head h / (q_heads / heads) of k and v; width up to 256.
+ *   s[e, h] = score_scale <q[d, h], k[ri[e], h']>,  p = softmax of s over the edges of d,  out[d, h] = sum of drop(p[e, h]) v[ri[e], h']
+ *   lse[d, h] = log of the sum of exp(s[e, h]) (float)
+ * An edge whose ri[e] is not below Vs has no source and is left out (its rows are not read).  A destination without edges, or whose
+ * scores are all -infinity: out 0, lse -infinity and no gradient.  NaN or +infinity among a destination's scores: NaN.
+ * A probability below 2^-126 may count as 0.
+ * dropout: of the probabilities, NULL for none.  edges: at least co[Vd] - co[0].  max_degree: no destination has more edges than
+ * that; 0: no bound known.
+ * nts_dot_attention_grad computes the probabilities again from q, k and lse; gq, gk and gv are the gradients for g, that
+ * of out.  ro [Vs+1] and ci [edges]: the same edges by source (nts_csr_from_csc), those without a source left out; an entry of ci that
+ * is not below Vd is left out.  Every element of gq, gk and gv is written.  No atomics: the same bits on every call.
+ * work: nts_dot_attention_work_bytes / nts_dot_attention_grad_work_bytes of 16-byte-aligned device memory (0: may be NULL), in use
+ * until the call's work on `stream` is done. */
+size_t nts_dot_attention_work_bytes(uint32_t Vd, uint32_t edges, uint32_t q_heads, uint32_t width, uint32_t max_degree);
+int nts_dot_attention(void *out, float *lse, const void *q, const void *k, const void *v, int type, const uint32_t *co,
+                      const uint32_t *ri, uint32_t Vd, uint32_t Vs, uint32_t edges, uint32_t q_heads, uint32_t heads, uint32_t width,
+                      float score_scale, uint32_t max_degree, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
+size_t nts_dot_attention_grad_work_bytes(uint32_t Vd, uint32_t Vs, uint32_t edges, uint32_t q_heads, uint32_t heads, uint32_t width,
+                                         uint32_t max_degree);
+int nts_dot_attention_grad(void *gq, void *gk, void *gv, const void *g, const void *q, const void *k, const void *v, const float *lse,
+                           int type, const uint32_t *co, const uint32_t *ri, const uint32_t *ro, const uint32_t *ci, uint32_t Vd,
+                           uint32_t Vs, uint32_t edges, uint32_t q_heads, uint32_t heads, uint32_t width, float score_scale,
+                           uint32_t max_degree, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
+
+/* A dense layer: y[i, j] = residual[i, j] + drop(act(z[i, j])), z[i, j] = sum over f of x[i, f] w[j, f] + bias[j];
+ * x [n, F], w [N, F], bias [N], residual and y [n, N], all of one type; bias, residual and dropout may be NULL; N and F up to 2^17.
+ * Operands of 32 bits are multiplied as three bf16 parts each, with the accuracy of a 32-bit product but for parts below 2^-126, which
+ * may count as 0; an element whose sum is not finite that way is computed again term by term.
+ * nts_dense_grad: for g, the gradient of y, the gradients gx [n, F], gw [N, F] and gb [N], each NULL where it is not wanted (that of the
+ * residual is g itself).  z is computed again, not kept.  In 16 bits the gradient of z is rounded to the operands' type before the
+ * two products, as a layer that hands it on would; gb is summed before that.  relu's slope at 0 is 0.
+ * work: nts_dense_grad_work_bytes of 16-byte-aligned device memory (0: may be NULL), in use until the call's work on `stream` is done. */
+enum nts_activation { NTS_ACT_NONE = 0, NTS_ACT_RELU = 1, NTS_ACT_GELU = 2 /* z times the normal distribution's share below z */, NTS_ACT_SILU = 3 };
+int nts_dense(void *y, const void *x, const void *w, const void *bias, const void *residual, int type, uint32_t n, uint32_t N,
+              uint32_t F, int activation, const nts_dropout_t *dropout, nts_stream_t stream);
+size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_rows, int with_weight, int with_bias);
+int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, const void *w, const void *bias, int type, uint32_t n,
+                   uint32_t N, uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Sampled-layer index construction on the device (sampCSC, core/coocsc.hpp)
  * ------------------------------------------------------------------------------------------- */
 

@@ -4,6 +4,7 @@
 //   scales  [ceil(capacity / block_rows), 2, heads]
 #include <algorithm>
 
+#include "edge_spans.hpp"
 #include "launch_size.hpp"
 #include "lowbit.hpp"
 
@@ -154,22 +155,6 @@ struct AttendArgs {
   float *partial;
   uint32_t *tail_row;
 };
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-// Sum over an aligned group of ND lanes, the same in all of them; the exchanges are part of the additions.
-template <int CTRL>
-__device__ __forceinline__ float add_lane(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
-}
-template <int ND>
-__device__ __forceinline__ float lanes_sum(float v) {
-  if (ND > 1) v = add_lane<0xB1>(v);   // neighbours in pairs
-  if (ND > 2) v = add_lane<0x4E>(v);   // pairs in fours
-  if (ND > 4) v = add_lane<0x141>(v);  // fours, mirrored within eight
-  if (ND > 8) v = add_lane<0x140>(v);  // eights, mirrored within sixteen
-  return v;
-}
 
 // What the registers allow, measured: with one query head to a lane four wavefronts to a SIMD (2.48 M edges, 8 query heads of 64: 468 us at
 // the time; three 507, two edges at a time 600); with two, two wavefronts (500 K edges, 16 query heads of 128: 205 us; three and two
@@ -505,36 +490,7 @@ __global__ __launch_bounds__(kBlockWaves *kWave) void kv8_attend_block_kernel(At
   }
 }
 
-// Long rows are shared out and short ones bundled without a look at the degrees on the host: destinations and edges are
-// lined up -- destination r takes kRowCost positions from r * kRowCost + co[r] - co[0] on, which is what beginning and writing a
-// row costs in edges, and its edges the positions behind them -- and every walker takes the destinations that begin within its
-// span of `span` positions.  A destination of more than `span` edges is cut at the spans' ends: every span that it reaches into
-// sums its part into a record (1: the destination begins in this span, 0: in an earlier one) and join_spans_kernel adds the
-// parts in order.  No atomics: the same bits on every call.
-constexpr uint32_t kRowCost = 8;  // 2.48 M edges in 169 K rows, 4 heads of 32: 194 us when chosen (201 now); 4: 209, 16: 192, 1: 230
-__device__ __forceinline__ uint64_t position_of(const uint32_t *co, uint32_t co0, uint64_t r) { return r * kRowCost + (co[r] - co0); }
-
-// The last destination at or before position x: a candidate for every lane of the walker a step.
-__device__ __forceinline__ uint32_t destination_at(const uint32_t *co, uint32_t co0, uint32_t Vd, uint64_t x, uint32_t walker_shift) {
-  const uint32_t lanes = 1u << walker_shift, lane = threadIdx.x & (lanes - 1u);
-  const uint64_t group = lanes == 64u ? ~0ull : ((1ull << lanes) - 1ull) << ((threadIdx.x & 63u) & ~(lanes - 1u));
-  uint32_t lo = 0, hi = Vd;  // position_of(lo) <= x, the answer is in [lo, hi)
-  while (hi - lo > 1) {
-    const uint32_t step = lanes == 1u ? (hi - lo) / 2u : (hi - lo - 1u) / lanes + 1u;
-    const uint64_t r = static_cast<uint64_t>(lo) + static_cast<uint64_t>(lanes == 1u ? 1u : lane) * step;
-    const bool before = r < hi && position_of(co, co0, r) <= x;
-    if (lanes == 1u) {
-      if (before) lo += step; else hi = lo + step;
-      continue;
-    }
-    const uint32_t count = __popcll(__ballot(before) & group);  // lane 0 always counts
-    const uint32_t next = lo + (count - 1u) * step;
-    hi = hi - next > step ? next + step : hi;
-    lo = next;
-  }
-  return lo;
-}
-
+// Spans of positions: edge_spans.hpp.
 template <int ND, int G, bool NEAR>
 __global__ __launch_bounds__(256, kWavesOf<G>) void kv8_attend_spans_kernel(AttendArgs p) {
   uint32_t pass;
@@ -641,13 +597,6 @@ bool by_blocks(uint32_t Vd, uint32_t edges, uint32_t max_degree) {
 bool by_spans(uint32_t Vd, uint32_t edges, uint32_t max_degree) {
   return !by_blocks(Vd, edges, max_degree) && (max_degree == 0 || max_degree > kMostRowEdges);
 }
-
-uint32_t next_power(uint32_t v) {
-  uint32_t p = 1;
-  while (p < v) p <<= 1;
-  return p;
-}
-uint32_t shift_of(uint32_t power) { return static_cast<uint32_t>(__builtin_ctz(power)); }
 
 // How the lanes are laid out.  `slot_edges`: edges of a row for each of its slots.
 struct Lanes {

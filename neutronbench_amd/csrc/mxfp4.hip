@@ -4,6 +4,7 @@
 
 #include "launch_size.hpp"
 #include "lowbit.hpp"
+#include "tiles.hpp"
 
 namespace nts {
 namespace {
@@ -75,25 +76,6 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t *__restrict__ 
 // v_mfma_scale_f32_16x16x128 takes 16 rows of each operand, 128 values deep: lane l holds row l % 16, the 32 values of block
 // l / 16, which are 16 consecutive bytes of the row, and that block's scale.  So the operands go from memory to registers as
 // they lie.  W is the first operand: a lane then ends up with four neighbouring columns of one output row.
-
-// Blocks are handed to the eight chiplets, each with an L2 of its own, in turn.  Where there are kXcdTiles tiles of rows or more, a
-// chiplet takes `group` of them at a time, every column of tiles for all of the group before the next: blocks that run together share
-// rows and columns.  With fewer, tiles in turn fill the chip more evenly.  Product of 232,965 rows of 602 by 256: 79.5 -> 65.5 us, the
-// rows' gradient of 169,343 by 640 by 640: 607 -> 489.
-constexpr uint32_t kXcdTiles = 64;
-__device__ __forceinline__ void tile_of(uint32_t tiles_n, bool by_xcd, uint32_t group, uint32_t *tm, uint32_t *tn) {
-  if (by_xcd) {
-    const uint32_t x = blockIdx.x / 8u, of = group * tiles_n, within = x % of;
-    *tm = (x / of * group + within % group) * 8u + blockIdx.x % 8u;
-    *tn = within / group;
-  } else {
-    *tm = blockIdx.x / tiles_n;
-    *tn = blockIdx.x % tiles_n;
-  }
-}
-uint32_t tile_blocks(uint32_t tiles_m, uint32_t tiles_n, uint32_t group) {
-  return (tiles_m >= kXcdTiles ? ceil_div(tiles_m, 8 * group) * 8u * group : tiles_m) * tiles_n;
-}
 
 struct MxRows {
   const uint8_t *codes;

@@ -95,7 +95,7 @@ class FullGraphChunk:
             self.plan_forward = SpmmPlan(column_offset, V, self.E, chunk_edges, row_indices, V, n_slabs)
             self.plan_backward = SpmmPlan(row_offset, V, self.E, chunk_edges, column_indices, V, n_slabs)
         self.plan_build_s = time.perf_counter() - t0  # both schedules (host side, read-backs and uploads included)
-        self.v_size, self.e_size = V, self.E  # as a layer whose sources are the vertices themselves (dev_c_o, dev_r_i)
+        self.v_size, self.e_size, self.src_size = V, self.E, V  # as a layer whose sources are the vertices themselves
 
     @classmethod
     def from_edges(cls, src, dst, V, chunk_edges=0, n_slabs=1):
@@ -147,6 +147,12 @@ class FullGraphChunk:
 
     def dev_r_i(self):
         return self.row_indices_gpu
+
+    def dev_r_o(self):
+        return self.row_offset_gpu
+
+    def dev_c_i(self):
+        return self.column_indices_gpu
 
 
 class SampledLayer:
