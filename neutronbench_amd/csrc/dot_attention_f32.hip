@@ -1,0 +1,5 @@
+#include "dot_attention.hpp"
+
+namespace nts {
+int dot_launch_f32(int kind, const DotArgs &p, uint32_t nd, bool near, hipStream_t stream) { return launch_kind<float>(kind, p, nd, near, stream); }
+}  // namespace nts

@@ -14,7 +14,7 @@ inline size_t type_size(int type) { return type == NTS_F32 ? 4 : 2; }
 struct DropArgs {
   uint32_t threshold, key0, key1, step;
   float scale;
-  const uint32_t *step_device;  // the step is read there
+  const uint32_t *step_device;  // the step is read there, and `step` is 0
   uint32_t *step_kept;          // and written here
 };
 inline const char *bad_dropout(const nts_dropout_t *d) {
@@ -29,7 +29,7 @@ inline DropArgs drop_args(const nts_dropout_t *d) {
   a.threshold = static_cast<uint32_t>(__builtin_rint(static_cast<double>(d->p) * 65536.0));
   a.scale = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
   a.key0 = static_cast<uint32_t>(d->seed), a.key1 = static_cast<uint32_t>(d->seed >> 32);
-  a.step = d->step, a.step_device = d->step_device, a.step_kept = d->step_kept;
+  a.step = d->step_device ? 0u : d->step, a.step_device = d->step_device, a.step_kept = d->step_kept;
   return a;
 }
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint32_t k0, uint32_t k1) {
   }
   return c;
 }
-__device__ __forceinline__ uint32_t drop_step(const DropArgs &d) { return d.step_device ? *d.step_device : d.step; }
+__device__ __forceinline__ uint32_t drop_step(const DropArgs &d) { return d.step + (d.step_device ? *d.step_device : 0u); }
 __device__ __forceinline__ uint32_t half_of(const uint4 &n, int i) {
   const uint32_t w = i / 2 == 0 ? n.x : i / 2 == 1 ? n.y : i / 2 == 2 ? n.z : n.w;
   return i & 1 ? w >> 16 : w & 0xFFFFu;
