@@ -629,15 +629,20 @@ int nts_dot_attention_grad(void *gq, void *gk, void *gv, const void *g, const vo
  * Operands of 32 bits are multiplied as three bf16 parts each, with the accuracy of a 32-bit product but for parts below 2^-126, which
  * may count as 0; an element whose sum is not finite that way is computed again term by term.
  * nts_dense_grad: for g, the gradient of y, the gradients gx [n, F], gw [N, F] and gb [N], each NULL where it is not wanted (that of the
- * residual is g itself).  z is computed again, not kept.  In 16 bits the gradient of z is rounded to the operands' type before the
- * two products, as a layer that hands it on would; gb is summed before that.  relu's slope at 0 is 0.
- * work: nts_dense_grad_work_bytes of 16-byte-aligned device memory (0: may be NULL), in use until the call's work on `stream` is done. */
+ * residual is g itself).  z is computed again, not kept, but for relu without a residual where y (the layer's output, else NULL; never with a
+ * residual) says which sums were above 0 and kept: it has to be what it was, and a sum whose output was rounded to 0 counts as 0.  In 16
+ * bits the gradient of z is rounded to the operands' type before the two products, as a layer that hands it on would; gb is summed
+ * before that.  relu's slope at 0 is 0.
+ * work: nts_dense_work_bytes / nts_dense_grad_work_bytes of 16-byte-aligned device memory (0: may be NULL), in use until the call's work
+ * on `stream` is done. */
 enum nts_activation { NTS_ACT_NONE = 0, NTS_ACT_RELU = 1, NTS_ACT_GELU = 2 /* z times the normal distribution's share below z */, NTS_ACT_SILU = 3 };
+size_t nts_dense_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F);
 int nts_dense(void *y, const void *x, const void *w, const void *bias, const void *residual, int type, uint32_t n, uint32_t N,
-              uint32_t F, int activation, const nts_dropout_t *dropout, nts_stream_t stream);
-size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_rows, int with_weight, int with_bias);
-int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, const void *w, const void *bias, int type, uint32_t n,
-                   uint32_t N, uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
+              uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
+size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_y, int with_rows,
+                                 int with_weight, int with_bias);
+int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, const void *w, const void *bias, const void *y, int type,
+                   uint32_t n, uint32_t N, uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Sampled-layer index construction on the device (sampCSC, core/coocsc.hpp)

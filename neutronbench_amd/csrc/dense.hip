@@ -1,11 +1,12 @@
 // A dense layer on rows of vertices and its gradients.
 //   z = x w^T + bias, y = residual + drop(act(z))
 //   dz = drop(g) act'(z) with z computed again, gx = dz w, gw = dz^T x, gb = column sums of dz
+// With relu and no residual y says what dz needs: it is above 0 where z is and the value was kept.  Then dz is never stored: both products
+// make it from g and y as they read them.
 #include <algorithm>
 
 #include "launch_size.hpp"
 #include "layers.hpp"
-#include "tiles.hpp"
 
 namespace nts {
 namespace {
@@ -16,35 +17,67 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // What a product's result becomes.
-enum Use { kLayer, kSlope, kRows, kWeight };
+enum Use { kLayer, kSlope, kRows };
 
 struct DenseArgs {
-  const void *a, *b;  // result [M, N] = sum over K terms
+  const void *a, *b;  // result [M, N] = sum over K terms; b: the weight as prepared, or the second operand of the weight's gradient
+  const void *w;      // the weight itself
+  const void *y;      // masked gradients: a is g, and counts where y is not 0 or below, times mask_scale
+  float mask_scale;
   uint32_t M, N, K, a_stride, b_stride;
   void *out;
   const void *bias, *more;  // more: the residual, or the gradient of y
-  float *sums;              // kSlope: column sums of every row of tiles [tiles_m, N]; kWeight: the parts' results [parts, M, N], if there are several
+  float *sums;              // the workers' column sums [workers, N], or the parts of the weight's gradient [parts, M, N]; may be null
+  float *column_sums;       // the weight's gradient: the parts' sums of a's columns [parts, M], may be null
   int act;
   DropArgs drop;
-  uint32_t row0;  // of the launch, where dropout counts from
-  uint32_t tiles_m, tiles_n, part_terms;
+  uint32_t tiles_m, tiles_n, workers, part_terms;
   bool streamed;
 };
 
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == NTS_ACT_RELU) return z <= 0.0f ? 0.0f : z;
-  if (act == NTS_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-  if (act == NTS_ACT_SILU) return z / (1.0f + expf(-z));
-  return z;
+// The normal distribution's share below z, off by at most 0.75e-7, and density * sqrt(2 pi): half of M. Abramowitz and I. Stegun,
+// Handbook of Mathematical Functions, 7.1.26, for the error function of |z| / sqrt(2).
+__device__ __forceinline__ float normal_below(float z, float *bell) {
+  const float a = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678f, 1.0f));
+  const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+  const float tail = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f) * e;
+  *bell = e;
+  return z < 0.0f ? tail : 1.0f - tail;
 }
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == NTS_ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;
-  if (act == NTS_ACT_GELU) return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
-  if (act == NTS_ACT_SILU) {
-    const float f = 1.0f / (1.0f + expf(-z));
-    return f * (1.0f + z * (1.0f - f));
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+template <int N>
+__device__ __forceinline__ void activate(float *z, int act) {
+  if (act == NTS_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = z[k] <= 0.0f ? 0.0f : z[k];
+  } else if (act == NTS_ACT_GELU) {
+    float bell;
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] *= normal_below(z[k], &bell);
+  } else if (act == NTS_ACT_SILU) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] *= sigmoid(z[k]);
   }
-  return 1.0f;
+}
+// g times the activation's slopes at z.
+__device__ __forceinline__ void through_slope(float *z, const float *g, int act) {
+  if (act == NTS_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[k] = z[k] <= 0.0f ? 0.0f : g[k];
+  } else if (act == NTS_ACT_GELU) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float bell;
+      const float below = normal_below(z[k], &bell);
+      z[k] = g[k] * fmaf(z[k] * 0.39894228f, bell, below);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = sigmoid(z[k]);
+      z[k] = g[k] * (f * fmaf(z[k], 1.0f - f, 1.0f));
+    }
+  }
 }
 
 // Up to four neighbouring values of a row, those behind its end 0.
@@ -68,56 +101,29 @@ __device__ __forceinline__ void put_columns(T *at, uint32_t count, const float *
       if (c < count) put_value(at + c, v[c]);
   }
 }
-// Drops of the four columns of a row from c on, a multiple of 4.
-__device__ __forceinline__ void drop_columns(const DropArgs &d, uint32_t step, uint32_t row, uint32_t c, float *v) {
-  if (!d.threshold) return;
-  const uint4 n = row_numbers(d, step, row, c >> 3);
-  const uint32_t w0 = c & 4u ? n.z : n.x, w1 = c & 4u ? n.w : n.y;
-  v[0] = (w0 & 0xFFFFu) >= d.threshold ? v[0] * d.scale : 0.0f;
-  v[1] = (w0 >> 16) >= d.threshold ? v[1] * d.scale : 0.0f;
-  v[2] = (w1 & 0xFFFFu) >= d.threshold ? v[2] * d.scale : 0.0f;
-  v[3] = (w1 >> 16) >= d.threshold ? v[3] * d.scale : 0.0f;
-}
-// Columns c .. c + 3 of row i, sums of products in v: the layer's output, or the gradient of its sums, which v keeps.
-template <typename T, int USE>
-__device__ __forceinline__ void finish_columns(const DenseArgs &p, uint32_t step, uint64_t i, uint32_t c, float *v) {
-  const uint32_t count = p.N - c;
-  T *const to = static_cast<T *>(p.out) + i * p.N + c;
-  if (USE == kLayer || USE == kSlope) {
-    if (p.bias) {
-      float bias[4];
-      get_columns(static_cast<const T *>(p.bias) + c, count, bias);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += bias[k];
-    }
-    float more[4] = {};
-    if (p.more) get_columns(static_cast<const T *>(p.more) + i * p.N + c, count, more);
-    if (USE == kLayer) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = activate(v[k], p.act);
-      drop_columns(p.drop, step, p.row0 + static_cast<uint32_t>(i), c, v);
-      if (p.more) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += more[k];
-      }
-    } else {
-      drop_columns(p.drop, step, p.row0 + static_cast<uint32_t>(i), c, more);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = k < static_cast<int>(count) ? more[k] * slope(v[k], p.act) : 0.0f;
-    }
-  }
-  put_columns(to, count, v, p.streamed);
+__device__ __forceinline__ float dropped(uint32_t number, const DropArgs &d, float v) { return number >= d.threshold ? v * d.scale : 0.0f; }
+// Drops of the four columns from c on (a multiple of 4, neighbouring lanes take neighbouring fours) of two rows: a lane draws the eight
+// numbers of one of them, of the second one where its columns are the upper four, and neighbours exchange what the other needs.
+__device__ __forceinline__ void drop_two_rows(const DropArgs &d, uint32_t step, uint32_t row0, uint32_t row1, uint32_t c, float *v0, float *v1) {
+  const bool upper = (c & 4u) != 0;
+  const uint4 n = row_numbers(d, step, upper ? row1 : row0, c >> 3);
+  const int give0 = static_cast<int>(upper ? n.x : n.z), give1 = static_cast<int>(upper ? n.y : n.w);
+  const uint32_t got0 = __builtin_amdgcn_update_dpp(0, give0, 0xB1, 0xF, 0xF, true), got1 = __builtin_amdgcn_update_dpp(0, give1, 0xB1, 0xF, 0xF, true);
+  const uint32_t a0 = upper ? got0 : n.x, a1 = upper ? got1 : n.y, b0 = upper ? n.z : got0, b1 = upper ? n.w : got1;
+  v0[0] = dropped(a0 & 0xFFFFu, d, v0[0]), v0[1] = dropped(a0 >> 16, d, v0[1]);
+  v0[2] = dropped(a1 & 0xFFFFu, d, v0[2]), v0[3] = dropped(a1 >> 16, d, v0[3]);
+  v1[0] = dropped(b0 & 0xFFFFu, d, v1[0]), v1[1] = dropped(b0 >> 16, d, v1[1]);
+  v1[2] = dropped(b1 & 0xFFFFu, d, v1[2]), v1[3] = dropped(b1 >> 16, d, v1[3]);
 }
 
-// ---- tiles ------------------------------------------------------------------------------------------
-// A block of four wavefronts takes 128 rows of the result by 128 columns, 32 terms at a time through LDS, where both operands lie
-// with the terms of a row or column side by side.  Operands of 32 bits are split into three bf16 parts, each the nearest to what the ones
-// before it leave: x = hi + mid + lo up to 2^-27 of x, and of the nine products the three that are below 2^-26 of the whole are
-// left out, so that the sums in 32 bits are as good as a 32-bit product's.  An infinity's mid part is NaN: elements that are not finite
-// are computed again term by term.
-constexpr uint32_t kTile = 128, kTerms = 32;
-// Where 8 of a row's 32 terms lie: the 16 lanes that read one part of 16 rows meet all banks once.
-__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t part) { return row * kTerms + ((part ^ (row >> 2)) & 3u) * 8u; }
+// ---- products ---------------------------------------------------------------------------------------
+// Matrix instructions take 16 rows by 16 columns, 32 terms at a time.  Operands of 32 bits are split into three bf16 parts, each the nearest
+// to what the ones before it leave: x = hi + mid + lo up to 2^-27 of x, and of the nine products the three that are below 2^-26 of the whole
+// are left out, so that the sums in 32 bits are as good as a 32-bit product's.  An infinity's mid part is NaN: elements that are not
+// finite are computed again term by term.
+constexpr uint32_t kTile = 128, kTerms = 32, kPlane = kTile * kTerms;
+// Where 8 of a row's 32 terms lie in LDS: the 16 lanes that read one part of 16 rows meet all banks once.
+__host__ __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t part) { return row * kTerms + ((part ^ (row >> 2)) & 3u) * 8u; }
 
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
@@ -130,103 +136,445 @@ template <>
 __device__ __forceinline__ f32x4 multiply<F16>(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-
-// Sixteen terms of one row (ALONG: the terms lie side by side) or column of an operand, on their way from memory to LDS.
-template <typename T, bool ALONG>
-struct Terms {
-  typedef typename ValueOf<T>::raw raw;
-  raw v[16];
-  __device__ __forceinline__ void request(const T *from, uint32_t stride) {  // of the first of the sixteen
-    if (ALONG) {
-      constexpr int N = 16 / sizeof(raw);
-#pragma unroll
-      for (int i = 0; i < 16; i += N) {
-        const typename Pack<T, N>::type q = *reinterpret_cast<const typename Pack<T, N>::type *>(from + i);
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[i + k] = q[k];
-      }
-    } else {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) v[i] = *reinterpret_cast<const raw *>(from + static_cast<uint64_t>(i) * stride);
-    }
-  }
-  __device__ __forceinline__ void request_some(const T *from, uint32_t stride, uint32_t count) {
-#pragma unroll
-    for (uint32_t i = 0; i < 16; ++i)
-      v[i] = i < count ? *reinterpret_cast<const raw *>(from + (ALONG ? i : static_cast<uint64_t>(i) * stride)) : static_cast<raw>(0);
-  }
-};
 __device__ __forceinline__ uint32_t pair_of(float a, float b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
 }
-// Eight terms to the planes at `to`.
-__device__ __forceinline__ void keep(const float *v, uint16_t *to, uint32_t plane) {
-  u32x4 w[3];
+// The parts of eight terms.
+__device__ __forceinline__ void split8(const float *v, u32x4 *w) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-      w[c][i] = pair_of(a, b);
-      a -= __uint_as_float(w[c][i] << 16), b -= __uint_as_float(w[c][i] & 0xFFFF0000u);
+      const uint32_t both = pair_of(a, b);
+      w[c][i] = both;
+      a -= __uint_as_float(both << 16), b -= __uint_as_float(both & 0xFFFF0000u);
     }
   }
-#pragma unroll
-  for (int c = 0; c < 3; ++c) *reinterpret_cast<u32x4 *>(to + c * plane) = w[c];
 }
-__device__ __forceinline__ void keep(const uint16_t *v, uint16_t *to, uint32_t) {
-  u32x4 w;
+__device__ __forceinline__ void split8(const uint16_t *v, u32x4 *w) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = v[2 * i] | static_cast<uint32_t>(v[2 * i + 1]) << 16;
-  *reinterpret_cast<u32x4 *>(to) = w;
+  for (int i = 0; i < 4; ++i) w[0][i] = v[2 * i] | static_cast<uint32_t>(v[2 * i + 1]) << 16;
+}
+// The sum of an element's products term by term; mask: as DenseArgs' y, null for none.
+__device__ __forceinline__ float sum_of_terms(const float *x, const float *mask, float scale, uint64_t x_step, const float *y, uint64_t y_step, uint64_t count) {
+  float sum = 0.0f;
+  for (uint64_t f = 0; f < count; ++f) {
+    const float v = !mask ? x[f * x_step] : mask[f * x_step] <= 0.0f ? 0.0f : x[f * x_step] * scale;
+    sum = fmaf(v, y[f * y_step], sum);
+  }
+  return sum;
 }
 
-template <typename T, int USE>
-__global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
-  constexpr bool kAlongA = USE != kWeight, kAlongB = USE == kLayer || USE == kSlope;
+// The weight as the products want it: for every 128 columns of the result and 32 terms its parts, as they lie in LDS, zeros behind the
+// ends.  ALONG: a column's terms lie side by side.  A thread takes eight terms.
+struct PrepareArgs {
+  const void *from;
+  uint16_t *to;
+  uint32_t columns, terms, stride, stages, tiles;
+};
+template <typename T, bool ALONG>
+__global__ __launch_bounds__(256) void dense_prepare_kernel(PrepareArgs p) {
+  typedef typename ValueOf<T>::raw raw;
   constexpr int P = kPlanes<T>;
-  constexpr uint32_t kPlane = kTile * kTerms;
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  // neighbouring threads have neighbouring terms or columns, as they lie in memory
+  const uint32_t part = ALONG ? i % 4u : i / kTile % 4u, row = ALONG ? i / 4u % kTile : i % kTile, block = i / (4u * kTile);
+  if (block >= p.stages * p.tiles) return;
+  const uint32_t tile = block / p.stages, stage = block - tile * p.stages;
+  const uint32_t column = tile * kTile + row, term = stage * kTerms + part * 8u;
+  raw v[8];
+  if (ALONG && column < p.columns && term + 8u <= p.terms) {
+    const typename Pack<T, 8>::type got = *reinterpret_cast<const typename Pack<T, 8>::type *>(static_cast<const raw *>(p.from) + static_cast<uint64_t>(column) * p.stride + term);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = got[k];
+  } else {
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k) {
+    const uint64_t at = ALONG ? static_cast<uint64_t>(column) * p.stride + term + k : static_cast<uint64_t>(term + k) * p.stride + column;
+    v[k] = column < p.columns && term + k < p.terms ? static_cast<const raw *>(p.from)[at] : static_cast<raw>(0);
+  }
+  }
+  u32x4 w[3];
+  split8(v, w);
+#pragma unroll
+  for (int c = 0; c < P; ++c) *reinterpret_cast<u32x4 *>(p.to + (static_cast<uint64_t>(block) * P + c) * kPlane + tile_at(row, part)) = w[c];
+}
+
+typedef __attribute__((address_space(3))) void *LdsPointer;
+// 16 bytes a lane to 1,024 consecutive bytes of LDS.
+__device__ __forceinline__ void load_to_lds(const uint16_t *from, uint16_t *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (LdsPointer)to, 16, 0, 0);
+}
+// Waits for the wavefront's loads and LDS accesses, then for the block.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Many rows.  A block of 4 * WN wavefronts takes 64 * MR rows by 128 * WN columns, a stage of 32 terms after the other, and then its next
+// rows.  Rows go from memory to the registers that the matrix instructions read, each to the one wavefront (of a column group) that
+// needs them, and are split there; the prepared weight goes to LDS by loads that write it themselves.  Both are a stage ahead, past the end
+// of a tile too.
+// MR: 16 rows each, of a wavefront.
+template <typename T, int USE, int MR, int WN, bool MASKED>
+__global__ __launch_bounds__(256 * WN, MR == 4 || sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
+  constexpr int P = kPlanes<T>;
+  constexpr uint32_t kRows = 64 * MR, kStage = WN * P * kPlane;
+  // results are turned where the stage of the weight was that has been used last, if it is large enough
+  constexpr bool kApart = kStage * sizeof(uint16_t) < 4u * WN * 4096u;
+  __shared__ __attribute__((aligned(16))) uint16_t weight0[kStage], weight1[kStage], apart[kApart ? 4 * WN * 2048 : 8];
+  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
+  // neighbouring blocks of a chiplet take the columns of one worker's rows
+  const uint32_t x = blockIdx.x / 8u, tn = x % p.tiles_n, worker = x / p.tiles_n * 8u + blockIdx.x % 8u;
+  const uint32_t wr = wave & 3u, wc = wave >> 2, stages = (p.K + kTerms - 1u) / kTerms;
+  const uint32_t step = USE == kLayer || USE == kSlope ? drop_step(p.drop) : 0u;
+  if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
+  if (worker >= p.tiles_m) return;
+  const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * WN * stages * P * kPlane;
+  const T *const rows = static_cast<const T *>(p.a);
+  // stage s of the weight
+  auto request_weight = [&](uint16_t *to, uint32_t s) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2 * P; ++i) {
+      const uint32_t piece = i * 4 * WN + wave, group = piece / (8 * P), at = piece % (8 * P);  // 512 values each
+      load_to_lds(weight + ((static_cast<uint64_t>(group) * stages + s) * P * kPlane + at * 512u + lane * 8u), to + piece * 512u);
+    }
+  };
+  typedef typename ValueOf<T>::raw raw;
+  constexpr int L = 8 * sizeof(raw) / 16;  // loads of a lane's eight terms
+  constexpr int S = MASKED ? 2 : 1;  // operands: g and y
+  u32x4 next[S][MR][L];
+  const T *row_at[S][MR];
+  auto place = [&](uint32_t tile) __attribute__((always_inline)) {  // rows that the result does not have read the last one
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      const uint64_t row = static_cast<uint64_t>(tile) * kRows + wr * (16u * MR) + i * 16u + r;
+#pragma unroll
+      for (int o = 0; o < S; ++o)
+        row_at[o][i] = (o ? static_cast<const T *>(p.y) : rows) + min(row, static_cast<uint64_t>(p.M - 1u)) * p.a_stride + part * 8u;
+    }
+  };
+  auto request_rows = [&](uint32_t s) __attribute__((always_inline)) {
+    typedef typename Pack<T, 16 / sizeof(raw)>::type Whole;
+    const uint32_t k = s * kTerms;
+    if (k + kTerms <= p.K) {
+#pragma unroll
+      for (int o = 0; o < S; ++o)
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int l = 0; l < L; ++l) {
+            const Whole got = *reinterpret_cast<const Whole *>(row_at[o][i] + k + l * (16 / sizeof(raw)));
+            next[o][i][l] = __builtin_bit_cast(u32x4, got);
+          }
+    } else {
+      const uint32_t from = k + part * 8u, count = from < p.K ? min(p.K - from, 8u) : 0u;
+#pragma unroll
+      for (int o = 0; o < S; ++o)
+#pragma unroll
+        for (int i = 0; i < MR; ++i) {
+          raw v[8];
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) v[e] = e < count ? reinterpret_cast<const raw *>(row_at[o][i] + k)[e] : static_cast<raw>(0);
+          if (sizeof(raw) == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) next[o][i][e / 4 % L][e % 4] = __float_as_uint(v[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) next[o][i][0][e] = static_cast<uint32_t>(v[2 * e]) | static_cast<uint32_t>(v[2 * e + 1]) << 16;
+          }
+        }
+    }
+  };
+  // value e of the eight of fragment i
+  auto value = [&](int o, int i, int e) __attribute__((always_inline)) {
+    if (sizeof(raw) == 4) {
+      const uint32_t bits = next[o][i][e / 4 % L][e % 4];
+      return __uint_as_float(bits);
+    }
+    const uint32_t both = next[o][i][0][e / 2 % 4];
+    return ValueOf<T>::get(static_cast<raw>(e & 1 ? both >> 16 : both));
+  };
+  f32x4 acc[MR][8];
+  uint32_t half = 0;
+  float bias[2][4] = {};
+  if (USE != kRows && p.bias) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t c = tn * (kTile * WN) + wc * kTile + h * 64u + (lane & 15u) * 4u;
+      if (c < p.N) get_columns(static_cast<const T *>(p.bias) + c, p.N - c, bias[h]);
+    }
+  }
+  float sums[2][4] = {};
+  place(worker);
+  request_weight(weight0, 0);
+  request_rows(0);
+  for (uint32_t tile = worker; tile < p.tiles_m; tile += p.workers) {
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (uint32_t s = 0; s < stages; ++s) {
+      u32x4 a[MR][P];
+      stage_barrier();
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        if (P == 3 || MASKED) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = value(0, i, e);
+            if (MASKED) v[e] = value(S - 1, i, e) <= 0.0f ? 0.0f : v[e] * p.mask_scale;
+          }
+          if constexpr (P == 3) {
+            split8(v, a[i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[i][0][e] = ValueOf<T>::put(v[2 * e]) | static_cast<uint32_t>(ValueOf<T>::put(v[2 * e + 1])) << 16;
+          }
+        } else {
+          a[i][0] = next[0][i][0];
+        }
+      }
+      const bool last = s + 1u == stages;
+      if (!last || tile + p.workers < p.tiles_m) {
+        if (last) place(tile + p.workers);
+        request_weight(half ? weight0 : weight1, last ? 0u : s + 1u);
+        request_rows(last ? 0u : s + 1u);
+      }
+      const uint16_t *const w = (half ? weight1 : weight0) + wc * (P * kPlane);
+      half ^= 1u;
+      u32x4 b[2][P];
+#pragma unroll
+      for (int c = 0; c < P; ++c) b[0][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at(r, part));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < 7) {
+#pragma unroll
+          for (int c = 0; c < P; ++c) b[(j + 1) & 1][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at((j + 1) * 16 + r, part));
+        }
+        // the weight is the first operand: a lane then ends up with four neighbouring columns of one row; small products first
+#pragma unroll
+        for (int q = P - 1; q >= 0; --q)
+#pragma unroll
+          for (int c = 0; c <= q; ++c)
+#pragma unroll
+            for (int i = 0; i < MR; ++i) acc[i][j] = multiply<T>(b[j & 1][q - c], a[i][c], acc[i][j]);
+      }
+    }
+    // Through LDS, 16 rows by 64 columns at a time, a lane's columns become lines (part c of row r at c ^ r).
+    if (!kApart) __builtin_amdgcn_s_barrier();  // all have read it
+    f32x4 *const mine = reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u;
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[r * 16u + ((j * 4u + part) ^ r)] = acc[i][h * 4 + j];
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t c = tn * (kTile * WN) + wc * kTile + h * 64u + (lane & 15u) * 4u;
+        const uint64_t row0 = static_cast<uint64_t>(tile) * kRows + wr * (16u * MR) + i * 16u + lane / 16u;
+        // two rows of a lane at a time, the next ones' second operand on its way; not unrolled, or the registers do not hold what is behind it
+        float ahead[2][4] = {};
+        auto read = [&](uint32_t q) __attribute__((always_inline)) {
+#pragma unroll
+          for (uint32_t u = 0; u < 2; ++u)
+            if (USE != kRows && p.more && row0 + (q + u) * 4u < p.M && c < p.N)
+              get_columns(static_cast<const T *>(p.more) + (row0 + (q + u) * 4u) * p.N + c, p.N - c, ahead[u]);
+        };
+        read(0);
+#pragma unroll 1
+        for (uint32_t q = 0; q < 4; q += 2) {
+          float v[2][4], more[2][4];
+#pragma unroll
+          for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t row = (q + u) * 4u + lane / 16u;
+            const uint64_t at = row0 + (q + u) * 4u;
+            const f32x4 got = mine[row * 16u + ((lane & 15u) ^ row)];
+            v[u][0] = got.x, v[u][1] = got.y, v[u][2] = got.z, v[u][3] = got.w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) more[u][k] = ahead[u][k];
+            if (P == 3) {
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k) {
+                if (fabsf(v[u][k]) < INFINITY || at >= p.M || c + k >= p.N) continue;
+                const float *const b = static_cast<const float *>(p.w);
+                v[u][k] = sum_of_terms(static_cast<const float *>(p.a) + at * p.a_stride,
+                                       MASKED ? static_cast<const float *>(p.y) + at * p.a_stride : nullptr, p.mask_scale, 1,
+                                       USE == kRows ? b + c + k : b + static_cast<uint64_t>(c + k) * p.K, USE == kRows ? p.N : 1u, p.K);
+              }
+            }
+            if (USE != kRows) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[u][k] += bias[h][k];
+            }
+            if (USE == kLayer) activate<4>(v[u], p.act);
+          }
+          if (q == 0) read(2);
+          if (USE != kRows && p.drop.threshold) {
+            float(*const dropping)[4] = USE == kLayer ? v : more;
+            drop_two_rows(p.drop, step, static_cast<uint32_t>(row0) + q * 4u, static_cast<uint32_t>(row0) + q * 4u + 4u, c, dropping[0], dropping[1]);
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 2; ++u) {
+            const uint64_t at = row0 + (q + u) * 4u;
+            if (USE == kLayer && p.more) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[u][k] += more[u][k];
+            }
+            if (USE == kSlope) through_slope(v[u], more[u], p.act);
+            if (at >= p.M || c >= p.N) continue;
+            put_columns(static_cast<T *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
+            if (USE == kSlope) {  // columns that are not there are summed and not stored
+#pragma unroll
+              for (int k = 0; k < 4; ++k) sums[h][k] += v[u][k];
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+  }
+  if (USE != kSlope || !p.sums) return;
+  __syncthreads();
+  // the block's column sums: of a wavefront's four rows of lanes, then of its four wavefronts of rows
+  float(*const of_wave)[kTile] = reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v = sums[h][k];
+      v += __shfl_xor(v, 16, kWave);
+      v += __shfl_xor(v, 32, kWave);
+      if (lane < 16u) of_wave[wave][h * 64u + lane * 4u + k] = v;
+    }
+  __syncthreads();
+  if (t < kTile * WN) {
+    const uint32_t group = t / kTile, c = tn * (kTile * WN) + t;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v += of_wave[group * 4 + w][t % kTile];
+    if (c < p.N) p.sums[static_cast<uint64_t>(worker) * p.N + c] = v;
+  }
+}
+
+// ---- the weight's gradient --------------------------------------------------------------------------
+// Few results and many terms: blockIdx.z takes its part of the terms, the parts' sums are added in order by a second launch, so results do
+// not depend on scheduling.  A block of four wavefronts takes 128 rows of the result by 128 columns, 32 terms at a time through LDS, where
+// both operands are written with the terms of a row or column side by side.
+// Sixteen terms of one column of an operand, or eight of each of two neighbouring columns (PAIRS: rows of 16-bit values of an even number),
+// on their way from memory to LDS.  MASKED: as DenseArgs' y.
+template <typename T, bool PAIRS, bool MASKED>
+struct Terms {
+  typedef typename ValueOf<T>::raw raw;
+  static constexpr int S = MASKED ? 2 : 1, N = PAIRS ? 8 : 16;
+  typedef uint32_t Word __attribute__((aligned(2)));
+  uint32_t v[S][N];
+  const T *from[S];  // the operands' beginning, so that a row's address is a scalar, and the lane's place from there
+  uint32_t lane_at, stride, column, first;  // the thread's column of 128, its first term of 32
+  __device__ __forceinline__ void place(const void *a, const void *y, uint32_t row_stride, uint32_t first_column, uint32_t columns) {
+    const uint32_t t = threadIdx.x;
+    column = PAIRS ? t % 64u * 2u : t & 127u;
+    first = PAIRS ? t / 64u * 8u : (t >> 7) * 16u;
+    stride = row_stride;
+    // neighbouring threads have neighbouring columns; columns that the operand does not have read some other of it
+    const uint32_t c = min(first_column + column, columns - (PAIRS ? 2u : 1u));
+    lane_at = first * stride + c;
+    from[0] = static_cast<const T *>(a);
+    if (MASKED) from[S - 1] = static_cast<const T *>(y);
+  }
+  template <bool SOME>
+  __device__ __forceinline__ void request(uint64_t term, uint32_t left) {
+#pragma unroll
+    for (int o = 0; o < S; ++o) {
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) {
+        const T *const one = from[o] + (term + i) * stride + lane_at;
+        if (SOME && first + i >= left) v[o][i] = 0u;
+        else if (PAIRS) v[o][i] = *reinterpret_cast<const Word *>(one);
+        else if (sizeof(raw) == 4) v[o][i] = *reinterpret_cast<const uint32_t *>(one);
+        else v[o][i] = static_cast<uint32_t>(*reinterpret_cast<const raw *>(one));
+      }
+    }
+  }
+  // Term i of the thread's column, or of the second one of a pair.
+  __device__ __forceinline__ float value(int i, int which) const {
+    auto get = [&](uint32_t word) { return sizeof(raw) == 4 ? __uint_as_float(word) : ValueOf<T>::get(static_cast<raw>(which ? word >> 16 : word)); };
+    const float x = get(v[0][i]);
+    return !MASKED ? x : get(v[S - 1][i]) <= 0.0f ? 0.0f : x;
+  }
+  // To the planes; sums: of the columns' terms, times scale.
+  __device__ __forceinline__ void keep(uint16_t *planes, float scale, float *sums) const {
+#pragma unroll
+    for (int which = 0; which < (PAIRS ? 2 : 1); ++which)
+#pragma unroll
+      for (int i = 0; i < N; i += 8) {
+        u32x4 w[3];
+        if (sizeof(raw) == 4 || MASKED) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = value(i + e, which) * (MASKED ? scale : 1.0f);
+            if (sums) sums[which] += f[e];
+          }
+          if constexpr (sizeof(raw) == 4) {
+            split8(f, w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[0][e] = ValueOf<T>::put(f[2 * e]) | static_cast<uint32_t>(ValueOf<T>::put(f[2 * e + 1])) << 16;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = v[0][i + 2 * e], y = v[0][i + 2 * e + 1];
+            w[0][e] = which ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+          }
+          if (sums) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums[which] += value(i + e, which);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kPlanes<T>; ++c) *reinterpret_cast<u32x4 *>(planes + c * kPlane + tile_at(column + which, (first + i) / 8u)) = w[c];
+      }
+  }
+};
+
+template <typename T, bool PAIRS, bool MASKED>
+__global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
+  constexpr int P = kPlanes<T>;
   __shared__ __attribute__((aligned(16))) uint16_t tile[2 * P * kPlane > 8192 ? 2 * P * kPlane : 8192];
   uint16_t *const ta = tile, *const tb = tile + P * kPlane;
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
-  uint32_t tm, tn;
-  tile_of(p.tiles_n, p.tiles_m >= kXcdTiles, 1, &tm, &tn);
-  if (tm >= p.tiles_m) return;
-  const uint32_t step = USE == kLayer || USE == kSlope ? drop_step(p.drop) : 0u;
-  if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
-  const uint64_t m0 = static_cast<uint64_t>(tm) * kTile;
-  const uint32_t n0 = tn * kTile;
+  const uint32_t tm = blockIdx.x / p.tiles_n, tn = blockIdx.x % p.tiles_n;
+  const uint32_t m0 = tm * kTile, n0 = tn * kTile;
   const uint64_t begin = static_cast<uint64_t>(blockIdx.z) * p.part_terms, end = min(static_cast<uint64_t>(p.K), begin + p.part_terms);
-  // Two threads take a row's 32 terms where they lie side by side, otherwise neighbouring threads have neighbouring columns.  Rows and
-  // columns that the result does not have read some other of it.
-  const uint32_t ra = kAlongA ? t >> 1 : t & 127u, ka = kAlongA ? (t & 1u) * 16u : (t >> 7) * 16u;
-  const uint32_t rb = kAlongB ? t >> 1 : t & 127u, kb = kAlongB ? (t & 1u) * 16u : (t >> 7) * 16u;
-  const uint64_t ma = min(m0 + ra, static_cast<uint64_t>(p.M - 1u)), nb = min(n0 + rb, p.N - 1u);
-  const T *const from_a = static_cast<const T *>(p.a) + (kAlongA ? ma * p.a_stride + ka : ka * static_cast<uint64_t>(p.a_stride) + ma);
-  const T *const from_b = static_cast<const T *>(p.b) + (kAlongB ? nb * p.b_stride + kb : kb * static_cast<uint64_t>(p.b_stride) + nb);
-  Terms<T, kAlongA> va;
-  Terms<T, kAlongB> vb;
+  Terms<T, PAIRS, MASKED> va;
+  Terms<T, PAIRS, false> vb;
+  va.place(p.a, p.y, p.a_stride, m0, p.M);
+  vb.place(p.b, nullptr, p.b_stride, n0, p.N);
+  float sums[2] = {};
+  const bool summing = p.column_sums && tn == 0;
   auto request = [&](uint64_t k) __attribute__((always_inline)) {
-    const T *const at_a = from_a + (kAlongA ? k : k * p.a_stride), *const at_b = from_b + (kAlongB ? k : k * p.b_stride);
     if (k + kTerms <= end) {
-      va.request(at_a, p.a_stride);
-      vb.request(at_b, p.b_stride);
+      va.template request<false>(k, 0u);
+      vb.template request<false>(k, 0u);
     } else {
       const uint32_t left = k < end ? static_cast<uint32_t>(end - k) : 0u;
-      va.request_some(at_a, p.a_stride, left > ka ? left - ka : 0u);
-      vb.request_some(at_b, p.b_stride, left > kb ? left - kb : 0u);
+      va.template request<true>(k, left);
+      vb.template request<true>(k, left);
     }
   };
   const uint32_t wm = wave / 2u * 64u, wn = wave % 2u * 64u;
   f32x4 acc[4][4] = {};
   request(begin);
   for (uint64_t k = begin; k < end; k += kTerms) {
-#pragma unroll
-    for (uint32_t i = 0; i < 16; i += 8) {
-      keep(va.v + i, ta + tile_at(ra, (ka + i) / 8u), kPlane);
-      keep(vb.v + i, tb + tile_at(rb, (kb + i) / 8u), kPlane);
-    }
+    if (summing) va.keep(ta, p.mask_scale, sums);
+    else va.keep(ta, p.mask_scale, nullptr);
+    vb.keep(tb, 1.0f, nullptr);
     __syncthreads();
     if (k + kTerms < end) request(k + kTerms);
     u32x4 b[P][4];
@@ -239,7 +587,6 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
       u32x4 a[P];
 #pragma unroll
       for (int c = 0; c < P; ++c) a[c] = *reinterpret_cast<const u32x4 *>(ta + c * kPlane + tile_at(wm + i * 16 + r, part));
-      // b is the first operand: a lane then ends up with four neighbouring columns of one row of the result
 #pragma unroll
       for (int s = P - 1; s >= 0; --s)
 #pragma unroll
@@ -249,9 +596,8 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     }
     __syncthreads();
   }
-  // A lane has four columns of 16 rows: through LDS, 16 rows at a time, they become lines of 64 columns (part c of row r at c ^ r).
+  // as the rows' kernel: lines of 64 columns
   f32x4 *const mine = reinterpret_cast<f32x4 *>(tile) + wave * 256u;
-  float sums[4] = {};
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -259,8 +605,7 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (uint32_t q = 0; q < 4; ++q) {
-      const uint32_t row = q * 4u + lane / 16u, c = n0 + wn + (lane & 15u) * 4u;
-      const uint64_t i = m0 + wm + m * 16u + row;
+      const uint32_t row = q * 4u + lane / 16u, c = n0 + wn + (lane & 15u) * 4u, i = m0 + wm + m * 16u + row;
       const f32x4 got = mine[row * 16u + ((lane & 15u) ^ row)];
       if (i >= p.M || c >= p.N) continue;
       float v[4] = {got.x, got.y, got.z, got.w};
@@ -268,34 +613,27 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(DenseArgs p) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
           if (fabsf(v[k]) < INFINITY || c + k >= p.N) continue;
-          const float *x = static_cast<const float *>(p.a) + (kAlongA ? i * p.a_stride : i), *y = static_cast<const float *>(p.b) + (kAlongB ? static_cast<uint64_t>(c + k) * p.b_stride : c + k);
-          v[k] = 0.0f;
-          for (uint64_t f = begin; f < end; ++f) v[k] = fmaf(x[kAlongA ? f : f * p.a_stride], y[kAlongB ? f : f * p.b_stride], v[k]);
+          v[k] = sum_of_terms(static_cast<const float *>(p.a) + begin * p.a_stride + i, MASKED ? static_cast<const float *>(p.y) + begin * p.a_stride + i : nullptr,
+                              p.mask_scale, p.a_stride, static_cast<const float *>(p.b) + begin * p.b_stride + c + k, p.b_stride, end - begin);
         }
       }
-      if (USE == kWeight && p.sums) {
-        put_columns(p.sums + (static_cast<uint64_t>(blockIdx.z) * p.M + i) * p.N + c, p.N - c, v, false);
-        continue;
-      }
-      finish_columns<T, USE>(p, step, i, c, v);
-      if (USE == kSlope) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sums[k] += v[k];
-      }
+      if (p.sums) put_columns(p.sums + (static_cast<uint64_t>(blockIdx.z) * p.M + i) * p.N + c, p.N - c, v, false);
+      else put_columns(static_cast<T *>(p.out) + static_cast<uint64_t>(i) * p.N + c, p.N - c, v, false);
     }
     __builtin_amdgcn_wave_barrier();
   }
-  if (USE != kSlope || !p.sums) return;
+  if (!summing) return;
   __syncthreads();
-  float(*const both)[kTile] = reinterpret_cast<float(*)[kTile]>(tile);
+  float(*const of_terms)[kTile] = reinterpret_cast<float(*)[kTile]>(tile);
+  of_terms[va.first / Terms<T, PAIRS, MASKED>::N][va.column] = sums[0];
+  if (PAIRS) of_terms[va.first / 8u][va.column + 1u] = sums[1];
+  __syncthreads();
+  if (t < kTile && m0 + t < p.M) {
+    float sum = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    sums[k] += __shfl_xor(sums[k], 16, kWave);
-    sums[k] += __shfl_xor(sums[k], 32, kWave);
-    if (lane < 16u) both[wave / 2u][wn + lane * 4u + k] = sums[k];
+    for (int i = 0; i < (PAIRS ? 4 : 2); ++i) sum += of_terms[i][t];
+    p.column_sums[static_cast<uint64_t>(blockIdx.z) * p.M + m0 + t] = sum;
   }
-  __syncthreads();
-  if (t < kTile && n0 + t < p.N) p.sums[static_cast<uint64_t>(tm) * p.N + n0 + t] = both[0][t] + both[1][t];
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------
@@ -309,7 +647,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void dense_few_kernel(DenseArgs p
   const uint32_t step = drop_step(p.drop);
   if (p.drop.step_kept && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.drop.step_kept = step;
   if (c >= p.N) return;
-  const T *const x = static_cast<const T *>(p.a), *const w = static_cast<const T *>(p.b) + static_cast<uint64_t>(c) * p.K;
+  const T *const x = static_cast<const T *>(p.a), *const w = static_cast<const T *>(p.w) + static_cast<uint64_t>(c) * p.K;
   float acc[R] = {};
   for (uint32_t k = lane * 8u; k < p.K; k += kWave * 8u) {
     float wv[8], xv[R][8];
@@ -341,7 +679,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void dense_few_kernel(DenseArgs p
   const uint64_t i = i0 + lane;
   if (lane >= R || i >= p.M) return;
   if (p.bias) v += get_value(static_cast<const T *>(p.bias) + c);
-  v = activate(v, p.act);
+  activate<1>(&v, p.act);
   if (p.drop.threshold) {
     const uint4 n = row_numbers(p.drop, step, static_cast<uint32_t>(i), c >> 3);
     const uint32_t word = c & 4u ? (c & 2u ? n.w : n.z) : (c & 2u ? n.y : n.x);
@@ -402,31 +740,65 @@ __global__ __launch_bounds__(kSumWaves *kWave) void dense_sum_kernel(T *__restri
 // ---- launches ---------------------------------------------------------------------------------------
 constexpr uint64_t kStreamed = 32ull << 20;  // an output from this size on is more than the L2s hold
 
-template <int USE>
-int launch_tiles(DenseArgs p, int type, uint32_t parts, hipStream_t stream) {
-  p.tiles_n = ceil_div(p.N, kTile);
-  const size_t size = type_size(type);
-  p.streamed = static_cast<uint64_t>(p.M) * p.N * size >= kStreamed;
-  // launches of at most 2^24 - 1 blocks: rows of the result in turns
-  const uint64_t turn = USE == kWeight ? p.M : static_cast<uint64_t>(kMostBlocks / p.tiles_n - kXcdTiles) * kTile;
-  for (uint64_t first = 0; first < p.M; first += turn) {
-    DenseArgs q = p;
-    q.M = static_cast<uint32_t>(std::min<uint64_t>(turn, p.M - first));
-    q.tiles_m = ceil_div(q.M, kTile);
-    q.row0 = static_cast<uint32_t>(first);
-    if (first) {
-      q.a = static_cast<const char *>(p.a) + first * p.a_stride * size;
-      q.out = static_cast<char *>(p.out) + first * p.N * size;
-      if (p.more) q.more = static_cast<const char *>(p.more) + first * p.N * size;
-      if (p.sums) q.sums = p.sums + first / kTile * p.N;
-    }
-    const dim3 grid(tile_blocks(q.tiles_m, q.tiles_n, 1), 1, parts);
-    if (type == NTS_F32) hipLaunchKernelGGL((dense_tile_kernel<float, USE>), grid, dim3(256), 0, stream, q);
-    else if (type == NTS_BF16) hipLaunchKernelGGL((dense_tile_kernel<Bf16, USE>), grid, dim3(256), 0, stream, q);
-    else hipLaunchKernelGGL((dense_tile_kernel<F16, USE>), grid, dim3(256), 0, stream, q);
-    NTS_LAUNCH_CHECK("dense_tile_kernel");
-  }
+// Bytes of a prepared weight.
+uint32_t tile_groups(uint32_t columns) { return ceil_div(columns, 2 * kTile) * 2u; }
+size_t prepared_bytes(int type, uint32_t columns, uint32_t terms) {
+  return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * (type == NTS_F32 ? 6 : 2);
+}
+template <bool ALONG>
+int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t terms, uint32_t stride, hipStream_t stream) {
+  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns)};
+  const dim3 grid(ceil_div(static_cast<uint64_t>(p.stages) * p.tiles * 4u * kTile, 256));
+  if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, ALONG>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied
+  NTS_LAUNCH_CHECK("dense_prepare_kernel");
   return NTS_OK;
+}
+
+// Workers that share the rows: two blocks to a compute unit.
+bool wide_rows(int type, uint32_t n, uint32_t N, uint32_t K) {
+  return type != NTS_F32 && K >= 512 && static_cast<uint64_t>(ceil_div(n, 256)) * ceil_div(N, kTile) >= 1024;
+}
+uint32_t workers_for(int type, uint32_t n, uint32_t N, bool wide) {
+  const uint32_t tiles = ceil_div(n, wide ? 256 : 128), columns = ceil_div(N, kTile);
+  return std::min(tiles, std::max(8u, (wide || type == NTS_F32 ? 512u : 768u) / columns / 8u * 8u));
+}
+template <typename T, int USE, int MR, bool MASKED = false>
+void launch_rows(DenseArgs p, hipStream_t stream) {
+  p.tiles_m = ceil_div(p.M, 64 * MR);
+  p.tiles_n = ceil_div(p.N, kTile);
+  p.streamed = static_cast<uint64_t>(p.M) * p.N * sizeof(T) >= kStreamed;
+  hipLaunchKernelGGL((dense_rows_kernel<T, USE, MR, 1, MASKED>), dim3(ceil_div(p.workers, 8) * 8u * p.tiles_n), dim3(256), 0, stream, p);
+}
+template <typename T, int USE>
+void launch_rows_of(const DenseArgs &p, bool wide, hipStream_t stream) {
+  constexpr int kWide = sizeof(T) == 4 ? 2 : 4;
+  if constexpr (USE == kRows) {
+    if (p.y) return launch_rows<T, USE, 2, true>(p, stream);  // four fragments of two operands do not fit the registers
+  }
+  wide ? launch_rows<T, USE, kWide>(p, stream) : launch_rows<T, USE, 2>(p, stream);
+}
+template <int USE>
+int launch_product(DenseArgs p, int type, hipStream_t stream) {
+  const bool wide = !p.y && wide_rows(type, p.M, p.N, p.K);
+  p.workers = workers_for(type, p.M, p.N, wide);
+  if (type == NTS_F32) launch_rows_of<float, USE>(p, wide, stream);
+  else if (type == NTS_BF16) launch_rows_of<Bf16, USE>(p, wide, stream);
+  else launch_rows_of<F16, USE>(p, wide, stream);
+  NTS_LAUNCH_CHECK("dense_rows_kernel");
+  return NTS_OK;
+}
+template <typename T>
+void launch_weight(const DenseArgs &p, const dim3 &grid, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.M % 2 == 0 && p.N % 2 == 0) {
+      if (p.y) hipLaunchKernelGGL((dense_weight_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
+      else hipLaunchKernelGGL((dense_weight_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
+      return;
+    }
+  }
+  if (p.y) hipLaunchKernelGGL((dense_weight_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dense_weight_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
 }
 template <typename T>
 void launch_few(const DenseArgs &p, hipStream_t stream) {
@@ -457,22 +829,28 @@ Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
   return p;
 }
 
-// The gradient's work: dz, the parts of the bias's sums and of the weight's.
+// The gradient's work: dz, the prepared weight, the parts of the bias's sums and of the weight's.
 struct Work {
-  size_t sums, parts, bytes;
-  uint32_t sum_parts;
-  Parts weight;
+  bool masked;   // dz comes from g and y
+  bool stored;   // dz is stored
+  bool beside;   // the bias's sums are made beside the weight's gradient
+  size_t weight_at, sums_at, parts_at, bytes;
+  uint32_t sums;
+  Parts parts;
 };
-Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, bool dropout, bool rows, bool weight, bool bias) {
+Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, bool dropout, bool has_y, bool rows, bool weight, bool bias) {
   Work w{};
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  const bool keeps = (act != NTS_ACT_NONE || dropout) && n;
-  w.sums = keeps ? up(static_cast<size_t>(n) * N * type_size(type)) : 0;
-  w.sum_parts = act != NTS_ACT_NONE ? ceil_div(n, kTile) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
-  w.parts = w.sums + (bias ? up(static_cast<size_t>(w.sum_parts) * N * sizeof(float)) : 0);
-  w.weight = weight_parts(n, N, F);
-  w.bytes = w.parts + (weight && w.weight.count > 1 ? static_cast<size_t>(w.weight.count) * N * F * sizeof(float) : 0);
-  (void)rows;
+  w.masked = act == NTS_ACT_RELU && has_y && (weight || !bias);
+  w.stored = !w.masked && (act != NTS_ACT_NONE || dropout) && n;
+  w.beside = bias && weight && !w.stored;
+  const bool again = w.stored && act != NTS_ACT_NONE;
+  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * type_size(type)) : 0;
+  w.sums_at = w.weight_at + up(std::max(again ? prepared_bytes(type, N, F) : 0, rows && n ? prepared_bytes(type, F, N) : 0));
+  w.parts = weight_parts(n, N, F);
+  w.sums = w.beside ? w.parts.count : again ? workers_for(type, n, N, wide_rows(type, n, N, F)) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
+  w.parts_at = w.sums_at + (bias ? up(static_cast<size_t>(w.sums) * N * sizeof(float)) : 0);
+  w.bytes = w.parts_at + (weight && w.parts.count > 1 ? static_cast<size_t>(w.parts.count) * N * F * sizeof(float) : 0);
   return w;
 }
 
@@ -495,8 +873,12 @@ using namespace nts;
 
 extern "C" {
 
+size_t nts_dense_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F) {
+  return bad_shapes(type, N, F, 0, nullptr) || n <= kFewRows ? 0 : prepared_bytes(type, N, F);
+}
+
 int nts_dense(void *y, const void *x, const void *w, const void *bias, const void *residual, int type, uint32_t n, uint32_t N,
-              uint32_t F, int activation, const nts_dropout_t *dropout, nts_stream_t stream) {
+              uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream) {
   NTS_TRACE_RANGE("nts_dense");
   if (const char *why = bad_shapes(type, N, F, activation, dropout)) return fail_in("nts_dense", why);
   if (n == 0) return NTS_OK;
@@ -504,8 +886,8 @@ int nts_dense(void *y, const void *x, const void *w, const void *bias, const voi
   for (const void *at : {static_cast<const void *>(y), x, w, bias, residual})
     if (!aligned_to(at, type_size(type))) return fail_in("nts_dense", "a value's alignment");
   DenseArgs p{};
-  p.a = x, p.b = w, p.M = n, p.N = N, p.K = F, p.a_stride = F, p.b_stride = F, p.out = y, p.bias = bias, p.more = residual;
-  p.act = activation, p.drop = drop_args(dropout), p.part_terms = F;
+  p.a = x, p.b = work, p.w = w, p.M = n, p.N = N, p.K = F, p.a_stride = F, p.out = y, p.bias = bias, p.more = residual;
+  p.act = activation, p.drop = drop_args(dropout);
   if (n <= kFewRows) {
     if (type == NTS_F32) launch_few<float>(p, stream);
     else if (type == NTS_BF16) launch_few<Bf16>(p, stream);
@@ -513,63 +895,76 @@ int nts_dense(void *y, const void *x, const void *w, const void *bias, const voi
     NTS_LAUNCH_CHECK("nts_dense");
     return NTS_OK;
   }
-  return launch_tiles<kLayer>(p, type, 1, stream);
+  if (!work || !aligned_to(work, 16)) return fail_in("nts_dense", "needs nts_dense_work_bytes of 16-byte-aligned work");
+  if (const int status = launch_prepare<true>(work, w, type, N, F, F, stream)) return status;
+  return launch_product<kLayer>(p, type, stream);
 }
 
-size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_rows, int with_weight, int with_bias) {
+size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_y, int with_rows,
+                                 int with_weight, int with_bias) {
   if (bad_shapes(type, N, F, activation, nullptr)) return 0;
-  return grad_work(type, n, N, F, activation, with_dropout != 0, with_rows != 0, with_weight != 0, with_bias != 0).bytes;
+  return grad_work(type, n, N, F, activation, with_dropout != 0, with_y != 0, with_rows != 0, with_weight != 0, with_bias != 0).bytes;
 }
 
-int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, const void *w, const void *bias, int type, uint32_t n,
-                   uint32_t N, uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream) {
+int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, const void *w, const void *bias, const void *y, int type,
+                   uint32_t n, uint32_t N, uint32_t F, int activation, const nts_dropout_t *dropout, void *work, nts_stream_t stream) {
   NTS_TRACE_RANGE("nts_dense_grad");
   const char *const name = "nts_dense_grad";
   if (const char *why = bad_shapes(type, N, F, activation, dropout)) return fail_in(name, why);
   if ((n == 0 || !gx) && !gw && !gb) return NTS_OK;
-  const bool again = activation != NTS_ACT_NONE;  // z is needed
+  const Work layout = grad_work(type, n, N, F, activation, dropout != nullptr, y != nullptr, gx != nullptr, gw != nullptr, gb != nullptr);
+  const bool again = layout.stored && activation != NTS_ACT_NONE;  // z is needed
   if (n && (!g || ((gw || again) && !x) || ((gx || again) && !w))) return fail_in(name, "null pointer");
-  for (const void *at : {static_cast<const void *>(gx), static_cast<const void *>(gw), static_cast<const void *>(gb), g, x, w, bias})
+  for (const void *at : {static_cast<const void *>(gx), static_cast<const void *>(gw), static_cast<const void *>(gb), g, x, w, bias, y})
     if (!aligned_to(at, type_size(type))) return fail_in(name, "a value's alignment");
-  const Work layout = grad_work(type, n, N, F, activation, dropout != nullptr, gx != nullptr, gw != nullptr, gb != nullptr);
   if (layout.bytes && (!work || !aligned_to(work, 16))) return fail_in(name, "needs nts_dense_grad_work_bytes of 16-byte-aligned work");
   char *const base = static_cast<char *>(work);
-  float *const sums = gb ? reinterpret_cast<float *>(base + layout.sums) : nullptr;
+  void *const prepared = base + layout.weight_at;
+  float *const sums = gb ? reinterpret_cast<float *>(base + layout.sums_at) : nullptr;
   const void *dz = g;
   DenseArgs p{};
-  p.drop = drop_args(dropout), p.act = activation;
+  p.drop = drop_args(dropout), p.act = activation, p.w = w, p.b = prepared, p.mask_scale = 1.0f;
   p.drop.step_kept = nullptr;
-  if (n && (again || dropout || gb)) {
+  if (n && (layout.stored || (gb && !layout.beside))) {
     DenseArgs q = p;
     q.more = g, q.M = n, q.N = N, q.sums = sums;
-    if (again || dropout) dz = q.out = work;
+    if (layout.stored) dz = q.out = work;
     if (again) {
-      q.a = x, q.b = w, q.K = F, q.a_stride = F, q.b_stride = F, q.bias = bias, q.part_terms = F;
-      if (const int status = launch_tiles<kSlope>(q, type, 1, stream)) return status;
+      q.a = x, q.K = F, q.a_stride = F, q.bias = bias;
+      if (const int status = launch_prepare<true>(prepared, w, type, N, F, F, stream)) return status;
+      if (const int status = launch_product<kSlope>(q, type, stream)) return status;
     } else {
-      const dim3 grid(ceil_div(N, kWave), layout.sum_parts);
+      const dim3 grid(ceil_div(N, kWave), layout.sums);
       if (type == NTS_F32) hipLaunchKernelGGL(dense_columns_kernel<float>, grid, dim3(256), 0, stream, q);
       else if (type == NTS_BF16) hipLaunchKernelGGL(dense_columns_kernel<Bf16>, grid, dim3(256), 0, stream, q);
       else hipLaunchKernelGGL(dense_columns_kernel<F16>, grid, dim3(256), 0, stream, q);
       NTS_LAUNCH_CHECK("dense_columns_kernel");
     }
   }
-  if (gb)
-    if (const int status = launch_sum(gb, type, sums, N, n ? layout.sum_parts : 0u, stream)) return status;
+  if (layout.masked) p.y = y, p.mask_scale = p.drop.scale;
   if (gx && n) {
     DenseArgs q = p;
-    q.a = dz, q.b = w, q.M = n, q.N = F, q.K = N, q.a_stride = N, q.b_stride = F, q.out = gx, q.part_terms = N;
-    if (const int status = launch_tiles<kRows>(q, type, 1, stream)) return status;
+    q.a = dz, q.M = n, q.N = F, q.K = N, q.a_stride = N, q.out = gx;
+    if (const int status = launch_prepare<false>(prepared, w, type, F, N, F, stream)) return status;
+    if (const int status = launch_product<kRows>(q, type, stream)) return status;
   }
   if (gw) {
     DenseArgs q = p;
-    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = N, q.b_stride = F, q.out = gw, q.part_terms = layout.weight.terms;
-    const uint32_t parts = layout.weight.count;
-    q.sums = parts > 1 ? reinterpret_cast<float *>(base + layout.parts) : nullptr;
-    if (const int status = launch_tiles<kWeight>(q, type, parts, stream)) return status;
+    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = N, q.b_stride = F, q.out = gw, q.part_terms = layout.parts.terms;
+    q.tiles_m = ceil_div(N, kTile), q.tiles_n = ceil_div(F, kTile);
+    if (layout.beside) q.column_sums = sums;
+    const uint32_t parts = layout.parts.count;
+    q.sums = parts > 1 ? reinterpret_cast<float *>(base + layout.parts_at) : nullptr;
+    const dim3 grid(q.tiles_m * q.tiles_n, 1, parts);
+    if (type == NTS_F32) launch_weight<float>(q, grid, stream);
+    else if (type == NTS_BF16) launch_weight<Bf16>(q, grid, stream);
+    else launch_weight<F16>(q, grid, stream);
+    NTS_LAUNCH_CHECK("dense_weight_kernel");
     if (parts > 1)
       if (const int status = launch_sum(gw, type, q.sums, static_cast<uint64_t>(N) * F, parts, stream)) return status;
   }
+  if (gb)
+    if (const int status = launch_sum(gb, type, sums, N, n || layout.beside ? layout.sums : 0u, stream)) return status;
   return NTS_OK;
 }
 

@@ -587,9 +587,25 @@ __global__ __launch_bounds__(256, (kWavesOf<T, KIND, REACH, WIDE ? kWide : kNarr
   if (pass == 0 && (threadIdx.x & ((1u << p.walker_shift) - 1u)) == 0) p.tail_row[span] = tail;
 }
 
-// The rows that were cut: 64 columns a block, its wavefronts take every kJoinWaves-th part, and the first adds up what they have, in
-// order.
-constexpr uint32_t kJoinWaves = 8, kJoinSpans = 8, kJoinAhead = 8;
+// The rows that were cut: 64 columns of kJoinSpans spans' rows a block.  Every wavefront takes rows of few parts of its own; of longer ones
+// all take every kJoinWaves-th part, and the first adds up what they have.  Parts in order, so the same bits on every call.
+constexpr uint32_t kJoinWaves = 16, kJoinSpans = 32, kJoinAhead = 8, kJoinAlone = 16;
+// What the parts of a column come to.  Forward: largest score, sum and weighted sum; by destination: none, mean, both sums.
+template <int KIND>
+struct Joined {
+  float top = KIND == kForward ? -INFINITY : 0.0f, sum = 0.0f, acc = 0.0f;
+  __device__ __forceinline__ void add(float t, float l, float v) {
+    if (KIND == kForward) {
+      const float now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
+      const float f = __builtin_amdgcn_exp2f(top - base), o = __builtin_amdgcn_exp2f(t - base);
+      top = now;
+      sum = sum * f + l * o;
+      acc = acc * f + v * o;
+    } else {
+      top += t, sum += l, acc += v;
+    }
+  }
+};
 template <typename T, int KIND>
 __global__ __launch_bounds__(kJoinWaves *kWave) void join_dot_spans_kernel(DotArgs p) {
   __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave];
@@ -598,75 +614,65 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_dot_spans_kernel(DotAr
   const uint64_t size = record_size<KIND>(p.q_heads, p.heads, p.D);
   const uint64_t span0 = static_cast<uint64_t>(blockIdx.x) * kJoinSpans;
   const uint32_t rows = lane < kJoinSpans && span0 + lane < p.spans ? p.tail_row[span0 + lane] : kNoSlot;
-  if (__ballot(rows != kNoSlot) == 0) return;  // the same in every wavefront
-  // where a record has the three numbers of a column: forward top, sum and weighted sum; by destination none, mean, both sums
+  uint64_t cut = __ballot(rows != kNoSlot);  // the same in every wavefront
+  // where a record has the three numbers of a column
   const uint64_t at_a = KIND == kForward ? columns + h : columns + cc, at_b = KIND == kForward ? columns + p.q_heads + h : 2ull * columns + h;
-  for (uint32_t k = 0; k < kJoinSpans; ++k) {
-    const uint64_t span = span0 + k;
-    const uint32_t row = wave_read(rows, k);
-    if (row == kNoSlot) continue;
-    const uint64_t last_at = static_cast<uint64_t>(row) * kRowCost + (kRowCost - 1u) + (p.offsets[row + 1] - p.offsets[0]);  // its last edge's
-    const uint64_t last = min<uint64_t>(last_at / p.span, p.spans - 1u);
-    float top = KIND == kForward ? -INFINITY : 0.0f, sum = 0.0f, acc = 0.0f;
-    for (uint64_t s = span + wave; s <= last; s += kJoinAhead * kJoinWaves) {
+  auto parts_of = [&](uint64_t first, uint64_t last, uint64_t from, uint64_t step) {
+    Joined<KIND> j;
+    for (uint64_t s = from; s <= last; s += kJoinAhead * step) {
       float t[kJoinAhead], l[kJoinAhead], v[kJoinAhead];
 #pragma unroll
       for (uint32_t u = 0; u < kJoinAhead; ++u) {
-        const uint64_t part = s + u * kJoinWaves;
+        const uint64_t part = s + u * step;
         t[u] = KIND == kForward ? -INFINITY : 0.0f, l[u] = v[u] = 0.0f;
         if (part <= last) {
-          const float *const record = p.partial + (part * 2u + (part == span ? 1u : 0u)) * size;
+          const float *const record = p.partial + (part * 2u + (part == first ? 1u : 0u)) * size;
           v[u] = record[cc];
           if (KIND != kBySource) t[u] = record[at_a], l[u] = record[at_b];
         }
       }
-      if (KIND == kForward) {
-        float now = top;
 #pragma unroll
-        for (uint32_t u = 0; u < kJoinAhead; ++u) now = fmaxf(now, t[u]);
-        const float base = now == -INFINITY ? 0.0f : now, f = __builtin_amdgcn_exp2f(top - base);
-        top = now;
-        sum *= f;
-        acc *= f;
-#pragma unroll
-        for (uint32_t u = 0; u < kJoinAhead; ++u) {
-          const float o = __builtin_amdgcn_exp2f(t[u] - base);
-          sum = fmaf(l[u], o, sum);
-          acc = fmaf(v[u], o, acc);
-        }
-      } else {
-#pragma unroll
-        for (uint32_t u = 0; u < kJoinAhead; ++u) top += t[u], sum += l[u], acc += v[u];
-      }
+      for (uint32_t u = 0; u < kJoinAhead; ++u) j.add(t[u], l[u], v[u]);
     }
-    tops[wave][lane] = top, sums[wave][lane] = sum, accs[wave][lane] = acc;
+    return j;
+  };
+  auto write = [&](uint32_t row, const Joined<KIND> &j) {
+    if (c >= columns) return;
+    const uint64_t head = static_cast<uint64_t>(row) * p.q_heads + h;
+    if (KIND == kForward) {
+      put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, j.sum == 0.0f ? 0.0f : j.acc / j.sum);
+      if (c == h * p.D) p.lse[head] = j.sum == 0.0f ? -INFINITY : (j.top + __builtin_amdgcn_logf(j.sum)) * kLn2;
+    } else if (KIND == kByDestination) {
+      put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, fmaf(-j.sum, j.top, j.acc) * p.score_scale);
+      if (c == h * p.D) {
+        const float l = p.lse[head];
+        p.ends[head] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, j.sum);
+      }
+    } else {
+      const bool second = c >= columns / 2u;
+      put_value(static_cast<T *>(second ? p.out2 : p.out) + static_cast<uint64_t>(row) * (columns / 2u) + (second ? c - columns / 2u : c), j.acc);
+    }
+  };
+  auto last_part = [&](uint32_t row) {  // where its last edge lies
+    const uint64_t at = static_cast<uint64_t>(row) * kRowCost + (kRowCost - 1u) + (offset_at(p.offsets, row + 1ull) - offset_at(p.offsets, 0));
+    return min<uint64_t>(at / p.span, p.spans - 1u);
+  };
+  uint64_t together = 0;
+  for (uint32_t taker = 0; cut; cut &= cut - 1, ++taker) {
+    const uint32_t k = __builtin_ctzll(cut), row = wave_read(rows, k);
+    const uint64_t first = span0 + k, last = last_part(row);
+    if (last - first >= kJoinAlone) together |= 1ull << k;
+    else if (taker % kJoinWaves == wave) write(row, parts_of(first, last, first, 1u));
+  }
+  for (; together; together &= together - 1) {
+    const uint32_t k = __builtin_ctzll(together), row = wave_read(rows, k);
+    const uint64_t first = span0 + k;
+    Joined<KIND> j = parts_of(first, last_part(row), first + wave, kJoinWaves);
+    tops[wave][lane] = j.top, sums[wave][lane] = j.sum, accs[wave][lane] = j.acc;
     __syncthreads();
-    if (wave == 0 && c < columns) {
-      for (uint32_t w = 1; w < kJoinWaves; ++w) {
-        if (KIND == kForward) {
-          const float t = tops[w][lane], now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
-          const float f = __builtin_amdgcn_exp2f(top - base), o = __builtin_amdgcn_exp2f(t - base);
-          top = now;
-          sum = sum * f + sums[w][lane] * o;
-          acc = acc * f + accs[w][lane] * o;
-        } else {
-          top += tops[w][lane], sum += sums[w][lane], acc += accs[w][lane];
-        }
-      }
-      const uint64_t head = static_cast<uint64_t>(row) * p.q_heads + h;
-      if (KIND == kForward) {
-        put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, sum == 0.0f ? 0.0f : acc / sum);
-        if (c == h * p.D) p.lse[head] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-      } else if (KIND == kByDestination) {
-        put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, fmaf(-sum, top, acc) * p.score_scale);
-        if (c == h * p.D) {
-          const float l = p.lse[head];
-          p.ends[head] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, sum);
-        }
-      } else {
-        const bool second = c >= columns / 2u;
-        put_value(static_cast<T *>(second ? p.out2 : p.out) + static_cast<uint64_t>(row) * (columns / 2u) + (second ? c - columns / 2u : c), acc);
-      }
+    if (wave == 0) {
+      for (uint32_t w = 1; w < kJoinWaves; ++w) j.add(tops[w][lane], sums[w][lane], accs[w][lane]);
+      write(row, j);
     }
     __syncthreads();
   }

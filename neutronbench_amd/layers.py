@@ -127,8 +127,8 @@ class DropoutOp:
 class DenseOp:
     """y = residual + drop(act(x W^T + bias)), W with a row per output; activation: none, relu, gelu or silu.  backward returns the
     gradient of x (None with rows_grad=False: feature rows are constants), get_additional_grad() those of W and bias (None without
-    one); the residual's is the gradient of y itself.  The sums are computed again in the backward pass: x, W and bias have to be
-    what they were."""
+    one); the residual's is the gradient of y itself.  The backward pass computes the sums again, or with relu and no residual reads from y
+    which were above 0: x, W, bias and y have to be what they were."""
 
     def __init__(self, activation="none", dropout=None, rows_grad=True):
         if activation not in ACTIVATIONS:
@@ -136,7 +136,7 @@ class DenseOp:
         if dropout is not None and not isinstance(dropout, Dropout):
             raise ValueError("dropout: a Dropout or None")
         self.activation, self.dropout, self.rows_grad = activation, dropout, rows_grad
-        self.x = self.weight = self.bias = self.drawn = self.gw = self.gb = None
+        self.x = self.weight = self.bias = self.y = self.drawn = self.gw = self.gb = None
 
     def forward(self, x, weight, bias=None, residual=None):
         kind = _type(x, "x")
@@ -152,9 +152,11 @@ class DenseOp:
         drawn = _drawn(self.dropout, dev)
         y = allocate(torch.empty, n, N, dtype=x.dtype, device=dev)
         with _on(dev):
+            work = _work(call("nts_dense_work_bytes", kind, n, N, F), dev)
             call("nts_dense", ptr(y), ptr(x), ptr(weight), ptr(bias), ptr(residual), kind, n, N, F, ACTIVATIONS[self.activation],
-                 _ref(drawn and drawn.desc), _stream(dev))
+                 _ref(drawn and drawn.desc), ptr(work), _stream(dev))
         self.x, self.weight, self.bias, self.drawn = x, weight, bias, drawn
+        self.y = y if self.activation == "relu" and residual is None else None
         return y
 
     def backward(self, g_out):
@@ -169,9 +171,10 @@ class DenseOp:
         self.gb = None if bias is None else allocate(torch.empty_like, bias)
         drawn = self.drawn and self.drawn.again()
         with _on(dev):
-            work = _work(call("nts_dense_grad_work_bytes", kind, n, N, F, act, drawn is not None, gx is not None, 1, bias is not None), dev)
-            call("nts_dense_grad", ptr(gx), ptr(self.gw), ptr(self.gb), ptr(g_out), ptr(x), ptr(weight), ptr(bias), kind, n, N, F, act,
-                 _ref(drawn), ptr(work), _stream(dev))
+            work = _work(call("nts_dense_grad_work_bytes", kind, n, N, F, act, drawn is not None, self.y is not None, gx is not None, 1,
+                              bias is not None), dev)
+            call("nts_dense_grad", ptr(gx), ptr(self.gw), ptr(self.gb), ptr(g_out), ptr(x), ptr(weight), ptr(bias), ptr(self.y), kind, n, N, F,
+                 act, _ref(drawn), ptr(work), _stream(dev))
         return gx
 
     def get_additional_grad(self):

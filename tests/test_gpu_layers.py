@@ -288,8 +288,9 @@ def test_dense_is_the_same_every_time_and_leaves_rows_behind(device):
         assert all(torch.equal(a, c) for a, c in zip(runs[0], other))
     out = torch.full((5100, 96), 7.0, dtype=BF16, device=device)
     desc = layers._Drawn(dropout, device).desc
+    work = layers._work(layers.call("nts_dense_work_bytes", 1, 5000, 96, 64), device)
     layers.call("nts_dense", out.data_ptr(), x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), 1, 5000, 96, 64, 2, layers._ref(desc),
-                layers._stream(x.device))
+                work.data_ptr(), layers._stream(x.device))
     assert torch.equal(out[:5000], runs[0][0]) and (out[5000:] == 7.0).all()
 
 

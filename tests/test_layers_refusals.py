@@ -44,48 +44,53 @@ def test_dropout():
 
 def test_dense():
     name = "nts_dense"
+    good = [P, P, P, 0, 0, 0, 40, 8, 8, 0, 0, P, 0]
     for N, F in ((0, 8), (8, 0), (BIG, 8), (8, BIG)):
-        refused("N or F", name, P, P, P, 0, 0, 0, 4, N, F, 0, 0, 0)
-    refused("unknown type", name, P, P, P, 0, 0, 7, 4, 8, 8, 0, 0, 0)
+        refused("N or F", name, *good[:7], N, F, *good[9:])
+    refused("unknown type", name, *good[:5], 7, *good[6:])
     for act in (-1, 4):
-        refused("unknown activation", name, P, P, P, 0, 0, 0, 4, 8, 8, act, 0, 0)
+        refused("unknown activation", name, *good[:9], act, *good[10:])
     for hole in range(3):
-        args = [P, P, P, 0, 0, 0, 4, 8, 8, 0, 0, 0]
+        args = list(good)
         args[hole] = 0
         refused("null pointer", name, *args)
     for at in range(5):
-        args = [P, P, P, P, P, 0, 4, 8, 8, 0, 0, 0]
+        args = list(good)
         args[at] = P + 2
         refused("alignment", name, *args)
+    for work in (0, P + 8):
+        refused("work_bytes", name, *good[:11], work, 0)
     bad = drop(2.0)
-    refused("within 0 .. 1", name, P, P, P, 0, 0, 0, 4, 8, 8, 0, ref(bad), 0)
-    assert abi.status(name, 0, 0, 0, 0, 0, 0, 0, 8, 8, 0, 0, 0) == abi.NTS_OK
+    refused("within 0 .. 1", name, *good[:10], ref(bad), P, 0)
+    assert abi.status(name, 0, 0, 0, 0, 0, 0, 0, 8, 8, 0, 0, 0, 0) == abi.NTS_OK
+    assert abi.call("nts_dense_work_bytes", 0, 1, 8, 8) == 0
 
 
 def test_dense_gradients():
     name = "nts_dense_grad"
-    good = [P, P, P, P, P, P, P, 0, 4, 8, 8, 1, 0, P, 0]
+    good = [P, P, P, P, P, P, P, 0, 0, 40, 8, 8, 2, 0, P, 0]
     for N, F in ((0, 8), (8, 0), (BIG, 8), (8, BIG)):
-        refused("N or F", name, *good[:9], N, F, *good[11:])
-    refused("unknown activation", name, *good[:11], 9, *good[12:])
+        refused("N or F", name, *good[:10], N, F, *good[12:])
+    refused("unknown activation", name, *good[:12], 9, *good[13:])
     for hole in (3, 4, 5):
         args = list(good)
         args[hole] = 0
         refused("null pointer", name, *args)
     for work in (0, P + 8):
-        refused("work_bytes", name, *good[:13], work, 0)
-    for at in range(7):
+        refused("work_bytes", name, *good[:14], work, 0)
+    for at in range(8):
         args = list(good)
         args[at] = P + 1
         refused("alignment", name, *args)
-    assert abi.status(name, 0, 0, 0, P, P, P, 0, 0, 4, 8, 8, 1, 0, 0, 0) == abi.NTS_OK  # nothing wanted
-    assert abi.call("nts_dense_grad_work_bytes", 0, 4, 0, 8, 1, 0, 1, 1, 1) == 0
-    assert abi.call("nts_dense_grad_work_bytes", 0, 100, 8, 8, 0, 0, 1, 0, 0) == 0
+    assert abi.status(name, 0, 0, 0, P, P, P, 0, 0, 0, 4, 8, 8, 1, 0, 0, 0) == abi.NTS_OK  # nothing wanted
+    # y says what relu's gradient needs: neither z nor the gradient of z is stored
+    with_y, without = (abi.call("nts_dense_grad_work_bytes", 0, 1000, 128, 64, 1, 1, y, 1, 1, 1) for y in (1, 0))
+    assert without - with_y >= 1000 * 128 * 4
 
 
 def test_attention():
     name = "nts_dot_attention"
-    good = [P, P, P, P, P, 0, P, P, 4, 5, 6, 4, 2, 16, 1.0, 0, 0, P, 0]
+    good = [P, P, P, P, P, 0, P, P, 100, 5, 6, 4, 2, 16, 1.0, 0, 0, P, 0]
     for q_heads, heads in ((0, 1), (4, 0), (4, 3), (2048, 2), (2, 4)):
         refused("q_heads", name, *good[:11], q_heads, heads, *good[13:])
     for width in (0, 257):
