@@ -7,6 +7,7 @@
 
 #include "launch_size.hpp"
 #include "layers.hpp"
+#include "tiles.hpp"
 
 namespace nts {
 namespace {
@@ -122,8 +123,11 @@ __device__ __forceinline__ void drop_two_rows(const DropArgs &d, uint32_t step, 
 // are left out, so that the sums in 32 bits are as good as a 32-bit product's.  An infinity's mid part is NaN: elements that are not
 // finite are computed again term by term.
 constexpr uint32_t kTile = 128, kTerms = 32, kPlane = kTile * kTerms;
-// Where 8 of a row's 32 terms lie in LDS: the 16 lanes that read one part of 16 rows meet all banks once.
-__host__ __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t part) { return row * kTerms + ((part ^ (row >> 2)) & 3u) * 8u; }
+// Where 8 of a row's 32 terms lie in LDS.  A read of 16 bytes by a wavefront goes in quarters of 16 lanes, four neighbours' worth each of two
+// parts (rows 0..3 and 12..15 of one with 4..11 of the next, and so on): with the four groups of rows at 0, 2, 3, 1 such a quarter meets
+// every bank once, as 16 rows of one part do.  At 0, 1, 2, 3 every read took half as long again.
+__host__ __device__ __forceinline__ uint32_t part_at(uint32_t row, uint32_t part) { return (part ^ (0x78u >> ((row >> 2 & 3u) * 2u))) & 3u; }
+__host__ __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t part) { return row * kTerms + part_at(row, part) * 8u; }
 
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
@@ -215,13 +219,124 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// What a wavefront's 16 * MR rows by 128 columns of sums become.  Through LDS (`mine`, 4 KB), 16 rows by 64 columns at a time, a lane's columns
+// become lines (part c of row r at c ^ r).  sums: of the columns, kept over tiles.
+template <typename T, int USE, int MR, bool MASKED>
+__device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f32x4 (&acc)[MR][8], f32x4 *mine, uint64_t first_row, uint32_t column0,
+                                            const float (&bias)[2][4], float (&sums)[2][4]) {
+  constexpr int P = kPlanes<T>;
+  const uint32_t lane = threadIdx.x & (kWave - 1), r = lane & 15u, part = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < MR; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine[r * 16u + ((j * 4u + part) ^ r)] = acc[i][h * 4 + j];
+      __builtin_amdgcn_wave_barrier();
+      const uint32_t c = column0 + h * 64u + (lane & 15u) * 4u;
+      const uint64_t row0 = first_row + i * 16u + lane / 16u;
+      // two rows of a lane at a time, the next ones' second operand on its way; not unrolled, or the registers do not hold what is behind it
+      float ahead[2][4] = {};
+      auto read = [&](uint32_t q) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u)
+          if (USE != kRows && p.more && row0 + (q + u) * 4u < p.M && c < p.N)
+            get_columns(static_cast<const T *>(p.more) + (row0 + (q + u) * 4u) * p.N + c, p.N - c, ahead[u]);
+      };
+      read(0);
+#pragma unroll 1
+      for (uint32_t q = 0; q < 4; q += 2) {
+        float v[2][4], more[2][4];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+          const uint32_t row = (q + u) * 4u + lane / 16u;
+          const uint64_t at = row0 + (q + u) * 4u;
+          const f32x4 got = mine[row * 16u + ((lane & 15u) ^ row)];
+          v[u][0] = got.x, v[u][1] = got.y, v[u][2] = got.z, v[u][3] = got.w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) more[u][k] = ahead[u][k];
+          if (P == 3) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              if (fabsf(v[u][k]) < INFINITY || at >= p.M || c + k >= p.N) continue;
+              const float *const b = static_cast<const float *>(p.w);
+              v[u][k] = sum_of_terms(static_cast<const float *>(p.a) + at * p.a_stride,
+                                     MASKED ? static_cast<const float *>(p.y) + at * p.a_stride : nullptr, p.mask_scale, 1,
+                                     USE == kRows ? b + c + k : b + static_cast<uint64_t>(c + k) * p.K, USE == kRows ? p.N : 1u, p.K);
+            }
+          }
+          if (USE != kRows) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[u][k] += bias[h][k];
+          }
+          if (USE == kLayer) activate<4>(v[u], p.act);
+        }
+        if (q == 0) read(2);
+        if (USE != kRows && p.drop.threshold) {
+          float(*const dropping)[4] = USE == kLayer ? v : more;
+          drop_two_rows(p.drop, step, static_cast<uint32_t>(row0) + q * 4u, static_cast<uint32_t>(row0) + q * 4u + 4u, c, dropping[0], dropping[1]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+          const uint64_t at = row0 + (q + u) * 4u;
+          if (USE == kLayer && p.more) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[u][k] += more[u][k];
+          }
+          if (USE == kSlope) through_slope(v[u], more[u], p.act);
+          if (at >= p.M || c >= p.N) continue;
+          put_columns(static_cast<T *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
+          if (USE == kSlope) {  // columns that are not there are summed and not stored
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sums[h][k] += v[u][k];
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void bias_of_columns(const DenseArgs &p, uint32_t column0, float (&bias)[2][4]) {
+  if (!p.bias) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t c = column0 + h * 64u + (threadIdx.x & 15u) * 4u;
+    if (c < p.N) get_columns(static_cast<const T *>(p.bias) + c, p.N - c, bias[h]);
+  }
+}
+// The block's column sums to row `to` of p.sums: of a wavefront's four rows of lanes, then of the ROWS wavefronts of rows of each group of 128
+// columns.
+template <int WAVES, int ROWS>
+__device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sums)[2][4], float (*of_wave)[kTile], uint32_t to, uint32_t column0) {
+  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block();
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v = sums[h][k];
+      v += __shfl_xor(v, 16, kWave);
+      v += __shfl_xor(v, 32, kWave);
+      if (lane < 16u) of_wave[wave][h * 64u + lane * 4u + k] = v;
+    }
+  __syncthreads();
+  if (t < kTile * (WAVES / ROWS)) {
+    const uint32_t group = t / kTile, c = column0 + t;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < ROWS; ++w) v += of_wave[group * ROWS + w][t % kTile];
+    if (c < p.N) p.sums[static_cast<uint64_t>(to) * p.N + c] = v;
+  }
+}
+
 // Many rows.  A block of 4 * WN wavefronts takes 64 * MR rows by 128 * WN columns, a stage of 32 terms after the other, and then its next
 // rows.  Rows go from memory to the registers that the matrix instructions read, each to the one wavefront (of a column group) that
 // needs them, and are split there; the prepared weight goes to LDS by loads that write it themselves.  Both are a stage ahead, past the end
 // of a tile too.
 // MR: 16 rows each, of a wavefront.
 template <typename T, int USE, int MR, int WN, bool MASKED>
-__global__ __launch_bounds__(256 * WN, MR == 4 || sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
+__global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
   constexpr int P = kPlanes<T>;
   constexpr uint32_t kRows = 64 * MR, kStage = WN * P * kPlane;
   // results are turned where the stage of the weight was that has been used last, if it is large enough
@@ -302,13 +417,7 @@ __global__ __launch_bounds__(256 * WN, MR == 4 || sizeof(T) == 4 ? 2 : 3) void d
   f32x4 acc[MR][8];
   uint32_t half = 0;
   float bias[2][4] = {};
-  if (USE != kRows && p.bias) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t c = tn * (kTile * WN) + wc * kTile + h * 64u + (lane & 15u) * 4u;
-      if (c < p.N) get_columns(static_cast<const T *>(p.bias) + c, p.N - c, bias[h]);
-    }
-  }
+  if (USE != kRows) bias_of_columns<T>(p, tn * (kTile * WN) + wc * kTile, bias);
   float sums[2][4] = {};
   place(worker);
   request_weight(weight0, 0);
@@ -366,99 +475,111 @@ __global__ __launch_bounds__(256 * WN, MR == 4 || sizeof(T) == 4 ? 2 : 3) void d
             for (int i = 0; i < MR; ++i) acc[i][j] = multiply<T>(b[j & 1][q - c], a[i][c], acc[i][j]);
       }
     }
-    // Through LDS, 16 rows by 64 columns at a time, a lane's columns become lines (part c of row r at c ^ r).
     if (!kApart) __builtin_amdgcn_s_barrier();  // all have read it
-    f32x4 *const mine = reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u;
-#pragma unroll
-    for (int i = 0; i < MR; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mine[r * 16u + ((j * 4u + part) ^ r)] = acc[i][h * 4 + j];
-        __builtin_amdgcn_wave_barrier();
-        const uint32_t c = tn * (kTile * WN) + wc * kTile + h * 64u + (lane & 15u) * 4u;
-        const uint64_t row0 = static_cast<uint64_t>(tile) * kRows + wr * (16u * MR) + i * 16u + lane / 16u;
-        // two rows of a lane at a time, the next ones' second operand on its way; not unrolled, or the registers do not hold what is behind it
-        float ahead[2][4] = {};
-        auto read = [&](uint32_t q) __attribute__((always_inline)) {
-#pragma unroll
-          for (uint32_t u = 0; u < 2; ++u)
-            if (USE != kRows && p.more && row0 + (q + u) * 4u < p.M && c < p.N)
-              get_columns(static_cast<const T *>(p.more) + (row0 + (q + u) * 4u) * p.N + c, p.N - c, ahead[u]);
-        };
-        read(0);
-#pragma unroll 1
-        for (uint32_t q = 0; q < 4; q += 2) {
-          float v[2][4], more[2][4];
-#pragma unroll
-          for (uint32_t u = 0; u < 2; ++u) {
-            const uint32_t row = (q + u) * 4u + lane / 16u;
-            const uint64_t at = row0 + (q + u) * 4u;
-            const f32x4 got = mine[row * 16u + ((lane & 15u) ^ row)];
-            v[u][0] = got.x, v[u][1] = got.y, v[u][2] = got.z, v[u][3] = got.w;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) more[u][k] = ahead[u][k];
-            if (P == 3) {
-#pragma unroll
-              for (uint32_t k = 0; k < 4; ++k) {
-                if (fabsf(v[u][k]) < INFINITY || at >= p.M || c + k >= p.N) continue;
-                const float *const b = static_cast<const float *>(p.w);
-                v[u][k] = sum_of_terms(static_cast<const float *>(p.a) + at * p.a_stride,
-                                       MASKED ? static_cast<const float *>(p.y) + at * p.a_stride : nullptr, p.mask_scale, 1,
-                                       USE == kRows ? b + c + k : b + static_cast<uint64_t>(c + k) * p.K, USE == kRows ? p.N : 1u, p.K);
-              }
-            }
-            if (USE != kRows) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[u][k] += bias[h][k];
-            }
-            if (USE == kLayer) activate<4>(v[u], p.act);
-          }
-          if (q == 0) read(2);
-          if (USE != kRows && p.drop.threshold) {
-            float(*const dropping)[4] = USE == kLayer ? v : more;
-            drop_two_rows(p.drop, step, static_cast<uint32_t>(row0) + q * 4u, static_cast<uint32_t>(row0) + q * 4u + 4u, c, dropping[0], dropping[1]);
-          }
-#pragma unroll
-          for (uint32_t u = 0; u < 2; ++u) {
-            const uint64_t at = row0 + (q + u) * 4u;
-            if (USE == kLayer && p.more) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[u][k] += more[u][k];
-            }
-            if (USE == kSlope) through_slope(v[u], more[u], p.act);
-            if (at >= p.M || c >= p.N) continue;
-            put_columns(static_cast<T *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
-            if (USE == kSlope) {  // columns that are not there are summed and not stored
-#pragma unroll
-              for (int k = 0; k < 4; ++k) sums[h][k] += v[u][k];
-            }
-          }
-        }
-        __builtin_amdgcn_wave_barrier();
-      }
+    finish_tile<T, USE, MR, MASKED>(p, step, acc, reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u,
+                                    static_cast<uint64_t>(tile) * kRows + wr * (16u * MR), tn * (kTile * WN) + wc * kTile, bias, sums);
   }
-  if (USE != kSlope || !p.sums) return;
-  __syncthreads();
-  // the block's column sums: of a wavefront's four rows of lanes, then of its four wavefronts of rows
-  float(*const of_wave)[kTile] = reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0);
+  if (USE == kSlope && p.sums) block_sums<4 * WN, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0), worker, tn * (kTile * WN));
+}
+
+// Large products of 16-bit values whose rows begin at multiples of 16 bytes: a block of eight wavefronts takes 256 rows by 256 columns, 32
+// terms at a time, which loads write to LDS themselves, three stages ahead of the one that is multiplied.  Both operands lie as they do in
+// memory: b's row j holds column j's terms; in LDS as tile_at says.  65,536 rows of 4,096 by 4,096 with GELU, drops and a residual take 2,110
+// us, 1,040 TF/s.  LDS bounds it: a stage's 96 reads and 32 KB of writes hold it for 1,024 cycles, as long as the matrix instructions take.
+// (Four wavefronts of 128 by 128 read a third less, but their 256 sums leave too few registers: 3,170 us, moves between the two halves of the
+// register file; all wavefronts in step: 2,510; dense_rows_kernel: 2,830.)
+constexpr uint32_t kWideTile = 256, kWideStages = 4;
+__device__ __attribute__((aligned(16))) uint16_t zero_part[8];
+template <typename T, int USE>
+__global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
+  constexpr uint32_t kOperand = kWideTile * kTerms;
+  __shared__ __attribute__((aligned(16))) uint16_t stages[kWideStages][2 * kOperand];
+  const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
+  uint32_t tm, tn;
+  tile_of(p.tiles_n, p.tiles_m >= kXcdTiles, 8, &tm, &tn);
+  if (tm >= p.tiles_m) return;
+  const uint32_t step = USE == kRows ? 0u : drop_step(p.drop);
+  if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
+  // A load takes 16 rows' 64 bytes, and a wavefront every eighth of the 32 loads of a stage.  Rows that are not there read the last one.
+  const uint64_t row_a = static_cast<uint64_t>(tm) * kWideTile, row_b = static_cast<uint64_t>(tn) * kWideTile;
+  const char *const from_a = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.a) + row_a * p.a_stride);
+  const char *const from_b = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.b) + row_b * p.b_stride);
+  const uint32_t chunk = part_at(lane / 4u, lane & 3u);  // the same for all of the lane's rows, which are 16 apart
+  uint32_t at[4];  // in bytes: below 2^26, as 256 rows of 2^17 values are
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t row = ((i & 1) * 8u + wave) * 16u + lane / 4u;
+    at[i] = (i < 2 ? static_cast<uint32_t>(min(static_cast<uint64_t>(row), p.M - 1u - row_a)) * p.a_stride
+                   : static_cast<uint32_t>(min(static_cast<uint64_t>(row), p.N - 1u - row_b)) * p.b_stride) * 2u + chunk * 16u;
+  }
+  auto request = [&](uint16_t *to, uint32_t k) __attribute__((always_inline)) {
+    const char *const a = from_a + k * 2ull, *const b = from_b + k * 2ull;
+    if (k + kTerms <= p.K) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float v = sums[h][k];
-      v += __shfl_xor(v, 16, kWave);
-      v += __shfl_xor(v, 32, kWave);
-      if (lane < 16u) of_wave[wave][h * 64u + lane * 4u + k] = v;
+      for (int i = 0; i < 4; ++i) load_to_lds(reinterpret_cast<const uint16_t *>((i < 2 ? a : b) + at[i]), to + (i * 8u + wave) * 512u);
+      return;
     }
-  __syncthreads();
-  if (t < kTile * WN) {
-    const uint32_t group = t / kTile, c = tn * (kTile * WN) + t;
-    float v = 0.0f;
+    const bool inside = k + chunk * 8u < p.K;  // whole parts: rows are of multiples of eight
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v += of_wave[group * 4 + w][t % kTile];
-    if (c < p.N) p.sums[static_cast<uint64_t>(worker) * p.N + c] = v;
+    for (int i = 0; i < 4; ++i)
+      load_to_lds(inside ? reinterpret_cast<const uint16_t *>((i < 2 ? a : b) + at[i]) : zero_part, to + (i * 8u + wave) * 512u);
+  };
+  const uint32_t wr = wave & 3u, wc = wave >> 2;
+  f32x4 acc[4][8] = {};
+  u32x4 rows[4], columns[8];
+#pragma unroll
+  for (uint32_t s = 0; s < kWideStages - 1; ++s) request(stages[s], s * kTerms);
+  // Two wavefronts share a SIMD, and while one multiplies the other reads LDS: those of the upper columns are half a stage behind.  A stage
+  // is read by the lower ones in slot 2s and by the upper ones in slot 2s + 1, so its loads are waited for in the slots before, and its place
+  // is written again three stages on.
+  auto slot_ends = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // All LDS reads are done, and of the wavefront's loads all but those of two stages, eight.
+  auto stage_comes = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0078);
+  };
+  stage_comes();
+  if (wc) slot_ends();
+  // Whole turns, so that the stages' places are constants; stages behind the last term are zeros that no memory is read for.
+  for (uint32_t k = 0; k < p.K; k += kWideStages * kTerms) {
+#pragma unroll
+    for (uint32_t s = 0; s < kWideStages; ++s) {
+      slot_ends();
+      request(stages[(s + kWideStages - 1) % kWideStages], k + (s + kWideStages - 1) * kTerms);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = *reinterpret_cast<const u32x4 *>(stages[s] + tile_at(wr * 64u + i * 16u + r, part));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) columns[j] = *reinterpret_cast<const u32x4 *>(stages[s] + kOperand + wc * kPlane + tile_at(j * 16u + r, part));
+      stage_comes();
+      slot_ends();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][j] = multiply<T>(columns[j], rows[i], acc[i][j]);
+    }
   }
+  if (!wc) slot_ends();
+  stage_barrier();  // no load may reach the LDS any more
+  float bias[2][4] = {}, sums[2][4] = {};
+  if (USE != kRows) bias_of_columns<T>(p, tn * kWideTile + wc * kTile, bias);
+  finish_tile<T, USE, 4, false>(p, step, acc, reinterpret_cast<f32x4 *>(&stages[0][0]) + wave * 256u, static_cast<uint64_t>(tm) * kWideTile + wr * 64u,
+                                tn * kWideTile + wc * kTile, bias, sums);
+  if (USE == kSlope && p.sums) block_sums<8, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(&stages[2][0]), tm, tn * kWideTile);
+}
+// The weight with rows and columns exchanged, rows of `stride` values: [columns, stride], zeros behind `rows` of them.
+__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns, uint32_t stride) {
+  __shared__ uint16_t tile[64][66];
+  const uint32_t x = threadIdx.x % 64u, y = threadIdx.x / 64u, c0 = blockIdx.x * 64u, r0 = blockIdx.y * 64u;
+  for (uint32_t i = y; i < 64u; i += 4u) tile[i][x] = r0 + i < rows && c0 + x < columns ? from[static_cast<uint64_t>(r0 + i) * columns + c0 + x] : uint16_t{0};
+  __syncthreads();
+  for (uint32_t i = y; i < 64u; i += 4u)
+    if (c0 + i < columns && r0 + x < stride) to[static_cast<uint64_t>(c0 + i) * stride + r0 + x] = tile[x][i];
 }
 
 // ---- the weight's gradient --------------------------------------------------------------------------
@@ -690,30 +811,49 @@ __global__ __launch_bounds__(kFewWaves *kWave) void dense_few_kernel(DenseArgs p
 }
 
 // ---- sums -------------------------------------------------------------------------------------------
-// The gradient of y where the activation's slope is 1: dropped (if out is not null) and summed by columns.  A block takes 64 columns and
-// every gridDim.y-th group of 4 rows.
+// The gradient of y where no sums are needed: dropped, or by y as DenseArgs say (if out is not null), and summed by columns.  A lane has four
+// columns, a wavefront four rows of 64; a block takes every gridDim.y-th group of 32 rows.
 template <typename T>
 __global__ __launch_bounds__(256) void dense_columns_kernel(DenseArgs p) {
-  __shared__ float sums[4][kWave];
-  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block(), c = blockIdx.x * kWave + lane;
-  const uint32_t step = drop_step(p.drop);
-  float sum = 0.0f;
-  if (c < p.N) {
-    for (uint64_t i = blockIdx.y * 4ull + wave; i < p.M; i += gridDim.y * 4ull) {
-      float v = get_value(static_cast<const T *>(p.more) + i * p.N + c);
-      if (p.drop.threshold) {
-        const uint4 n = row_numbers(p.drop, step, static_cast<uint32_t>(i), c >> 3);
-        const uint32_t word = c & 4u ? (c & 2u ? n.w : n.z) : (c & 2u ? n.y : n.x);
-        v = (c & 1u ? word >> 16 : word & 0xFFFFu) >= p.drop.threshold ? v * p.drop.scale : 0.0f;
-      }
-      if (p.out) put_value(static_cast<T *>(p.out) + i * p.N + c, v);
-      sum += v;
+  __shared__ float of_wave[4][kWave];
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block(), c = blockIdx.x * kWave + (lane & 15u) * 4u;
+  const uint32_t step = drop_step(p.drop), count = c < p.N ? p.N - c : 0u;
+  float sums[4] = {};
+  for (uint64_t i0 = blockIdx.y * 32ull + wave * 8u + lane / 16u; i0 < p.M; i0 += gridDim.y * 32ull) {
+    float v[2][4] = {}, y[2][4] = {};
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      if (i0 + u * 4u >= p.M || !count) continue;
+      get_columns(static_cast<const T *>(p.more) + (i0 + u * 4u) * p.N + c, count, v[u]);
+      if (p.y) get_columns(static_cast<const T *>(p.y) + (i0 + u * 4u) * p.N + c, count, y[u]);
+    }
+    if (p.y) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[u][k] = y[u][k] <= 0.0f ? 0.0f : v[u][k] * p.mask_scale;
+    } else if (p.drop.threshold) {
+      drop_two_rows(p.drop, step, static_cast<uint32_t>(i0), static_cast<uint32_t>(i0) + 4u, c, v[0], v[1]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      if (i0 + u * 4u >= p.M || !count) continue;
+      if (p.out) put_columns(static_cast<T *>(p.out) + (i0 + u * 4u) * p.N + c, count, v[u], false);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sums[k] += v[u][k];
     }
   }
   if (!p.sums) return;
-  sums[wave][lane] = sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    sums[k] += __shfl_xor(sums[k], 16, kWave);
+    sums[k] += __shfl_xor(sums[k], 32, kWave);
+    if (lane < 16u) of_wave[wave][lane * 4u + k] = sums[k];
+  }
   __syncthreads();
-  if (wave == 0 && c < p.N) p.sums[static_cast<uint64_t>(blockIdx.y) * p.N + c] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  const uint32_t column = blockIdx.x * kWave + threadIdx.x;
+  if (threadIdx.x < kWave && column < p.N)
+    p.sums[static_cast<uint64_t>(blockIdx.y) * p.N + column] = (of_wave[0][threadIdx.x] + of_wave[1][threadIdx.x]) + (of_wave[2][threadIdx.x] + of_wave[3][threadIdx.x]);
 }
 
 // out = the sum of `parts` arrays of `count` floats, in order: the wavefronts take every kSumWaves-th part of 64 values, and the first
@@ -755,36 +895,66 @@ int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t
   return NTS_OK;
 }
 
-// Workers that share the rows: two blocks to a compute unit.
-bool wide_rows(int type, uint32_t n, uint32_t N, uint32_t K) {
-  return type != NTS_F32 && K >= 512 && static_cast<uint64_t>(ceil_div(n, 256)) * ceil_div(N, kTile) >= 1024;
+// Large products by large tiles, where there are enough of them for the chip and rows of many terms; in us by large tiles and by rows:
+// 16,384 x 1,024 x 512 26 and 38, 65,536 x 256 x 1,024 42 and 63; of 256 terms 32,768 x 4,096 150 and 129; of 128 tiles 8,192 x 1,024 x 1,024
+// 34 and 34.
+bool by_wide_tiles(int type, uint32_t n, uint32_t N, uint32_t K) {
+  return type != NTS_F32 && K >= 512 && K % 8 == 0 && static_cast<uint64_t>(ceil_div(n, kWideTile)) * ceil_div(N, kWideTile) >= 256;
 }
-uint32_t workers_for(int type, uint32_t n, uint32_t N, bool wide) {
-  const uint32_t tiles = ceil_div(n, wide ? 256 : 128), columns = ceil_div(N, kTile);
-  return std::min(tiles, std::max(8u, (wide || type == NTS_F32 ? 512u : 768u) / columns / 8u * 8u));
+uint32_t turned_stride(uint32_t terms) { return (terms + 7u) / 8u * 8u; }
+// Bytes of a product's weight in the work: as the rows' kernel wants it, or turned for large tiles.
+size_t weight_bytes(int type, uint32_t n, uint32_t columns, uint32_t terms, bool turned) {
+  // operands between aligned addresses take the rows' kernel all the same
+  return std::max(prepared_bytes(type, columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * turned_stride(terms) * 2 : size_t{0});
 }
-template <typename T, int USE, int MR, bool MASKED = false>
+// Workers that share the rows: two blocks to a compute unit, three of 16-bit values.
+uint32_t workers_for(int type, uint32_t n, uint32_t N, uint32_t K) {
+  if (by_wide_tiles(type, n, N, K)) return ceil_div(n, kWideTile);
+  const uint32_t tiles = ceil_div(n, kTile), columns = ceil_div(N, kTile);
+  return std::min(tiles, std::max(8u, (type == NTS_F32 ? 512u : 768u) / columns / 8u * 8u));
+}
+template <typename T, int USE, bool MASKED = false>
 void launch_rows(DenseArgs p, hipStream_t stream) {
-  p.tiles_m = ceil_div(p.M, 64 * MR);
+  p.tiles_m = ceil_div(p.M, kTile);
   p.tiles_n = ceil_div(p.N, kTile);
-  p.streamed = static_cast<uint64_t>(p.M) * p.N * sizeof(T) >= kStreamed;
-  hipLaunchKernelGGL((dense_rows_kernel<T, USE, MR, 1, MASKED>), dim3(ceil_div(p.workers, 8) * 8u * p.tiles_n), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((dense_rows_kernel<T, USE, 2, 1, MASKED>), dim3(ceil_div(p.workers, 8) * 8u * p.tiles_n), dim3(256), 0, stream, p);
 }
 template <typename T, int USE>
-void launch_rows_of(const DenseArgs &p, bool wide, hipStream_t stream) {
-  constexpr int kWide = sizeof(T) == 4 ? 2 : 4;
-  if constexpr (USE == kRows) {
-    if (p.y) return launch_rows<T, USE, 2, true>(p, stream);  // four fragments of two operands do not fit the registers
+void launch_product_of(DenseArgs p, bool wide, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (wide) {
+      p.tiles_m = ceil_div(p.M, kWideTile);
+      p.tiles_n = ceil_div(p.N, kWideTile);
+      hipLaunchKernelGGL((dense_wide_kernel<T, USE>), dim3(tile_blocks(p.tiles_m, p.tiles_n, 8)), dim3(512), 0, stream, p);
+      return;
+    }
   }
-  wide ? launch_rows<T, USE, kWide>(p, stream) : launch_rows<T, USE, 2>(p, stream);
+  if constexpr (USE == kRows) {
+    if (p.y) return launch_rows<T, USE, true>(p, stream);
+  }
+  launch_rows<T, USE>(p, stream);
 }
+// The product of p.a and the weight p.w, whose form for it goes to `work`.
 template <int USE>
-int launch_product(DenseArgs p, int type, hipStream_t stream) {
-  const bool wide = !p.y && wide_rows(type, p.M, p.N, p.K);
-  p.workers = workers_for(type, p.M, p.N, wide);
-  if (type == NTS_F32) launch_rows_of<float, USE>(p, wide, stream);
-  else if (type == NTS_BF16) launch_rows_of<Bf16, USE>(p, wide, stream);
-  else launch_rows_of<F16, USE>(p, wide, stream);
+int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
+  const bool wide = !p.y && by_wide_tiles(type, p.M, p.N, p.K) && aligned_to(p.a, 16) && (USE == kRows || aligned_to(p.w, 16));
+  p.workers = workers_for(type, p.M, p.N, p.K);
+  p.streamed = static_cast<uint64_t>(p.M) * p.N * type_size(type) >= kStreamed;
+  p.b = work;
+  if (!wide) {
+    const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, stream) : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, stream);
+    if (status) return status;
+  } else if (USE == kRows) {
+    p.b_stride = turned_stride(p.K);
+    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(p.b_stride, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
+                       static_cast<const uint16_t *>(p.w), p.K, p.N, p.b_stride);
+    NTS_LAUNCH_CHECK("dense_turn_kernel");
+  } else {
+    p.b = p.w, p.b_stride = p.K;
+  }
+  if (type == NTS_F32) launch_product_of<float, USE>(p, wide, stream);
+  else if (type == NTS_BF16) launch_product_of<Bf16, USE>(p, wide, stream);
+  else launch_product_of<F16, USE>(p, wide, stream);
   NTS_LAUNCH_CHECK("dense_rows_kernel");
   return NTS_OK;
 }
@@ -815,7 +985,9 @@ int launch_sum(void *out, int type, const float *from, uint64_t count, uint32_t 
   return NTS_OK;
 }
 
-// Parts of the weight's gradient, of few results and many terms: 512 blocks, two for a compute unit, and none of fewer than 256 terms.
+// Parts of the weight's gradient, of few results and many terms: two blocks for a compute unit, and no part of fewer than 256 terms.
+// (All tiles of a part on one chiplet, whose L2 then reads its rows once, took 620 us instead of 515 at 232,965 terms of 256 by 602: the parts
+// are then a multiple of eight and fewer.)
 struct Parts {
   uint32_t count, terms;
 };
@@ -831,7 +1003,8 @@ Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
 
 // The gradient's work: dz, the prepared weight, the parts of the bias's sums and of the weight's.
 struct Work {
-  bool masked;   // dz comes from g and y
+  bool from_y;   // y says what dz needs
+  bool masked;   // and dz is made where it is read
   bool stored;   // dz is stored
   bool beside;   // the bias's sums are made beside the weight's gradient
   size_t weight_at, sums_at, parts_at, bytes;
@@ -841,14 +1014,17 @@ struct Work {
 Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, bool dropout, bool has_y, bool rows, bool weight, bool bias) {
   Work w{};
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  w.masked = act == NTS_ACT_RELU && has_y && (weight || !bias);
+  // Where more than one tile of columns reads it, dz is made once: a step of 232,965 rows of 602 by 256 takes 1,506 us so, and
+  // 1,685 where it is read; one of 337,000 of 100 by 128 takes 421 and 396.
+  w.from_y = act == NTS_ACT_RELU && has_y;
+  w.masked = w.from_y && F <= kTile && (weight || !bias);
   w.stored = !w.masked && (act != NTS_ACT_NONE || dropout) && n;
   w.beside = bias && weight && !w.stored;
-  const bool again = w.stored && act != NTS_ACT_NONE;
+  const bool again = w.stored && act != NTS_ACT_NONE && !w.from_y;
   w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * type_size(type)) : 0;
-  w.sums_at = w.weight_at + up(std::max(again ? prepared_bytes(type, N, F) : 0, rows && n ? prepared_bytes(type, F, N) : 0));
+  w.sums_at = w.weight_at + up(std::max(again ? weight_bytes(type, n, N, F, false) : 0, rows && n ? weight_bytes(type, n, F, N, true) : 0));
   w.parts = weight_parts(n, N, F);
-  w.sums = w.beside ? w.parts.count : again ? workers_for(type, n, N, wide_rows(type, n, N, F)) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
+  w.sums = w.beside ? w.parts.count : again ? workers_for(type, n, N, F) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
   w.parts_at = w.sums_at + (bias ? up(static_cast<size_t>(w.sums) * N * sizeof(float)) : 0);
   w.bytes = w.parts_at + (weight && w.parts.count > 1 ? static_cast<size_t>(w.parts.count) * N * F * sizeof(float) : 0);
   return w;
@@ -874,7 +1050,7 @@ using namespace nts;
 extern "C" {
 
 size_t nts_dense_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F) {
-  return bad_shapes(type, N, F, 0, nullptr) || n <= kFewRows ? 0 : prepared_bytes(type, N, F);
+  return bad_shapes(type, N, F, 0, nullptr) || n <= kFewRows ? 0 : weight_bytes(type, n, N, F, false);
 }
 
 int nts_dense(void *y, const void *x, const void *w, const void *bias, const void *residual, int type, uint32_t n, uint32_t N,
@@ -886,7 +1062,7 @@ int nts_dense(void *y, const void *x, const void *w, const void *bias, const voi
   for (const void *at : {static_cast<const void *>(y), x, w, bias, residual})
     if (!aligned_to(at, type_size(type))) return fail_in("nts_dense", "a value's alignment");
   DenseArgs p{};
-  p.a = x, p.b = work, p.w = w, p.M = n, p.N = N, p.K = F, p.a_stride = F, p.out = y, p.bias = bias, p.more = residual;
+  p.a = x, p.w = w, p.M = n, p.N = N, p.K = F, p.a_stride = F, p.out = y, p.bias = bias, p.more = residual;
   p.act = activation, p.drop = drop_args(dropout);
   if (n <= kFewRows) {
     if (type == NTS_F32) launch_few<float>(p, stream);
@@ -896,8 +1072,7 @@ int nts_dense(void *y, const void *x, const void *w, const void *bias, const voi
     return NTS_OK;
   }
   if (!work || !aligned_to(work, 16)) return fail_in("nts_dense", "needs nts_dense_work_bytes of 16-byte-aligned work");
-  if (const int status = launch_prepare<true>(work, w, type, N, F, F, stream)) return status;
-  return launch_product<kLayer>(p, type, stream);
+  return launch_product<kLayer>(p, type, work, stream);
 }
 
 size_t nts_dense_grad_work_bytes(int type, uint32_t n, uint32_t N, uint32_t F, int activation, int with_dropout, int with_y, int with_rows,
@@ -913,7 +1088,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   if (const char *why = bad_shapes(type, N, F, activation, dropout)) return fail_in(name, why);
   if ((n == 0 || !gx) && !gw && !gb) return NTS_OK;
   const Work layout = grad_work(type, n, N, F, activation, dropout != nullptr, y != nullptr, gx != nullptr, gw != nullptr, gb != nullptr);
-  const bool again = layout.stored && activation != NTS_ACT_NONE;  // z is needed
+  const bool again = layout.stored && activation != NTS_ACT_NONE && !layout.from_y;  // z is needed
   if (n && (!g || ((gw || again) && !x) || ((gx || again) && !w))) return fail_in(name, "null pointer");
   for (const void *at : {static_cast<const void *>(gx), static_cast<const void *>(gw), static_cast<const void *>(gb), g, x, w, bias, y})
     if (!aligned_to(at, type_size(type))) return fail_in(name, "a value's alignment");
@@ -923,16 +1098,16 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   float *const sums = gb ? reinterpret_cast<float *>(base + layout.sums_at) : nullptr;
   const void *dz = g;
   DenseArgs p{};
-  p.drop = drop_args(dropout), p.act = activation, p.w = w, p.b = prepared, p.mask_scale = 1.0f;
+  p.drop = drop_args(dropout), p.act = activation, p.w = w, p.mask_scale = 1.0f;
   p.drop.step_kept = nullptr;
   if (n && (layout.stored || (gb && !layout.beside))) {
     DenseArgs q = p;
     q.more = g, q.M = n, q.N = N, q.sums = sums;
     if (layout.stored) dz = q.out = work;
+    if (layout.from_y) q.y = y, q.mask_scale = p.drop.scale;
     if (again) {
       q.a = x, q.K = F, q.a_stride = F, q.bias = bias;
-      if (const int status = launch_prepare<true>(prepared, w, type, N, F, F, stream)) return status;
-      if (const int status = launch_product<kSlope>(q, type, stream)) return status;
+      if (const int status = launch_product<kSlope>(q, type, prepared, stream)) return status;
     } else {
       const dim3 grid(ceil_div(N, kWave), layout.sums);
       if (type == NTS_F32) hipLaunchKernelGGL(dense_columns_kernel<float>, grid, dim3(256), 0, stream, q);
@@ -945,8 +1120,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   if (gx && n) {
     DenseArgs q = p;
     q.a = dz, q.M = n, q.N = F, q.K = N, q.a_stride = N, q.out = gx;
-    if (const int status = launch_prepare<false>(prepared, w, type, F, N, F, stream)) return status;
-    if (const int status = launch_product<kRows>(q, type, stream)) return status;
+    if (const int status = launch_product<kRows>(q, type, prepared, stream)) return status;
   }
   if (gw) {
     DenseArgs q = p;

@@ -65,7 +65,7 @@ def activation(z, act):
     if act == "relu":
         return np.where(z <= 0, 0.0, z), np.where(z <= 0, 0.0, 1.0), 1.0, 0.0
     if act == "gelu":
-        below = 0.5 * np.vectorize(math.erfc)(-z / math.sqrt(2)) if z.size else z
+        below = 0.5 * torch.erfc(torch.from_numpy(-z / math.sqrt(2))).numpy()
         density = np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
         return z * below, below + z * density, 1.13, 0.8  # the slope's own is (2 - z^2) density <= 2 / sqrt(2 pi)
     if act == "silu":

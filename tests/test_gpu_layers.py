@@ -196,6 +196,14 @@ def test_dense_of_many_rows(device, dtype):
     check_dense(device, 20000, 65, 130, dtype, "silu", True, False, 0.5)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("F,N,act", [(520, 3900, "gelu"), (3900, 520, "silu"), (1000, 4090, "none")])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_dense_of_wide_layers(device, dtype, F, N, act, shift):
+    """Large tiles: of the layer, of its gradient, and none where operands lie between aligned addresses."""
+    check_dense(device, 4099, F, N, dtype, act, True, act == "gelu", 0.1 if act == "silu" else 0.0, shift=shift)
+
+
 def test_dense_of_large_and_small_values(device):
     """Rows whose parts in 16 bits reach the ends of the exponents' range."""
     n, F, N = 40, 64, 32
