@@ -1,6 +1,6 @@
 """Per-epoch time of the sampled mini-batch path with the stage breakdown of the reference's log
 line (toolkits/GCN_GPU_NEIGHBOR.hpp:1498-1506): sample / structure / gather / aggregate forward /
-aggregate backward.  Dense layers are not part of this library and are left out.
+aggregate backward.  Dense layers are left out except with --attention dot.
 
     python -m neutronbench_amd.epoch --config arxiv|products|gat [--scale S]
 
@@ -18,8 +18,10 @@ stream-ordered sequence with one read-back (nts_batch_builder_*; "sample" then h
 structure together); --sampler library goes hop by hop through the per-step entry points;
 --sampler harness uses the torch sampler of the test harness instead.  --features mxfp4 rounds the feature
 table to 4 bits and holds it in device memory: the gather reads it there, and in the gat configuration the
-first dense layer is part of the pass, as a product that gathers the rows itself.  Stages are separated by
-stream synchronisation, as every reference operator synchronises its stream.  --pipeline 2 samples
+first dense layer is part of the pass, as a product that gathers the rows itself.  --attention dot makes the
+gat configuration a graph transformer: a first dense layer, then for every hop projections, attention with dot
+products as scores, and two dense layers behind it, all forward and backward and with --dropout; the stages
+"dense_fwd" and "dense_bwd" hold what lies between the attentions.  Stages are separated by stream synchronisation, as every reference operator synchronises its stream.  --pipeline 2 samples
 the next batch on a second stream while the current one is gathered and aggregated; --pipeline P >= 3
 keeps P batches in flight: P - 2 are sampled ahead, each on a stream of its own, and the next
 batch's features and labels are gathered on another, so that sampling (small dependent kernels), the
@@ -36,6 +38,7 @@ import torch
 from . import synth
 from .batch import (BatchBuilder, FeatureCache, MappedHostTable, load_feature_gpu_cache, load_feature_mxfp4, load_label_gpu,
                     sample_hop)
+from .layers import DenseOp, DotAttentionOp, Dropout, DropoutOp
 from .layout import SampledLayer, as_u32
 from .lowbit import MxProductOp, MxTable
 from .ops import GATAggregateOp, GATAttentionOp, SingleGPUSampleGraphOp
@@ -49,6 +52,60 @@ CONFIGS = {
     "gat": dict(V=2_449_029, E=126_200_000, F=100, hidden=128, classes=47, fanout=[10, 10], batch=4096, train=196_615,
                 seed=4, cache=0.2, heads=4),
 }
+
+
+class DotLayer:
+    """A graph transformer's layer over one sampled hop: h = own + drop(attention Wo), out = h + Wd drop(gelu(Wu h)).  `weights`: (weight, bias) of queries, keys, values, output, up and down, shared by all batches; their gradients of
+    the last batch are in `grads` after backward.  Row i of x modulo its rows stands in for destination i's own row, which a sampled hop
+    need not hold.  timer: called with the stage's name after the dense layers and after the attention."""
+
+    def __init__(self, weights, heads, dropout, seed):
+        self.weights, self.heads, self.dropout, self.seed = weights, heads, dropout, seed
+        self.grads = None
+
+    @staticmethod
+    def make(width, seed, device):
+        """Weights of six dense layers and their biases."""
+        shapes = [(width, width)] * 4 + [(2 * width, width), (width, 2 * width)]
+        return [(synth.normal_features(n, f, seed=seed + i, device=device) * f ** -0.5, torch.zeros(n, device=device))
+                for i, (n, f) in enumerate(shapes)]
+
+    def forward(self, sg, x, step, timer):
+        drop = [Dropout(self.dropout, self.seed + i, step) if self.dropout else None for i in range(3)]
+        n, m = sg.src_size, sg.v_size
+        self.own = None if m <= n else torch.arange(m, device=x.device) % n
+        top = x[:m] if self.own is None else x[self.own]
+        self.rows = n
+        self.proj = [DenseOp() for _ in range(3)]
+        q, k, v = (op.forward(rows, *w) for op, rows, w in zip(self.proj, (top, x, x), self.weights))
+        timer("dense_fwd")
+        self.att = DotAttentionOp(sg, self.heads, dropout=drop[0])
+        a = self.att.forward(q, k, v)
+        timer("aggregate_fwd")
+        self.mix, self.up, self.down = DenseOp("none", drop[1]), DenseOp("gelu", drop[2]), DenseOp()
+        h = self.mix.forward(a, *self.weights[3], top)
+        y = self.down.forward(self.up.forward(h, *self.weights[4]), *self.weights[5], h)
+        timer("dense_fwd")
+        return y
+
+    def backward(self, g, timer):
+        gh = self.up.backward(self.down.backward(g)).add_(g)
+        ga = self.mix.backward(gh)
+        timer("dense_bwd")
+        gq = self.att.backward(ga)
+        gk, gv = self.att.get_additional_grad()
+        timer("aggregate_bwd")
+        gx = self.proj[1].backward(gk).add_(self.proj[2].backward(gv))
+        gtop = self.proj[0].backward(gq).add_(gh)
+        if self.own is None:
+            gx[:len(gtop)].add_(gtop)
+        else:  # row r stands in for destinations r, r + n, ...: added in order
+            for at in range(0, len(gtop), self.rows):
+                part = gtop[at:at + self.rows]
+                gx[:len(part)].add_(part)
+        self.grads = [op.get_additional_grad() for op in (*self.proj, self.mix, self.up, self.down)]
+        timer("dense_bwd")
+        return gx
 
 
 class Timer:
@@ -77,10 +134,16 @@ def graph_mode(graph, pipeline, cache=0.0):
 
 
 def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pipeline=1, quiet=False, checksum=False,
-        stage_sync=None, graph=True, features="f32"):
+        stage_sync=None, graph=True, features="f32", attention="gat", dropout=0.0):
     if features not in ("f32", "mxfp4"):
         raise ValueError("features: f32 or mxfp4")
     cfg = dict(CONFIGS[name])
+    if attention not in ("gat", "dot"):
+        raise ValueError("attention: gat or dot")
+    if attention == "dot" and not cfg.get("heads"):
+        raise ValueError("attention: dot needs a configuration with heads")
+    if not 0.0 <= dropout <= 1.0 or (dropout and attention != "dot"):
+        raise ValueError("dropout: 0 .. 1, with attention dot")
     graph = graph_mode(graph, pipeline, cfg["cache"])
     dev = torch.device("cuda:0")
     V, E = int(cfg["V"] * scale), int(cfg["E"] * scale)
@@ -104,6 +167,13 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
     else:
         table = MappedHostTable(feat_cpu)
         cache = FeatureCache(feat_cpu, out_deg.cpu(), int(V * cfg["cache"]), dev) if cfg["cache"] > 0 else None
+    dot = embed = None
+    if attention == "dot":
+        dot = [DotLayer(DotLayer.make(cfg["hidden"], cfg["seed"] + 50 + 10 * l, dev), heads, dropout, 16 * (l + 1))
+               for l in range(len(cfg["fanout"]))]
+        if mx_weight is None:
+            embed = (synth.normal_features(cfg["hidden"], cfg["F"], seed=cfg["seed"] + 44, device=dev) * cfg["F"] ** -0.5,
+                     torch.zeros(cfg["hidden"], device=dev))
     train_nodes = synth.permutation(V, cfg["seed"] + 42, dev)[:n_train]
     cs = CudaStream()
     # Stages separated by a stream synchronisation, as every reference operator ends with one -- except
@@ -138,7 +208,7 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
                      for _ in range(pipeline - 1)]
         sample_streams = [torch.cuda.Stream(device=dev) for _ in range(max(1, pipeline - 2))]
         gather_stream = torch.cuda.Stream(device=dev) if staged_gather else None
-    totals = {"edges": 0, "hits": 0, "rows": 0}
+    totals = {"edges": 0, "hits": 0, "rows": 0, "steps": 0}
     hits_on_device = torch.zeros(1, dtype=torch.int64, device=dev)  # summed there when no stage is waited for
     checksum_on_device = torch.zeros((), dtype=torch.float64, device=dev)
 
@@ -201,6 +271,33 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
             tm.add("aggregate_bwd", t0)
         return x, g
 
+    def transform(layers, x):
+        """The same with attention dot: a batch's own step draws what is dropped."""
+        clock = [time.perf_counter()]
+
+        def timer(stage):
+            tm.add(stage, clock[0])
+            clock[0] = time.perf_counter()
+
+        step = totals["steps"]
+        totals["steps"] += 1
+        drop, first = DropoutOp(Dropout(dropout, 1, step)) if dropout else None, DenseOp("relu") if embed else None
+        if drop:
+            x = drop.forward(x)
+        if first:
+            x = first.forward(x, *embed)
+        for block, layer in zip(dot, layers):
+            x = block.forward(layer, x, step, timer)
+        g = torch.ones_like(x)
+        for block in reversed(dot):
+            g = block.backward(g, timer)
+        if first:
+            g = first.backward(g)
+        if drop:
+            g = drop.backward(g)
+        timer("dense_bwd")
+        return x, g
+
     def sample_hop_by_hop(b):
         layers, dst_ids = [], train_nodes[b * cfg["batch"]:(b + 1) * cfg["batch"]]
         for hop, fan in enumerate(cfg["fanout"]):
@@ -228,7 +325,7 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
                 totals["hits"] += int(hits.item())
             else:
                 hits_on_device.add_(hits)
-        y, g = aggregate(layers, x)
+        y, g = (transform if dot else aggregate)(layers, x)
         if checksum:  # of the last layer's output and the first layer's input gradient: equal in every mode
             checksum_on_device.add_(y.double().sum() + g.double().sum())  # no read-back: nothing waits here
 
@@ -332,7 +429,7 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
     run_batches(list(range(n_warm)))
     torch.cuda.synchronize()
     tm.t.clear()
-    totals.update(edges=0, hits=0, rows=0)
+    totals.update(edges=0, hits=0, rows=0, steps=0)
     hits_on_device.zero_()
     checksum_on_device.zero_()
     t_epoch = time.perf_counter()
@@ -344,7 +441,7 @@ def run(name, scale=1.0, max_batches=0, sampler="builder", warmup_batches=2, pip
         table.close()
     out = {
         "config": name, "scale": scale, "vertices": V, "edges": E, "batches": n_batches, "batch_size": cfg["batch"],
-        "features": features, "warmup_batches": n_warm,
+        "features": features, "attention": attention if heads else None, "dropout": dropout, "warmup_batches": n_warm,
         "fanout_output_side_first": cfg["fanout"], "epoch_s": round(epoch_s, 4),
         "stage_s": {k: round(v, 4) for k, v in tm.t.items()},
         "library_s": round(sum(v for k, v in tm.t.items() if k != "sample" or sampler != "harness"), 4),
@@ -465,6 +562,11 @@ if __name__ == "__main__":
                     help="mxfp4: the feature table rounded to 4 bits and held in device memory; attention configurations "
                          "then read it through the product with the first layer's weight (not with --native or "
                          "--write-inputs)")
+    ap.add_argument("--attention", choices=["gat", "dot"], default="gat",
+                    help="dot, of the gat configuration: a graph transformer with its dense layers (not with --native or "
+                         "--write-inputs)")
+    ap.add_argument("--dropout", type=float, default=0.0,
+                    help="with --attention dot: rate for features, probabilities and the dense layers' outputs")
     ap.add_argument("--native", action="store_true",
                     help="drive the epoch from C++ (lib/nts_epoch) instead of this module's Python loop")
     ap.add_argument("--write-inputs", metavar="DIR", default=None,
@@ -473,6 +575,12 @@ if __name__ == "__main__":
     a = ap.parse_args()
     if a.features != "f32" and (a.native or a.write_inputs):
         ap.error("--native and --write-inputs take --features f32")
+    if a.attention != "gat" and (a.native or a.write_inputs):
+        ap.error("--native and --write-inputs take --attention gat")
+    if a.attention == "dot" and not CONFIGS[a.config].get("heads"):
+        ap.error("--attention dot needs a configuration with heads")
+    if not 0.0 <= a.dropout <= 1.0 or (a.dropout and a.attention != "dot"):
+        ap.error("--dropout: 0 .. 1, with --attention dot")
     if a.write_inputs:
         import os
 
@@ -491,4 +599,4 @@ if __name__ == "__main__":
     else:
         run(a.config, a.scale, a.max_batches, a.sampler, a.warmup_batches, a.pipeline,
             stage_sync=None if a.stage_sync is None else bool(a.stage_sync),
-            graph=True if a.graph is None else a.graph, features=a.features)
+            graph=True if a.graph is None else a.graph, features=a.features, attention=a.attention, dropout=a.dropout)

@@ -1,11 +1,14 @@
 """Arguments that the operators of layers in training refuse, before any device work (no GPU)."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
-from neutronbench_amd import abi, layers
+from neutronbench_amd import abi, epoch, layers
 from neutronbench_amd.layout import SampledLayer
 
 P = 4096  # stands for a device pointer with any alignment that is asked for: refused calls never follow it
@@ -188,3 +191,22 @@ def test_attention_objects():
     sg.dev_column_offset, sg.dev_row_indices = torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError, match="offsets"):
         op.forward(q, k, k)
+
+
+@pytest.mark.parametrize("options,text", [
+    (["--config", "arxiv", "--attention", "dot"], "heads"), (["--config", "gat", "--attention", "dot", "--native"], "--attention gat"),
+    (["--config", "gat", "--attention", "dot", "--write-inputs", "inputs"], "--attention gat"),
+    (["--config", "gat", "--dropout", "0.5"], "--dropout"), (["--config", "gat", "--attention", "dot", "--dropout", "1.5"], "--dropout"),
+    (["--config", "gat", "--attention", "dot", "--dropout", "nan"], "--dropout"), (["--config", "gat", "--attention", "add"], "--attention")])
+def test_options_of_the_epoch(options, text, tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(epoch.__file__)))
+    got = subprocess.run([sys.executable, "-m", "neutronbench_amd.epoch", *options], cwd=tmp_path, env={**os.environ, "PYTHONPATH": root},
+                         capture_output=True, text=True)
+    assert got.returncode == 2 and text in got.stderr and not os.listdir(tmp_path)
+
+
+def test_arguments_of_the_epoch():
+    for args in (dict(name="gat", attention="add"), dict(name="arxiv", attention="dot"), dict(name="gat", dropout=0.5),
+                 dict(name="gat", attention="dot", dropout=-0.1), dict(name="gat", attention="dot", dropout=math.nan)):
+        with pytest.raises(ValueError, match="attention|dropout"):
+            epoch.run(**args)
