@@ -572,14 +572,14 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
                                 tn * kWideTile + wc * kTile, bias, sums);
   if (USE == kSlope && p.sums) block_sums<8, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(&stages[2][0]), tm, tn * kWideTile);
 }
-// The weight with rows and columns exchanged, rows of `stride` values: [columns, stride], zeros behind `rows` of them.
-__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns, uint32_t stride) {
+// The weight with rows and columns exchanged.
+__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns) {
   __shared__ uint16_t tile[64][66];
   const uint32_t x = threadIdx.x % 64u, y = threadIdx.x / 64u, c0 = blockIdx.x * 64u, r0 = blockIdx.y * 64u;
   for (uint32_t i = y; i < 64u; i += 4u) tile[i][x] = r0 + i < rows && c0 + x < columns ? from[static_cast<uint64_t>(r0 + i) * columns + c0 + x] : uint16_t{0};
   __syncthreads();
   for (uint32_t i = y; i < 64u; i += 4u)
-    if (c0 + i < columns && r0 + x < stride) to[static_cast<uint64_t>(c0 + i) * stride + r0 + x] = tile[x][i];
+    if (c0 + i < columns && r0 + x < rows) to[static_cast<uint64_t>(c0 + i) * rows + r0 + x] = tile[x][i];
 }
 
 // ---- the weight's gradient --------------------------------------------------------------------------
@@ -901,11 +901,10 @@ int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t
 bool by_wide_tiles(int type, uint32_t n, uint32_t N, uint32_t K) {
   return type != NTS_F32 && K >= 512 && K % 8 == 0 && static_cast<uint64_t>(ceil_div(n, kWideTile)) * ceil_div(N, kWideTile) >= 256;
 }
-uint32_t turned_stride(uint32_t terms) { return (terms + 7u) / 8u * 8u; }
 // Bytes of a product's weight in the work: as the rows' kernel wants it, or turned for large tiles.
 size_t weight_bytes(int type, uint32_t n, uint32_t columns, uint32_t terms, bool turned) {
   // operands between aligned addresses take the rows' kernel all the same
-  return std::max(prepared_bytes(type, columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * turned_stride(terms) * 2 : size_t{0});
+  return std::max(prepared_bytes(type, columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * terms * 2 : size_t{0});
 }
 // Workers that share the rows: two blocks to a compute unit, three of 16-bit values.
 uint32_t workers_for(int type, uint32_t n, uint32_t N, uint32_t K) {
@@ -945,9 +944,9 @@ int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
     const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, stream) : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, stream);
     if (status) return status;
   } else if (USE == kRows) {
-    p.b_stride = turned_stride(p.K);
-    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(p.b_stride, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
-                       static_cast<const uint16_t *>(p.w), p.K, p.N, p.b_stride);
+    p.b_stride = p.K;
+    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(p.K, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
+                       static_cast<const uint16_t *>(p.w), p.K, p.N);
     NTS_LAUNCH_CHECK("dense_turn_kernel");
   } else {
     p.b = p.w, p.b_stride = p.K;

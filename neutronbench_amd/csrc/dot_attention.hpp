@@ -19,11 +19,14 @@ enum Form { kPerRow, kNarrow, kWide };
 
 // Wavefronts to a SIMD that the registers allow, and edges of a slot that are requested together.  2.48 M edges, 8 heads of 64 in bf16 with
 // gradients: 2,390 us; two edges and wavefronts in place of four and four, three, two: 2,420 with 6, 3, 2, 2,350 with 5, 4, 3, with which 360,000
-// edges of 4 heads of 32 in 32 bits take 464 instead of 350.
+// edges of 4 heads of 32 in 32 bits take 464 instead of 350.  Of walkers per row, 410,000 edges of 8 heads of 32 in 16 bits take 64 us forward
+// with three and 69 with four, which spill; 1,020,000 of 8 query heads of 64 that share 2 heads 113 and 106.
 template <typename T, int KIND, int REACH, int FORM>
-constexpr int kWavesOf = KIND == kForward         ? (REACH == kWhole && sizeof(T) == 2 && FORM != kNarrow ? 4 : REACH != kWhole && FORM == kNarrow ? 2 : 3)
-                         : KIND == kByDestination ? (REACH == kWhole && (FORM == kWide || (FORM == kPerRow && sizeof(T) == 2)) ? 3 : 2)
-                                                  : 2;
+constexpr int kWavesOf = KIND == kForward         ? (REACH == kWhole && FORM == kWide && sizeof(T) == 2            ? 4
+                                                     : (REACH != kWhole && FORM == kNarrow) || (REACH == kFar && FORM == kPerRow) ? 2
+                                                                                                                                  : 3)
+                         : KIND == kByDestination && REACH == kWhole && FORM == kWide ? 3
+                                                                                      : 2;
 template <typename T>
 constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
 
