@@ -39,8 +39,11 @@ Lanes lanes_for(uint32_t units, uint32_t share, uint32_t D, uint64_t slot_edges)
   return l;
 }
 
-// Positions of a span: 256, so that a part's record is little beside its edges, but as few as 64 where that takes 8,192 wavefronts, and
-// no more spans than 16,384 wavefronts have walkers or have records of 256 MB, but up to 256 spans whatever theirs take.
+// Positions of a span: 256, so that a part's record is little beside its edges, but as few as `shortest` where that takes 8,192 wavefronts.
+// That is 64, as a destination's parts have to be joined (393 destinations of 166 edges, 6 heads of 256 in fp16: 64 us; with 16 78), and by
+// source, whose rows wait for each other and have few edges, 32, or 16 of walkers that share a wavefront (35,587 sources of 138,125 edges, a
+// head of 20 in bf16: the step 109 us, with 32 158, with 64 194; 1,132 of 39,000, 16 query heads of 200 on 4: 328, 302 and 361).  And no more spans
+// than 16,384 wavefronts have walkers or have records of 256 MB, but up to 256 spans whatever theirs take.
 struct Spans {
   uint64_t positions, count;
   uint32_t length;
@@ -49,11 +52,12 @@ struct Spans {
 template <int KIND>
 Spans spans_for(uint32_t rows, uint32_t edges, uint32_t q_heads, uint32_t heads, uint32_t D, const Lanes &l) {
   Spans s;
+  const uint64_t shortest = KIND != kBySource ? 64 : l.walker_shift == 6 ? 32 : 16;
   const uint64_t records = 2 * record_size<KIND>(q_heads, heads, D) * sizeof(float), walkers = kWave >> l.walker_shift;
   s.positions = static_cast<uint64_t>(rows) * kRowCost + edges;
   const uint64_t most = std::max<uint64_t>(256, std::min<uint64_t>(16384 * walkers, (256ull << 20) / records));
-  const uint64_t wanted = std::min(most, std::max({uint64_t{1024}, s.positions / 256, std::min(s.positions / 64, 8192 * walkers)}));
-  s.length = static_cast<uint32_t>(std::max<uint64_t>((s.positions + wanted - 1) / wanted, 64));
+  const uint64_t wanted = std::min(most, std::max({uint64_t{1024}, s.positions / 256, std::min(s.positions / shortest, 8192 * walkers)}));
+  s.length = static_cast<uint32_t>(std::max<uint64_t>((s.positions + wanted - 1) / wanted, shortest));
   s.count = (s.positions + s.length - 1) / s.length;
   s.bytes = static_cast<size_t>(s.count * (records + sizeof(uint32_t)));
   return s;
