@@ -1,5 +1,7 @@
 // Dropout whose mask is never stored: y = x * 65536 / (65536 - t) where the value's number is at least t, else 0.  The backward
 // pass is the same on the gradient.
+// A thread takes 8 values, which share one drawing of ten rounds.  2,449,029 rows of 100 in 32 bits: 480 us, 4.08 TB/s, where a copy of as
+// much reaches 4.7; vector instructions are under way for a quarter of the time.
 #include <algorithm>
 
 #include "launch_size.hpp"

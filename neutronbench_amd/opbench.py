@@ -19,6 +19,7 @@ import torch
 from . import synth
 from .abi import call, ptr
 from .batch import MappedHostTable
+from .layers import DenseOp, DotAttentionOp, Dropout, DropoutOp
 from .layout import SampledLayer, SpmmPlan, as_u32
 from .lowbit import Kv8Cache, MxProductOp, MxTable, NeighborAttentionOp
 
@@ -164,6 +165,24 @@ def main():
     layer.v_size, layer.e_size, layer.dev_column_offset, layer.dev_row_indices = V, E, co32, ri32
     attention = NeighborAttentionOp(layer, H)
     report("nts_kv8_attention", lambda: attention.forward(k, kv), E * (2 * F + 4) + V * (8 * F + 4 * H), whole + f", F'={F}")
+    del kv, attention
+
+    drop = Dropout(0.1, 3)
+    layer.src_size = V
+    attention, q = DotAttentionOp(layer, H, dropout=drop), torch.randn(V, F, device=dev)
+    report("nts_dot_attention", lambda: attention.forward(q, k, v), E * (8 * F + 4) + V * (8 * F + 4 * H), whole + f", F'={F}, dropout")
+    ro, ci = (torch.empty(n_, dtype=torch.int32, device=dev) for n_ in (V + 1, E))
+    work = torch.empty(call("nts_csr_from_csc_work_bytes", V, V, E) + 512, dtype=torch.uint8, device=dev)
+    call("nts_csr_from_csc", ptr(ro), ptr(ci), 0, ptr(co32), ptr(ri32), V, V, E, (work.data_ptr() + 255) // 256 * 256, s)
+    del work
+    layer.dev_row_offset, layer.dev_column_indices = ro, ci
+    report("nts_dot_attention_grad", lambda: attention.backward(q), 2 * E * (8 * F + 4) + V * (28 * F + 4 * H), "the same")
+    del attention, q, k, v, ro, ci
+    dense, weight, bias = DenseOp("relu", drop), torch.randn(F, Ff, device=dev), torch.randn(F, device=dev)
+    report("nts_dense", lambda: dense.forward(table_dev, weight, bias), 4 * V * (Ff + F), f"{V} rows of {Ff} by {F} outputs, relu, dropout")
+    g = torch.randn(V, F, device=dev)
+    report("nts_dense_grad", lambda: dense.backward(g), 4 * V * (2 * Ff + 2 * F), "the same, all gradients")
+    report("nts_dropout", lambda: DropoutOp(drop).forward(table_dev), 8 * V * Ff, f"{V} rows of {Ff} floats")
 
 
 if __name__ == "__main__":
