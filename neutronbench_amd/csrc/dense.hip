@@ -2,7 +2,9 @@
 //   z = x w^T + bias, y = residual + drop(act(z))
 //   dz = drop(g) act'(z) with z computed again, gx = dz w, gw = dz^T x, gb = column sums of dz
 // With relu and no residual y says what dz needs: it is above 0 where z is and the value was kept.  Then z is not computed again, and rows of up
-// to 128 values have dz never stored: both products make it from g and y as they read them.
+// to 128 values have dz never stored: both products make it from g and y as they read them.  dz of 16-bit operands is not rounded to 16 bits, which
+// would add an error as large as the results' own rounding: dz of a computed z is stored as the nearest value and what that leaves, both
+// of which are multiplied, and otherwise the products are of g itself, dropped, and the scale of what is kept comes after the sums.
 #include <algorithm>
 
 #include "launch_size.hpp"
@@ -25,6 +27,8 @@ struct DenseArgs {
   const void *w;      // the weight itself
   const void *y;      // masked gradients: a is g, and counts where y is not 0 or below, times mask_scale
   float mask_scale;
+  float after;  // the products of 16-bit values for gx and gw, times this
+  bool split;   // dz is rows of two parts of N values each
   uint32_t M, N, K, a_stride, b_stride;
   void *out;
   const void *bias, *more;  // more: the residual, or the gradient of y
@@ -176,7 +180,7 @@ __device__ __forceinline__ float sum_of_terms(const float *x, const float *mask,
 struct PrepareArgs {
   const void *from;
   uint16_t *to;
-  uint32_t columns, terms, stride, stages, tiles;
+  uint32_t columns, terms, stride, stages, tiles, wrap;  // wrap: terms from there on are the first ones again
 };
 template <typename T, bool ALONG>
 __global__ __launch_bounds__(256) void dense_prepare_kernel(PrepareArgs p) {
@@ -196,7 +200,8 @@ __global__ __launch_bounds__(256) void dense_prepare_kernel(PrepareArgs p) {
   } else {
 #pragma unroll
   for (uint32_t k = 0; k < 8; ++k) {
-    const uint64_t at = ALONG ? static_cast<uint64_t>(column) * p.stride + term + k : static_cast<uint64_t>(term + k) * p.stride + column;
+    const uint32_t one = term + k < p.wrap ? term + k : term + k - p.wrap;
+    const uint64_t at = ALONG ? static_cast<uint64_t>(column) * p.stride + one : static_cast<uint64_t>(one) * p.stride + column;
     v[k] = column < p.columns && term + k < p.terms ? static_cast<const raw *>(p.from)[at] : static_cast<raw>(0);
   }
   }
@@ -244,7 +249,7 @@ __device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f
             get_columns(static_cast<const T *>(p.more) + (row0 + (q + u) * 4u) * p.N + c, p.N - c, ahead[u]);
       };
       read(0);
-      // nothing for 64 columns that are not there: a step of 183,672 rows of 39 by 22 in bf16 takes 112 us and 134 with them
+      // nothing for 64 columns that are not there: a step of 183,672 rows of 39 by 22 in bf16 takes 134 us and some 20 more with them
       const uint32_t turns = column0 + h * 64u < p.N ? 4u : 0u;
 #pragma unroll 1
       for (uint32_t q = 0; q < turns; q += 2) {
@@ -287,7 +292,23 @@ __device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f
           }
           if (USE == kSlope) through_slope(v[u], more[u], p.act);
           if (at >= p.M || c >= p.N) continue;
-          put_columns(static_cast<T *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
+          if (USE == kSlope && P == 1) {
+            float rest[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float near = ValueOf<T>::get(ValueOf<T>::put(v[u][k]));
+              rest[k] = fabsf(near) < INFINITY ? v[u][k] - near : 0.0f;
+            }
+            T *const to = static_cast<T *>(p.out) + at * (2ull * p.N) + c;
+            put_columns(to, p.N - c, v[u], p.streamed);
+            put_columns(to + p.N, p.N - c, rest, p.streamed);
+          } else {
+            if (USE == kRows && P == 1) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[u][k] *= p.after;
+            }
+            put_columns(static_cast<T *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
+          }
           if (USE == kSlope) {  // columns that are not there are summed and not stored
 #pragma unroll
             for (int k = 0; k < 4; ++k) sums[h][k] += v[u][k];
@@ -443,7 +464,7 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             v[e] = value(0, i, e);
-            if (MASKED) v[e] = value(S - 1, i, e) <= 0.0f ? 0.0f : v[e] * p.mask_scale;
+            if (MASKED) v[e] = value(S - 1, i, e) <= 0.0f ? 0.0f : P == 3 ? v[e] * p.mask_scale : v[e];
           }
           if constexpr (P == 3) {
             split8(v, a[i]);
@@ -511,7 +532,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
   const char *const from_a = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.a) + row_a * p.a_stride);
   const char *const from_b = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.b) + row_b * p.b_stride);
   const uint32_t chunk = part_at(lane / 4u, lane & 3u);  // the same for all of the lane's rows, which are 16 apart
-  uint32_t at[4];  // in bytes: below 2^26, as 256 rows of 2^17 values are
+  uint32_t at[4];  // in bytes: below 2^27, as 256 rows of 2^18 values are
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t row = ((i & 1) * 8u + wave) * 16u + lane / 4u;
@@ -578,14 +599,15 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
                                 tn * kWideTile + wc * kTile, bias, sums);
   if (USE == kSlope && p.sums) block_sums<8, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(&stages[2][0]), tm, tn * kWideTile);
 }
-// The weight with rows and columns exchanged.
-__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns) {
+// The weight with rows and columns exchanged, `copies` times beside each other.
+__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns, uint32_t copies) {
   __shared__ uint16_t tile[64][66];
   const uint32_t x = threadIdx.x % 64u, y = threadIdx.x / 64u, c0 = blockIdx.x * 64u, r0 = blockIdx.y * 64u;
   for (uint32_t i = y; i < 64u; i += 4u) tile[i][x] = r0 + i < rows && c0 + x < columns ? from[static_cast<uint64_t>(r0 + i) * columns + c0 + x] : uint16_t{0};
   __syncthreads();
   for (uint32_t i = y; i < 64u; i += 4u)
-    if (c0 + i < columns && r0 + x < rows) to[static_cast<uint64_t>(c0 + i) * rows + r0 + x] = tile[x][i];
+    if (c0 + i < columns && r0 + x < rows)
+      for (uint32_t k = 0; k < copies; ++k) to[(static_cast<uint64_t>(c0 + i) * copies + k) * rows + r0 + x] = tile[x][i];
 }
 
 // ---- the weight's gradient --------------------------------------------------------------------------
@@ -593,18 +615,20 @@ __global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ 
 // not depend on scheduling.  A block of four wavefronts takes 128 rows of the result by 128 columns, 32 terms at a time through LDS, where
 // both operands are written with the terms of a row or column side by side.
 // 232,965 terms of 256 by 602 in 32 bits: 500-550 us, 130-143 TFLOP/s, splitting half of the time and matrix instructions for two fifths;
-// 169,343 of 128 by 128 in bf16: 19 us, 4.5 TB/s.
+// 169,343 of 128 by 128 in bf16: 19 us, 4.5 TB/s, and 25 with dz in two parts, 5.1 TB/s.
 // Sixteen terms of one column of an operand, or eight of each of two neighbouring columns (PAIRS: rows of 16-bit values of an even number),
-// on their way from memory to LDS.  MASKED: as DenseArgs' y.
-template <typename T, bool PAIRS, bool MASKED>
+// on their way from memory to LDS.  kMasked: as DenseArgs' y; kSplit: dz of two parts, which go to two planes.
+enum Source { kPlain, kMasked, kSplit };
+template <typename T, bool PAIRS, int SOURCE>
 struct Terms {
   typedef typename ValueOf<T>::raw raw;
-  static constexpr int S = MASKED ? 2 : 1, N = PAIRS ? 8 : 16;
+  static constexpr bool MASKED = SOURCE == kMasked;
+  static constexpr int S = SOURCE == kPlain ? 1 : 2, N = PAIRS ? 8 : 16, P = SOURCE == kSplit ? 2 : kPlanes<T>;
   typedef uint32_t Word __attribute__((aligned(2)));
   uint32_t v[S][N];
   const T *from[S];  // the operands' beginning, so that a row's address is a scalar, and the lane's place from there
   uint32_t lane_at, stride, column, first;  // the thread's column of 128, its first term of 32
-  __device__ __forceinline__ void place(const void *a, const void *y, uint32_t row_stride, uint32_t first_column, uint32_t columns) {
+  __device__ __forceinline__ void place(const void *a, const void *second, uint32_t row_stride, uint32_t first_column, uint32_t columns) {
     const uint32_t t = threadIdx.x;
     column = PAIRS ? t % 64u * 2u : t & 127u;
     first = PAIRS ? t / 64u * 8u : (t >> 7) * 16u;
@@ -613,7 +637,7 @@ struct Terms {
     const uint32_t c = min(first_column + column, columns - (PAIRS ? 2u : 1u));
     lane_at = first * stride + c;
     from[0] = static_cast<const T *>(a);
-    if (MASKED) from[S - 1] = static_cast<const T *>(y);
+    if (S == 2) from[S - 1] = static_cast<const T *>(second);
   }
   template <bool SOME>
   __device__ __forceinline__ void request(uint64_t term, uint32_t left) {
@@ -646,8 +670,8 @@ struct Terms {
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            f[e] = value(i + e, which) * (MASKED ? scale : 1.0f);
-            if (sums) sums[which] += f[e];
+            f[e] = value(i + e, which) * (MASKED && P == 3 ? scale : 1.0f);
+            if (sums) sums[which] += MASKED && P == 1 ? f[e] * scale : f[e];
           }
           if constexpr (sizeof(raw) == 4) {
             split8(f, w);
@@ -657,33 +681,36 @@ struct Terms {
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = v[0][i + 2 * e], y = v[0][i + 2 * e + 1];
-            w[0][e] = which ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
-          }
+          for (int o = 0; o < S; ++o)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = v[o][i + 2 * e], y = v[o][i + 2 * e + 1];
+              w[o][e] = which ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+            }
           if (sums) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sums[which] += value(i + e, which);
           }
         }
 #pragma unroll
-        for (int c = 0; c < kPlanes<T>; ++c) *reinterpret_cast<u32x4 *>(planes + c * kPlane + tile_at(column + which, (first + i) / 8u)) = w[c];
+        for (int c = 0; c < P; ++c) *reinterpret_cast<u32x4 *>(planes + c * kPlane + tile_at(column + which, (first + i) / 8u)) = w[c];
       }
   }
 };
 
-template <typename T, bool PAIRS, bool MASKED>
+template <typename T, bool PAIRS, int SOURCE>
 __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
-  constexpr int P = kPlanes<T>;
-  __shared__ __attribute__((aligned(16))) uint16_t tile[2 * P * kPlane > 8192 ? 2 * P * kPlane : 8192];
-  uint16_t *const ta = tile, *const tb = tile + P * kPlane;
+  constexpr bool MASKED = SOURCE == kMasked;
+  constexpr int P = kPlanes<T>, PA = Terms<T, PAIRS, SOURCE>::P;
+  __shared__ __attribute__((aligned(16))) uint16_t tile[(PA + P) * kPlane];
+  uint16_t *const ta = tile, *const tb = tile + PA * kPlane;
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
   const uint32_t tm = blockIdx.x / p.tiles_n, tn = blockIdx.x % p.tiles_n;
   const uint32_t m0 = tm * kTile, n0 = tn * kTile;
   const uint64_t begin = static_cast<uint64_t>(blockIdx.z) * p.part_terms, end = min(static_cast<uint64_t>(p.K), begin + p.part_terms);
-  Terms<T, PAIRS, MASKED> va;
-  Terms<T, PAIRS, false> vb;
-  va.place(p.a, p.y, p.a_stride, m0, p.M);
+  Terms<T, PAIRS, SOURCE> va;
+  Terms<T, PAIRS, kPlain> vb;
+  va.place(p.a, SOURCE == kSplit ? static_cast<const T *>(p.a) + p.M : p.y, p.a_stride, m0, p.M);
   vb.place(p.b, nullptr, p.b_stride, n0, p.N);
   float sums[2] = {};
   const bool summing = p.column_sums && tn == 0;
@@ -713,13 +740,13 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
       for (int j = 0; j < 4; ++j) b[c][j] = *reinterpret_cast<const u32x4 *>(tb + c * kPlane + tile_at(wn + j * 16 + r, part));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u32x4 a[P];
+      u32x4 a[PA];
 #pragma unroll
-      for (int c = 0; c < P; ++c) a[c] = *reinterpret_cast<const u32x4 *>(ta + c * kPlane + tile_at(wm + i * 16 + r, part));
+      for (int c = 0; c < PA; ++c) a[c] = *reinterpret_cast<const u32x4 *>(ta + c * kPlane + tile_at(wm + i * 16 + r, part));
 #pragma unroll
-      for (int s = P - 1; s >= 0; --s)
+      for (int s = PA - 1; s >= 0; --s)
 #pragma unroll
-        for (int c = 0; c <= s; ++c)
+        for (int c = PA == P ? 0 : s; c <= s; ++c)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] = multiply<T>(b[s - c][j], a[c], acc[i][j]);
     }
@@ -746,6 +773,10 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
                               p.mask_scale, p.a_stride, static_cast<const float *>(p.b) + begin * p.b_stride + c + k, p.b_stride, end - begin);
         }
       }
+      if (P == 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= p.after;
+      }
       if (p.sums) put_columns(p.sums + (static_cast<uint64_t>(blockIdx.z) * p.M + i) * p.N + c, p.N - c, v, false);
       else put_columns(static_cast<T *>(p.out) + static_cast<uint64_t>(i) * p.N + c, p.N - c, v, false);
     }
@@ -754,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
   if (!summing) return;
   __syncthreads();
   float(*const of_terms)[kTile] = reinterpret_cast<float(*)[kTile]>(tile);
-  of_terms[va.first / Terms<T, PAIRS, MASKED>::N][va.column] = sums[0];
+  of_terms[va.first / Terms<T, PAIRS, SOURCE>::N][va.column] = sums[0];
   if (PAIRS) of_terms[va.first / 8u][va.column + 1u] = sums[1];
   __syncthreads();
   if (t < kTile && m0 + t < p.M) {
@@ -827,6 +858,10 @@ __global__ __launch_bounds__(256) void dense_columns_kernel(DenseArgs p) {
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block(), c = blockIdx.x * kWave + (lane & 15u) * 4u;
   const uint32_t step = drop_step(p.drop), count = c < p.N ? p.N - c : 0u;
   float sums[4] = {};
+  // 16-bit values are stored as they are, and their sums scaled
+  const float scale = p.y ? p.mask_scale : p.drop.scale, inside = kPlanes<T> == 3 ? scale : 1.0f, outside = kPlanes<T> == 3 ? 1.0f : scale;
+  DropArgs drop = p.drop;
+  drop.scale = inside;
   for (uint64_t i0 = blockIdx.y * 32ull + wave * 8u + lane / 16u; i0 < p.M; i0 += gridDim.y * 32ull) {
     float v[2][4] = {}, y[2][4] = {};
 #pragma unroll
@@ -839,9 +874,9 @@ __global__ __launch_bounds__(256) void dense_columns_kernel(DenseArgs p) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[u][k] = y[u][k] <= 0.0f ? 0.0f : v[u][k] * p.mask_scale;
+        for (int k = 0; k < 4; ++k) v[u][k] = y[u][k] <= 0.0f ? 0.0f : v[u][k] * inside;
     } else if (p.drop.threshold) {
-      drop_two_rows(p.drop, step, static_cast<uint32_t>(i0), static_cast<uint32_t>(i0) + 4u, c, v[0], v[1]);
+      drop_two_rows(drop, step, static_cast<uint32_t>(i0), static_cast<uint32_t>(i0) + 4u, c, v[0], v[1]);
     }
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
@@ -854,6 +889,7 @@ __global__ __launch_bounds__(256) void dense_columns_kernel(DenseArgs p) {
   if (!p.sums) return;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    sums[k] *= outside;
     sums[k] += __shfl_xor(sums[k], 16, kWave);
     sums[k] += __shfl_xor(sums[k], 32, kWave);
     if (lane < 16u) of_wave[wave][lane * 4u + k] = sums[k];
@@ -894,8 +930,8 @@ size_t prepared_bytes(int type, uint32_t columns, uint32_t terms) {
   return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * (type == NTS_F32 ? 6 : 2);
 }
 template <bool ALONG>
-int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t terms, uint32_t stride, hipStream_t stream) {
-  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns)};
+int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t terms, uint32_t stride, uint32_t wrap, hipStream_t stream) {
+  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns), wrap};
   const dim3 grid(ceil_div(static_cast<uint64_t>(p.stages) * p.tiles * 4u * kTile, 256));
   if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, ALONG>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied
@@ -949,12 +985,14 @@ int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
   p.streamed = static_cast<uint64_t>(p.M) * p.N * type_size(type) >= kStreamed;
   p.b = work;
   if (!wide) {
-    const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, stream) : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, stream);
+    const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, p.split ? p.K / 2u : p.K, stream)
+                                    : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, p.K, stream);
     if (status) return status;
   } else if (USE == kRows) {
     p.b_stride = p.K;
-    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(p.K, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
-                       static_cast<const uint16_t *>(p.w), p.K, p.N);
+    const uint32_t copies = p.split ? 2u : 1u, rows = p.K / copies;
+    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(rows, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
+                       static_cast<const uint16_t *>(p.w), rows, p.N, copies);
     NTS_LAUNCH_CHECK("dense_turn_kernel");
   } else {
     p.b = p.w, p.b_stride = p.K;
@@ -965,17 +1003,23 @@ int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
   NTS_LAUNCH_CHECK("dense_rows_kernel");
   return NTS_OK;
 }
-template <typename T>
-void launch_weight(const DenseArgs &p, const dim3 &grid, hipStream_t stream) {
+template <typename T, bool PAIRS>
+void launch_weight_of(const DenseArgs &p, const dim3 &grid, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (p.M % 2 == 0 && p.N % 2 == 0) {
-      if (p.y) hipLaunchKernelGGL((dense_weight_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
-      else hipLaunchKernelGGL((dense_weight_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
+    if (p.split) {
+      hipLaunchKernelGGL((dense_weight_kernel<T, PAIRS, kSplit>), grid, dim3(256), 0, stream, p);
       return;
     }
   }
-  if (p.y) hipLaunchKernelGGL((dense_weight_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((dense_weight_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
+  if (p.y) hipLaunchKernelGGL((dense_weight_kernel<T, PAIRS, kMasked>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dense_weight_kernel<T, PAIRS, kPlain>), grid, dim3(256), 0, stream, p);
+}
+template <typename T>
+void launch_weight(const DenseArgs &p, const dim3 &grid, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.M % 2 == 0 && p.N % 2 == 0) return launch_weight_of<T, true>(p, grid, stream);
+  }
+  launch_weight_of<T, false>(p, grid, stream);
 }
 template <typename T>
 void launch_few(const DenseArgs &p, hipStream_t stream) {
@@ -1014,6 +1058,8 @@ struct Work {
   bool masked;   // and dz is made where it is read
   bool stored;   // dz is stored
   bool beside;   // the bias's sums are made beside the weight's gradient
+  bool again;    // z is computed again
+  bool split;    // dz is stored in two parts
   size_t weight_at, sums_at, parts_at, bytes;
   uint32_t sums;
   Parts parts;
@@ -1027,11 +1073,13 @@ Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, bool dropo
   w.masked = w.from_y && F <= kTile && (weight || !bias);
   w.stored = !w.masked && (act != NTS_ACT_NONE || dropout) && n;
   w.beside = bias && weight && !w.stored;
-  const bool again = w.stored && act != NTS_ACT_NONE && !w.from_y;
-  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * type_size(type)) : 0;
-  w.sums_at = w.weight_at + up(std::max(again ? weight_bytes(type, n, N, F, false) : 0, rows && n ? weight_bytes(type, n, F, N, true) : 0));
+  w.again = w.stored && act != NTS_ACT_NONE && !w.from_y;
+  w.split = w.again && type != NTS_F32;
+  const uint32_t parts = w.split ? 2u : 1u;
+  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * type_size(type) * parts) : 0;
+  w.sums_at = w.weight_at + up(std::max(w.again ? weight_bytes(type, n, N, F, false) : 0, rows && n ? weight_bytes(type, n, F, N * parts, true) : 0));
   w.parts = weight_parts(n, N, F);
-  w.sums = w.beside ? w.parts.count : again ? workers_for(type, n, N, F) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
+  w.sums = w.beside ? w.parts.count : w.again ? workers_for(type, n, N, F) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
   w.parts_at = w.sums_at + (bias ? up(static_cast<size_t>(w.sums) * N * sizeof(float)) : 0);
   w.bytes = w.parts_at + (weight && w.parts.count > 1 ? static_cast<size_t>(w.parts.count) * N * F * sizeof(float) : 0);
   return w;
@@ -1095,8 +1143,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   if (const char *why = bad_shapes(type, N, F, activation, dropout)) return fail_in(name, why);
   if ((n == 0 || !gx) && !gw && !gb) return NTS_OK;
   const Work layout = grad_work(type, n, N, F, activation, dropout != nullptr, y != nullptr, gx != nullptr, gw != nullptr, gb != nullptr);
-  const bool again = layout.stored && activation != NTS_ACT_NONE && !layout.from_y;  // z is needed
-  if (n && (!g || ((gw || again) && !x) || ((gx || again) && !w))) return fail_in(name, "null pointer");
+  if (n && (!g || ((gw || layout.again) && !x) || ((gx || layout.again) && !w))) return fail_in(name, "null pointer");
   for (const void *at : {static_cast<const void *>(gx), static_cast<const void *>(gw), static_cast<const void *>(gb), g, x, w, bias, y})
     if (!aligned_to(at, type_size(type))) return fail_in(name, "a value's alignment");
   if (layout.bytes && (!work || !aligned_to(work, 16))) return fail_in(name, "needs nts_dense_grad_work_bytes of 16-byte-aligned work");
@@ -1112,7 +1159,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
     q.more = g, q.M = n, q.N = N, q.sums = sums;
     if (layout.stored) dz = q.out = work;
     if (layout.from_y) q.y = y, q.mask_scale = p.drop.scale;
-    if (again) {
+    if (layout.again) {
       q.a = x, q.K = F, q.a_stride = F, q.bias = bias;
       if (const int status = launch_product<kSlope>(q, type, prepared, stream)) return status;
     } else {
@@ -1124,14 +1171,17 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
     }
   }
   if (layout.masked) p.y = y, p.mask_scale = p.drop.scale;
+  p.after = layout.masked || (layout.stored && !layout.again) ? p.drop.scale : 1.0f;
+  p.split = layout.split;
+  const uint32_t dz_width = layout.split ? 2u * N : N;
   if (gx && n) {
     DenseArgs q = p;
-    q.a = dz, q.M = n, q.N = F, q.K = N, q.a_stride = N, q.out = gx;
+    q.a = dz, q.M = n, q.N = F, q.K = dz_width, q.a_stride = dz_width, q.out = gx;
     if (const int status = launch_product<kRows>(q, type, prepared, stream)) return status;
   }
   if (gw) {
     DenseArgs q = p;
-    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = N, q.b_stride = F, q.out = gw, q.part_terms = layout.parts.terms;
+    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = dz_width, q.b_stride = F, q.out = gw, q.part_terms = layout.parts.terms;
     q.tiles_m = ceil_div(N, kTile), q.tiles_n = ceil_div(F, kTile);
     if (layout.beside) q.column_sums = sums;
     const uint32_t parts = layout.parts.count;

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from layers_ref import row_factors
 from neutronbench_amd import layers
 from test_gpu_layers import BF16, F16, F32, check_attention, check_dense, graph, layer_of
 
@@ -178,3 +179,29 @@ def test_an_operator_that_is_used_again(device):
     assert torch.equal(op.forward(x, w), other.forward(x, w)) and torch.equal(op.backward(g), other.backward(g))
     assert torch.equal(op.backward(g), other.backward(g))
     assert math.isfinite(float(op.get_additional_grad()[0].sum())) and op.get_additional_grad()[1] is None
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,F,N,act,residual,p", [(700, 100, 130, "gelu", True, 0.1), (700, 200, 61, "silu", False, 0.3), (600, 96, 128, "relu", False, 0.1),
+                                                  (600, 300, 64, "relu", False, 0.1), (500, 200, 72, "none", False, 0.1), (5000, 64, 520, "gelu", False, 0.0)])
+def test_dense_gradients_are_rounded_once(device, dtype, n, F, N, act, residual, p):
+    """Against 64 bits a 16-bit gradient is off by its own rounding, evenly spread over a step: with values m 2^e, m spread over 1 .. 2, by
+    eps / sqrt(12 * 7 / 3) = 0.38 eps / 2 of the whole in the norm, and with all at m = 1, by 0.58.  Normally distributed ones (a product's, of thousands
+    of elements) lie between, at 0.43; a second such error before the products would make it 0.61.  dz's parts (2^-16 of it), GELU's 10^-7 and
+    sums in 32 bits are far below.  The bias's gradient has too few elements for that: eps / 2 holds for each of them."""
+    x, w, b, g = ((torch.randn(*s, device=device, generator=torch.Generator(device=device).manual_seed(i)) * k).to(dtype)
+                  for i, (s, k) in enumerate((((n, F), 1.0), ((N, F), 1 / math.sqrt(F)), ((N,), 0.5), ((n, N), 1.0))))
+    r = torch.randn(n, N, device=device).to(dtype) if residual else None
+    op = layers.DenseOp(act, layers.Dropout(p, 17, 2) if p else None)
+    op.forward(x, w, b, r)
+    got = [op.backward(g), *op.get_additional_grad()]
+    xd, wd, bd = (t.double().cpu().requires_grad_() for t in (x, w, b))
+    z = xd @ wd.T + bd
+    z.retain_grad()
+    y = {"none": lambda v: v, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu}[act](z)
+    factors = torch.from_numpy(row_factors(n, N, p, 17, 2)) if p else 1.0
+    (y * factors).backward(g.double().cpu())
+    # sums so near 0 that 32 bits may fall on the other side of relu's border
+    assert act != "relu" or float(z.detach().abs().min()) > 1e-7
+    for a, e, most in zip(got, (xd.grad, wd.grad, bd.grad), (0.5, 0.5, 1.1)):
+        assert float((a.double().cpu() - e).norm() / e.norm()) < most * torch.finfo(dtype).eps / 2
