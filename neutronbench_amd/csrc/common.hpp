@@ -9,6 +9,7 @@
 #include <utility>
 
 #include "idle_blocks.hpp"
+#include "launch_size.hpp"
 #include "nts_hip.h"
 
 namespace nts {
@@ -133,8 +134,6 @@ inline bool sddmm_by_lanes(const void *in, const void *gout, uint32_t H, uint32_
   const uint32_t lanes = H * Fh / *vec;
   return lanes <= 64 && is_power_of_two(lanes) && is_power_of_two(Fh / *vec);
 }
-
-inline uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
 // A count that kernels need: known on the host (`n` null, value = `cap`), or produced earlier in the
 // same stream and read on the device -- the word `*n`, or `off[*n]` when `off` is set (an offsets

@@ -7,6 +7,7 @@
 // of which are multiplied, and otherwise the products are of g itself, dropped, and the scale of what is kept comes after the sums.
 #include <algorithm>
 
+#include "dense_layout.hpp"
 #include "launch_size.hpp"
 #include "layers.hpp"
 #include "tiles.hpp"
@@ -126,7 +127,6 @@ __device__ __forceinline__ void drop_two_rows(const DropArgs &d, uint32_t step, 
 // to what the ones before it leave: x = hi + mid + lo up to 2^-27 of x, and of the nine products the three that are below 2^-26 of the whole
 // are left out, so that the sums in 32 bits are as good as a 32-bit product's.  An infinity's mid part is NaN: elements that are not
 // finite are computed again term by term.
-constexpr uint32_t kTile = 128, kTerms = 32, kPlane = kTile * kTerms;
 // Where 8 of a row's 32 terms lie in LDS.  A read of 16 bytes by a wavefront goes in quarters of 16 lanes, four neighbours' worth each of two
 // parts (rows 0..3 and 12..15 of one with 4..11 of the next, and so on): with the four groups of rows at 0, 2, 3, 1 such a quarter meets
 // every bank once, as 16 rows of one part do.  At 0, 1, 2, 3 every read took half as long again.
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
   const uint32_t wr = wave & 3u, wc = wave >> 2, stages = (p.K + kTerms - 1u) / kTerms;
   const uint32_t step = USE == kLayer || USE == kSlope ? drop_step(p.drop) : 0u;
   if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
-  if (worker >= p.tiles_m) return;
+  if (!has_rows(worker, p.workers)) return;
   const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * WN * stages * P * kPlane;
   const T *const rows = static_cast<const T *>(p.a);
   // stage s of the weight
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
 // us, 1,040 TF/s.  LDS bounds it: a stage's 96 reads and 32 KB of writes hold it for 1,024 cycles, as long as the matrix instructions take.
 // (Four wavefronts of 128 by 128 read a third less, but their 256 sums leave too few registers: 3,170 us, moves between the two halves of the
 // register file; all wavefronts in step: 2,510; dense_rows_kernel: 2,830.)
-constexpr uint32_t kWideTile = 256, kWideStages = 4;
+constexpr uint32_t kWideStages = 4;
 __device__ __attribute__((aligned(16))) uint16_t zero_part[8];
 template <typename T, int USE>
 __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
@@ -924,11 +924,6 @@ __global__ __launch_bounds__(kSumWaves *kWave) void dense_sum_kernel(T *__restri
 // ---- launches ---------------------------------------------------------------------------------------
 constexpr uint64_t kStreamed = 32ull << 20;  // an output from this size on is more than the L2s hold
 
-// Bytes of a prepared weight.
-uint32_t tile_groups(uint32_t columns) { return ceil_div(columns, 2 * kTile) * 2u; }
-size_t prepared_bytes(int type, uint32_t columns, uint32_t terms) {
-  return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * (type == NTS_F32 ? 6 : 2);
-}
 template <bool ALONG>
 int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t terms, uint32_t stride, uint32_t wrap, hipStream_t stream) {
   const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns), wrap};
@@ -939,52 +934,35 @@ int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t
   return NTS_OK;
 }
 
-// Large products by large tiles, where there are enough of them for the chip and rows of many terms; in us by large tiles and by rows:
-// 16,384 x 1,024 x 512 26 and 38, 65,536 x 256 x 1,024 42 and 63; of 256 terms 32,768 x 4,096 150 and 129; of 128 tiles 8,192 x 1,024 x 1,024
-// 34 and 34.
-bool by_wide_tiles(int type, uint32_t n, uint32_t N, uint32_t K) {
-  return type != NTS_F32 && K >= 512 && K % 8 == 0 && static_cast<uint64_t>(ceil_div(n, kWideTile)) * ceil_div(N, kWideTile) >= 256;
-}
-// Bytes of a product's weight in the work: as the rows' kernel wants it, or turned for large tiles.
-size_t weight_bytes(int type, uint32_t n, uint32_t columns, uint32_t terms, bool turned) {
-  // operands between aligned addresses take the rows' kernel all the same
-  return std::max(prepared_bytes(type, columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * terms * 2 : size_t{0});
-}
-// Workers that share the rows: two blocks to a compute unit, three of 16-bit values.
-uint32_t workers_for(int type, uint32_t n, uint32_t N, uint32_t K) {
-  if (by_wide_tiles(type, n, N, K)) return ceil_div(n, kWideTile);
-  const uint32_t tiles = ceil_div(n, kTile), columns = ceil_div(N, kTile);
-  return std::min(tiles, std::max(8u, (type == NTS_F32 ? 512u : 768u) / columns / 8u * 8u));
-}
 template <typename T, int USE, bool MASKED = false>
-void launch_rows(DenseArgs p, hipStream_t stream) {
-  p.tiles_m = ceil_div(p.M, kTile);
-  p.tiles_n = ceil_div(p.N, kTile);
-  hipLaunchKernelGGL((dense_rows_kernel<T, USE, 2, 1, MASKED>), dim3(ceil_div(p.workers, 8) * 8u * p.tiles_n), dim3(256), 0, stream, p);
+void launch_rows(const DenseArgs &p, const Share &share, hipStream_t stream) {
+  hipLaunchKernelGGL((dense_rows_kernel<T, USE, 2, 1, MASKED>), dim3(launched_workers(share) * p.tiles_n), dim3(256), 0, stream, p);
 }
 template <typename T, int USE>
-void launch_product_of(DenseArgs p, bool wide, hipStream_t stream) {
+void launch_product_of(const DenseArgs &p, const Share &share, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (wide) {
-      p.tiles_m = ceil_div(p.M, kWideTile);
-      p.tiles_n = ceil_div(p.N, kWideTile);
+    if (share.wide) {
       hipLaunchKernelGGL((dense_wide_kernel<T, USE>), dim3(tile_blocks(p.tiles_m, p.tiles_n, 8)), dim3(512), 0, stream, p);
       return;
     }
   }
   if constexpr (USE == kRows) {
-    if (p.y) return launch_rows<T, USE, true>(p, stream);
+    if (p.y) return launch_rows<T, USE, true>(p, share, stream);
   }
-  launch_rows<T, USE>(p, stream);
+  launch_rows<T, USE>(p, share, stream);
+}
+template <int USE>
+Share share_for(const DenseArgs &p, int type) {
+  return share_of(type, p.M, p.N, p.K, !p.y && aligned_to(p.a, 16) && (USE == kRows || aligned_to(p.w, 16)));
 }
 // The product of p.a and the weight p.w, whose form for it goes to `work`.
 template <int USE>
 int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
-  const bool wide = !p.y && by_wide_tiles(type, p.M, p.N, p.K) && aligned_to(p.a, 16) && (USE == kRows || aligned_to(p.w, 16));
-  p.workers = workers_for(type, p.M, p.N, p.K);
+  const Share share = share_for<USE>(p, type);
+  p.tiles_m = share.tiles_m, p.tiles_n = share.tiles_n, p.workers = share.workers;
   p.streamed = static_cast<uint64_t>(p.M) * p.N * type_size(type) >= kStreamed;
   p.b = work;
-  if (!wide) {
+  if (!share.wide) {
     const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, p.split ? p.K / 2u : p.K, stream)
                                     : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, p.K, stream);
     if (status) return status;
@@ -997,9 +975,9 @@ int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
   } else {
     p.b = p.w, p.b_stride = p.K;
   }
-  if (type == NTS_F32) launch_product_of<float, USE>(p, wide, stream);
-  else if (type == NTS_BF16) launch_product_of<Bf16, USE>(p, wide, stream);
-  else launch_product_of<F16, USE>(p, wide, stream);
+  if (type == NTS_F32) launch_product_of<float, USE>(p, share, stream);
+  else if (type == NTS_BF16) launch_product_of<Bf16, USE>(p, share, stream);
+  else launch_product_of<F16, USE>(p, share, stream);
   NTS_LAUNCH_CHECK("dense_rows_kernel");
   return NTS_OK;
 }
@@ -1034,55 +1012,6 @@ int launch_sum(void *out, int type, const float *from, uint64_t count, uint32_t 
   else hipLaunchKernelGGL(dense_sum_kernel<F16>, grid, block, 0, stream, static_cast<F16 *>(out), from, count, parts);
   NTS_LAUNCH_CHECK("dense_sum_kernel");
   return NTS_OK;
-}
-
-// Parts of the weight's gradient, of few results and many terms: two blocks for a compute unit, and no part of fewer than 256 terms.
-// (All tiles of a part on one chiplet, whose L2 then reads its rows once, took 620 us instead of 515 at 232,965 terms of 256 by 602: the parts
-// are then a multiple of eight and fewer.)
-struct Parts {
-  uint32_t count, terms;
-};
-Parts weight_parts(uint32_t n, uint32_t N, uint32_t F) {
-  const uint64_t tiles = static_cast<uint64_t>(ceil_div(N, kTile)) * ceil_div(F, kTile);
-  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(512 / tiles, n / 256));
-  const uint64_t terms = (n + want - 1) / want;
-  Parts p;
-  p.terms = static_cast<uint32_t>(std::min<uint64_t>((terms + kTerms - 1) / kTerms * kTerms, 0xFFFFFFE0u));
-  p.count = std::max(1u, ceil_div(n, std::max(p.terms, 1u)));
-  return p;
-}
-
-// The gradient's work: dz, the prepared weight, the parts of the bias's sums and of the weight's.
-struct Work {
-  bool from_y;   // y says what dz needs
-  bool masked;   // and dz is made where it is read
-  bool stored;   // dz is stored
-  bool beside;   // the bias's sums are made beside the weight's gradient
-  bool again;    // z is computed again
-  bool split;    // dz is stored in two parts
-  size_t weight_at, sums_at, parts_at, bytes;
-  uint32_t sums;
-  Parts parts;
-};
-Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, bool dropout, bool has_y, bool rows, bool weight, bool bias) {
-  Work w{};
-  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  // Where more than one tile of columns reads it, dz is made once: a step of 232,965 rows of 602 by 256 takes 1,506 us so, and
-  // 1,685 where it is read; one of 337,000 of 100 by 128 takes 421 and 396.
-  w.from_y = act == NTS_ACT_RELU && has_y;
-  w.masked = w.from_y && F <= kTile && (weight || !bias);
-  w.stored = !w.masked && (act != NTS_ACT_NONE || dropout) && n;
-  w.beside = bias && weight && !w.stored;
-  w.again = w.stored && act != NTS_ACT_NONE && !w.from_y;
-  w.split = w.again && type != NTS_F32;
-  const uint32_t parts = w.split ? 2u : 1u;
-  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * type_size(type) * parts) : 0;
-  w.sums_at = w.weight_at + up(std::max(w.again ? weight_bytes(type, n, N, F, false) : 0, rows && n ? weight_bytes(type, n, F, N * parts, true) : 0));
-  w.parts = weight_parts(n, N, F);
-  w.sums = w.beside ? w.parts.count : w.again ? workers_for(type, n, N, F) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
-  w.parts_at = w.sums_at + (bias ? up(static_cast<size_t>(w.sums) * N * sizeof(float)) : 0);
-  w.bytes = w.parts_at + (weight && w.parts.count > 1 ? static_cast<size_t>(w.parts.count) * N * F * sizeof(float) : 0);
-  return w;
 }
 
 const char *bad_shapes(int type, uint32_t N, uint32_t F, int act, const nts_dropout_t *dropout) {
@@ -1149,6 +1078,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   if (layout.bytes && (!work || !aligned_to(work, 16))) return fail_in(name, "needs nts_dense_grad_work_bytes of 16-byte-aligned work");
   char *const base = static_cast<char *>(work);
   void *const prepared = base + layout.weight_at;
+  uint32_t sum_rows = n || layout.beside ? layout.sums : 0u;
   float *const sums = gb ? reinterpret_cast<float *>(base + layout.sums_at) : nullptr;
   const void *dz = g;
   DenseArgs p{};
@@ -1161,6 +1091,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
     if (layout.from_y) q.y = y, q.mask_scale = p.drop.scale;
     if (layout.again) {
       q.a = x, q.K = F, q.a_stride = F, q.bias = bias;
+      sum_rows = share_for<kSlope>(q, type).workers;
       if (const int status = launch_product<kSlope>(q, type, prepared, stream)) return status;
     } else {
       const dim3 grid(ceil_div(N, kWave), layout.sums);
@@ -1195,7 +1126,7 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
       if (const int status = launch_sum(gw, type, q.sums, static_cast<uint64_t>(N) * F, parts, stream)) return status;
   }
   if (gb)
-    if (const int status = launch_sum(gb, type, sums, N, n || layout.beside ? layout.sums : 0u, stream)) return status;
+    if (const int status = launch_sum(gb, type, sums, N, sum_rows, stream)) return status;
   return NTS_OK;
 }
 

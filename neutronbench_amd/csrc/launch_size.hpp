@@ -4,6 +4,8 @@
 
 namespace nts {
 
+inline uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
+
 // A launch has fewer than 2^32 threads: blocks of 256, at most.
 constexpr uint32_t kMostBlocks = (1u << 24) - 1;
 
