@@ -631,8 +631,8 @@ int nts_dot_attention_grad(void *gq, void *gk, void *gv, const void *g, const vo
  * nts_dense_grad: for g, the gradient of y, the gradients gx [n, F], gw [N, F] and gb [N], each NULL where it is not wanted (that of the
  * residual is g itself).  z is computed again, not kept, but for relu without a residual where y (the layer's output, else NULL; never with a
  * residual) says which sums were above 0 and kept: it has to be what it was, and a sum whose output was rounded to 0 counts as 0.  In 16
- * bits the gradient of z is not rounded to the operands' type before the two products: it is held as two values, the nearest one and what that
- * leaves (nothing where the nearest is infinite), or as g itself with the scale of what is kept after the sums.  relu's slope at 0 is 0.
+ * bits the gradient of z is not rounded to the operands' type before the two products: it is held in 32 bits and multiplied as operands of 32
+ * bits are, or is g itself with the scale of what is kept after the sums.  relu's slope at 0 is 0.
  * work: nts_dense_work_bytes / nts_dense_grad_work_bytes of 16-byte-aligned device memory (0: may be NULL), in use until the call's work
  * on `stream` is done. */
 enum nts_activation { NTS_ACT_NONE = 0, NTS_ACT_RELU = 1, NTS_ACT_GELU = 2 /* z times the normal distribution's share below z */, NTS_ACT_SILU = 3 };

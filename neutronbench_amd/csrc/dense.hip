@@ -3,9 +3,12 @@
 //   dz = drop(g) act'(z) with z computed again, gx = dz w, gw = dz^T x, gb = column sums of dz
 // With relu and no residual y says what dz needs: it is above 0 where z is and the value was kept.  Then z is not computed again, and rows of up
 // to 128 values have dz never stored: both products make it from g and y as they read them.  dz of 16-bit operands is not rounded to 16 bits, which
-// would add an error as large as the results' own rounding: dz of a computed z is stored as the nearest value and what that leaves, both
-// of which are multiplied, and otherwise the products are of g itself, dropped, and the scale of what is kept comes after the sums.
+// would add an error as large as the results' own rounding: dz of a computed z is stored in 32 bits and multiplied as three bf16 parts, with as
+// many parts of the other operand as it has (bf16 one, fp16 two), and otherwise the products are of g itself, dropped, and the scale of what is
+// kept comes after the sums.  (Two parts of the operands' own type take as much memory and one matrix instruction less, but hold 16 to 17
+// bits in bf16, and in fp16 nothing below 2^-25 or above 65,504.)
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_layout.hpp"
 #include "launch_size.hpp"
@@ -29,7 +32,7 @@ struct DenseArgs {
   const void *y;      // masked gradients: a is g, and counts where y is not 0 or below, times mask_scale
   float mask_scale;
   float after;  // the products of 16-bit values for gx and gw, times this
-  bool split;   // dz is rows of two parts of N values each
+  bool dz32;    // a is dz in 32 bits, the other operand and the result are of 16
   uint32_t M, N, K, a_stride, b_stride;
   void *out;
   const void *bias, *more;  // more: the residual, or the gradient of y
@@ -135,6 +138,11 @@ __host__ __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t part
 
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+// Parts of an operand of T that is multiplied by one of A: fp16 is two bf16 parts, whose exponents reach as far.
+template <typename A, typename T>
+constexpr int kPlanesBeside = sizeof(A) == sizeof(T) ? kPlanes<T> : 1;
+template <>
+constexpr int kPlanesBeside<float, F16> = 2;
 
 template <typename T>
 __device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
@@ -166,11 +174,12 @@ __device__ __forceinline__ void split8(const uint16_t *v, u32x4 *w) {
   for (int i = 0; i < 4; ++i) w[0][i] = v[2 * i] | static_cast<uint32_t>(v[2 * i + 1]) << 16;
 }
 // The sum of an element's products term by term, as far as it is not NaN; mask: as DenseArgs' y, null for none.
-__device__ __forceinline__ float sum_of_terms(const float *x, const float *mask, float scale, uint64_t x_step, const float *y, uint64_t y_step, uint64_t count) {
+template <typename T>
+__device__ __forceinline__ float sum_of_terms(const float *x, const float *mask, float scale, uint64_t x_step, const T *y, uint64_t y_step, uint64_t count) {
   float sum = 0.0f;
   for (uint64_t f = 0; f < count && sum == sum; ++f) {
     const float v = !mask ? x[f * x_step] : mask[f * x_step] <= 0.0f ? 0.0f : x[f * x_step] * scale;
-    sum = fmaf(v, y[f * y_step], sum);
+    sum = fmaf(v, get_value(y + f * y_step), sum);
   }
   return sum;
 }
@@ -180,12 +189,11 @@ __device__ __forceinline__ float sum_of_terms(const float *x, const float *mask,
 struct PrepareArgs {
   const void *from;
   uint16_t *to;
-  uint32_t columns, terms, stride, stages, tiles, wrap;  // wrap: terms from there on are the first ones again
+  uint32_t columns, terms, stride, stages, tiles;
 };
-template <typename T, bool ALONG>
+template <typename T, int P, bool ALONG>
 __global__ __launch_bounds__(256) void dense_prepare_kernel(PrepareArgs p) {
   typedef typename ValueOf<T>::raw raw;
-  constexpr int P = kPlanes<T>;
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   // neighbouring threads have neighbouring terms or columns, as they lie in memory
   const uint32_t part = ALONG ? i % 4u : i / kTile % 4u, row = ALONG ? i / 4u % kTile : i % kTile, block = i / (4u * kTile);
@@ -200,13 +208,19 @@ __global__ __launch_bounds__(256) void dense_prepare_kernel(PrepareArgs p) {
   } else {
 #pragma unroll
   for (uint32_t k = 0; k < 8; ++k) {
-    const uint32_t one = term + k < p.wrap ? term + k : term + k - p.wrap;
-    const uint64_t at = ALONG ? static_cast<uint64_t>(column) * p.stride + one : static_cast<uint64_t>(one) * p.stride + column;
+    const uint64_t at = ALONG ? static_cast<uint64_t>(column) * p.stride + term + k : static_cast<uint64_t>(term + k) * p.stride + column;
     v[k] = column < p.columns && term + k < p.terms ? static_cast<const raw *>(p.from)[at] : static_cast<raw>(0);
   }
   }
   u32x4 w[3];
-  split8(v, w);
+  if constexpr (P == 2) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = ValueOf<T>::get(v[k]);
+    split8(f, w);
+  } else {
+    split8(v, w);
+  }
 #pragma unroll
   for (int c = 0; c < P; ++c) *reinterpret_cast<u32x4 *>(p.to + (static_cast<uint64_t>(block) * P + c) * kPlane + tile_at(row, part)) = w[c];
 }
@@ -226,10 +240,9 @@ __device__ __forceinline__ void stage_barrier() {
 
 // What a wavefront's 16 * MR rows by 128 columns of sums become.  Through LDS (`mine`, 4 KB), 16 rows by 64 columns at a time, a lane's columns
 // become lines (part c of row r at c ^ r).  sums: of the columns, kept over tiles.
-template <typename T, int USE, int MR, bool MASKED>
+template <typename A, typename T, int USE, int MR, bool MASKED>
 __device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f32x4 (&acc)[MR][8], f32x4 *mine, uint64_t first_row, uint32_t column0,
                                             const float (&bias)[2][4], float (&sums)[2][4]) {
-  constexpr int P = kPlanes<T>;
   const uint32_t lane = threadIdx.x & (kWave - 1), r = lane & 15u, part = lane >> 4;
 #pragma unroll
   for (int i = 0; i < MR; ++i)
@@ -262,11 +275,11 @@ __device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f
           v[u][0] = got.x, v[u][1] = got.y, v[u][2] = got.z, v[u][3] = got.w;
 #pragma unroll
           for (int k = 0; k < 4; ++k) more[u][k] = ahead[u][k];
-          if (P == 3) {
+          if (sizeof(A) == 4) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
               if (fabsf(v[u][k]) < INFINITY || at >= p.M || c + k >= p.N) continue;
-              const float *const b = static_cast<const float *>(p.w);
+              const T *const b = static_cast<const T *>(p.w);
               v[u][k] = sum_of_terms(static_cast<const float *>(p.a) + at * p.a_stride,
                                      MASKED ? static_cast<const float *>(p.y) + at * p.a_stride : nullptr, p.mask_scale, 1,
                                      USE == kRows ? b + c + k : b + static_cast<uint64_t>(c + k) * p.K, USE == kRows ? p.N : 1u, p.K);
@@ -292,18 +305,10 @@ __device__ __forceinline__ void finish_tile(const DenseArgs &p, uint32_t step, f
           }
           if (USE == kSlope) through_slope(v[u], more[u], p.act);
           if (at >= p.M || c >= p.N) continue;
-          if (USE == kSlope && P == 1) {
-            float rest[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float near = ValueOf<T>::get(ValueOf<T>::put(v[u][k]));
-              rest[k] = fabsf(near) < INFINITY ? v[u][k] - near : 0.0f;
-            }
-            T *const to = static_cast<T *>(p.out) + at * (2ull * p.N) + c;
-            put_columns(to, p.N - c, v[u], p.streamed);
-            put_columns(to + p.N, p.N - c, rest, p.streamed);
+          if (USE == kSlope) {
+            put_columns(static_cast<float *>(p.out) + at * p.N + c, p.N - c, v[u], p.streamed);
           } else {
-            if (USE == kRows && P == 1) {
+            if (USE == kRows && sizeof(A) == 2) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[u][k] *= p.after;
             }
@@ -362,10 +367,11 @@ __device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sum
 // instructions a product, which are under way for half of the time, and the splitting for most of the other half; the clock falls to 1.8 GHz
 // (splitting one tile between the instructions of the other, or three blocks to a compute unit, which spill, did not help).  169,343 rows of
 // 128 by 128 in bf16 with GELU, drops and residual take 55 us, 2.4 TB/s: vector instructions of the epilogue for half of the time.
-template <typename T, int USE, int MR, int WN, bool MASKED>
-__global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
-  constexpr int P = kPlanes<T>;
-  constexpr uint32_t kRows = 64 * MR, kStage = WN * P * kPlane;
+// A: the rows' type.
+template <typename A, typename T, int USE, int MR, int WN, bool MASKED>
+__device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
+  constexpr int P = kPlanes<A>, PB = kPlanesBeside<A, T>;
+  constexpr uint32_t kRows = 64 * MR, kStage = WN * PB * kPlane;
   // results are turned where the stage of the weight was that has been used last, if it is large enough
   constexpr bool kApart = kStage * sizeof(uint16_t) < 4u * WN * 4096u;
   __shared__ __attribute__((aligned(16))) uint16_t weight0[kStage], weight1[kStage], apart[kApart ? 4 * WN * 2048 : 8];
@@ -376,32 +382,32 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
   const uint32_t step = USE == kLayer || USE == kSlope ? drop_step(p.drop) : 0u;
   if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
   if (!has_rows(worker, p.workers)) return;
-  const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * WN * stages * P * kPlane;
-  const T *const rows = static_cast<const T *>(p.a);
+  const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * WN * stages * PB * kPlane;
+  const A *const rows = static_cast<const A *>(p.a);
   // stage s of the weight
   auto request_weight = [&](uint16_t *to, uint32_t s) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t i = 0; i < 2 * P; ++i) {
-      const uint32_t piece = i * 4 * WN + wave, group = piece / (8 * P), at = piece % (8 * P);  // 512 values each
-      load_to_lds(weight + ((static_cast<uint64_t>(group) * stages + s) * P * kPlane + at * 512u + lane * 8u), to + piece * 512u);
+    for (uint32_t i = 0; i < 2 * PB; ++i) {
+      const uint32_t piece = i * 4 * WN + wave, group = piece / (8 * PB), at = piece % (8 * PB);  // 512 values each
+      load_to_lds(weight + ((static_cast<uint64_t>(group) * stages + s) * PB * kPlane + at * 512u + lane * 8u), to + piece * 512u);
     }
   };
-  typedef typename ValueOf<T>::raw raw;
+  typedef typename ValueOf<A>::raw raw;
   constexpr int L = 8 * sizeof(raw) / 16;  // loads of a lane's eight terms
   constexpr int S = MASKED ? 2 : 1;  // operands: g and y
   u32x4 next[S][MR][L];
-  const T *row_at[S][MR];
+  const A *row_at[S][MR];
   auto place = [&](uint32_t tile) __attribute__((always_inline)) {  // rows that the result does not have read the last one
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
       const uint64_t row = static_cast<uint64_t>(tile) * kRows + wr * (16u * MR) + i * 16u + r;
 #pragma unroll
       for (int o = 0; o < S; ++o)
-        row_at[o][i] = (o ? static_cast<const T *>(p.y) : rows) + min(row, static_cast<uint64_t>(p.M - 1u)) * p.a_stride + part * 8u;
+        row_at[o][i] = (o ? static_cast<const A *>(p.y) : rows) + min(row, static_cast<uint64_t>(p.M - 1u)) * p.a_stride + part * 8u;
     }
   };
   auto request_rows = [&](uint32_t s) __attribute__((always_inline)) {
-    typedef typename Pack<T, 16 / sizeof(raw)>::type Whole;
+    typedef typename Pack<A, 16 / sizeof(raw)>::type Whole;
     const uint32_t k = s * kTerms;
     if (k + kTerms <= p.K) {
 #pragma unroll
@@ -439,7 +445,7 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
       return __uint_as_float(bits);
     }
     const uint32_t both = next[o][i][0][e / 2 % 4];
-    return ValueOf<T>::get(static_cast<raw>(e & 1 ? both >> 16 : both));
+    return ValueOf<A>::get(static_cast<raw>(e & 1 ? both >> 16 : both));
   };
   f32x4 acc[MR][8];
   uint32_t half = 0;
@@ -470,7 +476,7 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
             split8(v, a[i]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[i][0][e] = ValueOf<T>::put(v[2 * e]) | static_cast<uint32_t>(ValueOf<T>::put(v[2 * e + 1])) << 16;
+            for (int e = 0; e < 4; ++e) a[i][0][e] = ValueOf<A>::put(v[2 * e]) | static_cast<uint32_t>(ValueOf<A>::put(v[2 * e + 1])) << 16;
           }
         } else {
           a[i][0] = next[0][i][0];
@@ -482,31 +488,42 @@ __global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_k
         request_weight(half ? weight0 : weight1, last ? 0u : s + 1u);
         request_rows(last ? 0u : s + 1u);
       }
-      const uint16_t *const w = (half ? weight1 : weight0) + wc * (P * kPlane);
+      const uint16_t *const w = (half ? weight1 : weight0) + wc * (PB * kPlane);
       half ^= 1u;
-      u32x4 b[2][P];
+      u32x4 b[2][PB];
 #pragma unroll
-      for (int c = 0; c < P; ++c) b[0][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at(r, part));
+      for (int c = 0; c < PB; ++c) b[0][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at(r, part));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (j < 7) {
 #pragma unroll
-          for (int c = 0; c < P; ++c) b[(j + 1) & 1][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at((j + 1) * 16 + r, part));
+          for (int c = 0; c < PB; ++c) b[(j + 1) & 1][c] = *reinterpret_cast<const u32x4 *>(w + c * kPlane + tile_at((j + 1) * 16 + r, part));
         }
         // the weight is the first operand: a lane then ends up with four neighbouring columns of one row; small products first
 #pragma unroll
         for (int q = P - 1; q >= 0; --q)
 #pragma unroll
-          for (int c = 0; c <= q; ++c)
+          for (int c = q >= PB ? q - PB + 1 : 0; c <= q; ++c)
 #pragma unroll
-            for (int i = 0; i < MR; ++i) acc[i][j] = multiply<T>(b[j & 1][q - c], a[i][c], acc[i][j]);
+            for (int i = 0; i < MR; ++i) acc[i][j] = multiply<A>(b[j & 1][q - c], a[i][c], acc[i][j]);
       }
     }
     if (!kApart) __builtin_amdgcn_s_barrier();  // all have read it
-    finish_tile<T, USE, MR, MASKED>(p, step, acc, reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u,
+    finish_tile<A, T, USE, MR, MASKED>(p, step, acc, reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u,
                                     static_cast<uint64_t>(tile) * kRows + wr * (16u * MR), tn * (kTile * WN) + wc * kTile, bias, sums);
   }
   if (USE == kSlope && p.sums) block_sums<4 * WN, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0), worker, tn * (kTile * WN));
+}
+template <typename T, int USE, int MR, int WN, bool MASKED>
+__global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
+  rows_of_tiles<T, T, USE, MR, WN, MASKED>(p);
+}
+// Rows of dz in 32 bits times a weight of 16.  169,343 rows of 128 by 128: 34 us in bf16, 3.8 TB/s, as with two bf16 parts of dz, whose products
+// read the weight twice from LDS; 49 in fp16.  Large products go this way, too: 65,536 x 4,096 x 4,096 in bf16 5.7 ms, three products at
+// 1,160 TFLOP/s, where large tiles took 3.5 for two parts; in fp16 8.9.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void dense_dz_kernel(DenseArgs p) {
+  rows_of_tiles<float, T, kRows, 2, 1, false>(p);
 }
 
 // Large products of 16-bit values whose rows begin at multiples of 16 bytes: a block of eight wavefronts takes 256 rows by 256 columns, 32
@@ -532,7 +549,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
   const char *const from_a = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.a) + row_a * p.a_stride);
   const char *const from_b = reinterpret_cast<const char *>(static_cast<const uint16_t *>(p.b) + row_b * p.b_stride);
   const uint32_t chunk = part_at(lane / 4u, lane & 3u);  // the same for all of the lane's rows, which are 16 apart
-  uint32_t at[4];  // in bytes: below 2^27, as 256 rows of 2^18 values are
+  uint32_t at[4];  // in bytes: below 2^26, as 256 rows of 2^17 values are
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t row = ((i & 1) * 8u + wave) * 16u + lane / 4u;
@@ -595,19 +612,18 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseArgs p) {
   stage_barrier();  // no load may reach the LDS any more
   float bias[2][4] = {}, sums[2][4] = {};
   if (USE != kRows) bias_of_columns<T>(p, tn * kWideTile + wc * kTile, bias);
-  finish_tile<T, USE, 4, false>(p, step, acc, reinterpret_cast<f32x4 *>(&stages[0][0]) + wave * 256u, static_cast<uint64_t>(tm) * kWideTile + wr * 64u,
+  finish_tile<T, T, USE, 4, false>(p, step, acc, reinterpret_cast<f32x4 *>(&stages[0][0]) + wave * 256u, static_cast<uint64_t>(tm) * kWideTile + wr * 64u,
                                 tn * kWideTile + wc * kTile, bias, sums);
   if (USE == kSlope && p.sums) block_sums<8, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(&stages[2][0]), tm, tn * kWideTile);
 }
-// The weight with rows and columns exchanged, `copies` times beside each other.
-__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns, uint32_t copies) {
+// The weight with rows and columns exchanged.
+__global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ to, const uint16_t *__restrict__ from, uint32_t rows, uint32_t columns) {
   __shared__ uint16_t tile[64][66];
   const uint32_t x = threadIdx.x % 64u, y = threadIdx.x / 64u, c0 = blockIdx.x * 64u, r0 = blockIdx.y * 64u;
   for (uint32_t i = y; i < 64u; i += 4u) tile[i][x] = r0 + i < rows && c0 + x < columns ? from[static_cast<uint64_t>(r0 + i) * columns + c0 + x] : uint16_t{0};
   __syncthreads();
   for (uint32_t i = y; i < 64u; i += 4u)
-    if (c0 + i < columns && r0 + x < rows)
-      for (uint32_t k = 0; k < copies; ++k) to[(static_cast<uint64_t>(c0 + i) * copies + k) * rows + r0 + x] = tile[x][i];
+    if (c0 + i < columns && r0 + x < rows) to[static_cast<uint64_t>(c0 + i) * rows + r0 + x] = tile[x][i];
 }
 
 // ---- the weight's gradient --------------------------------------------------------------------------
@@ -615,15 +631,14 @@ __global__ __launch_bounds__(256) void dense_turn_kernel(uint16_t *__restrict__ 
 // not depend on scheduling.  A block of four wavefronts takes 128 rows of the result by 128 columns, 32 terms at a time through LDS, where
 // both operands are written with the terms of a row or column side by side.
 // 232,965 terms of 256 by 602 in 32 bits: 500-550 us, 130-143 TFLOP/s, splitting half of the time and matrix instructions for two fifths;
-// 169,343 of 128 by 128 in bf16: 19 us, 4.5 TB/s, and 25 with dz in two parts, 5.1 TB/s.
+// 169,343 of 128 by 128 in bf16: 19 us, 4.5 TB/s, and 33 with dz in 32 bits, three matrix instructions a product and the splitting; in
+// fp16, with five, 38.
 // Sixteen terms of one column of an operand, or eight of each of two neighbouring columns (PAIRS: rows of 16-bit values of an even number),
-// on their way from memory to LDS.  kMasked: as DenseArgs' y; kSplit: dz of two parts, which go to two planes.
-enum Source { kPlain, kMasked, kSplit };
-template <typename T, bool PAIRS, int SOURCE>
+// on their way from memory to LDS, as P parts in planes of their own.  MASKED: as DenseArgs' y.
+template <typename T, bool PAIRS, bool MASKED, int P>
 struct Terms {
   typedef typename ValueOf<T>::raw raw;
-  static constexpr bool MASKED = SOURCE == kMasked;
-  static constexpr int S = SOURCE == kPlain ? 1 : 2, N = PAIRS ? 8 : 16, P = SOURCE == kSplit ? 2 : kPlanes<T>;
+  static constexpr int S = MASKED ? 2 : 1, N = PAIRS ? 8 : 16;
   typedef uint32_t Word __attribute__((aligned(2)));
   uint32_t v[S][N];
   const T *from[S];  // the operands' beginning, so that a row's address is a scalar, and the lane's place from there
@@ -666,14 +681,14 @@ struct Terms {
 #pragma unroll
       for (int i = 0; i < N; i += 8) {
         u32x4 w[3];
-        if (sizeof(raw) == 4 || MASKED) {
+        if (sizeof(raw) == 4 || MASKED || P == 2) {
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             f[e] = value(i + e, which) * (MASKED && P == 3 ? scale : 1.0f);
             if (sums) sums[which] += MASKED && P == 1 ? f[e] * scale : f[e];
           }
-          if constexpr (sizeof(raw) == 4) {
+          if constexpr (P > 1) {
             split8(f, w);
           } else {
 #pragma unroll
@@ -681,12 +696,10 @@ struct Terms {
           }
         } else {
 #pragma unroll
-          for (int o = 0; o < S; ++o)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = v[o][i + 2 * e], y = v[o][i + 2 * e + 1];
-              w[o][e] = which ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = v[0][i + 2 * e], y = v[0][i + 2 * e + 1];
+            w[0][e] = which ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+          }
           if (sums) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sums[which] += value(i + e, which);
@@ -698,19 +711,23 @@ struct Terms {
   }
 };
 
+// SOURCE, the first operand: g or dz as it is, g by y, dz in 32 bits beside operands of 16.
+enum Source { kPlain, kMasked, kInWords };
 template <typename T, bool PAIRS, int SOURCE>
 __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
+  typedef typename std::conditional<SOURCE == kInWords, float, T>::type A;
   constexpr bool MASKED = SOURCE == kMasked;
-  constexpr int P = kPlanes<T>, PA = Terms<T, PAIRS, SOURCE>::P;
+  constexpr int PA = kPlanes<A>, P = kPlanesBeside<A, T>;
+  typedef Terms<A, PAIRS && sizeof(A) == 2, MASKED, PA> First;
   __shared__ __attribute__((aligned(16))) uint16_t tile[(PA + P) * kPlane];
   uint16_t *const ta = tile, *const tb = tile + PA * kPlane;
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
   const uint32_t tm = blockIdx.x / p.tiles_n, tn = blockIdx.x % p.tiles_n;
   const uint32_t m0 = tm * kTile, n0 = tn * kTile;
   const uint64_t begin = static_cast<uint64_t>(blockIdx.z) * p.part_terms, end = min(static_cast<uint64_t>(p.K), begin + p.part_terms);
-  Terms<T, PAIRS, SOURCE> va;
-  Terms<T, PAIRS, kPlain> vb;
-  va.place(p.a, SOURCE == kSplit ? static_cast<const T *>(p.a) + p.M : p.y, p.a_stride, m0, p.M);
+  First va;
+  Terms<T, PAIRS, false, P> vb;
+  va.place(p.a, p.y, p.a_stride, m0, p.M);
   vb.place(p.b, nullptr, p.b_stride, n0, p.N);
   float sums[2] = {};
   const bool summing = p.column_sums && tn == 0;
@@ -746,9 +763,9 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
 #pragma unroll
       for (int s = PA - 1; s >= 0; --s)
 #pragma unroll
-        for (int c = PA == P ? 0 : s; c <= s; ++c)
+        for (int c = s >= P ? s - P + 1 : 0; c <= s; ++c)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = multiply<T>(b[s - c][j], a[c], acc[i][j]);
+          for (int j = 0; j < 4; ++j) acc[i][j] = multiply<A>(b[s - c][j], a[c], acc[i][j]);
     }
     __syncthreads();
   }
@@ -765,15 +782,15 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
       const f32x4 got = mine[row * 16u + ((lane & 15u) ^ row)];
       if (i >= p.M || c >= p.N) continue;
       float v[4] = {got.x, got.y, got.z, got.w};
-      if (P == 3) {
+      if (sizeof(A) == 4) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
           if (fabsf(v[k]) < INFINITY || c + k >= p.N) continue;
           v[k] = sum_of_terms(static_cast<const float *>(p.a) + begin * p.a_stride + i, MASKED ? static_cast<const float *>(p.y) + begin * p.a_stride + i : nullptr,
-                              p.mask_scale, p.a_stride, static_cast<const float *>(p.b) + begin * p.b_stride + c + k, p.b_stride, end - begin);
+                              p.mask_scale, p.a_stride, static_cast<const T *>(p.b) + begin * p.b_stride + c + k, p.b_stride, end - begin);
         }
       }
-      if (P == 1) {
+      if (sizeof(A) == 2) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] *= p.after;
       }
@@ -785,13 +802,13 @@ __global__ __launch_bounds__(256, 2) void dense_weight_kernel(DenseArgs p) {
   if (!summing) return;
   __syncthreads();
   float(*const of_terms)[kTile] = reinterpret_cast<float(*)[kTile]>(tile);
-  of_terms[va.first / Terms<T, PAIRS, SOURCE>::N][va.column] = sums[0];
-  if (PAIRS) of_terms[va.first / 8u][va.column + 1u] = sums[1];
+  of_terms[va.first / First::N][va.column] = sums[0];
+  if (First::N == 8) of_terms[va.first / 8u][va.column + 1u] = sums[1];
   __syncthreads();
   if (t < kTile && m0 + t < p.M) {
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < (PAIRS ? 4 : 2); ++i) sum += of_terms[i][t];
+    for (int i = 0; i < (First::N == 8 ? 4 : 2); ++i) sum += of_terms[i][t];
     p.column_sums[static_cast<uint64_t>(blockIdx.z) * p.M + m0 + t] = sum;
   }
 }
@@ -925,11 +942,12 @@ __global__ __launch_bounds__(kSumWaves *kWave) void dense_sum_kernel(T *__restri
 constexpr uint64_t kStreamed = 32ull << 20;  // an output from this size on is more than the L2s hold
 
 template <bool ALONG>
-int launch_prepare(void *to, const void *w, int type, uint32_t columns, uint32_t terms, uint32_t stride, uint32_t wrap, hipStream_t stream) {
-  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns), wrap};
+int launch_prepare(void *to, const void *w, int type, uint32_t planes, uint32_t columns, uint32_t terms, uint32_t stride, hipStream_t stream) {
+  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns)};
   const dim3 grid(ceil_div(static_cast<uint64_t>(p.stages) * p.tiles * 4u * kTile, 256));
-  if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, ALONG>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied
+  if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, 3, ALONG>), grid, dim3(256), 0, stream, p);
+  else if (planes == 2) hipLaunchKernelGGL((dense_prepare_kernel<F16, 2, ALONG>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, 1, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied
   NTS_LAUNCH_CHECK("dense_prepare_kernel");
   return NTS_OK;
 }
@@ -946,6 +964,12 @@ void launch_product_of(const DenseArgs &p, const Share &share, hipStream_t strea
       return;
     }
   }
+  if constexpr (USE == kRows && sizeof(T) == 2) {
+    if (p.dz32) {
+      hipLaunchKernelGGL((dense_dz_kernel<T>), dim3(launched_workers(share) * p.tiles_n), dim3(256), 0, stream, p);
+      return;
+    }
+  }
   if constexpr (USE == kRows) {
     if (p.y) return launch_rows<T, USE, true>(p, share, stream);
   }
@@ -953,24 +977,24 @@ void launch_product_of(const DenseArgs &p, const Share &share, hipStream_t strea
 }
 template <int USE>
 Share share_for(const DenseArgs &p, int type) {
-  return share_of(type, p.M, p.N, p.K, !p.y && aligned_to(p.a, 16) && (USE == kRows || aligned_to(p.w, 16)));
+  return share_of(type, p.M, p.N, p.K, !p.y && !p.dz32 && aligned_to(p.a, 16) && (USE == kRows || aligned_to(p.w, 16)));
 }
 // The product of p.a and the weight p.w, whose form for it goes to `work`.
 template <int USE>
 int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
   const Share share = share_for<USE>(p, type);
   p.tiles_m = share.tiles_m, p.tiles_n = share.tiles_n, p.workers = share.workers;
-  p.streamed = static_cast<uint64_t>(p.M) * p.N * type_size(type) >= kStreamed;
+  p.streamed = static_cast<uint64_t>(p.M) * p.N * (USE == kSlope ? sizeof(float) : type_size(type)) >= kStreamed;
   p.b = work;
   if (!share.wide) {
-    const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, p.N, p.K, p.N, p.split ? p.K / 2u : p.K, stream)
-                                    : launch_prepare<true>(work, p.w, type, p.N, p.K, p.K, p.K, stream);
+    const uint32_t planes = planes_of(type, p.dz32);
+    const int status = USE == kRows ? launch_prepare<false>(work, p.w, type, planes, p.N, p.K, p.N, stream)
+                                    : launch_prepare<true>(work, p.w, type, planes, p.N, p.K, p.K, stream);
     if (status) return status;
   } else if (USE == kRows) {
     p.b_stride = p.K;
-    const uint32_t copies = p.split ? 2u : 1u, rows = p.K / copies;
-    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(rows, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
-                       static_cast<const uint16_t *>(p.w), rows, p.N, copies);
+    hipLaunchKernelGGL(dense_turn_kernel, dim3(ceil_div(p.N, 64), ceil_div(p.K, 64)), dim3(256), 0, stream, static_cast<uint16_t *>(work),
+                       static_cast<const uint16_t *>(p.w), p.K, p.N);
     NTS_LAUNCH_CHECK("dense_turn_kernel");
   } else {
     p.b = p.w, p.b_stride = p.K;
@@ -984,8 +1008,8 @@ int launch_product(DenseArgs p, int type, void *work, hipStream_t stream) {
 template <typename T, bool PAIRS>
 void launch_weight_of(const DenseArgs &p, const dim3 &grid, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (p.split) {
-      hipLaunchKernelGGL((dense_weight_kernel<T, PAIRS, kSplit>), grid, dim3(256), 0, stream, p);
+    if (p.dz32) {
+      hipLaunchKernelGGL((dense_weight_kernel<T, PAIRS, kInWords>), grid, dim3(256), 0, stream, p);
       return;
     }
   }
@@ -1103,16 +1127,15 @@ int nts_dense_grad(void *gx, void *gw, void *gb, const void *g, const void *x, c
   }
   if (layout.masked) p.y = y, p.mask_scale = p.drop.scale;
   p.after = layout.masked || (layout.stored && !layout.again) ? p.drop.scale : 1.0f;
-  p.split = layout.split;
-  const uint32_t dz_width = layout.split ? 2u * N : N;
+  p.dz32 = layout.dz32;
   if (gx && n) {
     DenseArgs q = p;
-    q.a = dz, q.M = n, q.N = F, q.K = dz_width, q.a_stride = dz_width, q.out = gx;
+    q.a = dz, q.M = n, q.N = F, q.K = N, q.a_stride = N, q.out = gx;
     if (const int status = launch_product<kRows>(q, type, prepared, stream)) return status;
   }
   if (gw) {
     DenseArgs q = p;
-    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = dz_width, q.b_stride = F, q.out = gw, q.part_terms = layout.parts.terms;
+    q.a = dz, q.b = x, q.M = N, q.N = F, q.K = n, q.a_stride = N, q.b_stride = F, q.out = gw, q.part_terms = layout.parts.terms;
     q.tiles_m = ceil_div(N, kTile), q.tiles_n = ceil_div(F, kTile);
     if (layout.beside) q.column_sums = sums;
     const uint32_t parts = layout.parts.count;

@@ -15,9 +15,11 @@ constexpr uint32_t kWideTile = 256;
 
 // Bytes of a prepared weight.
 inline uint32_t tile_groups(uint32_t columns) { return ceil_div(columns, 2 * kTile) * 2u; }
-inline size_t prepared_bytes(int type, uint32_t columns, uint32_t terms) {
-  return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * (type == NTS_F32 ? 6 : 2);
+inline size_t prepared_bytes(uint32_t planes, uint32_t columns, uint32_t terms) {
+  return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * planes * 2u;
 }
+// Parts of a weight: three of 32 bits; beside dz in 32 bits, which is multiplied as bf16 parts, two of fp16; else the weight itself.
+inline uint32_t planes_of(int type, bool dz32) { return type == NTS_F32 ? 3u : dz32 && type == NTS_F16 ? 2u : 1u; }
 // Large products by large tiles, where there are enough of them for the chip and rows of many terms; in us by large tiles and by rows:
 // 16,384 x 1,024 x 512 26 and 38, 65,536 x 256 x 1,024 42 and 63; of 256 terms 32,768 x 4,096 150 and 129; of 128 tiles 8,192 x 1,024 x 1,024
 // 34 and 34.
@@ -27,7 +29,7 @@ inline bool by_wide_tiles(int type, uint32_t n, uint32_t N, uint32_t K) {
 // Bytes of a product's weight in the work: as the rows' kernel wants it, or turned for large tiles.
 inline size_t weight_bytes(int type, uint32_t n, uint32_t columns, uint32_t terms, bool turned) {
   // operands between aligned addresses take the rows' kernel all the same
-  return std::max(prepared_bytes(type, columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * terms * 2 : size_t{0});
+  return std::max(prepared_bytes(planes_of(type, false), columns, terms), turned && by_wide_tiles(type, n, columns, terms) ? static_cast<size_t>(columns) * terms * 2 : size_t{0});
 }
 // How a product's tiles of rows are shared out: every worker takes every `workers`-th of them and leaves a row of column sums.  aligned: the
 // operands begin at multiples of 16 bytes, without which there are no large tiles.
@@ -73,7 +75,7 @@ struct Work {
   bool stored;   // dz is stored
   bool beside;   // the bias's sums are made beside the weight's gradient
   bool again;    // z is computed again
-  bool split;    // dz is stored in two parts
+  bool dz32;     // and dz is stored in 32 bits, though the operands have 16
   size_t weight_at, sums_at, parts_at, bytes;
   uint32_t sums;  // rows of them that there is room for
   Parts parts;
@@ -88,10 +90,11 @@ inline Work grad_work(int type, uint32_t n, uint32_t N, uint32_t F, int act, boo
   w.stored = !w.masked && (act != NTS_ACT_NONE || dropout) && n;
   w.beside = bias && weight && !w.stored;
   w.again = w.stored && act != NTS_ACT_NONE && !w.from_y;
-  w.split = w.again && type != NTS_F32;
-  const uint32_t parts = w.split ? 2u : 1u;
-  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * (type == NTS_F32 ? 4u : 2u) * parts) : 0;
-  w.sums_at = w.weight_at + up(std::max(w.again ? weight_bytes(type, n, N, F, false) : 0, rows && n ? weight_bytes(type, n, F, N * parts, true) : 0));
+  w.dz32 = w.again && type != NTS_F32;
+  w.weight_at = w.stored ? up(static_cast<size_t>(n) * N * (type == NTS_F32 || w.dz32 ? 4u : 2u)) : 0;
+  const size_t for_z = w.again ? weight_bytes(type, n, N, F, false) : 0;
+  const size_t for_rows = !rows || !n ? 0 : w.dz32 ? prepared_bytes(planes_of(type, true), F, N) : weight_bytes(type, n, F, N, true);
+  w.sums_at = w.weight_at + up(std::max(for_z, for_rows));
   w.parts = weight_parts(n, N, F);
   w.sums = w.beside ? w.parts.count : w.again ? most_workers(type, n, N, F) : static_cast<uint32_t>(std::min<uint64_t>(1024, ceil_div(n, 64)));
   w.parts_at = w.sums_at + (bias ? up(static_cast<size_t>(w.sums) * N * sizeof(float)) : 0);

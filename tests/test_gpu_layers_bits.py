@@ -1,0 +1,132 @@
+"""Dense layers of 16-bit operands: the gradient of z is as good as in 32 bits, whatever its size, and infinities come out as in the formulas."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import layers_ref as ref
+from neutronbench_amd import layers
+from test_gpu_layers import BF16, F16
+
+pytestmark = pytest.mark.gpu
+
+
+def doubles(t):
+    return t.double().cpu().numpy()
+
+
+def backward(act, x, w, b, g, residual=False, dropout=None):
+    """Gradients of rows, weight and bias."""
+    op = layers.DenseOp(act, dropout)
+    op.forward(x, w, b, torch.zeros_like(g) if residual else None)
+    return op.backward(g), *op.get_additional_grad()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("p", [0.1, 0.2, 0.3, 0.45, 0.6, 0.7, 0.85])
+def test_gradients_where_terms_cancel(device, dtype, p):
+    """relu's slopes are 1 here, so dz is g times the scale of what is kept, rounded to 32 bits.  Two terms of it, (1 + e) (1 - e) - 1 with e = eps,
+    leave e^2 of it: of its 32 bits 10 in bf16 and none in fp16, but none at all of the first 17."""
+    n, k, e = 2, 40, torch.finfo(dtype).eps
+    drop, s = (p, 5, 3), float(ref.factor(p))
+    pair = torch.tensor([1 + e, -1.0], dtype=dtype, device=device)
+    near = torch.tensor([1 - e, 1.0], dtype=dtype, device=device)
+    small = torch.tensor(2.0 ** -7, dtype=dtype, device=device)
+    for across in (False, True):  # the weight's gradient: two rows; the rows' gradient: two columns
+        if across:
+            x, w, g = small.expand(k, 8).contiguous(), near[:, None].expand(n, 8).contiguous(), pair[None].expand(k, n).contiguous()
+        else:
+            x, w, g = near[:, None].expand(n, 8).contiguous(), small.expand(k, 8).contiguous(), pair[:, None].expand(n, k).contiguous()
+        b = torch.ones(w.shape[0], dtype=dtype, device=device)
+        gx, gw, _ = backward("relu", x, w, b, g, residual=True, dropout=layers.Dropout(*drop))
+        factors = ref.row_factors(*g.shape, *drop)
+        dz = doubles(g) * factors
+        got, want, size = (gx, dz @ doubles(w), np.abs(dz) @ np.abs(doubles(w))) if across else (gw, dz.T @ doubles(x), np.abs(dz).T @ np.abs(doubles(x)))
+        assert (np.abs(want) > 0).any() and (np.abs(want) < 2 * e * e * s).any()
+        # dz's rounding and six of the sum's (two terms, among 32 places)
+        ref.check(got, (want, 7 * ref.U * size + ref.rounding(want, dtype)), f"gradient of {'x' if across else 'w'}")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-5, 1e-6])
+def test_small_gradients_in_fp16(device, act, size):
+    """Of the weight, with g as small as a mean over many rows makes it: the sums are normal values, rounded once (test_dense_gradients_are_rounded_once
+    says why 0.5 eps / 2 of the whole is more than that).  g itself is among fp16's subnormal values there and exact as it is."""
+    n, F, N = 8192, 64, 64
+    gen = torch.Generator(device=device).manual_seed(3)
+    up = min(256.0, 1 / math.sqrt(size))  # of x, and down of w, so that z stays
+    x, w, g = (torch.randn(*s, device=device, generator=gen) * k for s, k in (((n, F), up), ((N, F), 1 / (8 * up)), ((n, N), size)))
+    x, w, b, g = x.to(F16), w.to(F16), torch.zeros(N, dtype=F16, device=device), g.to(F16)
+    gx, gw, gb = backward(act, x, w, b, g)
+    z = doubles(x) @ doubles(w).T
+    dz = doubles(g) * ref.activation(z, act)[1]
+    want = dz.T @ doubles(x)
+    assert np.median(np.abs(want)) > 2.0 ** -14
+    assert np.linalg.norm(doubles(gw) - want) / np.linalg.norm(want) < 0.5 * torch.finfo(F16).eps / 2
+    # and every element of all three: 32-bit sums, one rounding, to a subnormal value where it is one
+    for got, name in ((gx, "x"), (gw, "w"), (gb, "b")):
+        value, bound = ref.dense(doubles(x), doubles(w), doubles(b), None, doubles(g), act, np.ones((n, N)), torch.float32)[name]
+        ref.check(got, (value, bound + ref.rounding(value, F16)), f"gradient of {name}")
+
+
+def test_large_gradients_in_fp16(device):
+    """dz above the largest fp16 value, of which the sums are none."""
+    n, F, N = 300, 40, 24
+    gen = torch.Generator(device=device).manual_seed(4)
+    x, w = (torch.randn(*s, device=device, generator=gen).to(F16) * 2.0 ** -10 for s in ((n, F), (N, F)))
+    b, g = torch.ones(N, dtype=F16, device=device), torch.randn(n, N, device=device, generator=gen).sign().to(F16) * 60000
+    drop = (0.75, 6, 1)
+    factors = ref.row_factors(n, N, *drop)
+    gx, gw, _ = backward("relu", x, w, b, g, residual=True, dropout=layers.Dropout(*drop))
+    want = ref.dense(doubles(x), doubles(w), doubles(b), None, doubles(g), "relu", factors, torch.float32)
+    assert np.abs(want["x"][0]).max() < 60000 and np.abs(want["w"][0]).max() < 60000
+    for got, name in ((gx, "x"), (gw, "w")):
+        ref.check(got, (want[name][0], want[name][1] + ref.rounding(want[name][0], F16)), f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_beside_infinities(device, dtype):
+    """A finite dz times an infinite operand is infinite, with its sign; a dz of 0 (relu's slope) makes it NaN, as in the formulas."""
+    n, F, N = 40, 33, 20
+    gen = torch.Generator(device=device).manual_seed(5)
+    x, w, g = (torch.randn(*s, device=device, generator=gen).to(dtype) for s in ((n, F), (N, F), (n, N)))
+    w = w.abs()
+    x[3, 7], x[9, 8] = math.inf, -math.inf
+    w[4, 11] = math.inf
+    x[:, 11] = x[:, 11].abs() + 0.5  # the sums with w's infinity are infinite, not NaN
+    x[9, 8] = -math.inf
+    b = torch.full((N,), 0.25, dtype=dtype, device=device)
+    gx, gw, gb = backward("relu", x, w, b, g, residual=True)
+    with np.errstate(invalid="ignore", over="ignore"):
+        xd, wd, gd = doubles(x), doubles(w), doubles(g)
+        # sums with infinities by hand: BLAS may meet them in any order, but NaN and signs do not depend on it
+        z = (xd[:, None, :] * wd[None]).sum(2) + 0.25
+        dz = np.where(z <= 0, 0.0, gd)
+        wx, ww = (dz[:, :, None] * wd[None]).sum(1), (dz[:, :, None] * xd[:, None, :]).sum(0)
+    assert np.isinf(wx).any() and np.isinf(ww).any() and np.isnan(ww).any()
+    for got, want, terms, what in ((gx, wx, N, "x"), (gw, ww, n, "w"), (gb, dz.sum(0), n, "b")):
+        fine = np.where(np.isfinite(want), want, 0.0)
+        # as many terms as there are, each below 16 here
+        ref.check(got, (want, (terms + 8) * ref.U * 16 * terms + ref.rounding(fine, dtype)), f"gradient of {what}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,F,N,act,residual,p", [(4099, 3900, 520, "silu", False, 0.1), (4099, 3900, 520, "none", False, 0.1), (4099, 520, 3900, "gelu", True, 0.1),
+                                                  (4352, 1024, 4096, "relu", False, 0.0), (700, 200, 61, "relu", True, 0.3)])
+def test_gradients_of_wide_layers_are_rounded_once(device, dtype, n, F, N, act, residual, p):
+    """As test_dense_gradients_are_rounded_once, at sizes whose products go by large tiles."""
+    gen = torch.Generator(device=device).manual_seed(7)
+    x, w, b, g = ((torch.randn(*s, device=device, generator=gen) * k).to(dtype) for s, k in (((n, F), 1.0), ((N, F), F ** -0.5), ((N,), 0.5), ((n, N), 1.0)))
+    r = torch.zeros(n, N, dtype=dtype, device=device) if residual else None
+    op = layers.DenseOp(act, layers.Dropout(p, 17, 2) if p else None)
+    y = op.forward(x, w, b, r)
+    got = [op.backward(g), *op.get_additional_grad()]
+    xd, wd, bd, gd = (t.double() for t in (x, w, b, g))
+    if act == "relu":  # which sums are above 0 the layer's output says: some are so near it that 64 bits would say otherwise
+        dz = gd * float(ref.factor(p)) * (y > 0)
+    else:
+        slope = torch.from_numpy(ref.activation((xd @ wd.t() + bd).cpu().numpy(), act)[1]).to(device)
+        dz = gd * slope * (torch.from_numpy(ref.row_factors(n, N, p, 17, 2)).to(device) if p else 1.0)
+    for a, e, most in zip(got, (dz @ wd, dz.t() @ xd, dz.sum(0)), (0.5, 0.5, 1.1)):
+        assert float((a.double() - e).norm() / e.norm()) < most * torch.finfo(dtype).eps / 2
