@@ -604,7 +604,8 @@ int nts_dropout(void *out, const void *in, int type, uint32_t n, uint32_t F, con
  *   s[e, h] = score_scale <q[d, h], k[ri[e], h']>,  p = softmax of s over the edges of d,  out[d, h] = sum of drop(p[e, h]) v[ri[e], h']
  *   lse[d, h] = log of the sum of exp(s[e, h]) (float)
  * An edge whose ri[e] is not below Vs has no source and is left out (its rows are not read).  A destination without edges, or whose
- * scores are all -infinity: out 0, lse -infinity and no gradient.  NaN or +infinity among a destination's scores: NaN.
+ * scores are all -infinity: out 0, lse -infinity and no gradient.  NaN or +infinity among a destination's scores: NaN.  An edge whose score
+ * is -infinity has no part in the gradients, whatever its rows hold.
  * A probability below 2^-126 may count as 0.
  * dropout: of the probabilities, NULL for none.  edges: at least co[Vd] - co[0].  max_degree: no destination has more edges than
  * that; 0: no bound known.

@@ -233,6 +233,13 @@ struct Walk {
   }
   static __device__ __forceinline__ bool there(uint32_t where) { return NEAR ? where < kNowhere : where != kNoSlot; }
 
+  // In the gradients an edge whose score is -infinity has no part, whatever its rows hold: 0 times their infinities would be NaN.
+  static __device__ __forceinline__ void leave_out(bool out, u32x4 *x, u32x4 *y, float *gv, float *mean) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) x[j] = out ? u32x4{0, 0, 0, 0} : x[j], y[j] = out ? u32x4{0, 0, 0, 0} : y[j];
+    *gv = out ? 0.0f : *gv, *mean = out ? 0.0f : *mean;
+  }
+
   template <int U>
   __device__ __forceinline__ void step(const uint32_t *where, const uint32_t *ids, const uint32_t *words, uint32_t from) {
     const float scale2 = p.score_scale * kLog2e;
@@ -253,8 +260,11 @@ struct Walk {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float qk = dot(x[u], a), gv = dot(y[u], b);
-          const float w = there(where[u]) ? __builtin_amdgcn_exp2f(fmaf(qk, scale2, -e[u].x)) : 0.0f;
+          const float qk = dot(x[u], a);
+          float gv = dot(y[u], b);
+          const float z = fmaf(qk, scale2, -e[u].x);
+          const float w = there(where[u]) ? __builtin_amdgcn_exp2f(z) : 0.0f;
+          if (__any(z == -INFINITY)) leave_out(z == -INFINITY, x[u], y[u], &gv, &e[u].y);
           const float m = drop_factor(words[u], h - first_head - from);
           const float c = m == 0.0f ? 0.0f : gv * m;
           const float ds = w * (c - e[u].y) * p.score_scale, wm = w * m;
@@ -270,8 +280,10 @@ struct Walk {
     if (KIND == kByDestination) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float qk = dot(a, x[u]), gv = dot(b, y[u]);
-        const float w = there(where[u]) ? __builtin_amdgcn_exp2f(fmaf(qk, scale2, -base2)) : 0.0f;
+        const float qk = dot(a, x[u]), z = fmaf(qk, scale2, -base2);
+        float gv = dot(b, y[u]), none;
+        const float w = there(where[u]) ? __builtin_amdgcn_exp2f(z) : 0.0f;
+        if (__any(z == -INFINITY)) leave_out(z == -INFINITY, x[u], y[u], &gv, &none);
         const float m = drop_factor(words[u], unit - first_head), wc = m == 0.0f ? 0.0f : w * (gv * m);
         sum += wc;
 #pragma unroll
