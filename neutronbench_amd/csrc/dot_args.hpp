@@ -6,7 +6,9 @@
 //   by source     (offsets, ids: the edges by source)
 //                 gk[s] = scale sum_e p_e (c_e - mean[dst e]) q[dst e], gv[s] = sum_e m_e p_e g[dst e]
 // per query head, which shares its keys and values with the other heads of its group; m is the dropout's 0 or 1 / (1 - p).
-// Both sums of gq and the mean come from one pass over the edges, so neither `out` nor the scores are kept.
+// Both sums of gq and the mean come from one pass over the edges, so neither `out` nor the scores are kept.  lse was rounded, by
+// half a step of its own size, which every p of a destination is off by: the pass sums them, too, and both passes divide by that.  One
+// neighbour's p is then 1 whatever its score; with scores of 10^5 it was off by a hundredth.
 #pragma once
 
 #include "layers.hpp"
@@ -14,6 +16,11 @@
 namespace nts {
 
 enum Kind { kForward, kByDestination, kBySource };
+
+// What the pass by destination leaves of a destination's head for the one by source: lse over log 2, mean, 1 / sum of p.
+struct Ends {
+  float base2, mean, share;
+};
 
 // A lane holds 16 columns of one head ("unit": a query head, by source a head of keys) in pieces of 16 bytes that lie ND lanes
 // apart, so that neighbouring lanes read neighbouring pieces.  ND lanes (a power of two) cover a unit, 2^hw_shift units lie side by
@@ -23,7 +30,7 @@ enum Kind { kForward, kByDestination, kBySource };
 struct DotArgs {
   void *out, *out2;  // out; gq; gk and gv
   float *lse;
-  float2 *ends;  // [Vd, q_heads]: lse over log 2, mean
+  Ends *ends;  // [Vd, q_heads]
   const void *q, *k, *v, *g;
   const uint32_t *offsets, *ids;
   uint32_t rows, others;  // rows that are walked over; rows that ids may name
@@ -43,7 +50,7 @@ struct DotArgs {
 template <int KIND>
 __host__ __device__ __forceinline__ uint64_t record_size(uint32_t q_heads, uint32_t heads, uint32_t D) {
   if (KIND == kForward) return static_cast<uint64_t>(q_heads) * (D + 2u);
-  if (KIND == kByDestination) return static_cast<uint64_t>(q_heads) * (2u * D + 1u);
+  if (KIND == kByDestination) return static_cast<uint64_t>(q_heads) * (2u * D + 2u);
   return 2ull * heads * D;
 }
 

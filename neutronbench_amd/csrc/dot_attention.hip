@@ -94,7 +94,7 @@ int run(DotArgs p, int type, uint32_t edges, uint32_t max_degree, void *work, hi
   }
   const uint64_t width = static_cast<uint64_t>(KIND == kBySource ? p.q_heads : p.heads) * p.D * size;
   const void *const x = KIND == kBySource ? p.q : p.k, *const y = KIND == kBySource ? p.g : p.v;
-  const bool near = !p.narrow && p.others <= (1u << 24) && p.others * std::max<uint64_t>(width, p.q_heads * sizeof(float2)) <= kMostNear &&
+  const bool near = !p.narrow && p.others <= (1u << 24) && p.others * std::max<uint64_t>(width, p.q_heads * sizeof(Ends)) <= kMostNear &&
                     p.D * size % 4 == 0 && aligned_to(x, 4) && aligned_to(y, 4);
   const auto launch_it = type == NTS_F32 ? dot_launch_f32 : type == NTS_BF16 ? dot_launch_bf16 : dot_launch_f16;
   return launch_it(KIND, p, l.nd, near, stream);
@@ -119,7 +119,7 @@ size_t spans_work(uint32_t rows, uint32_t edges, uint32_t q_heads, uint32_t head
   if (rows == 0 || !by_spans<KIND>(rows, edges, max_degree)) return 0;
   return spans_for<KIND>(rows, edges, q_heads, heads, D, lanes_of<KIND>(rows, edges, q_heads, heads, D, max_degree)).bytes;
 }
-size_t ends_bytes(uint32_t Vd, uint32_t q_heads) { return (static_cast<size_t>(Vd) * q_heads * sizeof(float2) + 15) / 16 * 16; }
+size_t ends_bytes(uint32_t Vd, uint32_t q_heads) { return (static_cast<size_t>(Vd) * q_heads * sizeof(Ends) + 15) / 16 * 16; }
 
 }  // namespace
 }  // namespace nts
@@ -173,7 +173,7 @@ int nts_dot_attention_grad(void *gq, void *gk, void *gv, const void *g, const vo
     if (!aligned_to(at, size)) return fail_in("nts_dot_attention_grad", "a value's alignment");
   if (!work || !aligned_to(work, 16)) return fail_in("nts_dot_attention_grad", "needs nts_dot_attention_grad_work_bytes of 16-byte-aligned work");
   DotArgs p{};
-  p.lse = const_cast<float *>(lse), p.ends = static_cast<float2 *>(work), p.q = q, p.k = k, p.v = v, p.g = g;
+  p.lse = const_cast<float *>(lse), p.ends = static_cast<Ends *>(work), p.q = q, p.k = k, p.v = v, p.g = g;
   p.q_heads = q_heads, p.heads = heads, p.share = q_heads / heads, p.D = width, p.score_scale = score_scale, p.drop = drop_args(dropout);
   p.drop.step_kept = nullptr;
   void *const rest = static_cast<char *>(work) + ends_bytes(Vd, q_heads);

@@ -30,6 +30,11 @@ constexpr int kWavesOf = KIND == kForward         ? (REACH == kWhole && FORM == 
 template <typename T>
 constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
 
+// sum: of p c, norm: of p.  Where no p counts, nothing does.
+__device__ __forceinline__ Ends ends_of(float base2, float sum, float norm) {
+  return norm == 0.0f ? Ends{base2, 0.0f, 0.0f} : Ends{base2, sum / norm, 1.0f / norm};
+}
+
 // What an edge without a row reads.
 __device__ __attribute__((aligned(16))) float zero_row[256];
 // Offsets behind the end of every buffer, which read zeros: of an edge without a row, also with a row's bytes added, and of a piece that a
@@ -96,7 +101,7 @@ struct Walk {
   uint32_t row;
   // forward: a = q, s = sum of w v.  By destination: a = q, b = g, s = sum of p c k, t = sum of p k.  By source: a = k, b = v, s = gk, t = gv.
   u32x4 a[NC], b[NC];
-  float s[C], t[C], top, sum, base2;
+  float s[C], t[C], top, sum, norm, base2;  // norm: by destination, sum of p
   uint32_t at;  // the lane's first column (of 16) after join()
 
   __device__ __forceinline__ Walk(const DotArgs &args, uint32_t pass) : p(args) {
@@ -131,7 +136,7 @@ struct Walk {
       const uint64_t bytes = static_cast<uint64_t>(p.others) * row_bytes;
       rx = buffer_of(KIND == kBySource ? p.q : p.k, bytes);
       ry = buffer_of(KIND == kBySource ? p.g : p.v, bytes);
-      if (KIND == kBySource) rends = buffer_of(p.ends, static_cast<uint64_t>(p.others) * p.q_heads * sizeof(float2));
+      if (KIND == kBySource) rends = buffer_of(p.ends, static_cast<uint64_t>(p.others) * p.q_heads * sizeof(Ends));
     }
     step_now = p.drop.threshold ? drop_step(p.drop) : 0u;
   }
@@ -182,7 +187,7 @@ struct Walk {
     row = r;
 #pragma unroll
     for (int i = 0; i < C; ++i) s[i] = t[i] = 0.0f;
-    sum = 0.0f;
+    sum = norm = 0.0f;
     top = -INFINITY;
     base2 = INFINITY;
     if (KIND == kBySource && !some) return;  // elsewhere few rows have none, and the load need not wait for the offsets
@@ -247,27 +252,27 @@ struct Walk {
       const uint32_t h0 = unit * p.share + from, h1 = min(h0 + 32u, unit * p.share + p.share);
       for (uint32_t h = h0; h < h1; ++h) {
         u32x4 x[U][NC], y[U][NC];
-        float2 e[U];
+        Ends e[U];
         request<U>(where, (h - unit * p.share) * p.D * static_cast<uint32_t>(sizeof(T)), x, y);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (NEAR) {
-            const auto got = __builtin_amdgcn_raw_buffer_load_b64(rends, there(where[u]) ? (__umul24(ids[u], p.q_heads) + h) * 8u : kNowhere, 0, 0);
-            e[u] = make_float2(__uint_as_float(got[0]), __uint_as_float(got[1]));
+            const auto got = __builtin_amdgcn_raw_buffer_load_b96(rends, there(where[u]) ? (__umul24(ids[u], p.q_heads) + h) * static_cast<uint32_t>(sizeof(Ends)) : kNowhere, 0, 0);
+            e[u] = Ends{__uint_as_float(got[0]), __uint_as_float(got[1]), __uint_as_float(got[2])};
           } else {
-            e[u] = *(there(where[u]) ? p.ends + static_cast<uint64_t>(ids[u]) * p.q_heads + h : reinterpret_cast<const float2 *>(zero_row));
+            e[u] = *(there(where[u]) ? p.ends + static_cast<uint64_t>(ids[u]) * p.q_heads + h : reinterpret_cast<const Ends *>(zero_row));
           }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float qk = dot(x[u], a);
           float gv = dot(y[u], b);
-          const float z = fmaf(qk, scale2, -e[u].x);
-          const float w = there(where[u]) ? __builtin_amdgcn_exp2f(z) : 0.0f;
-          if (__any(z == -INFINITY)) leave_out(z == -INFINITY, x[u], y[u], &gv, &e[u].y);
+          const float z = fmaf(qk, scale2, -e[u].base2);
+          const float w = there(where[u]) ? __builtin_amdgcn_exp2f(z) * e[u].share : 0.0f;
+          if (__any(z == -INFINITY)) leave_out(z == -INFINITY, x[u], y[u], &gv, &e[u].mean);
           const float m = drop_factor(words[u], h - first_head - from);
           const float c = m == 0.0f ? 0.0f : gv * m;
-          const float ds = w * (c - e[u].y) * p.score_scale, wm = w * m;
+          const float ds = w * (c - e[u].mean) * p.score_scale, wm = w * m;
 #pragma unroll
           for (int i = 0; i < C; ++i)
             s[i] = fmaf(ds, value_of<T>(x[u][i / CH], i % CH), s[i]), t[i] = fmaf(wm, value_of<T>(y[u][i / CH], i % CH), t[i]);
@@ -285,7 +290,7 @@ struct Walk {
         const float w = there(where[u]) ? __builtin_amdgcn_exp2f(z) : 0.0f;
         if (__any(z == -INFINITY)) leave_out(z == -INFINITY, x[u], y[u], &gv, &none);
         const float m = drop_factor(words[u], unit - first_head), wc = m == 0.0f ? 0.0f : w * (gv * m);
-        sum += wc;
+        sum += wc, norm += w;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const float k = value_of<T>(x[u][i / CH], i % CH);
@@ -395,6 +400,7 @@ struct Walk {
       return KIND == kForward ? fmaf(v.y, o, v.x * f) : v.x + v.y;
     };
     if (KIND != kBySource) sum = joined(sum, sum);
+    if (KIND == kByDestination) norm = joined(norm, norm);
 #pragma unroll
     for (int i = 0; i < (HALF ? HALF : 1); ++i) {
       s[i] = joined(s[i], s[i + HALF]);
@@ -472,9 +478,10 @@ struct Walk {
       for (int i = 0; i < C; ++i) s[i] = sum == 0.0f ? 0.0f : s[i] * f;
       if (dl == 0 && slot == 0) (p.lse + head)[unit] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
+      const Ends e = ends_of(base2, sum, norm);
 #pragma unroll
-      for (int i = 0; i < C; ++i) s[i] = fmaf(-sum, t[i], s[i]) * p.score_scale;
-      if (dl == 0 && slot == 0) (p.ends + head)[unit] = make_float2(base2, sum);
+      for (int i = 0; i < C; ++i) s[i] = fmaf(-e.mean, t[i], s[i]) * (p.score_scale * e.share);
+      if (dl == 0 && slot == 0) (p.ends + head)[unit] = e;
     }
     store(static_cast<T *>(p.out) + first, own_at, s);
   }
@@ -488,7 +495,7 @@ struct Walk {
     if (KIND != kForward) store(to, columns + own_at, t);
     if (dl == 0 && slot == 0) {
       if (KIND == kForward) to[columns + unit] = top, to[columns + p.q_heads + unit] = sum;
-      if (KIND == kByDestination) to[2u * columns + unit] = sum;
+      if (KIND == kByDestination) to[2u * columns + unit] = sum, to[2u * columns + p.q_heads + unit] = norm;
     }
   }
 };
@@ -609,11 +616,11 @@ __global__ __launch_bounds__(256, (kWavesOf<T, KIND, REACH, WIDE ? kWide : kNarr
 // all take every kJoinWaves-th part, and the first adds up what they have.  Parts in order, so the same bits on every call.  2.48 M edges of 8
 // heads of 64: 20-30 us.
 constexpr uint32_t kJoinWaves = 16, kJoinSpans = 32, kJoinAhead = 8, kJoinAlone = 16;
-// What the parts of a column come to.  Forward: largest score, sum and weighted sum; by destination: none, mean, both sums.
+// What the parts of a column come to.  Forward: largest score, sum and weighted sum; by destination: the sums of p k, p c, p c k and p.
 template <int KIND>
 struct Joined {
-  float top = KIND == kForward ? -INFINITY : 0.0f, sum = 0.0f, acc = 0.0f;
-  __device__ __forceinline__ void add(float t, float l, float v) {
+  float top = KIND == kForward ? -INFINITY : 0.0f, sum = 0.0f, acc = 0.0f, norm = 0.0f;
+  __device__ __forceinline__ void add(float t, float l, float v, float n) {
     if (KIND == kForward) {
       const float now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
       const float f = __builtin_amdgcn_exp2f(top - base), o = __builtin_amdgcn_exp2f(t - base);
@@ -621,37 +628,39 @@ struct Joined {
       sum = sum * f + l * o;
       acc = acc * f + v * o;
     } else {
-      top += t, sum += l, acc += v;
+      top += t, sum += l, acc += v, norm += n;
     }
   }
 };
 template <typename T, int KIND>
 __global__ __launch_bounds__(kJoinWaves *kWave) void join_dot_spans_kernel(DotArgs p) {
-  __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave];
-  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block();
+  __shared__ float tops[kJoinWaves][kWave], sums[kJoinWaves][kWave], accs[kJoinWaves][kWave], norms[KIND == kByDestination ? kJoinWaves : 1][kWave];
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = wave_of_block(), of_norms = KIND == kByDestination ? wave : 0u;
   const uint32_t columns = (KIND == kBySource ? 2u * p.heads : p.q_heads) * p.D, c = blockIdx.y * kWave + lane, cc = min(c, columns - 1u), h = cc / p.D;
   const uint64_t size = record_size<KIND>(p.q_heads, p.heads, p.D);
   const uint64_t span0 = static_cast<uint64_t>(blockIdx.x) * kJoinSpans;
   const uint32_t rows = lane < kJoinSpans && span0 + lane < p.spans ? p.tail_row[span0 + lane] : kNoSlot;
   uint64_t cut = __ballot(rows != kNoSlot);  // the same in every wavefront
-  // where a record has the three numbers of a column
+  // where a record has the other numbers of a column
   const uint64_t at_a = KIND == kForward ? columns + h : columns + cc, at_b = KIND == kForward ? columns + p.q_heads + h : 2ull * columns + h;
+  const uint64_t at_c = 2ull * columns + p.q_heads + h;
   auto parts_of = [&](uint64_t first, uint64_t last, uint64_t from, uint64_t step) {
     Joined<KIND> j;
     for (uint64_t s = from; s <= last; s += kJoinAhead * step) {
-      float t[kJoinAhead], l[kJoinAhead], v[kJoinAhead];
+      float t[kJoinAhead], l[kJoinAhead], v[kJoinAhead], n[kJoinAhead];
 #pragma unroll
       for (uint32_t u = 0; u < kJoinAhead; ++u) {
         const uint64_t part = s + u * step;
-        t[u] = KIND == kForward ? -INFINITY : 0.0f, l[u] = v[u] = 0.0f;
+        t[u] = KIND == kForward ? -INFINITY : 0.0f, l[u] = v[u] = n[u] = 0.0f;
         if (part <= last) {
           const float *const record = p.partial + (part * 2u + (part == first ? 1u : 0u)) * size;
           v[u] = record[cc];
           if (KIND != kBySource) t[u] = record[at_a], l[u] = record[at_b];
+          if (KIND == kByDestination) n[u] = record[at_c];
         }
       }
 #pragma unroll
-      for (uint32_t u = 0; u < kJoinAhead; ++u) j.add(t[u], l[u], v[u]);
+      for (uint32_t u = 0; u < kJoinAhead; ++u) j.add(t[u], l[u], v[u], n[u]);
     }
     return j;
   };
@@ -662,11 +671,10 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_dot_spans_kernel(DotAr
       put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, j.sum == 0.0f ? 0.0f : j.acc / j.sum);
       if (c == h * p.D) p.lse[head] = j.sum == 0.0f ? -INFINITY : (j.top + __builtin_amdgcn_logf(j.sum)) * kLn2;
     } else if (KIND == kByDestination) {
-      put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, fmaf(-j.sum, j.top, j.acc) * p.score_scale);
-      if (c == h * p.D) {
-        const float l = p.lse[head];
-        p.ends[head] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, j.sum);
-      }
+      const float l = p.lse[head];
+      const Ends e = ends_of(l == -INFINITY ? INFINITY : l * kLog2e, j.sum, j.norm);
+      put_value(static_cast<T *>(p.out) + static_cast<uint64_t>(row) * columns + c, fmaf(-e.mean, j.top, j.acc) * (p.score_scale * e.share));
+      if (c == h * p.D) p.ends[head] = e;
     } else {
       const bool second = c >= columns / 2u;
       put_value(static_cast<T *>(second ? p.out2 : p.out) + static_cast<uint64_t>(row) * (columns / 2u) + (second ? c - columns / 2u : c), j.acc);
@@ -688,9 +696,10 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_dot_spans_kernel(DotAr
     const uint64_t first = span0 + k;
     Joined<KIND> j = parts_of(first, last_part(row), first + wave, kJoinWaves);
     tops[wave][lane] = j.top, sums[wave][lane] = j.sum, accs[wave][lane] = j.acc;
+    if (KIND == kByDestination) norms[of_norms][lane] = j.norm;
     __syncthreads();
     if (wave == 0) {
-      for (uint32_t w = 1; w < kJoinWaves; ++w) j.add(tops[w][lane], sums[w][lane], accs[w][lane]);
+      for (uint32_t w = 1; w < kJoinWaves; ++w) j.add(tops[w][lane], sums[w][lane], accs[w][lane], norms[KIND == kByDestination ? w : 0][lane]);
       write(row, j);
     }
     __syncthreads();

@@ -51,3 +51,54 @@ def test_no_gradient_from_scores_of_minus_infinity(device, dtype, D, form, where
     assert np.isneginf(want["lse"][0][5]).all()
     for name, t in zip(("out", "lse", "q", "k", "v"), got):
         ref.check(t, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [16, 20])
+@pytest.mark.parametrize("form", ["spans", "rows"])
+def test_one_neighbour_has_all(device, dtype, D, form):
+    """Destinations of one edge: its probability is 1, however large its score is."""
+    Vd, Vs, H = 300, 40, 4
+    rng = np.random.default_rng(7)
+    co, ri = np.arange(Vd + 1, dtype=np.uint32), rng.integers(0, Vs, Vd).astype(np.uint32)
+    (q, _), (k, _), (v, v64), (g, g64) = (rows(n, H * D, 50 + i, dtype, device, s) for i, (n, s) in enumerate(((Vd, 300.0), (Vs, 300.0), (Vs, 1.0), (Vd, 1.0))))
+    drop = (0.25, 9, 1)
+    out, lse, gq, gk, gv = gradients(device, co, ri, q, k, v, g, H, drop, 1 if form == "rows" else 0)
+    assert float(lse.abs().max()) > 1e5
+    m = ref.edge_factors(ri, np.arange(Vd), H, *drop)[:, :, None]
+    ge, ve = g64.reshape(Vd, H, D), v64.reshape(Vs, H, D)[ri]
+    want, size = np.zeros((Vs, H, D)), np.zeros((Vs, H, D))
+    np.add.at(want, ri, m * ge)
+    np.add.at(size, ri, m * np.abs(ge))
+    uses = np.bincount(ri, minlength=Vs)[:, None, None]
+    # p is a quotient of a number by itself (2 half steps), then a product and a sum of as many terms as the source has edges
+    bound = (uses + 6) * ref.U * size + ref.rounding(want, dtype)
+    ref.check(gv, (want.reshape(Vs, -1), bound.reshape(Vs, -1)), "gradient of v")
+    # Scores do not matter to the output: p (c - mean) is 0, up to roundings of c, which is a sum of D terms in the same order in
+    # both passes but for the order of lanes: 2 (D + 4) half steps of its terms, times the other operand and the scale.
+    c = m[:, :, 0] * (np.abs(ge) * np.abs(ve)).sum(2) * 0.25 * 2 * (D + 4) * ref.U
+    most_q = c[:, :, None] * np.abs(k.double().cpu().numpy().reshape(Vs, H, D)[ri])
+    most_k = np.zeros((Vs, H, D))
+    np.add.at(most_k, ri, c[:, :, None] * np.abs(q.double().cpu().numpy().reshape(Vd, H, D)))
+    assert (np.abs(gq.double().cpu().numpy().reshape(Vd, H, D)) <= most_q * 1.01).all()
+    assert (np.abs(gk.double().cpu().numpy().reshape(Vs, H, D)) <= most_k * 1.01).all()
+
+
+@pytest.mark.parametrize("form", ["spans", "rows", "cut"])
+@pytest.mark.parametrize("H,Hk,D", [(4, 4, 32), (6, 2, 20), (2, 2, 256)])
+def test_probabilities_sum_to_one(device, form, H, Hk, D):
+    """With a gradient of ones every value's is the sum of its probabilities, and all of them together are one for every destination that has edges:
+    also with scores of some ten thousand, whose lse is rounded by a thousandth."""
+    Vs = 50
+    rng = np.random.default_rng(D)
+    co, ri = graph(rng, 80, Vs, 10, hub=6000 if form == "cut" else 0)
+    degrees = np.diff(co.astype(np.int64))
+    (q, _), (k, _), (v, _) = (rows(n, h * D, 70 + i, F32, device, s) for i, (n, h, s) in enumerate(((80, H, 60.0), (Vs, Hk, 60.0), (Vs, Hk, 1.0))))
+    op = layers.DotAttentionOp(layer_of(co, ri, Vs, device, int(degrees.max()) if form == "rows" else 0), H, Hk, 1.0)
+    op.forward(q, k, v)
+    assert float(op.lse[torch.from_numpy(degrees > 0).to(device)].abs().median()) > 5e3
+    op.backward(torch.ones_like(q))
+    gv = op.get_additional_grad()[1].double().cpu().numpy().reshape(Vs, Hk, D).sum(0)
+    # a destination's p: as many additions in the sum that they are divided by, the division, a product, and as many additions by source
+    terms = degrees.max() + np.bincount(ri, minlength=Vs).max() * (H // Hk) + 20
+    assert (np.abs(gv - (degrees > 0).sum() * (H // Hk)) <= terms * ref.U * (degrees > 0).sum() * (H // Hk)).all()
