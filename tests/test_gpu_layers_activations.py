@@ -1,0 +1,57 @@
+"""GELU and SiLU of dense layers and their slopes, value by value: as good as in 32 bits, also where they are small."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import layers_ref as ref
+from neutronbench_amd import layers
+from test_gpu_layers import BF16, F16, F32, TYPES
+
+pytestmark = pytest.mark.gpu
+
+
+def values(dtype, seed):
+    """-14 .. 14 evenly, and normally distributed values, as `dtype` holds them: 16 bits hold few, 32 bits 40,000."""
+    rng = np.random.default_rng(seed)
+    z = np.concatenate([np.linspace(-14, 14, 20001), rng.standard_normal(20000), [0.0, -0.0, 1.25, -1.25, 1e-30, -1e-30, 30.0, -30.0, 80.0]])
+    return torch.from_numpy(z.astype(np.float32)).to(dtype).unique()[:, None].contiguous()
+
+
+def gelu(z):
+    """Value, slope and what a computation in 32 bits may be off by (u half steps): the share behind |z| by its density's argument, z^2 / 2, which is
+    rounded twice, and some 14 further roundings; the share's larger part by three of its own; below 2^-126 it may count as 0."""
+    below = 0.5 * torch.erfc(torch.from_numpy(-z / math.sqrt(2))).numpy()
+    density = np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    off = ref.U * ((14 + z * z) * np.minimum(below, 1 - below) + 3 * below) + 2.0 ** -126
+    slope = below + z * density
+    return z * below, np.abs(z) * off + ref.U * np.abs(z * below), slope, off + np.abs(z) * (density * (z * z + 8) * ref.U + 2.0 ** -126) + 2 * ref.U * np.abs(slope)
+
+
+def check(device, dtype, act, value):
+    z = values(dtype, 3)
+    zd = z.double().numpy()
+    y64, dy, slope64, dslope = value(zd)
+    one = torch.ones(1, 1, dtype=dtype, device=device)
+    op = layers.DenseOp(act)
+    y = op.forward(z.to(device), one)
+    ref.check(y, (y64, dy + ref.rounding(y64, dtype)), act)
+    slope = op.backward(torch.ones_like(y))
+    ref.check(slope, (slope64, dslope + ref.rounding(slope64, dtype)), f"slope of {act}")
+    few = layers.DenseOp(act)
+    for i in range(0, len(z), 997):  # up to eight rows go another way
+        ref.check(few.forward(z[i:i + 8].to(device), one), (y64[i:i + 8], (dy + ref.rounding(y64, dtype))[i:i + 8]), f"{act} of few rows")
+    if dtype == F32:  # and of the whole: as a 32-bit erf or exponential
+        rng = np.random.default_rng(4)
+        z = torch.from_numpy(rng.standard_normal((100000, 1)).astype(np.float32))
+        y64, _, slope64, _ = value(z.double().numpy())
+        y = op.forward(z.to(device), one)
+        # about one half step of rounding for each of a handful of operations, which add like random numbers
+        for got, want in ((y, y64), (op.backward(torch.ones_like(y)), slope64)):
+            assert np.linalg.norm(got.double().cpu().numpy() - want) / np.linalg.norm(want) < ref.U
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu(device, dtype):
+    check(device, dtype, "gelu", gelu)
