@@ -68,7 +68,16 @@ __device__ __forceinline__ float normal_below(float z, float *bell) {
   }
   return z < 0.0f ? far : 1.0f - far;
 }
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+// 1 / (1 + e^-z).  z log2 e is rounded by as much as it is large, which the exponential of 16 is off by 1e-6 for.  For operands of 32 bits what
+// that leaves goes into a factor near 1 (beyond 200 nothing changes, and the factor is a number there); results of 16 bits do not see it, and
+// forward 169,343 rows of 128 by 128 in bf16 would take 31.4 us instead of 29.1.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  if (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+  const float to = __builtin_amdgcn_fmed3f(z, -200.0f, 200.0f), x = to * -1.44269504f;
+  const float rest = fmaf(to, -1.92596299e-8f, fmaf(to, -1.44269504f, -x));
+  return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(x), fmaf(rest, 0.693147181f, 1.0f), 1.0f));
+}
 template <typename T, int N>
 __device__ __forceinline__ void activate(float *z, int act) {
   if (act == NTS_ACT_RELU) {
@@ -80,7 +89,7 @@ __device__ __forceinline__ void activate(float *z, int act) {
     for (int k = 0; k < N; ++k) z[k] *= normal_below<T>(z[k], &bell);
   } else if (act == NTS_ACT_SILU) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) z[k] *= sigmoid(z[k]);
+    for (int k = 0; k < N; ++k) z[k] *= sigmoid<T>(z[k]);
   }
 }
 // g times the activation's slopes at z.
@@ -99,7 +108,7 @@ __device__ __forceinline__ void through_slope(float *z, const float *g, int act)
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float f = sigmoid(z[k]);
+      const float f = sigmoid<T>(z[k]);
       z[k] = g[k] * (f * fmaf(z[k], 1.0f - f, 1.0f));
     }
   }

@@ -55,3 +55,33 @@ def check(device, dtype, act, value):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gelu(device, dtype):
     check(device, dtype, "gelu", gelu)
+
+
+def silu(z, argument=0.0):
+    """Likewise: an exponential, a sum and a quotient are off by six half steps together, whatever z; below 2^-126 the quotient may count as 0.
+    argument: times |z| half steps more, from an exponential whose argument was rounded."""
+    f = 1 / (1 + np.exp(-z))
+    behind = 1 / (1 + np.exp(z))
+    slope = f * (1 + z * behind)
+    off = (6 + argument * np.abs(z)) * ref.U * f + 2.0 ** -126
+    # 1 - f is off by as much as f and by its own rounding
+    return z * f, np.abs(z) * (off + ref.U * f), slope, off * (1 + np.abs(z)) + f * np.abs(z) * 2 * ref.U * ((1 + argument * np.abs(z)) * f + 2 * behind) + 3 * ref.U * np.abs(slope)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu(device, dtype):
+    check(device, dtype, "silu", silu if dtype == F32 else lambda z: silu(z, 1.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_activations_far_out(device, dtype):
+    """Where the sigmoid and the share below are 0 or 1: the value is z or 0, the slope 1 or 0."""
+    most = torch.finfo(dtype).max
+    z = torch.tensor([[200.0], [1e4], [most], [-200.0], [-1e4], [-most]] * 3, dtype=dtype, device=device)
+    one = torch.ones(1, 1, dtype=dtype, device=device)
+    for act in ("gelu", "silu"):
+        for x in (z, z[:6]):
+            op = layers.DenseOp(act)
+            assert torch.equal(op.forward(x, one), torch.where(x > 0, x, torch.zeros_like(x)))
+            assert torch.equal(op.backward(torch.ones_like(x)), (x > 0).to(dtype))
+        assert float(layers.DenseOp(act).forward(torch.full((9, 1), math.inf, dtype=dtype, device=device), one).min()) == math.inf
