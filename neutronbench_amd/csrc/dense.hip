@@ -383,8 +383,7 @@ __device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sum
   }
 }
 
-// Many rows.  A block of 4 * WN wavefronts takes 64 * MR rows by 128 * WN columns, a stage of 32 terms after the other, and then its next
-// rows.  Rows go from memory to the registers that the matrix instructions read, each to the one wavefront (of a column group) that
+// Many rows.  A block of four wavefronts takes 64 * MR rows by 128 columns, a stage of 32 terms after the other, and then its next rows.  Rows go from memory to the registers that the matrix instructions read, each to the one wavefront that
 // needs them, and are split there; the prepared weight goes to LDS by loads that write it themselves.  Both are a stage ahead, past the end
 // of a tile too.
 // MR: 16 rows each, of a wavefront.
@@ -393,28 +392,28 @@ __device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sum
 // (splitting one tile between the instructions of the other, or three blocks to a compute unit, which spill, did not help).  169,343 rows of
 // 128 by 128 in bf16 with GELU, drops and residual take 55 us, 2.4 TB/s: vector instructions of the epilogue for half of the time.
 // A: the rows' type.
-template <typename A, typename T, int USE, int MR, int WN, bool MASKED>
+template <typename A, typename T, int USE, int MR, bool MASKED>
 __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
   constexpr int P = kPlanes<A>, PB = kPlanesBeside<A, T>;
-  constexpr uint32_t kRows = 64 * MR, kStage = WN * PB * kPlane;
+  constexpr uint32_t kTileRows = 64 * MR, kStage = PB * kPlane;
   // results are turned where the stage of the weight was that has been used last, if it is large enough
-  constexpr bool kApart = kStage * sizeof(uint16_t) < 4u * WN * 4096u;
-  __shared__ __attribute__((aligned(16))) uint16_t weight0[kStage], weight1[kStage], apart[kApart ? 4 * WN * 2048 : 8];
+  constexpr bool kApart = kStage * sizeof(uint16_t) < 4u * 4096u;
+  __shared__ __attribute__((aligned(16))) uint16_t weight0[kStage], weight1[kStage], apart[kApart ? 4 * 2048 : 8];
   const uint32_t t = threadIdx.x, lane = t & (kWave - 1), wave = wave_of_block(), r = lane & 15u, part = lane >> 4;
   // neighbouring blocks of a chiplet take the columns of one worker's rows
   const uint32_t x = blockIdx.x / 8u, tn = x % p.tiles_n, worker = x / p.tiles_n * 8u + blockIdx.x % 8u;
-  const uint32_t wr = wave & 3u, wc = wave >> 2, stages = (p.K + kTerms - 1u) / kTerms;
+  const uint32_t stages = (p.K + kTerms - 1u) / kTerms;
   const uint32_t step = USE == kLayer || USE == kSlope ? drop_step(p.drop) : 0u;
   if (USE == kLayer && p.drop.step_kept && blockIdx.x == 0 && t == 0) *p.drop.step_kept = step;
   if (!has_rows(worker, p.workers)) return;
-  const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * WN * stages * PB * kPlane;
+  const uint16_t *const weight = static_cast<const uint16_t *>(p.b) + static_cast<uint64_t>(tn) * stages * PB * kPlane;
   const A *const rows = static_cast<const A *>(p.a);
   // stage s of the weight
   auto request_weight = [&](uint16_t *to, uint32_t s) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t i = 0; i < 2 * PB; ++i) {
-      const uint32_t piece = i * 4 * WN + wave, group = piece / (8 * PB), at = piece % (8 * PB);  // 512 values each
-      load_to_lds(weight + ((static_cast<uint64_t>(group) * stages + s) * PB * kPlane + at * 512u + lane * 8u), to + piece * 512u);
+      const uint32_t piece = i * 4 + wave;  // 512 values each
+      load_to_lds(weight + (static_cast<uint64_t>(s) * PB * kPlane + piece * 512u + lane * 8u), to + piece * 512u);
     }
   };
   typedef typename ValueOf<A>::raw raw;
@@ -425,7 +424,7 @@ __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
   auto place = [&](uint32_t tile) __attribute__((always_inline)) {  // rows that the result does not have read the last one
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-      const uint64_t row = static_cast<uint64_t>(tile) * kRows + wr * (16u * MR) + i * 16u + r;
+      const uint64_t row = static_cast<uint64_t>(tile) * kTileRows + wave * (16u * MR) + i * 16u + r;
 #pragma unroll
       for (int o = 0; o < S; ++o)
         row_at[o][i] = (o ? static_cast<const A *>(p.y) : rows) + min(row, static_cast<uint64_t>(p.M - 1u)) * p.a_stride + part * 8u;
@@ -475,7 +474,7 @@ __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
   f32x4 acc[MR][8];
   uint32_t half = 0;
   float bias[2][4] = {};
-  if (USE != kRows) bias_of_columns<T>(p, tn * (kTile * WN) + wc * kTile, bias);
+  if (USE != kRows) bias_of_columns<T>(p, tn * kTile, bias);
   float sums[2][4] = {};
   place(worker);
   request_weight(weight0, 0);
@@ -513,7 +512,7 @@ __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
         request_weight(half ? weight0 : weight1, last ? 0u : s + 1u);
         request_rows(last ? 0u : s + 1u);
       }
-      const uint16_t *const w = (half ? weight1 : weight0) + wc * (PB * kPlane);
+      const uint16_t *const w = half ? weight1 : weight0;
       half ^= 1u;
       u32x4 b[2][PB];
 #pragma unroll
@@ -535,20 +534,20 @@ __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
     }
     if (!kApart) __builtin_amdgcn_s_barrier();  // all have read it
     finish_tile<A, T, USE, MR, MASKED>(p, step, acc, reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u,
-                                    static_cast<uint64_t>(tile) * kRows + wr * (16u * MR), tn * (kTile * WN) + wc * kTile, bias, sums);
+                                    static_cast<uint64_t>(tile) * kTileRows + wave * (16u * MR), tn * kTile, bias, sums);
   }
-  if (USE == kSlope && p.sums) block_sums<4 * WN, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0), worker, tn * (kTile * WN));
+  if (USE == kSlope && p.sums) block_sums<4, 4>(p, sums, reinterpret_cast<float(*)[kTile]>(kApart ? apart : weight0), worker, tn * kTile);
 }
-template <typename T, int USE, int MR, int WN, bool MASKED>
-__global__ __launch_bounds__(256 * WN, sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
-  rows_of_tiles<T, T, USE, MR, WN, MASKED>(p);
+template <typename T, int USE, int MR, bool MASKED>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void dense_rows_kernel(DenseArgs p) {
+  rows_of_tiles<T, T, USE, MR, MASKED>(p);
 }
 // Rows of dz in 32 bits times a weight of 16.  169,343 rows of 128 by 128: 34 us in bf16, 3.8 TB/s, as with two bf16 parts of dz, whose products
 // read the weight twice from LDS; 49 in fp16.  Large products go this way, too: 65,536 x 4,096 x 4,096 in bf16 5.7 ms, three products at
 // 1,160 TFLOP/s, where large tiles took 3.5 for two parts; in fp16 8.9.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void dense_dz_kernel(DenseArgs p) {
-  rows_of_tiles<float, T, kRows, 2, 1, false>(p);
+  rows_of_tiles<float, T, kRows, 2, false>(p);
 }
 
 // Large products of 16-bit values whose rows begin at multiples of 16 bytes: a block of eight wavefronts takes 256 rows by 256 columns, 32
@@ -968,7 +967,7 @@ constexpr uint64_t kStreamed = 32ull << 20;  // an output from this size on is m
 
 template <bool ALONG>
 int launch_prepare(void *to, const void *w, int type, uint32_t planes, uint32_t columns, uint32_t terms, uint32_t stride, hipStream_t stream) {
-  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), tile_groups(columns)};
+  const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), ceil_div(columns, kTile)};
   const dim3 grid(ceil_div(static_cast<uint64_t>(p.stages) * p.tiles * 4u * kTile, 256));
   if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, 3, ALONG>), grid, dim3(256), 0, stream, p);
   else if (planes == 2) hipLaunchKernelGGL((dense_prepare_kernel<F16, 2, ALONG>), grid, dim3(256), 0, stream, p);
@@ -979,7 +978,7 @@ int launch_prepare(void *to, const void *w, int type, uint32_t planes, uint32_t 
 
 template <typename T, int USE, bool MASKED = false>
 void launch_rows(const DenseArgs &p, const Share &share, hipStream_t stream) {
-  hipLaunchKernelGGL((dense_rows_kernel<T, USE, 2, 1, MASKED>), dim3(launched_workers(share) * p.tiles_n), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((dense_rows_kernel<T, USE, 2, MASKED>), dim3(launched_workers(share) * p.tiles_n), dim3(256), 0, stream, p);
 }
 template <typename T, int USE>
 void launch_product_of(const DenseArgs &p, const Share &share, hipStream_t stream) {

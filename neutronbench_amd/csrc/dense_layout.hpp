@@ -14,9 +14,8 @@ constexpr uint32_t kTile = 128, kTerms = 32, kPlane = kTile * kTerms;  // rows o
 constexpr uint32_t kWideTile = 256;
 
 // Bytes of a prepared weight.
-inline uint32_t tile_groups(uint32_t columns) { return ceil_div(columns, 2 * kTile) * 2u; }
 inline size_t prepared_bytes(uint32_t planes, uint32_t columns, uint32_t terms) {
-  return static_cast<size_t>(tile_groups(columns)) * ceil_div(terms, kTerms) * kPlane * planes * 2u;
+  return static_cast<size_t>(ceil_div(columns, kTile)) * ceil_div(terms, kTerms) * kPlane * planes * 2u;
 }
 // Parts of a weight: three of 32 bits; beside dz in 32 bits, which is multiplied as bf16 parts, two of fp16; else the weight itself.
 inline uint32_t planes_of(int type, bool dz32) { return type == NTS_F32 ? 3u : dz32 && type == NTS_F16 ? 2u : 1u; }
