@@ -263,6 +263,14 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// The block has read what it wanted from LDS, and the compiler moves no access past that; loads that are on their way stay so.
+__device__ __forceinline__ void block_has_read() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // What a wavefront's 16 * MR rows by 128 columns of sums become.  Through LDS (`mine`, 4 KB), 16 rows by 64 columns at a time, a lane's columns
 // become lines (part c of row r at c ^ r).  sums: of the columns, kept over tiles.
 template <typename A, typename T, int USE, int MR, bool MASKED>
@@ -532,7 +540,7 @@ __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
             for (int i = 0; i < MR; ++i) acc[i][j] = multiply<A>(b[j & 1][q - c], a[i][c], acc[i][j]);
       }
     }
-    if (!kApart) __builtin_amdgcn_s_barrier();  // all have read it
+    if (!kApart) block_has_read();
     finish_tile<A, T, USE, MR, MASKED>(p, step, acc, reinterpret_cast<f32x4 *>(kApart ? apart : half ? weight0 : weight1) + wave * 256u,
                                     static_cast<uint64_t>(tile) * kTileRows + wave * (16u * MR), tn * kTile, bias, sums);
   }
