@@ -216,7 +216,7 @@ struct Walk {
     return word;
   }
   __device__ __forceinline__ float drop_factor(uint32_t word, uint32_t bit) const {
-    return !p.drop.threshold ? 1.0f : word >> bit & 1u ? p.drop.scale : 0.0f;
+    return !p.drop.threshold ? 1.0f : word >> (bit & 31u) & 1u ? p.drop.scale : 0.0f;  // lanes without a unit have a bit that no word has
   }
 
   // Rows of U edges, requested together.  where[u]: NEAR the offset of the edge's row, kNowhere for none; else its id, kNoSlot for none.
