@@ -33,6 +33,8 @@ def _rows(t, rows, columns, like, what):
             columns is not None and t.shape[1] != columns):
         shape = f"[{'n' if rows is None else rows}, {'columns' if columns is None else columns}]"
         raise ValueError(f"{what}: a contiguous {like.dtype} tensor {shape}")
+    if max(t.shape) >= 1 << 32:
+        raise ValueError(f"{what}: fewer than 2^32 rows and columns")
 
 
 class Dropout:
