@@ -976,7 +976,7 @@ constexpr uint64_t kStreamed = 32ull << 20;  // an output from this size on is m
 template <bool ALONG>
 int launch_prepare(void *to, const void *w, int type, uint32_t planes, uint32_t columns, uint32_t terms, uint32_t stride, hipStream_t stream) {
   const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), ceil_div(columns, kTile)};
-  const dim3 grid(ceil_div(static_cast<uint64_t>(p.stages) * p.tiles * 4u * kTile, 256));
+  const dim3 grid(ceil_div(prepare_threads(columns, terms), 256));
   if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, 3, ALONG>), grid, dim3(256), 0, stream, p);
   else if (planes == 2) hipLaunchKernelGGL((dense_prepare_kernel<F16, 2, ALONG>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, 1, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied

@@ -17,6 +17,10 @@ constexpr uint32_t kWideTile = 256;
 inline size_t prepared_bytes(uint32_t planes, uint32_t columns, uint32_t terms) {
   return static_cast<size_t>(ceil_div(columns, kTile)) * ceil_div(terms, kTerms) * kPlane * planes * 2u;
 }
+// Threads that prepare it, eight terms each; columns and terms of up to 2^17 take 2^31.
+inline uint64_t prepare_threads(uint32_t columns, uint32_t terms) {
+  return static_cast<uint64_t>(ceil_div(columns, kTile)) * kTile * ceil_div(terms, kTerms) * (kTerms / 8);
+}
 // Parts of a weight: three of 32 bits; beside dz in 32 bits, which is multiplied as bf16 parts, two of fp16; else the weight itself.
 inline uint32_t planes_of(int type, bool dz32) { return type == NTS_F32 ? 3u : dz32 && type == NTS_F16 ? 2u : 1u; }
 // Large products by large tiles, where there are enough of them for the chip and rows of many terms; in us by large tiles and by rows:

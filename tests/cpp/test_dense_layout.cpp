@@ -31,6 +31,11 @@ static bool fits(const Share &s, uint32_t room, const char *what, int type, uint
 }
 
 int main() {
+  // what the gradient's products prepare: columns of x or of dz and as many terms as the other has, each once
+  for (uint32_t columns : {1u, 127u, 131071u, 131072u})
+    for (uint32_t terms : {1u, 33u, 131071u, 131072u})
+      if (prepare_threads(columns, terms) / 256 > kMostBlocks || prepare_threads(columns, terms) < static_cast<uint64_t>(columns) * terms / 8)
+        return printf("%u by %u: a launch of %llu threads\n", columns, terms, static_cast<unsigned long long>(prepare_threads(columns, terms))), 1;
   for (int type : {NTS_F32, NTS_BF16, NTS_F16})
     for (uint32_t n : {1u, 9u, 128u, 129u, 1000u, 1025u, 4099u, 4352u, 7424u, 9000u, 65536u, 65537u, 337000u})
       for (uint32_t N : {1u, 64u, 129u, 520u, 2048u, 2176u, 3900u, 4096u, 8192u, 131072u})
