@@ -398,7 +398,7 @@ __device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sum
 // 232,965 rows of 602 by 256 in 32 bits take 440-500 us, 72 GFLOP at 145-160 TFLOP/s, as the library's product of such size (152): six matrix
 // instructions a product, which are under way for half of the time, and the splitting for most of the other half; the clock falls to 1.8 GHz
 // (splitting one tile between the instructions of the other, or three blocks to a compute unit, which spill, did not help).  169,343 rows of
-// 128 by 128 in bf16 with GELU, drops and residual take 55 us, 2.4 TB/s: vector instructions of the epilogue for half of the time.
+// 128 by 128 in bf16 with GELU, drops and residual take 56 us, 2.4 TB/s: vector instructions of the epilogue for half of the time.
 // A: the rows' type.
 template <typename A, typename T, int USE, int MR, bool MASKED>
 __device__ __forceinline__ void rows_of_tiles(DenseArgs p) {
