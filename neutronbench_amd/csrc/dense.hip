@@ -391,9 +391,9 @@ __device__ __forceinline__ void block_sums(const DenseArgs &p, const float (&sum
   }
 }
 
-// Many rows.  A block of four wavefronts takes 64 * MR rows by 128 columns, a stage of 32 terms after the other, and then its next rows.  Rows go from memory to the registers that the matrix instructions read, each to the one wavefront that
-// needs them, and are split there; the prepared weight goes to LDS by loads that write it themselves.  Both are a stage ahead, past the end
-// of a tile too.
+// Many rows.  A block of four wavefronts takes 64 * MR rows by 128 columns, a stage of 32 terms after the other, and then its next rows.  Rows
+// go from memory to the registers that the matrix instructions read, each to the one wavefront that needs them, and are split there; the
+// prepared weight goes to LDS by loads that write it themselves.  Both are a stage ahead, past the end of a tile too.
 // MR: 16 rows each, of a wavefront.
 // 232,965 rows of 602 by 256 in 32 bits take 440-500 us, 72 GFLOP at 145-160 TFLOP/s, as the library's product of such size (152): six matrix
 // instructions a product, which are under way for half of the time, and the splitting for most of the other half; the clock falls to 1.8 GHz
@@ -978,7 +978,7 @@ int launch_prepare(void *to, const void *w, int type, uint32_t planes, uint32_t 
   const PrepareArgs p{w, static_cast<uint16_t *>(to), columns, terms, stride, ceil_div(terms, kTerms), ceil_div(columns, kTile)};
   const dim3 grid(ceil_div(prepare_threads(columns, terms), 256));
   if (type == NTS_F32) hipLaunchKernelGGL((dense_prepare_kernel<float, 3, ALONG>), grid, dim3(256), 0, stream, p);
-  else if (planes == 2) hipLaunchKernelGGL((dense_prepare_kernel<F16, 2, ALONG>), grid, dim3(256), 0, stream, p);
+  else if (!ALONG && planes == 2) hipLaunchKernelGGL((dense_prepare_kernel<F16, 2, false>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((dense_prepare_kernel<Bf16, 1, ALONG>), grid, dim3(256), 0, stream, p);  // the bits of both 16-bit types are copied
   NTS_LAUNCH_CHECK("dense_prepare_kernel");
   return NTS_OK;
