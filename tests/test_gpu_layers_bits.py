@@ -130,3 +130,27 @@ def test_gradients_of_wide_layers_are_rounded_once(device, dtype, n, F, N, act, 
         dz = gd * slope * (torch.from_numpy(ref.row_factors(n, N, p, 17, 2)).to(device) if p else 1.0)
     for a, e, most in zip(got, (dz @ wd, dz.t() @ xd, dz.sum(0)), (0.5, 0.5, 1.1)):
         assert float((a.double() - e).norm() / e.norm()) < most * torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act,residual", [("relu", True), ("gelu", False), ("silu", False)])
+@pytest.mark.parametrize("n", [6, 300])
+def test_infinite_gradients(device, dtype, act, residual, n):
+    """They stay in their row (of the rows' gradient) and their column's row (of the weight's), with the signs of what they are multiplied by."""
+    F, N = 40, 21
+    x, w = torch.ones(n, F, dtype=dtype, device=device), torch.full((N, F), 0.25, dtype=dtype, device=device)
+    b = torch.ones(N, dtype=dtype, device=device)
+    w[6, 3], x[2, 5], w[9, 4] = -0.25, -1.0, 0.0
+    g = torch.ones(n, N, dtype=dtype, device=device)
+    g[2, 6], g[3, 9], g[4, 1] = math.inf, -math.inf, math.nan
+    gx, gw, gb = (t.float().cpu() for t in backward(act, x, w, b, g, residual))
+    row = torch.full((F,), math.inf)
+    row[3] = -math.inf
+    assert torch.equal(gx[2], row) and torch.isnan(gx[4]).all()
+    assert torch.isnan(gx[3, 4]) and (gx[3, torch.arange(F) != 4] == -math.inf).all()  # infinity times 0
+    row = torch.full((F,), math.inf)
+    row[5] = -math.inf
+    assert torch.equal(gw[6], row) and (gw[9] == -math.inf).all() and torch.isnan(gw[1]).all()
+    assert gb[6] == math.inf and gb[9] == -math.inf and torch.isnan(gb[1])
+    others = [j for j in range(N) if j not in (1, 6, 9)]
+    assert torch.isfinite(gw[others]).all() and torch.isfinite(gb[others]).all() and torch.isfinite(gx[[i for i in range(n) if i not in (2, 3, 4)]]).all()
